@@ -416,6 +416,83 @@ int pace_kv_batch_indices_positions(const int32_t* append_indptr, const int32_t*
                                     int32_t* positions, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Quantised cache: append and page conversion                               */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of rows and of pools that are not quantised. */
+#define PACE_KV_BF16 0
+#define PACE_KV_FP16 1
+#define PACE_KV_FP32 2
+
+/* Cache formats: the element type itself, 8-bit e4m3 or 4-bit e2m1. */
+#define PACE_KV_PLAIN 0
+#define PACE_KV_MXFP8 1
+#define PACE_KV_MXFP4 2
+
+/*
+ * A quantised cache holds blocks of 32 elements along head_dim with one
+ * power-of-two scale each: the smallest 2^e (-117 <= e <= 127) with
+ * max |x| <= top * 2^e, top = 448 (PACE_KV_MXFP8) or 6 (PACE_KV_MXFP4).  An
+ * element is x * 2^-e rounded to nearest even; the scale byte is e + 127.  A
+ * block with an infinity or a NaN has the scale byte 255 and zero elements,
+ * and every value of it reads as NaN.
+ *
+ * A page is two halves, keys then values, each [page_size, H, D] elements
+ * (e4m3 bytes, or two e2m1 to a byte, the even one low) followed by
+ * [page_size, H, D / 32] scale bytes: page_size * H * D * 33 / 32 or 17 / 32
+ * bytes, which must be a multiple of 16.  The page carries its scales, so
+ * pack, unpack, move, swap, the channel and promotion take quantised pages as
+ * they are.
+ */
+
+/*
+ * pace_kv_append and pace_kv_append_indptr into a quantised cache: the same
+ * tokens, slots, skips and limits, with each row quantised as it is written.
+ * keys / values hold nnz rows of row_elems = H * D elements of elem_type.
+ */
+int pace_kv_append_mx(const void* keys, const void* values, int elem_type,
+                      int64_t token_stride_bytes, int64_t nnz,
+                      const int32_t* batch_indices, const int32_t* positions,
+                      int batch_size, void* cache, int format,
+                      int64_t num_pages, const int32_t* kv_indices,
+                      int64_t num_indices, const int32_t* kv_indptr,
+                      int page_size, int64_t row_elems, int32_t* err_count,
+                      void* stream);
+int pace_kv_append_mx_indptr(const void* keys, const void* values,
+                             int elem_type, int64_t token_stride_bytes,
+                             int64_t nnz, const int32_t* append_indptr,
+                             int batch_size, void* cache, int format,
+                             int64_t num_pages, const int32_t* kv_indices,
+                             int64_t num_indices, const int32_t* kv_indptr,
+                             const int32_t* kv_last_page_len, int page_size,
+                             int64_t row_elems, int32_t* err_count,
+                             void* stream);
+
+/*
+ * Pages from a pool of elem_type into a quantised pool, and back, all layers
+ * in one call: page dst_ids[j] of layer l becomes the quantised page src_ids[j]
+ * of layer l (every slot of it, stale ones included), or its values rounded to
+ * elem_type (a value past the type's range reads as infinity).  half_elems =
+ * page_size * H * D.  Ids are device arrays of n_pages; a page whose id is out
+ * of range on either side is skipped and counted once per layer in err_count.
+ * Destination ids must be distinct, and the pools must not share memory.
+ */
+int pace_kv_quantize_pages(const void* const* src_layers,
+                           int64_t src_pool_pages, const int32_t* src_ids,
+                           int elem_type, void* const* dst_layers,
+                           int64_t dst_pool_pages, const int32_t* dst_ids,
+                           int format, int num_layers, int64_t n_pages,
+                           int64_t half_elems, int32_t* err_count,
+                           void* stream);
+int pace_kv_dequantize_pages(const void* const* src_layers,
+                             int64_t src_pool_pages, const int32_t* src_ids,
+                             int format, void* const* dst_layers,
+                             int64_t dst_pool_pages, const int32_t* dst_ids,
+                             int elem_type, int num_layers, int64_t n_pages,
+                             int64_t half_elems, int32_t* err_count,
+                             void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Native block allocation, batch planning and single-call promotion          */
 /* ------------------------------------------------------------------------ */
 

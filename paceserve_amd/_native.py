@@ -13,13 +13,15 @@ import threading
 from ctypes import POINTER, c_char_p, c_int, c_int32, c_int64, c_uint64, c_void_p
 from pathlib import Path
 
-import torch  # noqa: F401  (binds the HIP runtime before the library loads)
+import torch  # binds the HIP runtime before the library loads
 
 LIB_PATH = Path(__file__).resolve().parent / "libpace_kv.so"
 ABI_VERSION = 2
 MAX_LAYERS_PER_LAUNCH = 64
 NOALLOC_SCRATCH_BYTES = 64 << 20
 INLINE_IDS = 512
+ELEM_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+PLAIN, MXFP8, MXFP4 = 0, 1, 2
 
 PACE_KV_OK = 0
 PACE_KV_EINVAL = -1
@@ -60,6 +62,16 @@ SIGNATURES = {
     "pace_kv_append_indptr": (
         c_int, [_VP, _VP, c_int64, c_int64, _VP, c_int, _VP, c_int64, _VP, c_int64, _VP, _VP, c_int, c_int64,
                 _VP, _VP]),
+    "pace_kv_append_mx": (
+        c_int, [_VP, _VP, c_int, c_int64, c_int64, _VP, _VP, c_int, _VP, c_int, c_int64, _VP, c_int64, _VP, c_int,
+                c_int64, _VP, _VP]),
+    "pace_kv_append_mx_indptr": (
+        c_int, [_VP, _VP, c_int, c_int64, c_int64, _VP, c_int, _VP, c_int, c_int64, _VP, c_int64, _VP, _VP, c_int,
+                c_int64, _VP, _VP]),
+    "pace_kv_quantize_pages": (
+        c_int, [_VP, c_int64, _VP, c_int, _VP, c_int64, _VP, c_int, c_int, c_int64, c_int64, _VP, _VP]),
+    "pace_kv_dequantize_pages": (
+        c_int, [_VP, c_int64, _VP, c_int, _VP, c_int64, _VP, c_int, c_int, c_int64, c_int64, _VP, _VP]),
     "pace_kv_seq_lens": (c_int, [_VP, _VP, c_int, c_int, _VP, _VP]),
     "pace_kv_batch_indices_positions": (c_int, [_VP, _VP, c_int, c_int64, _VP, _VP, _VP]),
     "pace_kv_allocator_create": (c_int, [c_int64, _VP, c_int64, POINTER(c_void_p)]),

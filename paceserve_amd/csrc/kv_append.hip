@@ -39,6 +39,7 @@
 // 16384 tokens.  Every index is checked: a token whose request, page slot or
 // page id is out of range is skipped and counted.
 #include "internal.h"
+#include "mx.h"
 
 namespace pace_kv {
 namespace {
@@ -58,8 +59,6 @@ constexpr int64_t kCachedLoadBytes = int64_t(1) << 20;
 constexpr int kSearchBlocks = 4;
 // Most entries that a wave of several requests hands round one by one.
 constexpr uint32_t kHandRound = 8;
-
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 
 struct AppendParams {
   const char* key;
@@ -280,6 +279,51 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendParams p) 
   store_row_vec(reinterpret_cast<u32x4*>(row + half) + vec, v);
 }
 
+// The same append into a quantised cache (format: mx.h): a lane carries eight
+// elements of the key row and the same eight of the value row, and four lanes
+// settle a block's scale between them.  p.row_bytes counts elements here.
+template <bool FUSED, bool UNIFORM, int TYPE, int FORMAT>
+__global__ __launch_bounds__(kThreads) void append_mx_kernel(const AppendParams p) {
+  uint32_t i, vec, first_i, last_i;
+  bool live = true;
+  if (UNIFORM) {
+    const uint32_t t = over(p.by_row, blockIdx.x);
+    vec = (blockIdx.x - t * p.row_div) * kThreads + threadIdx.x;
+    i = first_i = last_i = p.first_token + t;
+  } else {
+    uint32_t g = blockIdx.x * kThreads + threadIdx.x;
+    live = g < p.total_items;
+    if (!live) g = p.total_items - 1;
+    const uint32_t t = over(p.by_row, g);
+    vec = g - t * p.row_div;
+    i = p.first_token + t;
+    first_i = __builtin_amdgcn_readlane(i, 0);
+    last_i = __builtin_amdgcn_readlane(i, kThreads - 1);
+  }
+  FirstRound f;
+  if (!UNIFORM) {
+    f = first_round<FUSED, false>(p, i);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  const int64_t at = static_cast<int64_t>(i) * p.token_stride + vec * (kLaneElems * elem_bytes(TYPE));
+  const Run<TYPE> k = load_run<TYPE>(p.key + at);
+  const Run<TYPE> v = load_run<TYPE>(p.value + at);
+  __builtin_amdgcn_sched_barrier(0);
+  if (UNIFORM) f = first_round<FUSED, true>(p, i);
+  uint32_t page = 0, slot = 0;
+  const bool placed = locate<FUSED, UNIFORM>(p, f, first_i, last_i, i, &page, &slot);
+  if (!placed && live && vec == 0 && p.err != nullptr) atomicAdd(p.err, 1);
+  const uint32_t kb = scale_byte<FORMAT>(block_amax<TYPE>(k)), vb = scale_byte<FORMAT>(block_amax<TYPE>(v));
+  if (!placed || !live) return;
+  const int64_t elems = static_cast<int64_t>(p.page_size) * p.row_bytes;
+  const int64_t bytes = elems * mx_bits(FORMAT) / 8, half = bytes + elems / kMxBlock;
+  const int64_t e = static_cast<int64_t>(slot) * p.row_bytes + vec * kLaneElems;
+  char* data = p.cache + 2 * half * page + e * mx_bits(FORMAT) / 8;
+  char* scale = p.cache + 2 * half * page + bytes + e / kMxBlock;
+  store_run<TYPE, FORMAT>(k, kb, data, scale);
+  store_run<TYPE, FORMAT>(v, vb, data + half, scale + half);
+}
+
 // Sequence length of each request, in 32-bit arithmetic that wraps as torch's
 // does.  Bound by its launch: one instead of the five elementwise ones that
 // tensor arithmetic takes (MI355X: FlashInfer's form of a prefill of 2 x 4095
@@ -393,6 +437,82 @@ int launch_append(AppendParams& p, int64_t nnz, int batch_size, int64_t num_page
   return PACE_KV_OK;
 }
 
+template <bool FUSED, int TYPE, int FORMAT>
+const void* mx_kernel_of(bool uniform) {
+  return uniform ? reinterpret_cast<const void*>(&append_mx_kernel<FUSED, true, TYPE, FORMAT>)
+                 : reinterpret_cast<const void*>(&append_mx_kernel<FUSED, false, TYPE, FORMAT>);
+}
+
+template <bool FUSED, int TYPE>
+const void* mx_kernel_of(int format, bool uniform) {
+  return format == PACE_KV_MXFP8 ? mx_kernel_of<FUSED, TYPE, PACE_KV_MXFP8>(uniform)
+                                 : mx_kernel_of<FUSED, TYPE, PACE_KV_MXFP4>(uniform);
+}
+
+template <bool FUSED>
+const void* pick_mx_kernel(int type, int format, bool uniform) {
+  switch (type) {
+    case PACE_KV_BF16: return mx_kernel_of<FUSED, PACE_KV_BF16>(format, uniform);
+    case PACE_KV_FP16: return mx_kernel_of<FUSED, PACE_KV_FP16>(format, uniform);
+    default: return mx_kernel_of<FUSED, PACE_KV_FP32>(format, uniform);
+  }
+}
+
+// launch_append for a quantised cache; row_elems = H * D.
+int launch_append_mx(AppendParams& p, int64_t nnz, int batch_size, int64_t num_pages, int64_t num_indices,
+                     int page_size, int64_t token_stride_bytes, int64_t row_elems, int type, int format, bool fused,
+                     hipStream_t stream) {
+  if (nnz < 0 || batch_size < 0 || num_pages < 0 || num_indices < 0)
+    return fail(PACE_KV_EINVAL, "append_mx: negative size");
+  if (!is_elem_type(type)) return fail(PACE_KV_EINVAL, "append_mx: unknown element type %d", type);
+  if (!is_mx_format(format)) return fail(PACE_KV_EINVAL, "append_mx: unknown format %d", format);
+  if (nnz == 0) return PACE_KV_OK;
+  if (!p.key || !p.value || !p.cache || !p.kv_indices || !p.kv_indptr)
+    return fail(PACE_KV_EINVAL, "append_mx: NULL argument");
+  if (page_size <= 0) return fail(PACE_KV_EINVAL, "append_mx: page_size must be >= 1");
+  if (row_elems <= 0 || row_elems % kMxBlock != 0)
+    return fail(PACE_KV_EINVAL, "append_mx: a row (H * D elements) must be whole blocks of 32");
+  if (row_elems > INT32_MAX) return fail(PACE_KV_ERANGE, "append_mx: row too large (%lld)", (long long)row_elems);
+  if (mx_half_bytes(page_size * row_elems, format) % 16 != 0)
+    return fail(PACE_KV_EINVAL, "append_mx: half a quantised page must be a multiple of 16 bytes");
+  const int64_t row_bytes = row_elems * elem_bytes(type);
+  if (token_stride_bytes < row_bytes || token_stride_bytes % kVecBytes != 0)
+    return fail(PACE_KV_EINVAL, "append_mx: token stride must be >= row bytes and a multiple of 16");
+  if ((reinterpret_cast<uintptr_t>(p.key) | reinterpret_cast<uintptr_t>(p.value) |
+       reinterpret_cast<uintptr_t>(p.cache)) & 15u)
+    return fail(PACE_KV_EINVAL, "append_mx: keys, values and cache must be 16-byte aligned");
+  if (num_pages > INT32_MAX) return fail(PACE_KV_ERANGE, "append_mx: too many pages");
+  const int64_t pieces = (row_bytes + (16 << 10) - 1) / (16 << 10);  // append's limit on a call
+  if (nnz > INT32_MAX || nnz * 2 * pieces >= (int64_t(1) << 25))
+    return fail(PACE_KV_ERANGE, "append_mx: too many tokens for one call (%lld)", (long long)nnz);
+  const int64_t row_runs = row_elems / kLaneElems;
+  p.token_stride = token_stride_bytes;
+  p.num_indices = num_indices;
+  p.row_bytes = row_elems;
+  p.batch_size = static_cast<uint32_t>(batch_size);
+  p.num_pages = static_cast<uint32_t>(num_pages);
+  p.page_size = static_cast<uint32_t>(page_size);
+  p.page_log2 = exact_log2(page_size);
+  p.row_vecs = static_cast<uint32_t>(row_runs);
+  p.guess_own_request = fused && nnz <= batch_size ? 1u : 0u;
+  const bool uniform = row_runs % kThreads == 0;
+  const int64_t waves_per_row = (row_runs + kThreads - 1) / kThreads;
+  p.row_div = static_cast<uint32_t>(uniform ? waves_per_row : row_runs);
+  p.by_row = fast_div(p.row_div);
+  const void* fn = fused ? pick_mx_kernel<true>(type, format, uniform) : pick_mx_kernel<false>(type, format, uniform);
+  const int64_t max_tokens = kMaxGroupsPerLaunch / waves_per_row;
+  if (max_tokens < 1) return fail(PACE_KV_ERANGE, "append_mx: row too large (%lld)", (long long)row_elems);
+  for (int64_t t0 = 0; t0 < nnz; t0 += max_tokens) {
+    const int64_t n = nnz - t0 < max_tokens ? nnz - t0 : max_tokens;
+    p.first_token = static_cast<uint32_t>(t0);
+    p.total_items = static_cast<uint32_t>(n * row_runs);
+    void* args[] = {&p};
+    PACE_KV_TRY(hip_status(hipLaunchKernel(fn, dim3(static_cast<uint32_t>((n * row_runs + kThreads - 1) / kThreads)),
+                                           dim3(kThreads), args, 0, stream), "append_mx launch"));
+  }
+  return PACE_KV_OK;
+}
+
 }  // namespace
 }  // namespace pace_kv
 
@@ -438,6 +558,44 @@ int pace_kv_append_indptr(const void* keys, const void* values, int64_t token_st
   p.err = err_count;
   return pace_kv::launch_append(p, nnz, batch_size, num_pages, num_indices, page_size, token_stride_bytes,
                                 row_bytes, true, static_cast<hipStream_t>(stream));
+}
+
+int pace_kv_append_mx(const void* keys, const void* values, int elem_type, int64_t token_stride_bytes, int64_t nnz,
+                      const int32_t* batch_indices, const int32_t* positions, int batch_size, void* cache, int format,
+                      int64_t num_pages, const int32_t* kv_indices, int64_t num_indices, const int32_t* kv_indptr,
+                      int page_size, int64_t row_elems, int32_t* err_count, void* stream) {
+  if (nnz > 0 && (!batch_indices || !positions)) return fail(PACE_KV_EINVAL, "append_mx: NULL argument");
+  pace_kv::AppendParams p = {};
+  p.key = static_cast<const char*>(keys);
+  p.value = static_cast<const char*>(values);
+  p.batch_indices = batch_indices;
+  p.positions = positions;
+  p.kv_indices = kv_indices;
+  p.kv_indptr = kv_indptr;
+  p.cache = static_cast<char*>(cache);
+  p.err = err_count;
+  return pace_kv::launch_append_mx(p, nnz, batch_size, num_pages, num_indices, page_size, token_stride_bytes,
+                                   row_elems, elem_type, format, false, static_cast<hipStream_t>(stream));
+}
+
+int pace_kv_append_mx_indptr(const void* keys, const void* values, int elem_type, int64_t token_stride_bytes,
+                             int64_t nnz, const int32_t* append_indptr, int batch_size, void* cache, int format,
+                             int64_t num_pages, const int32_t* kv_indices, int64_t num_indices,
+                             const int32_t* kv_indptr, const int32_t* kv_last_page_len, int page_size,
+                             int64_t row_elems, int32_t* err_count, void* stream) {
+  if (nnz > 0 && batch_size == 0) return fail(PACE_KV_EINVAL, "append_mx: tokens without requests");
+  if (nnz > 0 && (!append_indptr || !kv_last_page_len)) return fail(PACE_KV_EINVAL, "append_mx: NULL argument");
+  pace_kv::AppendParams p = {};
+  p.key = static_cast<const char*>(keys);
+  p.value = static_cast<const char*>(values);
+  p.append_indptr = append_indptr;
+  p.kv_last_page_len = kv_last_page_len;
+  p.kv_indices = kv_indices;
+  p.kv_indptr = kv_indptr;
+  p.cache = static_cast<char*>(cache);
+  p.err = err_count;
+  return pace_kv::launch_append_mx(p, nnz, batch_size, num_pages, num_indices, page_size, token_stride_bytes,
+                                   row_elems, elem_type, format, true, static_cast<hipStream_t>(stream));
 }
 
 int pace_kv_seq_lens(const int32_t* kv_indptr, const int32_t* kv_last_page_len, int batch_size, int page_size,
