@@ -493,6 +493,62 @@ int pace_kv_dequantize_pages(const void* const* src_layers,
                              void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Attention over a paged cache                                               */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Attention of each request's last tokens over its pages: one token per
+ * request (a decode step), or several drafted ones under a mask (a tree to be
+ * verified, or a chain).  For request b
+ *   kv_len = max(pages - 1, 0) * page_size + kv_last_page_len[b], its queries
+ *   being its last q_len = qo_indptr[b + 1] - qo_indptr[b] tokens (already
+ *   appended; one per request and nnz == batch_size where qo_indptr is NULL);
+ *   query i sees every token before those, and the j-th of them where bit
+ *   j % 64 of tree_mask[(qo_indptr[b] + i) * mask_words + j / 64] is set
+ *   (tree_mask NULL: j <= i);
+ *   s = scale * q . k, or soft_cap * tanh(scale * q . k / soft_cap) where
+ *   soft_cap > 0;  out = softmax(s) v;  lse = log(sum exp(s)).
+ * q and out are [nnz, num_kv_heads * group, head_dim] of elem_type
+ * (PACE_KV_BF16 or PACE_KV_FP16; token strides in bytes), head h of q reads KV
+ * head h / group; lse is [nnz, num_kv_heads * group] float or NULL.
+ * head_dim is 64, 128 or 256.  The cache is one layer's, of elem_type
+ * (format PACE_KV_PLAIN) or quantised, whose values are those that
+ * pace_kv_dequantize_pages gives in elem_type.
+ *
+ * A query that sees nothing gets zeros and lse = -infinity.  A token that a
+ * query does not see, and a slot past a request's last token, never affect it,
+ * whatever they hold.  Rows of q outside every request are not written, and a
+ * request with more than max_q_len tokens, or tokens outside [0, nnz), is
+ * skipped and counted in err_count.  Tokens on a page whose id is outside
+ * [0, num_pages) are not read and count as not seen.
+ *
+ * Contexts are split over workgroups by the sizes here alone, so a captured
+ * call follows tables that change between replays.  workspace (device,
+ * 16-byte aligned) holds the parts of split requests until they are joined:
+ * pace_kv_attention_workspace gives its size, 0 where none is needed; calls
+ * that may overlap take one each.
+ *
+ * Stands beside the producer's calls in
+ * paceserve/model_executor/attention/flashinfer_attention_wrapper.py, whose
+ * attention reads the pages they write.
+ */
+int pace_kv_attention_workspace(int batch_size, int num_kv_heads, int group,
+                                int head_dim, int max_q_len,
+                                int64_t num_indices, int page_size,
+                                int64_t* bytes);
+int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type,
+                      int64_t nnz, const int32_t* qo_indptr, int batch_size,
+                      int num_kv_heads, int group, int head_dim,
+                      const void* cache, int format, int64_t num_pages,
+                      int page_size, const int32_t* kv_indices,
+                      int64_t num_indices, const int32_t* kv_indptr,
+                      const int32_t* kv_last_page_len, int max_q_len,
+                      const uint64_t* tree_mask, int mask_words, float scale,
+                      float soft_cap, void* out, int64_t out_stride_bytes,
+                      float* lse, void* workspace, int64_t workspace_size,
+                      int32_t* err_count, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Native block allocation, batch planning and single-call promotion          */
 /* ------------------------------------------------------------------------ */
 

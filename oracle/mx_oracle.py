@@ -16,7 +16,7 @@ VALUES = {"mxfp8": _E4M3, "mxfp4": _E2M1}
 
 def quantize(x: np.ndarray, fmt: str):
     """(codes [..., D], scale bytes [..., D / 32]) of x [..., D] (float64)."""
-    b = x.reshape(x.shape[:-1] + (-1, BLOCK))
+    b = x.reshape(x.shape[:-1] + (x.shape[-1] // BLOCK, BLOCK))
     finite = np.isfinite(b).all(-1)
     amax = np.where(finite, np.abs(np.where(np.isfinite(b), b, 0)).max(-1), 0)
     e = np.full(amax.shape, -117)
@@ -45,12 +45,12 @@ def values(data: np.ndarray, byte: np.ndarray, fmt: str) -> np.ndarray:
         code, sign = data & 127, data >> 7
         v = np.append(_E4M3, np.nan)[code]
     else:
-        code = np.stack([data & 15, data >> 4], -1).reshape(data.shape[:-1] + (-1,))
+        code = np.stack([data & 15, data >> 4], -1).reshape(data.shape[:-1] + (2 * data.shape[-1],))
         code, sign = code & 7, code >> 3
         v = _E2M1[code]
     v = np.where(sign == 1, -v, v)
     scale = np.where(byte == 255, np.nan, 2.0 ** (byte.astype(np.float64) - 127))
-    b = v.reshape(v.shape[:-1] + (-1, BLOCK)) * scale[..., None]
+    b = v.reshape(v.shape[:-1] + (v.shape[-1] // BLOCK, BLOCK)) * scale[..., None]
     return b.reshape(v.shape)
 
 

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import POINTER, c_char_p, c_int, c_int32, c_int64, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_uint64, c_void_p
 from pathlib import Path
 
 import torch  # binds the HIP runtime before the library loads
@@ -72,6 +72,11 @@ SIGNATURES = {
         c_int, [_VP, c_int64, _VP, c_int, _VP, c_int64, _VP, c_int, c_int, c_int64, c_int64, _VP, _VP]),
     "pace_kv_dequantize_pages": (
         c_int, [_VP, c_int64, _VP, c_int, _VP, c_int64, _VP, c_int, c_int, c_int64, c_int64, _VP, _VP]),
+    "pace_kv_attention_workspace": (
+        c_int, [c_int, c_int, c_int, c_int, c_int, c_int64, c_int, POINTER(c_int64)]),
+    "pace_kv_attention": (
+        c_int, [_VP, c_int64, c_int, c_int64, _VP, c_int, c_int, c_int, c_int, _VP, c_int, c_int64, c_int, _VP,
+                c_int64, _VP, _VP, c_int, _VP, c_int, c_float, c_float, _VP, c_int64, _VP, _VP, c_int64, _VP, _VP]),
     "pace_kv_seq_lens": (c_int, [_VP, _VP, c_int, c_int, _VP, _VP]),
     "pace_kv_batch_indices_positions": (c_int, [_VP, _VP, c_int, c_int64, _VP, _VP, _VP]),
     "pace_kv_allocator_create": (c_int, [c_int64, _VP, c_int64, POINTER(c_void_p)]),
