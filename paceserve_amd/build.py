@@ -10,6 +10,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -19,8 +21,9 @@ INCLUDE_DIR = REPO_DIR / "include"
 LIB_NAME = "libpace_kv.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 
-SOURCES = ["kv_copy.hip", "kv_stage.hip", "kv_plan.cpp", "kv_append.hip", "kv_mx.hip", "kv_attention.hip", "kv_channel.cpp"]
-HEADERS = ["internal.h", "mx.h"]
+SOURCES = ["kv_attention_d128.hip", "kv_attention_d256.hip", "kv_attention_d64.hip", "kv_copy.hip", "kv_stage.hip",
+           "kv_plan.cpp", "kv_append.hip", "kv_mx.hip", "kv_attention.hip", "kv_channel.cpp"]
+HEADERS = ["internal.h", "mx.h", "attention.h"]
 
 # Packed-FP32 instructions are disabled for every HIP translation unit.
 HIPCC_FLAGS = [
@@ -28,7 +31,6 @@ HIPCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     "-Wall",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
@@ -45,11 +47,7 @@ def hipcc_path() -> str:
     return found
 
 
-def build_library(verbose: bool = False) -> Path:
-    """Compiles every HIP source into LIB_PATH (always recompiles)."""
-    srcs = [str(CSRC_DIR / s) for s in SOURCES]
-    tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [hipcc_path(), *HIPCC_FLAGS, f"-I{INCLUDE_DIR}", f"-I{CSRC_DIR}", "-o", str(tmp), *srcs]
+def _run(cmd, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
@@ -60,6 +58,20 @@ def build_library(verbose: bool = False) -> Path:
         raise RuntimeError("hipcc failed:\n" + "\n".join(msgs))
     if verbose and msgs:
         print("\n".join(msgs), flush=True)
+
+
+def build_library(verbose: bool = False) -> Path:
+    """Compiles every HIP source into LIB_PATH (always recompiles), sources
+    side by side: the attention kernels of one head_dim take a minute."""
+    tmp = LIB_PATH.with_suffix(".so.tmp")
+    hipcc = hipcc_path()
+    workers = min(len(SOURCES), os.cpu_count() or 1, int(os.environ.get("MAX_JOBS", "8")))
+    with tempfile.TemporaryDirectory() as folder:
+        objs = [str(Path(folder) / (s + ".o")) for s in SOURCES]
+        with ThreadPoolExecutor(workers) as pool:
+            list(pool.map(lambda so: _run([hipcc, *HIPCC_FLAGS, f"-I{INCLUDE_DIR}", f"-I{CSRC_DIR}", "-c",
+                                           str(CSRC_DIR / so[0]), "-o", so[1]], verbose), zip(SOURCES, objs)))
+        _run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", str(tmp), *objs], verbose)
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

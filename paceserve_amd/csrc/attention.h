@@ -1,0 +1,581 @@
+// Attention of each request's last tokens over its pages: single tokens of a
+// decode step, or a tree of drafted tokens, over a 16-bit or a quantised cache.
+//
+//   request b: kv_len tokens in pages kv_indices[kv_indptr[b] .. kv_indptr[b+1]),
+//   its last q_len are the queries; base = kv_len - q_len.
+//   query i sees position t < base, and t = base + j where bit j of its mask row
+//   is set (no mask: j <= i).
+//   s = scale * q . k, or cap * tanh(scale * q . k / cap);  o = softmax(s) v
+//
+// One pass over the keys and values with a running maximum m, sum l and
+// unnormalised output per query row (float32).  The queries of one KV head,
+// q_len * group rows, share every key and value that a workgroup loads.
+// Scores are computed transposed, S^T = K Q^T (v_mfma_f32_16x16x32: lane holds
+// four tokens of one query), so that a lane's exponentials are already the
+// operand of O^T = V^T P^T: its four tokens of two 16-token tiles are eight
+// consecutive entries of the product's k, for which V's rows are read in the
+// same order through the transposing LDS read.  P is rounded to the values'
+// type for the product (within 2^-8 of each weight in bfloat16, 2^-11 in float16,
+// errors that average out over the row); l sums the unrounded weights.
+//
+// Work split: a request's pages in chunks of C; chunk k of request b is work
+// item floor(kv_indptr[b] / C) + b + k, which a workgroup inverts by counting
+// the requests that start at or before its item, so a launch needs no plan and
+// a captured one follows the tables.  A request of one chunk is written
+// directly; the others leave (o, m, l) in a workspace for combine_kernel.
+#pragma once
+
+#include "mx.h"
+
+namespace pace_kv {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kXcds = 8;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+struct AttnParams {
+  const char* q;
+  int64_t q_stride;            // bytes between tokens
+  const int32_t* qo_indptr;    // batch + 1 entries, or nullptr: one token per request
+  const char* cache;
+  const int32_t* kv_indices;
+  const int32_t* kv_indptr;
+  const int32_t* kv_last_page_len;
+  const uint64_t* mask;        // [nnz, mask_words], or nullptr
+  char* out;
+  int64_t out_stride;
+  float* lse;                  // [nnz, heads * group], or nullptr
+  float* part_o;               // [items, heads, row_tiles, rows of a tile, D]
+  float* part_ml;              // [items, heads, row_tiles, rows of a tile, 2]
+  int32_t* err;
+  uint32_t num_indices, batch, nnz, heads, group, num_pages, page_size, max_q, mask_words;
+  uint32_t chunk_pages, items, row_tiles, tile_rows;
+  uint32_t page16, half16, row16;  // page, half page and token row, in 16-byte units
+  uint32_t scale_at, scale_row;    // scales within a half page, scale bytes of a token
+  FastDiv by_page, by_chunk, by_group, by_unit, by_tiles;
+  float scale_log2;            // scale * log2(e); with a cap: scale / cap * 2 * log2(e)
+  float cap_log2;              // cap * log2(e), or 0
+};
+
+// Swaps of half a wave and of neighbouring rows of 16 lanes bring the four
+// lanes of one query together.
+template <class F>
+__device__ __forceinline__ float across_groups(float x, F f) {
+  const uint32_t b = __float_as_uint(x);
+  auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  const uint32_t y = __float_as_uint(f(__uint_as_float(r[0]), __uint_as_float(r[1])));
+  r = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A request and the part of it that a work item covers.
+struct Request {
+  uint32_t b, chunk, chunks;
+  int32_t first_page;          // in kv_indices
+  uint32_t pages;
+  uint32_t kv_len;
+  uint32_t q0, q_len;
+};
+
+__device__ __forceinline__ uint32_t item_of(const AttnParams& p, uint32_t b, int32_t first) {
+  return over(p.by_chunk, static_cast<uint32_t>(max(first, 0))) + b;
+}
+
+// The sizes of request b; false where its queries are not nnz's or exceed max_q.
+__device__ __forceinline__ bool request_of(const AttnParams& p, uint32_t b, Request* r) {
+  const int32_t k0 = max(p.kv_indptr[b], 0), k1 = p.kv_indptr[b + 1];
+  r->b = b;
+  r->first_page = k0;
+  r->pages = k1 > k0 ? static_cast<uint32_t>(k1 - k0) : 0u;
+  r->pages = min(r->pages, p.num_indices - min(static_cast<uint32_t>(k0), p.num_indices));
+  const int64_t most = static_cast<int64_t>(r->pages) * p.page_size;
+  const int64_t len = (most > p.page_size ? most - p.page_size : 0) + p.kv_last_page_len[b];
+  r->kv_len = static_cast<uint32_t>(min(max(len, int64_t(0)), most));
+  const uint32_t n = over(p.by_chunk, r->pages);
+  r->chunks = max(n * p.chunk_pages < r->pages ? n + 1 : n, 1u);
+  if (p.qo_indptr == nullptr) {
+    r->q0 = b;
+    r->q_len = 1;
+    return b < p.nnz;
+  }
+  const int32_t a0 = p.qo_indptr[b], a1 = p.qo_indptr[b + 1];
+  r->q0 = static_cast<uint32_t>(a0);
+  r->q_len = static_cast<uint32_t>(a1 - a0);
+  return a0 >= 0 && a1 >= a0 && static_cast<uint32_t>(a1) <= p.nnz && r->q_len <= p.max_q;
+}
+
+// Largest b with f(b) <= x where f does not decrease, plus one; the wave counts
+// together, 64 entries a round.
+template <class F>
+__device__ __forceinline__ uint32_t count_upto(uint32_t n, uint32_t x, F f) {
+  uint32_t count = 0;
+  for (uint32_t e0 = 0; e0 < n; e0 += 64) {
+    const uint32_t e = e0 + threadIdx.x % 64;
+    count += __popcll(__ballot(e < n && f(e) <= x));
+  }
+  return __builtin_amdgcn_readfirstlane(count);
+}
+
+// Rows in LDS are padded so that neighbouring rows start 16 bytes (keys) or 32
+// (values) further along the banks: 16 rows' 16 bytes of a key fragment, and 8
+// rows' 32 bytes of a transposing read, each cover the 256 bytes of all banks
+// once.  Unlike a xor of the columns, a pad leaves every address one register and
+// an immediate offset.
+template <int D>
+constexpr uint32_t kKeyStride = D * 2 + 16;
+template <int D>
+constexpr uint32_t kValueStride = D * 2 + 32;
+
+template <int TYPE>
+__device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if constexpr (TYPE == PACE_KV_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0,
+                                                   0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint32_t pair_of(float a, float b) {
+  if constexpr (TYPE == PACE_KV_BF16) {
+    const bf16x2 x = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+    return __builtin_bit_cast(uint32_t, x);
+  } else {
+    const f16x2 x = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+    return __builtin_bit_cast(uint32_t, x);
+  }
+}
+
+template <int TYPE>
+__device__ __forceinline__ float value_of(uint32_t word, int half) {
+  const unsigned short h = static_cast<unsigned short>(word >> (16 * half));
+  if constexpr (TYPE == PACE_KV_BF16) return __uint_as_float(static_cast<uint32_t>(h) << 16);
+  else return static_cast<float>(__builtin_bit_cast(_Float16, h));
+}
+
+// Whether either half of a word is an infinity or a NaN.
+template <int TYPE>
+__device__ __forceinline__ bool odd_word(uint32_t w) {
+  constexpr uint32_t kExp = TYPE == PACE_KV_BF16 ? 0x7f80u : 0x7c00u;
+  return (w & kExp) == kExp || ((w >> 16) & kExp) == kExp;
+}
+
+// TYPE: of queries and output, and what a quantised cache is expanded to.
+// R tiles of 16 query rows per wave.  WR = 1: the waves take 32 tokens each of
+// a step and join at the end.  WR = 4: each wave takes its own 16 * R rows, and
+// all share a tile of 64 tokens.
+template <int D, int TYPE, int FORMAT, int R, int WR>
+__global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attention_kernel(const AttnParams p) {
+  constexpr int kBits = FORMAT == PACE_KV_PLAIN ? 16 : mx_bits(FORMAT);
+  constexpr int kWT = kWaves / WR;
+  constexpr uint32_t kTileRows = 16 * R * WR;
+  constexpr uint32_t kIdTokens = WR == 1 ? 32 : 64;      // tokens whose pages a wave looks up
+  constexpr uint32_t kStep = kIdTokens * kWT;            // tokens of a workgroup's step
+  constexpr uint32_t kLoadRows = WR == 1 ? 32 : 16;      // rows that a wave loads
+  constexpr uint32_t kPieces = D * kBits / 8 / 16;       // 16-byte pieces of a row
+  constexpr uint32_t kLoads = (kLoadRows * kPieces + 63) / 64;
+  constexpr uint32_t kLdsRows = WR == 1 ? 128 : 64;
+  constexpr int kDT = D / 16, kKS = D / 32;
+
+  __shared__ __attribute__((aligned(16))) char lds[kLdsRows * (kKeyStride<D> + kValueStride<D>)];
+  __shared__ float lds_ml[kWaves][kTileRows][2];
+
+  const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
+  const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+
+  // The heads and row tiles of one item run on one XCD, whose L2 then holds
+  // what they share.
+  const uint32_t unit = p.heads * p.row_tiles;
+  const uint32_t at = blockIdx.x / kXcds, nth = over(p.by_unit, at);
+  const uint32_t item = nth * kXcds + blockIdx.x % kXcds;
+  if (item >= p.items) return;
+  const uint32_t in_unit = at - nth * unit, head = over(p.by_tiles, in_unit), tile = in_unit - head * p.row_tiles;
+  const uint32_t count = count_upto(p.batch, item, [&](uint32_t e) { return item_of(p, e, p.kv_indptr[e]); });
+  if (count == 0) return;
+  Request r;
+  const bool valid_request = request_of(p, count - 1, &r);
+  r.chunk = item - item_of(p, r.b, r.first_page);
+  if (r.chunk >= r.chunks) return;
+  if (!valid_request) {
+    if (r.chunk == 0 && in_unit == 0 && threadIdx.x == 0 && p.err != nullptr) atomicAdd(p.err, 1);
+    return;
+  }
+  const uint32_t rows = r.q_len * p.group, row0 = tile * kTileRows;
+  if (row0 >= rows) return;
+  const int32_t base = static_cast<int32_t>(r.kv_len) - static_cast<int32_t>(r.q_len);
+  // Without a mask no row of the tile sees past its last query.
+  const int32_t first_q = static_cast<int32_t>(over(p.by_group, row0));
+  const int32_t last_q = static_cast<int32_t>(over(p.by_group, min(row0 + kTileRows, rows) - 1));
+  const int32_t chunk_tokens = static_cast<int32_t>(p.chunk_pages * p.page_size);
+  const int32_t t_begin = static_cast<int32_t>(r.chunk) * chunk_tokens;
+  int32_t t_end = static_cast<int32_t>(min(static_cast<int64_t>(t_begin) + chunk_tokens, static_cast<int64_t>(r.kv_len)));
+  if (p.mask == nullptr) t_end = min(t_end, base + last_q + 1);
+
+  // Query fragments: row n of each tile, eight elements from 32 * ks + 8 * g.
+  const uint32_t wave_row0 = row0 + (WR == 1 ? 0 : w * 16 * R);
+  u32x4 qf[R][kKS];
+  int32_t qi[R];
+#pragma unroll
+  for (int a = 0; a < R; ++a) {
+    const uint32_t row = wave_row0 + a * 16 + n;
+    const uint32_t i = over(p.by_group, row);
+    qi[a] = static_cast<int32_t>(i);
+    const char* src = p.q + static_cast<int64_t>(r.q0 + i) * p.q_stride +
+                      (static_cast<int64_t>(head) * p.group + (row - i * p.group)) * (D * 2);
+#pragma unroll
+    for (int k = 0; k < kKS; ++k) {
+      qf[a][k] = u32x4{0, 0, 0, 0};
+      if (row < rows) qf[a][k] = *reinterpret_cast<const u32x4*>(src + k * 64 + g * 16);
+    }
+  }
+
+  f32x4 acc[R][kDT];
+  float m[R], l[R];
+#pragma unroll
+  for (int a = 0; a < R; ++a) {
+    m[a] = -INFINITY;
+    l[a] = 0.f;
+#pragma unroll
+    for (int d = 0; d < kDT; ++d) acc[a][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  char* const lds_k = lds;
+  char* const lds_v = lds + kLdsRows * kKeyStride<D>;
+  const uint32_t lds_row0 = w * kLoadRows;               // first row that this wave loads
+
+  // A step's loads: page ids (one token per lane), then rows.
+  const uint32_t id_lane = lane % kIdTokens;
+  int32_t id = 0;
+  const auto load_id = [&](int32_t t0) {
+    const int32_t t = t0 + static_cast<int32_t>(id_lane);
+    id = -1;
+    if (t < t_end) id = p.kv_indices[r.first_page + static_cast<int32_t>(over(p.by_page, static_cast<uint32_t>(t)))];
+  };
+  u32x4 kr[kLoads], vr[kLoads];
+  uint64_t ks_byte = 0, vs_byte = 0;                     // the scales of the lane's token
+  uint64_t valid = 0;
+  const auto load_rows = [&](int32_t t0) {
+    const uint32_t t = static_cast<uint32_t>(t0) + id_lane;
+    const bool ok = t0 + static_cast<int32_t>(id_lane) < t_end && static_cast<uint32_t>(id) < p.num_pages;
+    valid = __ballot(ok);
+    if (kIdTokens == 32) valid &= 0xffffffffull;
+    const uint32_t slot = t - over(p.by_page, t) * p.page_size;
+    const uint32_t off = ok ? static_cast<uint32_t>(id) * p.page16 + slot * p.row16 + head * (D * kBits / 128) : ~0u;
+    if constexpr (FORMAT != PACE_KV_PLAIN) {
+      ks_byte = vs_byte = 0;
+      if (ok && id_lane / kLoadRows == (WR == 1 ? 0 : w)) {
+        const char* s = p.cache + static_cast<int64_t>(id) * p.page16 * 16 + p.scale_at +
+                        static_cast<int64_t>(slot) * p.scale_row + head * (D / 32);
+        const char* sv = s + static_cast<int64_t>(p.half16) * 16;
+        if constexpr (D == 64) {
+          ks_byte = *reinterpret_cast<const uint16_t*>(s);
+          vs_byte = *reinterpret_cast<const uint16_t*>(sv);
+        } else if constexpr (D == 128) {
+          ks_byte = *reinterpret_cast<const uint32_t*>(s);
+          vs_byte = *reinterpret_cast<const uint32_t*>(sv);
+        } else {
+          ks_byte = *reinterpret_cast<const uint64_t*>(s);
+          vs_byte = *reinterpret_cast<const uint64_t*>(sv);
+        }
+      }
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kLoads; ++j) {
+      const uint32_t piece = j * 64 + lane, row = piece / kPieces, c = piece % kPieces;
+      const uint32_t o = __shfl(off, (WR == 1 ? 0 : w * kLoadRows) + row % kLoadRows);
+      kr[j] = vr[j] = u32x4{0, 0, 0, 0};
+      if (o != ~0u && row < kLoadRows) {
+        const char* s = p.cache + (static_cast<int64_t>(o) + c) * 16;
+        kr[j] = *reinterpret_cast<const u32x4*>(s);
+        vr[j] = *reinterpret_cast<const u32x4*>(s + static_cast<int64_t>(p.half16) * 16);
+      }
+    }
+  };
+  const auto store_piece = [&](char* row, uint32_t c, const u32x4& x, uint64_t bytes) {
+    u32x4* to = reinterpret_cast<u32x4*>(row);
+    if constexpr (FORMAT == PACE_KV_PLAIN) {
+      to[c] = x;
+    } else if constexpr (FORMAT == PACE_KV_MXFP8) {      // 16 elements: half a block
+      const float s = scale_of(static_cast<uint32_t>(bytes >> (c / 2 * 8)) & 255u);
+      to[2 * c] = run_up<TYPE, FORMAT>(u32x2{x[0], x[1]}, s);
+      to[2 * c + 1] = run_up<TYPE, FORMAT>(u32x2{x[2], x[3]}, s);
+    } else {                                             // 32 elements: a block
+      const float s = scale_of(static_cast<uint32_t>(bytes >> (c * 8)) & 255u);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) to[4 * c + k] = run_up<TYPE, FORMAT>(u32x2{x[k], 0}, s);
+    }
+  };
+  const auto store_rows = [&]() {
+#pragma unroll
+    for (uint32_t j = 0; j < kLoads; ++j) {
+      const uint32_t piece = j * 64 + lane, row = piece / kPieces, c = piece % kPieces;
+      uint64_t kb = 0, vb = 0;
+      if constexpr (FORMAT != PACE_KV_PLAIN) {
+        const uint32_t from = (WR == 1 ? 0 : w * kLoadRows) + row % kLoadRows;
+        kb = static_cast<uint32_t>(__shfl(static_cast<uint32_t>(ks_byte), from));
+        vb = static_cast<uint32_t>(__shfl(static_cast<uint32_t>(vs_byte), from));
+        if constexpr (D == 256) {
+          kb |= static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ks_byte >> 32), from)) << 32;
+          vb |= static_cast<uint64_t>(__shfl(static_cast<uint32_t>(vs_byte >> 32), from)) << 32;
+        }
+      }
+      if (row < kLoadRows) {
+        store_piece(lds_k + (lds_row0 + row) * kKeyStride<D>, c, kr[j], kb);
+        store_piece(lds_v + (lds_row0 + row) * kValueStride<D>, c, vr[j], vb);
+      }
+    }
+  };
+
+  // Which of the 32 tokens from t0 query row a sees (bit i: token t0 + i).
+  const auto seen = [&](int32_t t0, int32_t query) -> uint32_t {
+    const int32_t d0 = t0 - base;                        // drafted token of bit 0, negative: before them
+    if (p.mask == nullptr) {
+      const int32_t upto = query - d0 + 1;
+      return upto >= 32 ? ~0u : upto <= 0 ? 0u : (1u << upto) - 1u;
+    }
+    if (d0 <= -32) return ~0u;
+    if (query >= static_cast<int32_t>(r.q_len)) return 0u;   // a row of padding
+    const uint64_t* bits = p.mask + static_cast<int64_t>(r.q0 + static_cast<uint32_t>(query)) * p.mask_words;
+    if (d0 < 0) return static_cast<uint32_t>(bits[0] << -d0) | ((1u << -d0) - 1u);
+    const uint32_t word = static_cast<uint32_t>(d0) / 64, sh = static_cast<uint32_t>(d0) % 64;
+    uint64_t x = word < p.mask_words ? bits[word] >> sh : 0ull;
+    if (sh > 32 && word + 1 < p.mask_words) x |= bits[word + 1] << (64 - sh);
+    return static_cast<uint32_t>(x);
+  };
+
+  // 32 tokens from t0 whose rows lie at lds_row; `ok`: the tokens that exist.
+  const auto attend = [&](int32_t t0, uint32_t lds_row, uint32_t ok) {
+    const char* key_at = lds_k + (lds_row + n) * kKeyStride<D> + g * 16;
+    const char* value_at = lds_v + lds_row * kValueStride<D>;
+    f32x4 s[R][2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int a = 0; a < R; ++a) s[a][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < kKS; ++k) {
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(key_at + t * 16 * kKeyStride<D> + k * 64);
+#pragma unroll
+        for (int a = 0; a < R; ++a) s[a][t] = mfma<TYPE>(kf, qf[a][k], s[a][t]);
+      }
+    }
+    const bool full = ok == ~0u && (t0 + 32 <= base || (p.mask == nullptr && t0 + 31 <= base + first_q));
+    bool odd = false;                                    // an infinite or NaN value that some row must not see
+    uint32_t sees[R];
+    if (!full) {
+#pragma unroll
+      for (int a = 0; a < R; ++a) sees[a] = seen(t0, qi[a]) & ok;
+      bool found = false;
+#pragma unroll
+      for (uint32_t k = 0; k < 32 * D / 8 / 64; ++k) {
+        const uint32_t c = k * 64 + lane;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(value_at + c / (D / 8) * kValueStride<D> + c % (D / 8) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) found |= odd_word<TYPE>(x[e]);
+      }
+      odd = __ballot(found) != 0;
+    }
+    u32x4 pf[R];
+#pragma unroll
+    for (int a = 0; a < R; ++a) {
+      float x[8];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float y = s[a][t][e] * p.scale_log2;
+          // tanh(z) = 1 - 2 / (1 + 2^(2 log2(e) z))
+          if (p.cap_log2 > 0.f) y = p.cap_log2 * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + exp2_of(y)));
+          if (!full && !((sees[a] >> (t * 16 + 4 * g + e)) & 1u)) y = -INFINITY;
+          x[t * 4 + e] = y;
+        }
+      float top = x[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, x[e]);
+      top = fmaxf(m[a], across_groups(top, max_of));
+      const float from = top == -INFINITY ? 0.f : top;   // nothing seen yet: weights of 2^-inf = 0
+      const float shrink = exp2_of(m[a] - from);
+      m[a] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = exp2_of(x[e] - from);
+        sum += x[e];
+      }
+      l[a] = l[a] * shrink + sum;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pf[a][e] = pair_of<TYPE>(x[2 * e], x[2 * e + 1]);
+      if (__ballot(shrink != 1.f) != 0) {
+#pragma unroll
+        for (int d = 0; d < kDT; ++d) acc[a][d] *= shrink;
+      }
+    }
+    if (!odd) {
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) {
+        // Lane: row 4 g + n / 4 of each 16 tokens, four columns; transposed over
+        // 16 lanes: four tokens of column n.
+        const char* from = value_at + (4 * g + n / 4) * kValueStride<D> + n % 4 * 8 + d * 32;
+        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)from);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(from + 16 * kValueStride<D>));
+        const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
+        const u32x4 vf = {lo2[0], lo2[1], hi2[0], hi2[1]};
+#pragma unroll
+        for (int a = 0; a < R; ++a) acc[a][d] = mfma<TYPE>(vf, pf[a], acc[a][d]);
+      }
+    } else {
+      // A product with weight zero would spread an infinity or a NaN to rows
+      // that do not see its token: the same sum, token by token, over those seen.
+#pragma unroll
+      for (int a = 0; a < R; ++a)
+#pragma unroll 1
+        for (uint32_t token = 0; token < 32; ++token) {
+          const uint32_t word = token / 16 * 2 + token % 4 / 2;
+          const uint32_t mine = word == 0 ? pf[a][0] : word == 1 ? pf[a][1] : word == 2 ? pf[a][2] : pf[a][3];
+          const float weight = value_of<TYPE>(__shfl(mine, token % 16 / 4 * 16 + n), token % 2);
+          if (!((sees[a] >> token) & 1u)) continue;
+#pragma unroll
+          for (int d = 0; d < kDT; ++d) {
+            const u32x2 v = *reinterpret_cast<const u32x2*>(value_at + token * kValueStride<D> + d * 32 + g * 8);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) acc[a][d][c] += weight * value_of<TYPE>(v[c / 2], c % 2);
+          }
+        }
+    }
+  };
+
+  const int32_t wave_t0 = t_begin + (WR == 1 ? static_cast<int32_t>(w * kIdTokens) : 0);
+  load_id(wave_t0);
+  load_rows(wave_t0);
+  load_id(wave_t0 + static_cast<int32_t>(kStep));
+  for (int32_t t0 = t_begin; t0 < t_end; t0 += static_cast<int32_t>(kStep)) {
+    const int32_t tw = t0 + (wave_t0 - t_begin);
+    if (WR != 1) __syncthreads();                        // the last step's reads are done
+    store_rows();
+    const uint64_t ok = valid;
+    if (WR != 1) __syncthreads();
+    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    load_rows(tw + static_cast<int32_t>(kStep));
+    load_id(tw + 2 * static_cast<int32_t>(kStep));
+    __builtin_amdgcn_sched_barrier(0);
+    if (WR == 1) {
+      if (ok != 0) attend(tw, lds_row0, static_cast<uint32_t>(ok));
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    } else {
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t part = static_cast<uint32_t>(ok >> (32 * h));
+        if (part != 0) attend(t0 + 32 * h, 32 * h, part);
+      }
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < R; ++a) l[a] = across_groups(l[a], sum_of);
+
+  const bool direct = r.chunks == 1;
+  const int64_t part_row0 = (static_cast<int64_t>(item) * unit + in_unit) * kTileRows;
+  // Row `in_tile` of the tile: four output columns from d, and its m and l.
+  const auto write = [&](uint32_t in_tile, uint32_t d, f32x4 o, float top, float sum, bool first) {
+    const uint32_t row = row0 + in_tile;
+    if (row >= rows) return;
+    if (!direct) {
+      *reinterpret_cast<f32x4*>(p.part_o + (part_row0 + in_tile) * D + d) = o;
+      if (first) {
+        p.part_ml[(part_row0 + in_tile) * 2] = top;
+        p.part_ml[(part_row0 + in_tile) * 2 + 1] = sum;
+      }
+      return;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const uint32_t i = over(p.by_group, row);
+    const uint32_t qh = head * p.group + (row - i * p.group);
+    const u32x2 x = {pair_of<TYPE>(o[0] * inv, o[1] * inv), pair_of<TYPE>(o[2] * inv, o[3] * inv)};
+    *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(r.q0 + i) * p.out_stride +
+                              (static_cast<int64_t>(qh) * D + d) * 2) = x;
+    if (first && p.lse != nullptr)
+      p.lse[static_cast<int64_t>(r.q0 + i) * p.heads * p.group + qh] =
+          sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.69314718055994531f;
+  };
+  if (WR != 1) {
+#pragma unroll
+    for (int a = 0; a < R; ++a)
+#pragma unroll
+      for (int d = 0; d < kDT; ++d) write(w * 16 * R + a * 16 + n, d * 16 + g * 4, acc[a][d], m[a], l[a], d == 0 && g == 0);
+    return;
+  }
+  // The waves' parts of a row join over their common maximum.
+  __syncthreads();
+  float* part = reinterpret_cast<float*>(lds);           // [wave][row][D], chunks of 4 xored with the row
+#pragma unroll
+  for (int a = 0; a < R; ++a) {
+    const uint32_t row = a * 16 + n;
+    if (g == 0) {
+      lds_ml[w][row][0] = m[a];
+      lds_ml[w][row][1] = l[a];
+    }
+#pragma unroll
+    for (int d = 0; d < kDT; ++d)
+      *reinterpret_cast<f32x4*>(part + (w * kTileRows + row) * D + ((d * 4 + g) ^ n) * 4) = acc[a][d];
+  }
+  __syncthreads();
+  for (uint32_t e = threadIdx.x; e < kTileRows * (D / 4); e += kThreads) {
+    const uint32_t row = e / (D / 4), c = e % (D / 4);
+    float top = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) top = fmaxf(top, lds_ml[v][row][0]);
+    const float from = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) {
+      const float weight = exp2_of(lds_ml[v][row][0] - from);
+      sum += weight * lds_ml[v][row][1];
+      o += weight * *reinterpret_cast<const f32x4*>(part + (v * kTileRows + row) * D + (c ^ (row & 15u)) * 4);
+    }
+    write(row, c * 4, o, top, sum, c == 0);
+  }
+}
+
+// The kernel for a head_dim; tile_rows 16 or 32 (the waves split the tokens), 64
+// or 128 (the waves split the rows).  One translation unit each.
+const void* attention_kernel_d64(int type, int format, uint32_t tile_rows);
+const void* attention_kernel_d128(int type, int format, uint32_t tile_rows);
+const void* attention_kernel_d256(int type, int format, uint32_t tile_rows);
+
+template <int D, int TYPE, int FORMAT>
+const void* pick_rows(uint32_t tile_rows) {
+  switch (tile_rows) {
+    case 16: return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 1, 1>);
+    case 32: return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 2, 1>);
+    case 64: return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 1, 4>);
+    default: return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 2, 4>);
+  }
+}
+
+template <int D, int TYPE>
+const void* pick_format(int format, uint32_t tile_rows) {
+  switch (format) {
+    case PACE_KV_PLAIN: return pick_rows<D, TYPE, PACE_KV_PLAIN>(tile_rows);
+    case PACE_KV_MXFP8: return pick_rows<D, TYPE, PACE_KV_MXFP8>(tile_rows);
+    default: return pick_rows<D, TYPE, PACE_KV_MXFP4>(tile_rows);
+  }
+}
+
+template <int D>
+const void* pick_attention(int type, int format, uint32_t tile_rows) {
+  return type == PACE_KV_BF16 ? pick_format<D, PACE_KV_BF16>(format, tile_rows)
+                              : pick_format<D, PACE_KV_FP16>(format, tile_rows);
+}
+
+}  // namespace pace_kv
