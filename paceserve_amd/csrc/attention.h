@@ -240,10 +240,11 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
   }
 
   f32x4 acc[R][kDT];
-  float m[R], l[R];
+  float m[R], from[R], l[R];
 #pragma unroll
   for (int a = 0; a < R; ++a) {
     m[a] = -INFINITY;
+    from[a] = 0.f;
     l[a] = 0.f;
 #pragma unroll
     for (int d = 0; d < kDT; ++d) acc[a][d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
     id = -1;
     if (t < t_end) id = p.kv_indices[r.first_page + static_cast<int32_t>(over(p.by_page, static_cast<uint32_t>(t)))];
   };
-  u32x4 kr[kLoads], vr[kLoads];
+  u32x4 kr[kLoads] = {}, vr[kLoads] = {};
   uint64_t ks_byte = 0, vs_byte = 0;                     // the scales of the lane's token
   uint64_t valid = 0;
   const auto load_rows = [&](int32_t t0) {
@@ -270,7 +271,10 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
     valid = __ballot(ok);
     if (kIdTokens == 32) valid &= 0xffffffffull;
     const uint32_t slot = t - over(p.by_page, t) * p.page_size;
-    const uint32_t off = ok ? static_cast<uint32_t>(id) * p.page16 + slot * p.row16 + head * (D * kBits / 128) : ~0u;
+    // A token that does not exist reads the pool's first row, which store_rows
+    // makes zeros: loads without a condition.
+    const uint32_t off = ok ? static_cast<uint32_t>(id) * p.page16 + slot * p.row16 + head * (D * kBits / 128) : 0u;
+    if (valid == 0) return;
     if constexpr (FORMAT != PACE_KV_PLAIN) {
       ks_byte = vs_byte = 0;
       if (ok && id_lane / kLoadRows == (WR == 1 ? 0 : w)) {
@@ -293,12 +297,9 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
     for (uint32_t j = 0; j < kLoads; ++j) {
       const uint32_t piece = j * 64 + lane, row = piece / kPieces, c = piece % kPieces;
       const uint32_t o = __shfl(off, (WR == 1 ? 0 : w * kLoadRows) + row % kLoadRows);
-      kr[j] = vr[j] = u32x4{0, 0, 0, 0};
-      if (o != ~0u && row < kLoadRows) {
-        const char* s = p.cache + (static_cast<int64_t>(o) + c) * 16;
-        kr[j] = *reinterpret_cast<const u32x4*>(s);
-        vr[j] = *reinterpret_cast<const u32x4*>(s + static_cast<int64_t>(p.half16) * 16);
-      }
+      const char* s = p.cache + (static_cast<int64_t>(o) + c) * 16;
+      kr[j] = *reinterpret_cast<const u32x4*>(s);
+      vr[j] = *reinterpret_cast<const u32x4*>(s + static_cast<int64_t>(p.half16) * 16);
     }
   };
   const auto store_piece = [&](char* row, uint32_t c, const u32x4& x, uint64_t bytes) {
@@ -316,6 +317,13 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
     }
   };
   const auto store_rows = [&]() {
+    if (valid != (kIdTokens == 32 ? 0xffffffffull : ~0ull)) {
+#pragma unroll
+      for (uint32_t j = 0; j < kLoads; ++j) {
+        const uint32_t token = (WR == 1 ? 0 : w * kLoadRows) + (j * 64 + lane) / kPieces % kLoadRows;
+        if (!((valid >> token) & 1)) kr[j] = vr[j] = u32x4{0, 0, 0, 0};
+      }
+    }
 #pragma unroll
     for (uint32_t j = 0; j < kLoads; ++j) {
       const uint32_t piece = j * 64 + lane, row = piece / kPieces, c = piece % kPieces;
@@ -359,16 +367,17 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
     const char* value_at = lds_v + lds_row * kValueStride<D>;
     f32x4 s[R][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int a = 0; a < R; ++a) s[a][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < kKS; ++k) {
+    for (int k = 0; k < kKS; ++k)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
         const u32x4 kf = *reinterpret_cast<const u32x4*>(key_at + t * 16 * kKeyStride<D> + k * 64);
 #pragma unroll
         for (int a = 0; a < R; ++a) s[a][t] = mfma<TYPE>(kf, qf[a][k], s[a][t]);
       }
-    }
     const bool full = ok == ~0u && (t0 + 32 <= base || (p.mask == nullptr && t0 + 31 <= base + first_q));
     bool odd = false;                                    // an infinite or NaN value that some row must not see
     uint32_t sees[R];
@@ -402,23 +411,24 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
       float top = x[0];
 #pragma unroll
       for (int e = 1; e < 8; ++e) top = fmaxf(top, x[e]);
-      top = fmaxf(m[a], across_groups(top, max_of));
-      const float from = top == -INFINITY ? 0.f : top;   // nothing seen yet: weights of 2^-inf = 0
-      const float shrink = exp2_of(m[a] - from);
-      m[a] = top;
-      float sum = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = exp2_of(x[e] - from);
-        sum += x[e];
-      }
-      l[a] = l[a] * shrink + sum;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pf[a][e] = pair_of<TYPE>(x[2 * e], x[2 * e + 1]);
-      if (__ballot(shrink != 1.f) != 0) {
+      // The maximum is raised only past 2^8 of it: weights stay below 2^8 (and
+      // their sums within float32), and most steps need no joint maximum.
+      if (__ballot(top > m[a] + 8.f) != 0) {
+        top = fmaxf(m[a], across_groups(top, max_of));
+        from[a] = top == -INFINITY ? 0.f : top;          // nothing seen yet: weights of 2^-inf = 0
+        const float shrink = exp2_of(m[a] - from[a]);
+        m[a] = top;
+        l[a] *= shrink;
 #pragma unroll
         for (int d = 0; d < kDT; ++d) acc[a][d] *= shrink;
       }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = exp2_of(x[e] - from[a]);
+        l[a] += x[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pf[a][e] = pair_of<TYPE>(x[2 * e], x[2 * e + 1]);
     }
     if (!odd) {
 #pragma unroll

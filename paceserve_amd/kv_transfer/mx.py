@@ -53,9 +53,12 @@ def empty_cache(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int
 
 def _format_of(row: int, head_dim: int) -> int:
     """The format whose rows of head_dim elements take `row` bytes."""
-    for name, value in FORMATS.items():
-        if head_dim > 0 and head_dim % BLOCK == 0 and row == row_width(head_dim, name):
-            return value
+    if head_dim > 0 and head_dim % BLOCK == 0:
+        blocks = head_dim // BLOCK
+        if row == 33 * blocks:
+            return _native.MXFP8
+        if row == 17 * blocks:
+            return _native.MXFP4
     raise ValueError(f"rows of {row} bytes hold {head_dim} elements in no format: mxfp8 takes head_dim * 33 / 32 "
                      "bytes, mxfp4 head_dim * 17 / 32")
 
@@ -81,8 +84,22 @@ def _call(device: torch.device, name: str, *args) -> None:
             _native.check(fn(*args, _stream_handle(device)))
 
 
-def _check_append(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor) -> int:
-    """Validates the rows and the quantised cache; returns the format."""
+def _append_format(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor) -> int:
+    """The format of an append's cache.  One look at each property settles an
+    append that is in order; any other gets _check_append's checks and message."""
+    if type(cache) is type(key) is type(value) is torch.Tensor and cache.dtype is torch.uint8:
+        index, shape, rows, stride, dtype = cache.get_device(), cache.shape, key.shape, key.stride(), key.dtype
+        if (index >= 0 and len(shape) == 5 and len(rows) == 3 and shape[1] == 2 and rows[1] == shape[3]
+                and stride[2] == 1 and stride[1] == rows[2] and value.shape == rows and value.stride() == stride
+                and value.dtype is dtype and dtype in _native.ELEM_TYPES and cache.is_cuda
+                and key.get_device() == value.get_device() == index and cache.is_contiguous()):
+            return _format_of(shape[4], rows[2])
+    _check_append(key, value, cache)
+    return _format_of(cache.shape[4], key.shape[2])
+
+
+def _check_append(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor) -> None:
+    """Validates the rows and the quantised cache."""
     if cache.dtype is not torch.uint8 or cache.dim() != 5 or cache.shape[1] != 2 or not cache.is_contiguous() \
             or not cache.is_cuda:
         raise ValueError("mx_cache must be a contiguous uint8 device tensor [num_pages, 2, page_size, H, row_width]")
@@ -94,7 +111,6 @@ def _check_append(key: torch.Tensor, value: torch.Tensor, cache: torch.Tensor) -
             raise ValueError(f"{name} rows must be contiguous [H, D] blocks")
     if key.shape != value.shape or key.dtype != value.dtype or key.stride(0) != value.stride(0):
         raise ValueError("append_key and append_value differ in shape, dtype or token stride")
-    return _format_of(cache.shape[4], key.shape[2])
 
 
 def append_paged_kv_cache_mx(append_key: torch.Tensor, append_value: torch.Tensor, batch_indices: torch.Tensor,
@@ -104,7 +120,7 @@ def append_paged_kv_cache_mx(append_key: torch.Tensor, append_value: torch.Tenso
     """append.append_paged_kv_cache into a quantised cache: the rows
     ([nnz, H, D] bfloat16, float16 or float32) are quantised as they are
     written.  Tokens of one call take distinct slots."""
-    fmt = _check_append(append_key, append_value, mx_cache)
+    fmt = _append_format(append_key, append_value, mx_cache)
     dev, at, nnz = mx_cache.device, mx_cache.get_device(), append_key.shape[0]
     bi = _i32(batch_indices, "batch_indices", dev, at)
     pos = _i32(positions, "positions", dev, at)
@@ -128,7 +144,7 @@ def append_paged_kv_cache_mx_indptr(append_key: torch.Tensor, append_value: torc
                                     err: Optional[torch.Tensor] = None) -> None:
     """append.append_paged_kv_cache_indptr into a quantised cache: one launch
     that also derives each token's request and position."""
-    fmt = _check_append(append_key, append_value, mx_cache)
+    fmt = _append_format(append_key, append_value, mx_cache)
     dev, at, nnz = mx_cache.device, mx_cache.get_device(), append_key.shape[0]
     ai = _i32(append_indptr, "append_indptr", dev, at)
     idx = _i32(kv_indices, "kv_indices", dev, at)
