@@ -25,6 +25,8 @@
 // directly; the others leave (o, m, l) in a workspace for combine_kernel.
 #pragma once
 
+#include <type_traits>
+
 #include "mx.h"
 
 namespace pace_kv {
@@ -57,7 +59,7 @@ struct AttnParams {
   uint32_t chunk_pages, items, row_tiles, tile_rows;
   uint32_t page16, half16, row16;  // page, half page and token row, in 16-byte units
   uint32_t scale_at, scale_row;    // scales within a half page, scale bytes of a token
-  FastDiv by_page, by_chunk, by_group, by_unit, by_tiles;
+  FastDiv by_page, by_chunk, by_group, by_unit, by_tiles, by_heads;
   float scale_log2;            // scale * log2(e); with a cap: scale / cap * 2 * log2(e)
   float cap_log2;              // cap * log2(e), or 0
 };
@@ -90,39 +92,77 @@ __device__ __forceinline__ uint32_t item_of(const AttnParams& p, uint32_t b, int
   return over(p.by_chunk, static_cast<uint32_t>(max(first, 0))) + b;
 }
 
-// The sizes of request b; false where its queries are not nnz's or exceed max_q.
-__device__ __forceinline__ bool request_of(const AttnParams& p, uint32_t b, Request* r) {
-  const int32_t k0 = max(p.kv_indptr[b], 0), k1 = p.kv_indptr[b + 1];
+// What the tables say of a request.
+struct Tables {
+  int32_t k0, k1, last, a0, a1;
+};
+
+__device__ __forceinline__ Tables tables_of(const AttnParams& p, uint32_t b) {
+  Tables t;
+  t.k0 = p.kv_indptr[b];
+  t.k1 = p.kv_indptr[b + 1];
+  t.last = p.kv_last_page_len[b];
+  t.a0 = static_cast<int32_t>(b);
+  t.a1 = t.a0 + 1;
+  if (p.qo_indptr != nullptr) {
+    t.a0 = p.qo_indptr[b];
+    t.a1 = p.qo_indptr[b + 1];
+  }
+  return t;
+}
+
+// The sizes of request b; false where its queries are not among nnz or exceed
+// max_q.
+__device__ __forceinline__ bool request_of(const AttnParams& p, uint32_t b, const Tables& t, Request* r) {
+  const int32_t k0 = max(t.k0, 0);
   r->b = b;
   r->first_page = k0;
-  r->pages = k1 > k0 ? static_cast<uint32_t>(k1 - k0) : 0u;
+  r->pages = t.k1 > k0 ? static_cast<uint32_t>(t.k1 - k0) : 0u;
   r->pages = min(r->pages, p.num_indices - min(static_cast<uint32_t>(k0), p.num_indices));
   const int64_t most = static_cast<int64_t>(r->pages) * p.page_size;
-  const int64_t len = (most > p.page_size ? most - p.page_size : 0) + p.kv_last_page_len[b];
+  const int64_t len = (most > p.page_size ? most - p.page_size : 0) + t.last;
   r->kv_len = static_cast<uint32_t>(min(max(len, int64_t(0)), most));
   const uint32_t n = over(p.by_chunk, r->pages);
   r->chunks = max(n * p.chunk_pages < r->pages ? n + 1 : n, 1u);
-  if (p.qo_indptr == nullptr) {
-    r->q0 = b;
-    r->q_len = 1;
-    return b < p.nnz;
-  }
-  const int32_t a0 = p.qo_indptr[b], a1 = p.qo_indptr[b + 1];
-  r->q0 = static_cast<uint32_t>(a0);
-  r->q_len = static_cast<uint32_t>(a1 - a0);
-  return a0 >= 0 && a1 >= a0 && static_cast<uint32_t>(a1) <= p.nnz && r->q_len <= p.max_q;
+  r->q0 = static_cast<uint32_t>(t.a0);
+  r->q_len = static_cast<uint32_t>(t.a1 - t.a0);
+  return t.a0 >= 0 && t.a1 >= t.a0 && static_cast<uint32_t>(t.a1) <= p.nnz && r->q_len <= p.max_q;
 }
 
-// Largest b with f(b) <= x where f does not decrease, plus one; the wave counts
-// together, 64 entries a round.
-template <class F>
-__device__ __forceinline__ uint32_t count_upto(uint32_t n, uint32_t x, F f) {
-  uint32_t count = 0;
-  for (uint32_t e0 = 0; e0 < n; e0 += 64) {
-    const uint32_t e = e0 + threadIdx.x % 64;
-    count += __popcll(__ballot(e < n && f(e) <= x));
+// The last request whose key is at most x, keys not decreasing, and what the
+// tables say of it; false if there is none.  The wave looks at 256 requests a
+// round, and holds what it loads of each, so up to 256 cost one load latency.
+template <class Key>
+__device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Key key, uint32_t* b, Tables* t) {
+  bool found = false;
+  for (uint32_t e0 = 0; e0 < p.batch; e0 += 256) {
+    Tables mine[4] = {};
+    uint64_t pass[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t e = e0 + k * 64 + threadIdx.x % 64;
+      if (e < p.batch) mine[k] = tables_of(p, e);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t e = e0 + k * 64 + threadIdx.x % 64;
+      pass[k] = __ballot(e < p.batch && key(e, mine[k]) <= x);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (pass[k] == 0) continue;
+      const int at = 63 - __builtin_clzll(pass[k]);
+      found = true;
+      *b = e0 + k * 64 + at;
+      t->k0 = __builtin_amdgcn_readlane(mine[k].k0, at);
+      t->k1 = __builtin_amdgcn_readlane(mine[k].k1, at);
+      t->last = __builtin_amdgcn_readlane(mine[k].last, at);
+      t->a0 = __builtin_amdgcn_readlane(mine[k].a0, at);
+      t->a1 = __builtin_amdgcn_readlane(mine[k].a1, at);
+    }
+    if (pass[3] != ~0ull) break;
   }
-  return __builtin_amdgcn_readfirstlane(count);
+  return found;
 }
 
 // Rows in LDS are padded so that neighbouring rows start 16 bytes (keys) or 32
@@ -156,6 +196,13 @@ __device__ __forceinline__ uint32_t pair_of(float a, float b) {
   }
 }
 
+// Hides where x comes from, so that what a loop derives from it is derived anew
+// each time (an add) instead of being held in a register throughout.
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 template <int TYPE>
 __device__ __forceinline__ float value_of(uint32_t word, int half) {
   const unsigned short h = static_cast<unsigned short>(word >> (16 * half));
@@ -170,12 +217,20 @@ __device__ __forceinline__ bool odd_word(uint32_t w) {
   return (w & kExp) == kExp || ((w >> 16) & kExp) == kExp;
 }
 
+// Waves per SIMD that the registers are held to.  Two workgroups a CU fit the
+// accumulators and loads of 32 rows of 128; a decode step over a quantised cache
+// leaves room for a third, whose loads in flight count.
+constexpr int min_waves(int D, int format, int R, int WR) {
+  if (D == 256) return R == 2 || format == PACE_KV_PLAIN ? 1 : 2;
+  return R == 1 && WR == 1 && format != PACE_KV_PLAIN ? 3 : 2;
+}
+
 // TYPE: of queries and output, and what a quantised cache is expanded to.
 // R tiles of 16 query rows per wave.  WR = 1: the waves take 32 tokens each of
 // a step and join at the end.  WR = 4: each wave takes its own 16 * R rows, and
 // all share a tile of 64 tokens.
 template <int D, int TYPE, int FORMAT, int R, int WR>
-__global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attention_kernel(const AttnParams p) {
+__global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attention_kernel(const AttnParams p) {
   constexpr int kBits = FORMAT == PACE_KV_PLAIN ? 16 : mx_bits(FORMAT);
   constexpr int kWT = kWaves / WR;
   constexpr uint32_t kTileRows = 16 * R * WR;
@@ -186,9 +241,16 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
   constexpr uint32_t kLoads = (kLoadRows * kPieces + 63) / 64;
   constexpr uint32_t kLdsRows = WR == 1 ? 128 : 64;
   constexpr int kDT = D / 16, kKS = D / 32;
+  // Rows that no other workgroup reads are loaded nontemporally.  MI355X, reading
+  // 2 GiB of pages in this pattern: 6.3 to 6.8 TB/s against 5.7 to 6.1.
+  constexpr bool kReadOnce = WR == 1 || R == 1;
 
-  __shared__ __attribute__((aligned(16))) char lds[kLdsRows * (kKeyStride<D> + kValueStride<D>)];
-  __shared__ float lds_ml[kWaves][kTileRows][2];
+  constexpr uint32_t kRowBytes = WR == 1 ? kValueStride<D> : kKeyStride<D> + kValueStride<D>;
+  constexpr uint32_t kJoinBytes = WR == 1 ? kWaves * kTileRows * D * 4 : 0;
+  __shared__ __attribute__((aligned(16))) char
+      lds[kLdsRows * kRowBytes > kJoinBytes ? kLdsRows * kRowBytes : kJoinBytes];
+  __shared__ __attribute__((aligned(16))) char lds_q[WR == 1 ? kTileRows * kKeyStride<D> : 16];
+  __shared__ float lds_ml[kWaves][WR == 1 ? kTileRows : 1][2];
 
   const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -200,10 +262,11 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
   const uint32_t item = nth * kXcds + blockIdx.x % kXcds;
   if (item >= p.items) return;
   const uint32_t in_unit = at - nth * unit, head = over(p.by_tiles, in_unit), tile = in_unit - head * p.row_tiles;
-  const uint32_t count = count_upto(p.batch, item, [&](uint32_t e) { return item_of(p, e, p.kv_indptr[e]); });
-  if (count == 0) return;
+  uint32_t b;
+  Tables tables;
+  if (!find_request(p, item, [&](uint32_t e, const Tables& t) { return item_of(p, e, t.k0); }, &b, &tables)) return;
   Request r;
-  const bool valid_request = request_of(p, count - 1, &r);
+  const bool valid_request = request_of(p, b, tables, &r);
   r.chunk = item - item_of(p, r.b, r.first_page);
   if (r.chunk >= r.chunks) return;
   if (!valid_request) {
@@ -221,23 +284,29 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
   int32_t t_end = static_cast<int32_t>(min(static_cast<int64_t>(t_begin) + chunk_tokens, static_cast<int64_t>(r.kv_len)));
   if (p.mask == nullptr) t_end = min(t_end, base + last_q + 1);
 
-  // Query fragments: row n of each tile, eight elements from 32 * ks + 8 * g.
+  // Query fragments: row n of each tile, eight elements from 32 * k + 8 * g.  In
+  // registers, or (WR = 1, whose registers hold more loads in flight) in LDS.
   const uint32_t wave_row0 = row0 + (WR == 1 ? 0 : w * 16 * R);
+  const auto query_at = [&](uint32_t row) {
+    const uint32_t i = over(p.by_group, row);
+    return p.q + static_cast<int64_t>(r.q0 + i) * p.q_stride +
+           (static_cast<int64_t>(head) * p.group + (row - i * p.group)) * (D * 2);
+  };
   u32x4 qf[R][kKS];
   int32_t qi[R];
 #pragma unroll
   for (int a = 0; a < R; ++a) {
     const uint32_t row = wave_row0 + a * 16 + n;
-    const uint32_t i = over(p.by_group, row);
-    qi[a] = static_cast<int32_t>(i);
-    const char* src = p.q + static_cast<int64_t>(r.q0 + i) * p.q_stride +
-                      (static_cast<int64_t>(head) * p.group + (row - i * p.group)) * (D * 2);
+    qi[a] = static_cast<int32_t>(over(p.by_group, row));
+    if constexpr (WR != 1) {
 #pragma unroll
-    for (int k = 0; k < kKS; ++k) {
-      qf[a][k] = u32x4{0, 0, 0, 0};
-      if (row < rows) qf[a][k] = *reinterpret_cast<const u32x4*>(src + k * 64 + g * 16);
+      for (int k = 0; k < kKS; ++k) {
+        qf[a][k] = u32x4{0, 0, 0, 0};
+        if (row < rows) qf[a][k] = *reinterpret_cast<const u32x4*>(query_at(row) + k * 64 + g * 16);
+      }
     }
   }
+  const char* const query = lds_q + n * kKeyStride<D> + g * 16;
 
   f32x4 acc[R][kDT];
   float m[R], from[R], l[R];
@@ -250,11 +319,12 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
     for (int d = 0; d < kDT; ++d) acc[a][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  char* const lds_k = lds;
-  char* const lds_v = lds + kLdsRows * kKeyStride<D>;
-  const uint32_t lds_row0 = w * kLoadRows;               // first row that this wave loads
+  // WR = 1: a wave's keys, then its values, pass through one region of its own.
+  char* const lds_k = WR == 1 ? lds + w * kLoadRows * kValueStride<D> : lds;
+  char* const lds_v = WR == 1 ? lds_k : lds + kLdsRows * kKeyStride<D>;
+  const uint32_t lds_row0 = WR == 1 ? 0 : w * kLoadRows;  // first row that this wave loads
 
-  // A step's loads: page ids (one token per lane), then rows.
+  // A step's loads: page ids (one token per lane), then key rows, then value rows.
   const uint32_t id_lane = lane % kIdTokens;
   int32_t id = 0;
   const auto load_id = [&](int32_t t0) {
@@ -262,45 +332,47 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
     id = -1;
     if (t < t_end) id = p.kv_indices[r.first_page + static_cast<int32_t>(over(p.by_page, static_cast<uint32_t>(t)))];
   };
+  // Load j of a lane: column lane % kPieces of row j * kRowStep + lane / kPieces.
+  constexpr uint32_t kRowStep = 64 / kPieces;
+  const uint32_t my_row = lane / kPieces, my_col = lane % kPieces;
   u32x4 kr[kLoads] = {}, vr[kLoads] = {};
-  uint64_t ks_byte = 0, vs_byte = 0;                     // the scales of the lane's token
+  uint32_t row_at = 0;                                   // the lane's token's row, in 16-byte units
+  uint64_t k_bytes = 0, v_bytes = 0;                     // the scales of the lane's token
   uint64_t valid = 0;
-  const auto load_rows = [&](int32_t t0) {
+  const auto fetch = [&](u32x4* to, int64_t from) {
+    const uint32_t first_row = opaque((WR == 1 ? 0 : w * kLoadRows) + my_row % kLoadRows);
+#pragma unroll
+    for (uint32_t j = 0; j < kLoads; ++j) {
+      const int64_t at = static_cast<int64_t>(static_cast<uint32_t>(__shfl(row_at, first_row + j * kRowStep))) + from;
+      const u32x4* const x = reinterpret_cast<const u32x4*>(p.cache + at * 16) + my_col;
+      to[j] = kReadOnce ? __builtin_nontemporal_load(x) : *x;
+    }
+  };
+  const auto load_keys = [&](int32_t t0) {
     const uint32_t t = static_cast<uint32_t>(t0) + id_lane;
     const bool ok = t0 + static_cast<int32_t>(id_lane) < t_end && static_cast<uint32_t>(id) < p.num_pages;
     valid = __ballot(ok);
     if (kIdTokens == 32) valid &= 0xffffffffull;
-    const uint32_t slot = t - over(p.by_page, t) * p.page_size;
-    // A token that does not exist reads the pool's first row, which store_rows
-    // makes zeros: loads without a condition.
-    const uint32_t off = ok ? static_cast<uint32_t>(id) * p.page16 + slot * p.row16 + head * (D * kBits / 128) : 0u;
     if (valid == 0) return;
+    const uint32_t slot = t - over(p.by_page, t) * p.page_size;
+    // A token that does not exist reads the pool's first row, which is made
+    // zeros on its way into LDS: loads without a condition.
+    row_at = ok ? static_cast<uint32_t>(id) * p.page16 + slot * p.row16 + head * (D * kBits / 128) : 0u;
     if constexpr (FORMAT != PACE_KV_PLAIN) {
-      ks_byte = vs_byte = 0;
+      k_bytes = v_bytes = 0;
       if (ok && id_lane / kLoadRows == (WR == 1 ? 0 : w)) {
         const char* s = p.cache + static_cast<int64_t>(id) * p.page16 * 16 + p.scale_at +
                         static_cast<int64_t>(slot) * p.scale_row + head * (D / 32);
         const char* sv = s + static_cast<int64_t>(p.half16) * 16;
-        if constexpr (D == 64) {
-          ks_byte = *reinterpret_cast<const uint16_t*>(s);
-          vs_byte = *reinterpret_cast<const uint16_t*>(sv);
-        } else if constexpr (D == 128) {
-          ks_byte = *reinterpret_cast<const uint32_t*>(s);
-          vs_byte = *reinterpret_cast<const uint32_t*>(sv);
-        } else {
-          ks_byte = *reinterpret_cast<const uint64_t*>(s);
-          vs_byte = *reinterpret_cast<const uint64_t*>(sv);
-        }
+        typedef std::conditional_t<D == 64, uint16_t, std::conditional_t<D == 128, uint32_t, uint64_t>> Scales;
+        k_bytes = *reinterpret_cast<const Scales*>(s);
+        v_bytes = *reinterpret_cast<const Scales*>(sv);
       }
     }
-#pragma unroll
-    for (uint32_t j = 0; j < kLoads; ++j) {
-      const uint32_t piece = j * 64 + lane, row = piece / kPieces, c = piece % kPieces;
-      const uint32_t o = __shfl(off, (WR == 1 ? 0 : w * kLoadRows) + row % kLoadRows);
-      const char* s = p.cache + (static_cast<int64_t>(o) + c) * 16;
-      kr[j] = *reinterpret_cast<const u32x4*>(s);
-      vr[j] = *reinterpret_cast<const u32x4*>(s + static_cast<int64_t>(p.half16) * 16);
-    }
+    fetch(kr, 0);
+  };
+  const auto load_values = [&]() {
+    if (valid != 0) fetch(vr, p.half16);
   };
   const auto store_piece = [&](char* row, uint32_t c, const u32x4& x, uint64_t bytes) {
     u32x4* to = reinterpret_cast<u32x4*>(row);
@@ -316,31 +388,24 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
       for (int k = 0; k < 4; ++k) to[4 * c + k] = run_up<TYPE, FORMAT>(u32x2{x[k], 0}, s);
     }
   };
-  const auto store_rows = [&]() {
-    if (valid != (kIdTokens == 32 ? 0xffffffffull : ~0ull)) {
+  // Loaded rows into LDS; unless WHOLE, those of tokens outside `exist` as zeros.
+  const auto store = [&](auto whole, char* to, uint32_t stride, u32x4* x, uint64_t bytes, uint64_t exist) {
+    const uint32_t from = opaque((WR == 1 ? 0 : w * kLoadRows) + my_row % kLoadRows);
+    if constexpr (!decltype(whole)::value) {
 #pragma unroll
-      for (uint32_t j = 0; j < kLoads; ++j) {
-        const uint32_t token = (WR == 1 ? 0 : w * kLoadRows) + (j * 64 + lane) / kPieces % kLoadRows;
-        if (!((valid >> token) & 1)) kr[j] = vr[j] = u32x4{0, 0, 0, 0};
-      }
+      for (uint32_t j = 0; j < kLoads; ++j)
+        if (!((exist >> (from + j * kRowStep)) & 1)) x[j] = u32x4{0, 0, 0, 0};
     }
+    char* const row = to + (lds_row0 + my_row) * stride;
 #pragma unroll
     for (uint32_t j = 0; j < kLoads; ++j) {
-      const uint32_t piece = j * 64 + lane, row = piece / kPieces, c = piece % kPieces;
-      uint64_t kb = 0, vb = 0;
+      uint64_t b = 0;
       if constexpr (FORMAT != PACE_KV_PLAIN) {
-        const uint32_t from = (WR == 1 ? 0 : w * kLoadRows) + row % kLoadRows;
-        kb = static_cast<uint32_t>(__shfl(static_cast<uint32_t>(ks_byte), from));
-        vb = static_cast<uint32_t>(__shfl(static_cast<uint32_t>(vs_byte), from));
-        if constexpr (D == 256) {
-          kb |= static_cast<uint64_t>(__shfl(static_cast<uint32_t>(ks_byte >> 32), from)) << 32;
-          vb |= static_cast<uint64_t>(__shfl(static_cast<uint32_t>(vs_byte >> 32), from)) << 32;
-        }
+        b = static_cast<uint32_t>(__shfl(static_cast<uint32_t>(bytes), from + j * kRowStep));
+        if constexpr (D == 256)
+          b |= static_cast<uint64_t>(__shfl(static_cast<uint32_t>(bytes >> 32), from + j * kRowStep)) << 32;
       }
-      if (row < kLoadRows) {
-        store_piece(lds_k + (lds_row0 + row) * kKeyStride<D>, c, kr[j], kb);
-        store_piece(lds_v + (lds_row0 + row) * kValueStride<D>, c, vr[j], vb);
-      }
+      if (kRowStep <= kLoadRows || my_row < kLoadRows) store_piece(row + j * kRowStep * stride, my_col, x[j], b);
     }
   };
 
@@ -361,56 +426,62 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
     return static_cast<uint32_t>(x);
   };
 
-  // 32 tokens from t0 whose rows lie at lds_row; `ok`: the tokens that exist.
-  const auto attend = [&](int32_t t0, uint32_t lds_row, uint32_t ok) {
+  // The weights of 32 tokens from t0, whose keys lie at lds_row; `ok`: the tokens
+  // that exist.
+  u32x4 pf[R];
+  uint32_t sees[R];
+  const auto weigh = [&](auto full, int32_t t0, uint32_t lds_row, uint32_t ok) {
     const char* key_at = lds_k + (lds_row + n) * kKeyStride<D> + g * 16;
-    const char* value_at = lds_v + lds_row * kValueStride<D>;
     f32x4 s[R][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int a = 0; a < R; ++a) s[a][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < kKS; ++k)
+    for (int k = 0; k < kKS; ++k) {
+      if constexpr (WR == 1) {
+#pragma unroll
+        for (int a = 0; a < R; ++a)
+          qf[a][k] = *reinterpret_cast<const u32x4*>(query + a * 16 * kKeyStride<D> + k * 64);
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         const u32x4 kf = *reinterpret_cast<const u32x4*>(key_at + t * 16 * kKeyStride<D> + k * 64);
 #pragma unroll
         for (int a = 0; a < R; ++a) s[a][t] = mfma<TYPE>(kf, qf[a][k], s[a][t]);
       }
-    const bool full = ok == ~0u && (t0 + 32 <= base || (p.mask == nullptr && t0 + 31 <= base + first_q));
-    bool odd = false;                                    // an infinite or NaN value that some row must not see
-    uint32_t sees[R];
-    if (!full) {
-#pragma unroll
-      for (int a = 0; a < R; ++a) sees[a] = seen(t0, qi[a]) & ok;
-      bool found = false;
-#pragma unroll
-      for (uint32_t k = 0; k < 32 * D / 8 / 64; ++k) {
-        const uint32_t c = k * 64 + lane;
-        const u32x4 x = *reinterpret_cast<const u32x4*>(value_at + c / (D / 8) * kValueStride<D> + c % (D / 8) * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) found |= odd_word<TYPE>(x[e]);
-      }
-      odd = __ballot(found) != 0;
     }
-    u32x4 pf[R];
+#pragma unroll
+    for (int a = 0; a < R; ++a)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[a][t] *= p.scale_log2;
+    if (p.cap_log2 > 0.f) {
+      // tanh(z) = 1 - 2 / (1 + 2^(2 log2(e) z))
+#pragma unroll
+      for (int a = 0; a < R; ++a)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[a][t][e] = p.cap_log2 * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + exp2_of(s[a][t][e])));
+    }
+    if constexpr (!decltype(full)::value) {
+#pragma unroll
+      for (int a = 0; a < R; ++a) {
+        sees[a] = seen(t0, qi[a]) & ok;
+        const uint32_t mine = sees[a] >> opaque(4 * g);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(mine & (1u << (t * 16 + e)))) s[a][t][e] = -INFINITY;
+      }
+    }
 #pragma unroll
     for (int a = 0; a < R; ++a) {
-      float x[8];
+      float top = fmaxf(s[a][0][0], s[a][1][0]);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float y = s[a][t][e] * p.scale_log2;
-          // tanh(z) = 1 - 2 / (1 + 2^(2 log2(e) z))
-          if (p.cap_log2 > 0.f) y = p.cap_log2 * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + exp2_of(y)));
-          if (!full && !((sees[a] >> (t * 16 + 4 * g + e)) & 1u)) y = -INFINITY;
-          x[t * 4 + e] = y;
-        }
-      float top = x[0];
-#pragma unroll
-      for (int e = 1; e < 8; ++e) top = fmaxf(top, x[e]);
+      for (int e = 1; e < 4; ++e) top = fmaxf(top, fmaxf(s[a][0][e], s[a][1][e]));
       // The maximum is raised only past 2^8 of it: weights stay below 2^8 (and
       // their sums within float32), and most steps need no joint maximum.
       if (__ballot(top > m[a] + 8.f) != 0) {
@@ -423,22 +494,38 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
         for (int d = 0; d < kDT; ++d) acc[a][d] *= shrink;
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = exp2_of(x[e] - from[a]);
-        l[a] += x[e];
-      }
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) pf[a][e] = pair_of<TYPE>(x[2 * e], x[2 * e + 1]);
+        for (int e = 0; e < 4; e += 2) {
+          const float x = exp2_of(s[a][t][e] - from[a]), y = exp2_of(s[a][t][e + 1] - from[a]);
+          l[a] += x + y;
+          pf[a][t * 2 + e / 2] = pair_of<TYPE>(x, y);
+        }
+    }
+  };
+  // Adds the weighted values of those tokens, at lds_row.
+  const auto gather = [&](auto full, uint32_t lds_row) {
+    const char* value_at = lds_v + lds_row * kValueStride<D>;
+    bool odd = false;                                    // an infinite or NaN value that some row must not see
+    if constexpr (!decltype(full)::value) {
+      bool found = false;
+#pragma unroll 1
+      for (uint32_t c = lane; c < 32 * D / 8; c += 64) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(value_at + c / (D / 8) * kValueStride<D> + c % (D / 8) * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) found |= odd_word<TYPE>(x[e]);
+      }
+      odd = __ballot(found) != 0;
     }
     if (!odd) {
 #pragma unroll
       for (int d = 0; d < kDT; ++d) {
         // Lane: row 4 g + n / 4 of each 16 tokens, four columns; transposed over
         // 16 lanes: four tokens of column n.
-        const char* from = value_at + (4 * g + n / 4) * kValueStride<D> + n % 4 * 8 + d * 32;
+        const char* at = value_at + (4 * g + n / 4) * kValueStride<D> + n % 4 * 8 + d * 32;
         typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)from);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(from + 16 * kValueStride<D>));
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 16 * kValueStride<D>));
         const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
         const u32x4 vf = {lo2[0], lo2[1], hi2[0], hi2[1]};
 #pragma unroll
@@ -464,32 +551,67 @@ __global__ __launch_bounds__(kThreads, D == 256 && R == 2 ? 1 : 2) void attentio
         }
     }
   };
-
-  const int32_t wave_t0 = t_begin + (WR == 1 ? static_cast<int32_t>(w * kIdTokens) : 0);
-  load_id(wave_t0);
-  load_rows(wave_t0);
-  load_id(wave_t0 + static_cast<int32_t>(kStep));
-  for (int32_t t0 = t_begin; t0 < t_end; t0 += static_cast<int32_t>(kStep)) {
-    const int32_t tw = t0 + (wave_t0 - t_begin);
-    if (WR != 1) __syncthreads();                        // the last step's reads are done
-    store_rows();
-    const uint64_t ok = valid;
-    if (WR != 1) __syncthreads();
-    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    load_rows(tw + static_cast<int32_t>(kStep));
-    load_id(tw + 2 * static_cast<int32_t>(kStep));
-    __builtin_amdgcn_sched_barrier(0);
-    if (WR == 1) {
-      if (ok != 0) attend(tw, lds_row0, static_cast<uint32_t>(ok));
+  // Whether every row sees all of a wave's tokens from t0.
+  constexpr uint64_t kAll = kIdTokens == 32 ? 0xffffffffull : ~0ull;
+  const int32_t seen_by_all = p.mask == nullptr ? base + first_q + 1 : base;
+  const auto all_seen = [&](int32_t t0) {
+    return valid == kAll && t0 + static_cast<int32_t>(kIdTokens) <= seen_by_all;
+  };
+  const int32_t step = static_cast<int32_t>(kStep);
+  int32_t t0 = t_begin + (WR == 1 ? static_cast<int32_t>(w * kIdTokens) : 0);
+  const auto one_step = [&](auto full) {
+    const uint64_t ok = valid, bytes = v_bytes;
+    if constexpr (WR == 1) {
+      // No barrier: the region is the wave's own, and its LDS operations run in order.
+      store(full, lds_k, kKeyStride<D>, kr, k_bytes, ok);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      load_keys(t0 + step);
+      load_id(t0 + 2 * step);
+      __builtin_amdgcn_sched_barrier(0);
+      weigh(full, t0, 0, static_cast<uint32_t>(ok));
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      store(full, lds_v, kValueStride<D>, vr, bytes, ok);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      load_values();
+      __builtin_amdgcn_sched_barrier(0);
+      gather(full, 0);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     } else {
+      __syncthreads();                                   // the last step's reads are done
+      store(full, lds_k, kKeyStride<D>, kr, k_bytes, ok);
+      store(full, lds_v, kValueStride<D>, vr, bytes, ok);
+      __syncthreads();
+      load_keys(t0 + step);
+      load_values();
+      load_id(t0 + 2 * step);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
-        const uint32_t part = static_cast<uint32_t>(ok >> (32 * h));
-        if (part != 0) attend(t0 + 32 * h, 32 * h, part);
+        weigh(full, t0 + 32 * h, 32 * h, static_cast<uint32_t>(ok >> (32 * h)));
+        gather(full, 32 * h);
       }
     }
+    t0 += step;
+  };
+  load_id(t0);
+  if constexpr (WR == 1) {
+#pragma unroll
+    for (uint32_t e = threadIdx.x; e < kTileRows * (D / 8); e += kThreads) {
+      const uint32_t row = e / (D / 8), c = e % (D / 8);
+      u32x4 x = {0, 0, 0, 0};
+      if (row0 + row < rows) x = *reinterpret_cast<const u32x4*>(query_at(row0 + row) + c * 16);
+      *reinterpret_cast<u32x4*>(lds_q + row * kKeyStride<D> + c * 16) = x;
+    }
   }
+  load_keys(t0);
+  load_values();
+  load_id(t0 + step);
+  if (WR == 1) __syncthreads();                          // the queries are in LDS
+  // The steps whose tokens every row sees, then the others: the first loop is
+  // free of masks, and of the registers that they take.
+  while (t0 < t_end && all_seen(t0)) one_step(std::true_type{});
+#pragma unroll 1
+  while (t0 < t_end) one_step(std::false_type{});
 #pragma unroll
   for (int a = 0; a < R; ++a) l[a] = across_groups(l[a], sum_of);
 

@@ -1,75 +1,105 @@
 // Attention over a paged cache: how a call is cut up, the kernel that joins the
 // parts, and the entry points.  The attention itself: attention.h.
 #include "attention.h"
+#include <stdlib.h>
 
 namespace pace_kv {
 namespace {
 
-// Joins the chunks of each row (token, head): a workgroup per row, its threads
-// D / 4 columns of four by as many chunks at a time as fit.
-template <int D, int TYPE>
+// Joins the chunks of each row (token, head) of a split request.  WAVES waves take
+// a row; within a wave D / 4 lanes take four columns each of a chunk, and the
+// wave as many chunks at a time as fit.  The chunks' weights come first, 64 at a
+// time, so that the loads of their outputs do not wait for one another.
+template <int D, int TYPE, int WAVES>
 __global__ __launch_bounds__(kThreads) void combine_kernel(const AttnParams p) {
-  constexpr uint32_t kCols = D / 4, kGroups = kThreads / kCols;
-  __shared__ f32x4 lds_o[kGroups][kCols];
-  __shared__ float lds_l[kGroups], lds_m[kGroups];
+  constexpr uint32_t kCols = D / 4, kGroups = 64 / kCols;
+  __shared__ f32x4 lds_o[WAVES][kCols];
+  __shared__ float lds_m[WAVES], lds_l[WAVES];
+  const uint32_t lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t all_heads = p.heads * p.group;
-  const uint32_t token = blockIdx.x / all_heads, qh = blockIdx.x % all_heads;
+  const uint32_t row_id = WAVES == 1 ? blockIdx.x * kWaves + w : blockIdx.x;
+  const uint32_t token = over(p.by_heads, row_id), qh = row_id - token * all_heads;
+  if (token >= p.nnz) return;
   uint32_t b = token;
-  if (p.qo_indptr != nullptr) {
-    const uint32_t count =
-        count_upto(p.batch, token, [&](uint32_t e) { return static_cast<uint32_t>(max(p.qo_indptr[e], 0)); });
-    if (count == 0) return;
-    b = count - 1;
+  Tables tables;
+  if (p.qo_indptr == nullptr) {
+    if (b >= p.batch) return;
+    tables = tables_of(p, b);
+  } else if (!find_request(p, token, [](uint32_t, const Tables& t) { return static_cast<uint32_t>(max(t.a0, 0)); }, &b,
+                           &tables)) {
+    return;
   }
-  if (b >= p.batch) return;
   Request r;
-  if (!request_of(p, b, &r) || token < r.q0 || token - r.q0 >= r.q_len || r.chunks == 1) return;
+  if (!request_of(p, b, tables, &r) || token < r.q0 || token - r.q0 >= r.q_len || r.chunks == 1) return;
   const uint32_t head = over(p.by_group, qh), row = (token - r.q0) * p.group + (qh - head * p.group);
   const uint32_t tile = row / p.tile_rows;
   const int64_t unit = static_cast<int64_t>(p.heads) * p.row_tiles;
   const int64_t first = (static_cast<int64_t>(item_of(p, b, r.first_page)) * unit +
                          static_cast<int64_t>(head) * p.row_tiles + tile) * p.tile_rows + row % p.tile_rows;
   const int64_t step = unit * p.tile_rows;
-  const uint32_t col = threadIdx.x % kCols, part = threadIdx.x / kCols;
+  const uint32_t col = lane % kCols, group = lane / kCols;
+  // The wave's part of the chunks.
+  const uint32_t per_wave = (r.chunks + WAVES - 1) / WAVES;
+  const uint32_t c_begin = WAVES == 1 ? 0 : w * per_wave, c_end = min(c_begin + per_wave, r.chunks);
   float m = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (uint32_t c = part; c < r.chunks; c += kGroups) {
-    const int64_t at = first + c * step;
-    const float mc = p.part_ml[at * 2], lc = p.part_ml[at * 2 + 1];
-    const f32x4 oc = *reinterpret_cast<const f32x4*>(p.part_o + at * D + col * 4);
-    const float top = fmaxf(m, mc), from = top == -INFINITY ? 0.f : top;
-    const float a = exp2_of(m - from), d = exp2_of(mc - from);
-    l = l * a + lc * d;
-    o = o * a + oc * d;
+  for (uint32_t c0 = c_begin; c0 < c_end; c0 += 64) {
+    float mc = -INFINITY, lc = 0.f;
+    if (c0 + lane < c_end) {
+      const int64_t at = first + (c0 + lane) * step;
+      mc = p.part_ml[at * 2];
+      lc = p.part_ml[at * 2 + 1];
+    }
+    float top = mc;
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
+    top = fmaxf(m, top);
+    const float from = top == -INFINITY ? 0.f : top, shrink = exp2_of(m - from);
+    const float weight = exp2_of(mc - from);
+    float sum = weight * lc;
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) sum += __shfl_xor(sum, k);
+    l = l * shrink + sum;
+    o *= shrink;
     m = top;
+    const uint32_t n = min(c_end - c0, 64u);
+#pragma unroll 8
+    for (uint32_t c = group; c < n; c += kGroups)
+      o += __shfl(weight, c) * *reinterpret_cast<const f32x4*>(p.part_o + (first + (c0 + c) * step) * D + col * 4);
   }
-  lds_o[part][col] = o;
-  if (col == 0) {
-    lds_m[part] = m;
-    lds_l[part] = l;
-  }
-  __syncthreads();
-  if (part != 0) return;
-  float top = -INFINITY;
 #pragma unroll
-  for (uint32_t v = 0; v < kGroups; ++v) top = fmaxf(top, lds_m[v]);
-  const float from = top == -INFINITY ? 0.f : top;
-  l = 0.f;
-  o = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int k = kCols; k < 64; k *= 2)
 #pragma unroll
-  for (uint32_t v = 0; v < kGroups; ++v) {
-    const float weight = exp2_of(lds_m[v] - from);
-    l += weight * lds_l[v];
-    o += weight * lds_o[v][col];
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], k);
+  if constexpr (WAVES > 1) {
+    if (group == 0) lds_o[w][col] = o;
+    if (lane == 0) {
+      lds_m[w] = m;
+      lds_l[w] = l;
+    }
+    __syncthreads();
+    if (w != 0) return;
+    m = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) m = fmaxf(m, lds_m[v]);
+    const float from = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < WAVES; ++v) {
+      const float weight = exp2_of(lds_m[v] - from);
+      l += weight * lds_l[v];
+      o += weight * lds_o[v][col];
+    }
   }
+  if (group != 0) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const u32x2 x = {pair_of<TYPE>(o[0] * inv, o[1] * inv), pair_of<TYPE>(o[2] * inv, o[3] * inv)};
   *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(token) * p.out_stride +
                             (static_cast<int64_t>(qh) * D + col * 4) * 2) = x;
   if (col == 0 && p.lse != nullptr)
     p.lse[static_cast<int64_t>(token) * all_heads + qh] =
-        l == 0.f ? -INFINITY : (top + __log2f(l)) * 0.69314718055994531f;
+        l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
 }
 
 // How a call is cut up.
@@ -89,8 +119,10 @@ Split split_of(int64_t batch, int64_t heads, int64_t group, int64_t max_q, int64
   s.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
   s.row_tiles = static_cast<uint32_t>((rows + s.tile_rows - 1) / s.tile_rows);
   const int64_t units = heads * s.row_tiles;
-  int64_t chunk = (num_indices * units + kTargetGroups - 1) / kTargetGroups;
-  const int64_t least = (kMinChunkTokens + page_size - 1) / page_size;
+  static const int64_t T = getenv("PK_T") ? atoi(getenv("PK_T")) : kTargetGroups, TR = getenv("PK_TR") ? atoi(getenv("PK_TR")) : kTargetGroups, MM = getenv("PK_M") ? atoi(getenv("PK_M")) : kMinChunkTokens;
+  const int64_t tgt = s.by_rows ? TR : T;
+  int64_t chunk = (num_indices * units + tgt - 1) / tgt;
+  const int64_t least = (MM + page_size - 1) / page_size;
   if (chunk < least) chunk = least;
   if (chunk > num_indices) chunk = num_indices;
   if (chunk < 1) chunk = 1;
@@ -99,10 +131,19 @@ Split split_of(int64_t batch, int64_t heads, int64_t group, int64_t max_q, int64
   return s;
 }
 
+// Calls of at least this many rows give each row one wave to join its chunks,
+// smaller ones a workgroup.
+constexpr int64_t kManyRows = 2048;
+
+template <int D, int TYPE>
+const void* pick_combine(bool many) {
+  return many ? reinterpret_cast<const void*>(&combine_kernel<D, TYPE, 1>)
+              : reinterpret_cast<const void*>(&combine_kernel<D, TYPE, kWaves>);
+}
+
 template <int D>
-const void* pick_combine(int type) {
-  return type == PACE_KV_BF16 ? reinterpret_cast<const void*>(&combine_kernel<D, PACE_KV_BF16>)
-                              : reinterpret_cast<const void*>(&combine_kernel<D, PACE_KV_FP16>);
+const void* pick_combine(int type, bool many) {
+  return type == PACE_KV_BF16 ? pick_combine<D, PACE_KV_BF16>(many) : pick_combine<D, PACE_KV_FP16>(many);
 }
 
 int check_sizes(int batch_size, int num_kv_heads, int group, int head_dim, int max_q_len, int64_t num_indices,
@@ -218,6 +259,7 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   p.by_page = fast_div(p.page_size);
   p.by_chunk = fast_div(p.chunk_pages);
   p.by_group = fast_div(p.group);
+  p.by_heads = fast_div(p.heads * p.group);
   p.by_unit = fast_div(p.heads * p.row_tiles);
   p.by_tiles = fast_div(p.row_tiles);
   const float log2e = 1.44269504088896341f;
@@ -226,16 +268,19 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   const void* attention = head_dim == 64    ? attention_kernel_d64(elem_type, format, s.tile_rows)
                           : head_dim == 128 ? attention_kernel_d128(elem_type, format, s.tile_rows)
                                             : attention_kernel_d256(elem_type, format, s.tile_rows);
-  const void* combine = head_dim == 64    ? pick_combine<64>(elem_type)
-                        : head_dim == 128 ? pick_combine<128>(elem_type)
-                                          : pick_combine<256>(elem_type);
+  const int64_t out_rows = nnz * num_kv_heads * group;
+  const bool many = out_rows >= kManyRows;
+  const void* combine = head_dim == 64    ? pick_combine<64>(elem_type, many)
+                        : head_dim == 128 ? pick_combine<128>(elem_type, many)
+                                          : pick_combine<256>(elem_type, many);
   const uint32_t items = (s.items + kXcds - 1) / kXcds * kXcds;
   void* args[] = {&p};
   PACE_KV_TRY(hip_status(hipLaunchKernel(attention, dim3(items * p.heads * p.row_tiles), dim3(kThreads), args, 0,
                                          static_cast<hipStream_t>(stream)), "attention launch"));
   if (need == 0) return PACE_KV_OK;
-  return hip_status(hipLaunchKernel(combine, dim3(static_cast<uint32_t>(nnz) * p.heads * p.group), dim3(kThreads),
-                                    args, 0, static_cast<hipStream_t>(stream)), "attention combine launch");
+  const uint32_t groups = static_cast<uint32_t>(many ? (out_rows + kWaves - 1) / kWaves : out_rows);
+  return hip_status(hipLaunchKernel(combine, dim3(groups), dim3(kThreads), args, 0, static_cast<hipStream_t>(stream)),
+                    "attention combine launch");
 }
 
 }  // extern "C"
