@@ -77,6 +77,15 @@ __device__ __forceinline__ float across_groups(float x, F f) {
 __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float sum_of(float a, float b) { return a + b; }
 
+// The larger of three, of the numbers among them where some are NaN.  Plain fmaxf
+// quiets its operands first, an instruction each, though no product here is a
+// signalling NaN.
+__device__ __forceinline__ float max3_of(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A request and the part of it that a work item covers.
@@ -165,15 +174,12 @@ __device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Ke
   return found;
 }
 
-// Rows in LDS are padded so that neighbouring rows start 16 bytes (keys) or 32
-// (values) further along the banks: 16 rows' 16 bytes of a key fragment, and 8
-// rows' 32 bytes of a transposing read, each cover the 256 bytes of all banks
-// once.  Unlike a xor of the columns, a pad leaves every address one register and
-// an immediate offset.
+// Rows in LDS are padded by 32 bytes, so that 8 rows' 32 bytes of a transposing
+// read cover the 256 bytes of all banks once (MI355X, keys and values padded so:
+// half the bank conflicts of keys padded by 16).  Unlike a xor of the columns, a
+// pad leaves every address one register and an immediate offset.
 template <int D>
-constexpr uint32_t kKeyStride = D * 2 + 16;
-template <int D>
-constexpr uint32_t kValueStride = D * 2 + 32;
+constexpr uint32_t kStride = D * 2 + 32;
 
 template <int TYPE>
 __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c) {
@@ -227,7 +233,7 @@ constexpr int min_waves(int D, int format, int R, int WR) {
 
 // TYPE: of queries and output, and what a quantised cache is expanded to.
 // R tiles of 16 query rows per wave.  WR = 1: the waves take 32 tokens each of
-// a step and join at the end.  WR = 4: each wave takes its own 16 * R rows, and
+// a step for the same rows and join at the end.  WR = 4: each wave takes its own 16 * R rows, and
 // all share a tile of 64 tokens.
 template <int D, int TYPE, int FORMAT, int R, int WR>
 __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attention_kernel(const AttnParams p) {
@@ -245,11 +251,11 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   // 2 GiB of pages in this pattern: 6.3 to 6.8 TB/s against 5.7 to 6.1.
   constexpr bool kReadOnce = WR == 1 || R == 1;
 
-  constexpr uint32_t kRowBytes = WR == 1 ? kValueStride<D> : kKeyStride<D> + kValueStride<D>;
-  constexpr uint32_t kJoinBytes = WR == 1 ? kWaves * kTileRows * D * 4 : 0;
+  constexpr uint32_t kRowBytes = WR == 1 ? kStride<D> : 2 * kStride<D>;
+  constexpr uint32_t kJoinBytes = WR == 1 ? kWaves * 16 * D * 4 : 0;
   __shared__ __attribute__((aligned(16))) char
       lds[kLdsRows * kRowBytes > kJoinBytes ? kLdsRows * kRowBytes : kJoinBytes];
-  __shared__ __attribute__((aligned(16))) char lds_q[WR == 1 ? kTileRows * kKeyStride<D> : 16];
+  __shared__ __attribute__((aligned(16))) char lds_q[WR == 1 ? kTileRows * kStride<D> : 16];
   __shared__ float lds_ml[kWaves][WR == 1 ? kTileRows : 1][2];
 
   const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
@@ -306,7 +312,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
       }
     }
   }
-  const char* const query = lds_q + n * kKeyStride<D> + g * 16;
+  const char* const query = lds_q + n * kStride<D> + g * 16;
 
   f32x4 acc[R][kDT];
   float m[R], from[R], l[R];
@@ -320,8 +326,8 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   }
 
   // WR = 1: a wave's keys, then its values, pass through one region of its own.
-  char* const lds_k = WR == 1 ? lds + w * kLoadRows * kValueStride<D> : lds;
-  char* const lds_v = WR == 1 ? lds_k : lds + kLdsRows * kKeyStride<D>;
+  char* const lds_k = WR == 1 ? lds + w * kLoadRows * kStride<D> : lds;
+  char* const lds_v = WR == 1 ? lds_k : lds + kLdsRows * kStride<D>;
   const uint32_t lds_row0 = WR == 1 ? 0 : w * kLoadRows;  // first row that this wave loads
 
   // A step's loads: page ids (one token per lane), then key rows, then value rows.
@@ -389,14 +395,14 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
     }
   };
   // Loaded rows into LDS; unless WHOLE, those of tokens outside `exist` as zeros.
-  const auto store = [&](auto whole, char* to, uint32_t stride, u32x4* x, uint64_t bytes, uint64_t exist) {
+  const auto store = [&](auto whole, char* to, u32x4* x, uint64_t bytes, uint64_t exist) {
     const uint32_t from = opaque((WR == 1 ? 0 : w * kLoadRows) + my_row % kLoadRows);
     if constexpr (!decltype(whole)::value) {
 #pragma unroll
       for (uint32_t j = 0; j < kLoads; ++j)
         if (!((exist >> (from + j * kRowStep)) & 1)) x[j] = u32x4{0, 0, 0, 0};
     }
-    char* const row = to + (lds_row0 + my_row) * stride;
+    char* const row = to + (lds_row0 + my_row) * kStride<D>;
 #pragma unroll
     for (uint32_t j = 0; j < kLoads; ++j) {
       uint64_t b = 0;
@@ -405,7 +411,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
         if constexpr (D == 256)
           b |= static_cast<uint64_t>(__shfl(static_cast<uint32_t>(bytes >> 32), from + j * kRowStep)) << 32;
       }
-      if (kRowStep <= kLoadRows || my_row < kLoadRows) store_piece(row + j * kRowStep * stride, my_col, x[j], b);
+      if (kRowStep <= kLoadRows || my_row < kLoadRows) store_piece(row + j * kRowStep * kStride<D>, my_col, x[j], b);
     }
   };
 
@@ -430,8 +436,9 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   // that exist.
   u32x4 pf[R];
   uint32_t sees[R];
+  const float per_score = p.cap_log2 > 0.f || p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
   const auto weigh = [&](auto full, int32_t t0, uint32_t lds_row, uint32_t ok) {
-    const char* key_at = lds_k + (lds_row + n) * kKeyStride<D> + g * 16;
+    const char* key_at = lds_k + (lds_row + n) * kStride<D> + g * 16;
     f32x4 s[R][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -442,28 +449,33 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
       if constexpr (WR == 1) {
 #pragma unroll
         for (int a = 0; a < R; ++a)
-          qf[a][k] = *reinterpret_cast<const u32x4*>(query + a * 16 * kKeyStride<D> + k * 64);
+          qf[a][k] = *reinterpret_cast<const u32x4*>(query + a * 16 * kStride<D> + k * 64);
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const u32x4 kf = *reinterpret_cast<const u32x4*>(key_at + t * 16 * kKeyStride<D> + k * 64);
+        const u32x4 kf = *reinterpret_cast<const u32x4*>(key_at + t * 16 * kStride<D> + k * 64);
 #pragma unroll
         for (int a = 0; a < R; ++a) s[a][t] = mfma<TYPE>(kf, qf[a][k], s[a][t]);
       }
     }
-#pragma unroll
-    for (int a = 0; a < R; ++a)
-#pragma unroll
-      for (int t = 0; t < 2; ++t) s[a][t] *= p.scale_log2;
+    // The weights are 2^(per_score * s - m).
     if (p.cap_log2 > 0.f) {
-      // tanh(z) = 1 - 2 / (1 + 2^(2 log2(e) z))
+      // tanh(z) = 1 - 2 / (1 + 2^(2 log2(e) z)), times the cap
 #pragma unroll
       for (int a = 0; a < R; ++a)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s[a][t][e] = p.cap_log2 * (1.f - 2.f * __builtin_amdgcn_rcpf(1.f + exp2_of(s[a][t][e])));
+          for (int e = 0; e < 4; ++e) {
+            const float half = __builtin_amdgcn_rcpf(1.f + exp2_of(s[a][t][e] * p.scale_log2));
+            s[a][t][e] = __builtin_fmaf(half, -2.f * p.cap_log2, p.cap_log2);
+          }
+    } else if (p.scale_log2 <= 0.f) {
+      const float sign = p.scale_log2 < 0.f ? -1.f : 0.f;
+#pragma unroll
+      for (int a = 0; a < R; ++a)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[a][t] *= sign;
     }
     if constexpr (!decltype(full)::value) {
 #pragma unroll
@@ -479,9 +491,10 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
     }
 #pragma unroll
     for (int a = 0; a < R; ++a) {
-      float top = fmaxf(s[a][0][0], s[a][1][0]);
-#pragma unroll
-      for (int e = 1; e < 4; ++e) top = fmaxf(top, fmaxf(s[a][0][e], s[a][1][e]));
+      float top = max3_of(s[a][0][0], s[a][0][1], s[a][0][2]);
+      top = max3_of(top, s[a][0][3], s[a][1][0]);
+      top = max3_of(top, s[a][1][1], s[a][1][2]);
+      top = max3_of(top, s[a][1][3], s[a][1][3]) * per_score;
       // The maximum is raised only past 2^8 of it: weights stay below 2^8 (and
       // their sums within float32), and most steps need no joint maximum.
       if (__ballot(top > m[a] + 8.f) != 0) {
@@ -497,7 +510,8 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
-          const float x = exp2_of(s[a][t][e] - from[a]), y = exp2_of(s[a][t][e + 1] - from[a]);
+          const float x = exp2_of(__builtin_fmaf(s[a][t][e], per_score, -from[a]));
+          const float y = exp2_of(__builtin_fmaf(s[a][t][e + 1], per_score, -from[a]));
           l[a] += x + y;
           pf[a][t * 2 + e / 2] = pair_of<TYPE>(x, y);
         }
@@ -505,13 +519,13 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   };
   // Adds the weighted values of those tokens, at lds_row.
   const auto gather = [&](auto full, uint32_t lds_row) {
-    const char* value_at = lds_v + lds_row * kValueStride<D>;
+    const char* value_at = lds_v + lds_row * kStride<D>;
     bool odd = false;                                    // an infinite or NaN value that some row must not see
     if constexpr (!decltype(full)::value) {
       bool found = false;
 #pragma unroll 1
       for (uint32_t c = lane; c < 32 * D / 8; c += 64) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(value_at + c / (D / 8) * kValueStride<D> + c % (D / 8) * 16);
+        const u32x4 x = *reinterpret_cast<const u32x4*>(value_at + c / (D / 8) * kStride<D> + c % (D / 8) * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) found |= odd_word<TYPE>(x[e]);
       }
@@ -522,10 +536,10 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
       for (int d = 0; d < kDT; ++d) {
         // Lane: row 4 g + n / 4 of each 16 tokens, four columns; transposed over
         // 16 lanes: four tokens of column n.
-        const char* at = value_at + (4 * g + n / 4) * kValueStride<D> + n % 4 * 8 + d * 32;
+        const char* at = value_at + (4 * g + n / 4) * kStride<D> + n % 4 * 8 + d * 32;
         typedef __attribute__((address_space(3))) s16x4* lds_ptr;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 16 * kValueStride<D>));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 16 * kStride<D>));
         const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
         const u32x4 vf = {lo2[0], lo2[1], hi2[0], hi2[1]};
 #pragma unroll
@@ -544,51 +558,61 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
           if (!((sees[a] >> token) & 1u)) continue;
 #pragma unroll
           for (int d = 0; d < kDT; ++d) {
-            const u32x2 v = *reinterpret_cast<const u32x2*>(value_at + token * kValueStride<D> + d * 32 + g * 8);
+            const u32x2 v = *reinterpret_cast<const u32x2*>(value_at + token * kStride<D> + d * 32 + g * 8);
 #pragma unroll
             for (int c = 0; c < 4; ++c) acc[a][d][c] += weight * value_of<TYPE>(v[c / 2], c % 2);
           }
         }
     }
   };
-  // Whether every row sees all of a wave's tokens from t0.
   constexpr uint64_t kAll = kIdTokens == 32 ? 0xffffffffull : ~0ull;
   const int32_t seen_by_all = p.mask == nullptr ? base + first_q + 1 : base;
+  // Whether every row sees all the tokens of a wave's step from t0.
   const auto all_seen = [&](int32_t t0) {
     return valid == kAll && t0 + static_cast<int32_t>(kIdTokens) <= seen_by_all;
   };
   const int32_t step = static_cast<int32_t>(kStep);
   int32_t t0 = t_begin + (WR == 1 ? static_cast<int32_t>(w * kIdTokens) : 0);
   const auto one_step = [&](auto full) {
-    const uint64_t ok = valid, bytes = v_bytes;
     if constexpr (WR == 1) {
       // No barrier: the region is the wave's own, and its LDS operations run in order.
-      store(full, lds_k, kKeyStride<D>, kr, k_bytes, ok);
+      const uint64_t ok = valid, bytes = v_bytes;
+      store(full, lds_k, kr, k_bytes, ok);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       load_keys(t0 + step);
       load_id(t0 + 2 * step);
       __builtin_amdgcn_sched_barrier(0);
       weigh(full, t0, 0, static_cast<uint32_t>(ok));
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      store(full, lds_v, kValueStride<D>, vr, bytes, ok);
+      store(full, lds_v, vr, bytes, ok);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       load_values();
       __builtin_amdgcn_sched_barrier(0);
       gather(full, 0);
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     } else {
+      // Two tiles in LDS would need one barrier, but cost a third workgroup its
+      // place (MI355X, 36 rows over a 4-bit cache: 70 us against 53).
+      const uint64_t ok = valid;
       __syncthreads();                                   // the last step's reads are done
-      store(full, lds_k, kKeyStride<D>, kr, k_bytes, ok);
-      store(full, lds_v, kValueStride<D>, vr, bytes, ok);
+      store(full, lds_k, kr, k_bytes, ok);
+      store(full, lds_v, vr, v_bytes, ok);
       __syncthreads();
       load_keys(t0 + step);
       load_values();
       load_id(t0 + 2 * step);
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (decltype(full)::value) {
+        weigh(full, t0, 0, 0);
+        gather(full, 0);
+        weigh(full, t0 + 32, 32, 0);
+        gather(full, 32);
+      } else {
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        weigh(full, t0 + 32 * h, 32 * h, static_cast<uint32_t>(ok >> (32 * h)));
-        gather(full, 32 * h);
+        for (int h = 0; h < 2; ++h) {
+          weigh(full, t0 + 32 * h, 32 * h, static_cast<uint32_t>(ok >> (32 * h)));
+          gather(full, 32 * h);
+        }
       }
     }
     t0 += step;
@@ -600,7 +624,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
       const uint32_t row = e / (D / 8), c = e % (D / 8);
       u32x4 x = {0, 0, 0, 0};
       if (row0 + row < rows) x = *reinterpret_cast<const u32x4*>(query_at(row0 + row) + c * 16);
-      *reinterpret_cast<u32x4*>(lds_q + row * kKeyStride<D> + c * 16) = x;
+      *reinterpret_cast<u32x4*>(lds_q + row * kStride<D> + c * 16) = x;
     }
   }
   load_keys(t0);
@@ -646,41 +670,50 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
       for (int d = 0; d < kDT; ++d) write(w * 16 * R + a * 16 + n, d * 16 + g * 4, acc[a][d], m[a], l[a], d == 0 && g == 0);
     return;
   }
-  // The waves' parts of a row join over their common maximum.
-  __syncthreads();
-  float* part = reinterpret_cast<float*>(lds);           // [wave][row][D], chunks of 4 xored with the row
+  // The waves' parts of a row join over their common maximum, 16 rows at a time.
+  float* const part = reinterpret_cast<float*>(lds);     // [wave][row][D], chunks of 4 xored with the row
+  if (g == 0) {
+#pragma unroll
+    for (int a = 0; a < R; ++a) {
+      lds_ml[w][a * 16 + n][0] = m[a];
+      lds_ml[w][a * 16 + n][1] = l[a];
+    }
+  }
 #pragma unroll
   for (int a = 0; a < R; ++a) {
-    const uint32_t row = a * 16 + n;
-    if (g == 0) {
-      lds_ml[w][row][0] = m[a];
-      lds_ml[w][row][1] = l[a];
-    }
+    if (row0 + a * 16 >= rows) break;
+    __syncthreads();
 #pragma unroll
     for (int d = 0; d < kDT; ++d)
-      *reinterpret_cast<f32x4*>(part + (w * kTileRows + row) * D + ((d * 4 + g) ^ n) * 4) = acc[a][d];
-  }
-  __syncthreads();
-  for (uint32_t e = threadIdx.x; e < kTileRows * (D / 4); e += kThreads) {
-    const uint32_t row = e / (D / 4), c = e % (D / 4);
-    float top = -INFINITY;
+      *reinterpret_cast<f32x4*>(part + (w * 16 + n) * D + ((d * 4 + g) ^ n) * 4) = acc[a][d];
+    __syncthreads();
+#pragma unroll 1
+    for (uint32_t e = threadIdx.x; e < 16 * (D / 4); e += kThreads) {
+      const uint32_t row = e / (D / 4), c = e % (D / 4);
+      float top = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) top = fmaxf(top, lds_ml[v][row][0]);
-    const float from = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int v = 0; v < kWaves; ++v) top = fmaxf(top, lds_ml[v][a * 16 + row][0]);
+      const float base_m = top == -INFINITY ? 0.f : top;
+      float sum = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) {
-      const float weight = exp2_of(lds_ml[v][row][0] - from);
-      sum += weight * lds_ml[v][row][1];
-      o += weight * *reinterpret_cast<const f32x4*>(part + (v * kTileRows + row) * D + (c ^ (row & 15u)) * 4);
+      for (int v = 0; v < kWaves; ++v) {
+        const float weight = exp2_of(lds_ml[v][a * 16 + row][0] - base_m);
+        sum += weight * lds_ml[v][a * 16 + row][1];
+        o += weight * *reinterpret_cast<const f32x4*>(part + (v * 16 + row) * D + (c ^ row) * 4);
+      }
+      write(a * 16 + row, c * 4, o, top, sum, c == 0);
     }
-    write(row, c * 4, o, top, sum, c == 0);
   }
 }
 
-// The kernel for a head_dim; tile_rows 16 or 32 (the waves split the tokens), 64
-// or 128 (the waves split the rows).  One translation unit each.
+// Rows that a workgroup takes, of `rows` that a request has for one KV head: up to 32
+// the waves split the tokens, past that the rows.  (48 or 64 rows with the tokens
+// split fill 256 registers and spill: MI355X, 36 rows over a 4-bit cache, 48 us
+// either way.)
+inline uint32_t tile_rows_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+// The kernel for a head_dim and those rows.  One translation unit each.
 const void* attention_kernel_d64(int type, int format, uint32_t tile_rows);
 const void* attention_kernel_d128(int type, int format, uint32_t tile_rows);
 const void* attention_kernel_d256(int type, int format, uint32_t tile_rows);

@@ -1,7 +1,6 @@
 // Attention over a paged cache: how a call is cut up, the kernel that joins the
 // parts, and the entry points.  The attention itself: attention.h.
 #include "attention.h"
-#include <stdlib.h>
 
 namespace pace_kv {
 namespace {
@@ -105,24 +104,29 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(const AttnParams p) {
 // How a call is cut up.
 struct Split {
   uint32_t tile_rows, row_tiles, chunk_pages, items;
-  bool by_rows;
   int64_t part_rows() const { return static_cast<int64_t>(items) * row_tiles * tile_rows; }  // times the KV heads
 };
 
-constexpr int64_t kTargetGroups = 1024;  // workgroups that a long context is split over
-constexpr int64_t kMinChunkTokens = 256;
+// Workgroups that a call's contexts are split over: about what the CUs hold at once
+// (three, or of 128 rows two, each); more pay for their starts and for joining
+// their parts.  MI355X, kernel and joining, at 512, 768 and 1024 workgroups:
+//   a decode step of 256 ragged requests    204, 204, 205 us
+//   12 rows over 32768 tokens               101,  99, 105
+//   36 rows over 16 ragged 4-bit contexts    63,  63,  53 (rounds of unequal length)
+//   504 rows over 8 x 4096 8-bit tokens     130, 193, 143
+constexpr int64_t target_groups(uint32_t tile_rows) { return tile_rows <= 32 ? 768 : tile_rows == 64 ? 1024 : 512; }
+// A chunk is at least one step of a workgroup that splits the tokens.
+constexpr int64_t kMinChunkTokens = 128;
 
 Split split_of(int64_t batch, int64_t heads, int64_t group, int64_t max_q, int64_t num_indices, int64_t page_size) {
   Split s = {};
   const int64_t rows = max_q * group;
-  s.by_rows = rows > 32;
-  s.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+  s.tile_rows = tile_rows_of(rows);
   s.row_tiles = static_cast<uint32_t>((rows + s.tile_rows - 1) / s.tile_rows);
   const int64_t units = heads * s.row_tiles;
-  static const int64_t T = getenv("PK_T") ? atoi(getenv("PK_T")) : kTargetGroups, TR = getenv("PK_TR") ? atoi(getenv("PK_TR")) : kTargetGroups, MM = getenv("PK_M") ? atoi(getenv("PK_M")) : kMinChunkTokens;
-  const int64_t tgt = s.by_rows ? TR : T;
-  int64_t chunk = (num_indices * units + tgt - 1) / tgt;
-  const int64_t least = (MM + page_size - 1) / page_size;
+  const int64_t target = target_groups(s.tile_rows);
+  int64_t chunk = (num_indices * units + target - 1) / target;
+  const int64_t least = (kMinChunkTokens + page_size - 1) / page_size;
   if (chunk < least) chunk = least;
   if (chunk > num_indices) chunk = num_indices;
   if (chunk < 1) chunk = 1;
