@@ -224,11 +224,12 @@ __device__ __forceinline__ bool odd_word(uint32_t w) {
 }
 
 // Waves per SIMD that the registers are held to.  Two workgroups a CU fit the
-// accumulators and loads of 32 rows of 128; a decode step over a quantised cache
-// leaves room for a third, whose loads in flight count.
+// accumulators and loads of 32 rows of 128 (and of 16 rows of 256, with a few spills
+// outside the loops: MI355X, 24 rows over 8 x 4096 bf16 tokens, 93 us against 114
+// with one); a decode step over a quantised cache leaves room for a third, whose
+// loads in flight count.
 constexpr int min_waves(int D, int format, int R, int WR) {
-  if (D == 256) return R == 2 || format == PACE_KV_PLAIN ? 1 : 2;
-  return R == 1 && WR == 1 && format != PACE_KV_PLAIN ? 3 : 2;
+  return D != 256 && R == 1 && WR == 1 && format != PACE_KV_PLAIN ? 3 : 2;
 }
 
 // TYPE: of queries and output, and what a quantised cache is expanded to.
@@ -710,8 +711,13 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
 // Rows that a workgroup takes, of `rows` that a request has for one KV head: up to 32
 // the waves split the tokens, past that the rows.  (48 or 64 rows with the tokens
 // split fill 256 registers and spill: MI355X, 36 rows over a 4-bit cache, 48 us
-// either way.)
-inline uint32_t tile_rows_of(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+// either way.)  With head_dim 256 a wave has registers for 16 rows: 320 rows over 8 x
+// 4096 8-bit tokens 235 us, 561 with 32.
+inline uint32_t tile_rows_of(int head_dim, int64_t rows) {
+  if (rows <= 16) return 16;
+  if (head_dim == 256) return 64;
+  return rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
+}
 
 // The kernel for a head_dim and those rows.  One translation unit each.
 const void* attention_kernel_d64(int type, int format, uint32_t tile_rows);
@@ -720,12 +726,12 @@ const void* attention_kernel_d256(int type, int format, uint32_t tile_rows);
 
 template <int D, int TYPE, int FORMAT>
 const void* pick_rows(uint32_t tile_rows) {
-  switch (tile_rows) {
-    case 16: return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 1, 1>);
-    case 32: return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 2, 1>);
-    case 64: return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 1, 4>);
-    default: return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 2, 4>);
+  if (tile_rows == 16) return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 1, 1>);
+  if constexpr (D != 256) {
+    if (tile_rows == 32) return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 2, 1>);
+    if (tile_rows == 128) return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 2, 4>);
   }
+  return reinterpret_cast<const void*>(&attention_kernel<D, TYPE, FORMAT, 1, 4>);
 }
 
 template <int D, int TYPE>

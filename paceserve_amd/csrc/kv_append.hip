@@ -55,6 +55,10 @@ constexpr int64_t kMaxGroupsPerLaunch = int64_t(1) << 25;
 // 2.4 us plain, 2.6 nontemporal; 1 MiB the same either way; 2 MiB 3.8 against
 // 4.05 and 32 MiB 24.0 against 23.1.
 constexpr int64_t kCachedLoadBytes = int64_t(1) << 20;
+// Quantising appends of more key bytes than this stream: rows loaded, elements
+// stored nontemporally.  Measured on MI355X, 8-bit elements: 20 MiB of keys 12.0 us
+// plain, 13.6 streamed; 64 MiB 39.2 against 37.2.
+constexpr int64_t kStreamBytes = int64_t(32) << 20;
 // Blocks of 64 append_indptr entries that one round of the search loads.
 constexpr int kSearchBlocks = 4;
 // Most entries that a wave of several requests hands round one by one.
@@ -282,7 +286,10 @@ __global__ __launch_bounds__(kThreads) void append_kernel(const AppendParams p) 
 // The same append into a quantised cache (format: mx.h): a lane carries eight
 // elements of the key row and the same eight of the value row, and four lanes
 // settle a block's scale between them.  p.row_bytes counts elements here.
-template <bool FUSED, bool UNIFORM, int TYPE, int FORMAT>
+// Bound as the append above is.  MI355X, rows of 8 x 128 bfloat16 to 8 bits: 64
+// tokens 2.7 us, 10094 tokens 12.0 us (5.2 TB/s); 8190 rows of 32 x 128 float16
+// 37.2 us (5.5 TB/s).
+template <bool FUSED, bool UNIFORM, int TYPE, int FORMAT, bool STREAM>
 __global__ __launch_bounds__(kThreads) void append_mx_kernel(const AppendParams p) {
   uint32_t i, vec, first_i, last_i;
   bool live = true;
@@ -306,8 +313,8 @@ __global__ __launch_bounds__(kThreads) void append_mx_kernel(const AppendParams 
     __builtin_amdgcn_sched_barrier(0);
   }
   const int64_t at = static_cast<int64_t>(i) * p.token_stride + vec * (kLaneElems * elem_bytes(TYPE));
-  const Run<TYPE> k = load_run<TYPE>(p.key + at);
-  const Run<TYPE> v = load_run<TYPE>(p.value + at);
+  const Run<TYPE> k = load_run<TYPE, STREAM>(p.key + at);
+  const Run<TYPE> v = load_run<TYPE, STREAM>(p.value + at);
   __builtin_amdgcn_sched_barrier(0);
   if (UNIFORM) f = first_round<FUSED, true>(p, i);
   uint32_t page = 0, slot = 0;
@@ -320,8 +327,8 @@ __global__ __launch_bounds__(kThreads) void append_mx_kernel(const AppendParams 
   const int64_t e = static_cast<int64_t>(slot) * p.row_bytes + vec * kLaneElems;
   char* data = p.cache + 2 * half * page + e * mx_bits(FORMAT) / 8;
   char* scale = p.cache + 2 * half * page + bytes + e / kMxBlock;
-  store_run<TYPE, FORMAT>(k, kb, data, scale);
-  store_run<TYPE, FORMAT>(v, vb, data + half, scale + half);
+  store_run<TYPE, FORMAT, STREAM>(k, kb, data, scale);
+  store_run<TYPE, FORMAT, STREAM>(v, vb, data + half, scale + half);
 }
 
 // Sequence length of each request, in 32-bit arithmetic that wraps as torch's
@@ -437,24 +444,29 @@ int launch_append(AppendParams& p, int64_t nnz, int batch_size, int64_t num_page
   return PACE_KV_OK;
 }
 
-template <bool FUSED, int TYPE, int FORMAT>
+template <bool FUSED, int TYPE, int FORMAT, bool STREAM>
 const void* mx_kernel_of(bool uniform) {
-  return uniform ? reinterpret_cast<const void*>(&append_mx_kernel<FUSED, true, TYPE, FORMAT>)
-                 : reinterpret_cast<const void*>(&append_mx_kernel<FUSED, false, TYPE, FORMAT>);
+  return uniform ? reinterpret_cast<const void*>(&append_mx_kernel<FUSED, true, TYPE, FORMAT, STREAM>)
+                 : reinterpret_cast<const void*>(&append_mx_kernel<FUSED, false, TYPE, FORMAT, STREAM>);
+}
+
+template <bool FUSED, int TYPE, int FORMAT>
+const void* mx_kernel_of(bool uniform, bool stream) {
+  return stream ? mx_kernel_of<FUSED, TYPE, FORMAT, true>(uniform) : mx_kernel_of<FUSED, TYPE, FORMAT, false>(uniform);
 }
 
 template <bool FUSED, int TYPE>
-const void* mx_kernel_of(int format, bool uniform) {
-  return format == PACE_KV_MXFP8 ? mx_kernel_of<FUSED, TYPE, PACE_KV_MXFP8>(uniform)
-                                 : mx_kernel_of<FUSED, TYPE, PACE_KV_MXFP4>(uniform);
+const void* mx_kernel_of(int format, bool uniform, bool stream) {
+  return format == PACE_KV_MXFP8 ? mx_kernel_of<FUSED, TYPE, PACE_KV_MXFP8>(uniform, stream)
+                                 : mx_kernel_of<FUSED, TYPE, PACE_KV_MXFP4>(uniform, stream);
 }
 
 template <bool FUSED>
-const void* pick_mx_kernel(int type, int format, bool uniform) {
+const void* pick_mx_kernel(int type, int format, bool uniform, bool stream) {
   switch (type) {
-    case PACE_KV_BF16: return mx_kernel_of<FUSED, PACE_KV_BF16>(format, uniform);
-    case PACE_KV_FP16: return mx_kernel_of<FUSED, PACE_KV_FP16>(format, uniform);
-    default: return mx_kernel_of<FUSED, PACE_KV_FP32>(format, uniform);
+    case PACE_KV_BF16: return mx_kernel_of<FUSED, PACE_KV_BF16>(format, uniform, stream);
+    case PACE_KV_FP16: return mx_kernel_of<FUSED, PACE_KV_FP16>(format, uniform, stream);
+    default: return mx_kernel_of<FUSED, PACE_KV_FP32>(format, uniform, stream);
   }
 }
 
@@ -499,7 +511,9 @@ int launch_append_mx(AppendParams& p, int64_t nnz, int batch_size, int64_t num_p
   const int64_t waves_per_row = (row_runs + kThreads - 1) / kThreads;
   p.row_div = static_cast<uint32_t>(uniform ? waves_per_row : row_runs);
   p.by_row = fast_div(p.row_div);
-  const void* fn = fused ? pick_mx_kernel<true>(type, format, uniform) : pick_mx_kernel<false>(type, format, uniform);
+  const bool streamed = nnz * row_bytes > kStreamBytes;
+  const void* fn = fused ? pick_mx_kernel<true>(type, format, uniform, streamed)
+                         : pick_mx_kernel<false>(type, format, uniform, streamed);
   const int64_t max_tokens = kMaxGroupsPerLaunch / waves_per_row;
   if (max_tokens < 1) return fail(PACE_KV_ERANGE, "append_mx: row too large (%lld)", (long long)row_elems);
   for (int64_t t0 = 0; t0 < nnz; t0 += max_tokens) {

@@ -115,20 +115,23 @@ struct Split {
 //   36 rows over 16 ragged 4-bit contexts    63,  63,  53 (rounds of unequal length)
 //   504 rows over 8 x 4096 8-bit tokens     130, 193, 143
 constexpr int64_t target_groups(uint32_t tile_rows) { return tile_rows <= 32 ? 768 : tile_rows == 64 ? 1024 : 512; }
-// A chunk is at least one step of a workgroup that splits the tokens.
-constexpr int64_t kMinChunkTokens = 128;
+// Tokens that a chunk has at least: four steps of a workgroup that splits the tokens,
+// two of one that splits the rows, whose steps are longer.  MI355X, 4 rows over 512
+// tokens: 13 us in one launch, 7 + 4 in two, which take the host 3 us more.
+constexpr int64_t min_chunk_tokens(uint32_t tile_rows) { return tile_rows <= 32 ? 512 : 128; }
 
-Split split_of(int64_t batch, int64_t heads, int64_t group, int64_t max_q, int64_t num_indices, int64_t page_size) {
+Split split_of(int64_t batch, int64_t heads, int64_t group, int head_dim, int64_t max_q, int64_t num_indices,
+               int64_t page_size) {
   Split s = {};
   const int64_t rows = max_q * group;
-  s.tile_rows = tile_rows_of(rows);
+  s.tile_rows = tile_rows_of(head_dim, rows);
   s.row_tiles = static_cast<uint32_t>((rows + s.tile_rows - 1) / s.tile_rows);
   const int64_t units = heads * s.row_tiles;
   const int64_t target = target_groups(s.tile_rows);
   int64_t chunk = (num_indices * units + target - 1) / target;
-  const int64_t least = (kMinChunkTokens + page_size - 1) / page_size;
+  const int64_t least = (min_chunk_tokens(s.tile_rows) + page_size - 1) / page_size;
   if (chunk < least) chunk = least;
-  if (chunk > num_indices) chunk = num_indices;
+  if (num_indices <= least + least / 2) chunk = num_indices;  // no short second chunk
   if (chunk < 1) chunk = 1;
   s.chunk_pages = static_cast<uint32_t>(chunk);
   s.items = static_cast<uint32_t>(num_indices / chunk + batch);
@@ -159,7 +162,7 @@ int check_sizes(int batch_size, int num_kv_heads, int group, int head_dim, int m
   const int64_t rows = static_cast<int64_t>(max_q_len) * group;
   if (num_indices * page_size > INT32_MAX / 2 || rows > INT32_MAX / 2)
     return fail(PACE_KV_ERANGE, "attention: more than 2^30 tokens or query rows");
-  const Split s = split_of(batch_size, num_kv_heads, group, max_q_len, num_indices, page_size);
+  const Split s = split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size);
   if ((static_cast<int64_t>(s.items) + kXcds) * num_kv_heads * s.row_tiles >= (int64_t(1) << 24))
     return fail(PACE_KV_ERANGE, "attention: too many requests, heads or query rows for one call");
   return PACE_KV_OK;
@@ -180,7 +183,7 @@ int pace_kv_attention_workspace(int batch_size, int num_kv_heads, int group, int
   using namespace pace_kv;
   if (!bytes) return fail(PACE_KV_EINVAL, "attention: NULL argument");
   PACE_KV_TRY(check_sizes(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size));
-  *bytes = workspace_bytes(split_of(batch_size, num_kv_heads, group, max_q_len, num_indices, page_size), num_kv_heads,
+  *bytes = workspace_bytes(split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size), num_kv_heads,
                            head_dim, num_indices);
   return PACE_KV_OK;
 }
@@ -223,7 +226,7 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   if (half_bytes % 16) return fail(PACE_KV_EINVAL, "attention: half a page must be a multiple of 16 bytes");
   if (num_pages * 2 * half_bytes / 16 >= UINT32_MAX)
     return fail(PACE_KV_ERANGE, "attention: a layer's cache must be smaller than 64 GiB");
-  const Split s = split_of(batch_size, num_kv_heads, group, max_q_len, num_indices, page_size);
+  const Split s = split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size);
   const int64_t need = workspace_bytes(s, num_kv_heads, head_dim, num_indices);
   if (need > 0 && (!workspace || workspace_size < need || reinterpret_cast<uintptr_t>(workspace) & 15u))
     return fail(PACE_KV_EINVAL, "attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);

@@ -56,12 +56,22 @@ struct Run {
   u32x4 v[kVecs];
 };
 
-template <int TYPE>
+// STREAM: nontemporally.
+template <int TYPE, bool STREAM>
 __device__ __forceinline__ Run<TYPE> load_run(const char* s) {
   Run<TYPE> r;
 #pragma unroll
-  for (int k = 0; k < Run<TYPE>::kVecs; ++k) r.v[k] = reinterpret_cast<const u32x4*>(s)[k];
+  for (int k = 0; k < Run<TYPE>::kVecs; ++k) {
+    const u32x4* const at = reinterpret_cast<const u32x4*>(s) + k;
+    r.v[k] = STREAM ? __builtin_nontemporal_load(at) : *at;
+  }
   return r;
+}
+
+template <bool STREAM, class T>
+__device__ __forceinline__ void put(T* to, T x) {
+  if constexpr (STREAM) __builtin_nontemporal_store(x, to);
+  else *to = x;
 }
 
 // Largest magnitude of the lane's block as float32 bits; infinities and NaN
@@ -134,7 +144,7 @@ __device__ __forceinline__ uint32_t pair_down(uint32_t to, const Run<TYPE>& r, i
 
 // Stores a lane's run as elements at `data`, its place among the half page's
 // elements, and the block's scale byte at `scale` (from the block's first lane).
-template <int TYPE, int FORMAT>
+template <int TYPE, int FORMAT, bool STREAM>
 __device__ __forceinline__ void store_run(const Run<TYPE>& r, uint32_t byte, char* data, char* scale) {
   const float s = scale_of(byte);
   const uint32_t keep = byte == 255u ? 0u : ~0u;
@@ -144,15 +154,14 @@ __device__ __forceinline__ void store_run(const Run<TYPE>& r, uint32_t byte, cha
     q[0] = pair_down<TYPE, FORMAT, 1>(q[0], r, 1, s);
     q[1] = pair_down<TYPE, FORMAT, 0>(q[1], r, 2, s);
     q[1] = pair_down<TYPE, FORMAT, 1>(q[1], r, 3, s);
-    q &= keep;
-    *reinterpret_cast<u32x2*>(data) = q;
+    put<STREAM>(reinterpret_cast<u32x2*>(data), q & keep);
   } else {
     uint32_t q = 0;
     q = pair_down<TYPE, FORMAT, 0>(q, r, 0, s);
     q = pair_down<TYPE, FORMAT, 1>(q, r, 1, s);
     q = pair_down<TYPE, FORMAT, 2>(q, r, 2, s);
     q = pair_down<TYPE, FORMAT, 3>(q, r, 3, s);
-    *reinterpret_cast<uint32_t*>(data) = q & keep;
+    put<STREAM>(reinterpret_cast<uint32_t*>(data), q & keep);
   }
   if (threadIdx.x % 4 == 0) *reinterpret_cast<uint8_t*>(scale) = static_cast<uint8_t>(byte);
 }

@@ -120,7 +120,7 @@ def paged_attention(q: torch.Tensor, paged_kv_cache: torch.Tensor, kv_indices: t
     if not math.isfinite(sm_scale) or not math.isfinite(logits_soft_cap) or logits_soft_cap < 0:
         raise ValueError("sm_scale must be finite, logits_soft_cap finite and >= 0")
     if out is None:
-        out = torch.empty((nnz, heads, D), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(2) != 1 \
             or out.stride(1) != D:
         raise ValueError("out must be like q, its rows contiguous [num_qo_heads, head_dim] blocks")
