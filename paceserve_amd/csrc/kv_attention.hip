@@ -62,9 +62,14 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(const AttnParams p) {
     o *= shrink;
     m = top;
     const uint32_t n = min(c_end - c0, 64u);
+    // Every lane takes part in every turn: a lane that had left would hand no weight
+    // to the others.
 #pragma unroll 8
-    for (uint32_t c = group; c < n; c += kGroups)
-      o += __shfl(weight, c) * *reinterpret_cast<const f32x4*>(p.part_o + (first + (c0 + c) * step) * D + col * 4);
+    for (uint32_t c = 0; c < n; c += kGroups) {
+      const float mine = __shfl(weight, c + group);      // 0 past the last chunk
+      if (c + group < n)
+        o += mine * *reinterpret_cast<const f32x4*>(p.part_o + (first + (c0 + c + group) * step) * D + col * 4);
+    }
   }
 #pragma unroll
   for (int k = kCols; k < 64; k *= 2)

@@ -388,3 +388,126 @@ def test_python_refusals(gpu):
     bad("is on cpu", tables=(t[0].cpu(), t[1], t[2]))
     empty = paged_attention(b.q[:0], b.cache, t[0][:0], i32([0], gpu), t[2][:0], i32([0], gpu), max_q_len=1)
     assert empty.shape == (0, 8, 128)
+
+
+def test_pages_of_one_and_three_tokens(gpu):
+    for P, D, fmt in ((1, 128, None), (3, 64, None), (1, 256, "mxfp8"), (16, 64, "mxfp4")):
+        b = Batch(gpu, [70, 1, 131], [3, 1, 2], H=2, G=2, D=D, P=P, fmt=fmt, seed=12)
+        out, lse = b.run()
+        torch.cuda.synchronize()
+        b.check(out, lse)
+
+
+@pytest.mark.parametrize("R", [256, 257, 700])
+def test_many_requests(gpu, R):
+    """More requests than one round of the search takes, some without tokens."""
+    rng = np.random.default_rng(R)
+    kv, new = rng.integers(1, 40, R), rng.integers(0, 3, R)
+    new = np.minimum(new, kv)
+    b = Batch(gpu, kv, new, H=1, G=2, D=64, seed=R)
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    b.check(out, lse)
+
+
+@pytest.mark.parametrize("G,T,n", [(1, 1, 40000), (2, 2, 36000), (12, 40, 3000)])
+def test_many_chunks(gpu, G, T, n):
+    """More chunks of a request than a wave weighs at once, and more rows than the
+    joining workgroups take one by one (12 * 40 * 8 heads)."""
+    b = Batch(gpu, [n, 100], [T, 1], H=8 if n == 3000 else 1, G=G, D=64, seed=n, tree=n == 3000)
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    b.check(out, lse)
+
+
+def test_fewer_tokens_than_queries(gpu):
+    """Queries whose own place lies before the first token see nothing."""
+    b = Batch(gpu, [2, 0, 30, 0], [5, 3, 2, 1], seed=13)
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    b.check(out, lse)
+    assert (out[:3] == 0).all() and (out[5:8] == 0).all() and torch.isneginf(lse[5:8]).all()
+    none = Batch(gpu, [0, 0], [1, 1], seed=13)             # no pages at all
+    out, lse = none.run()
+    assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+def test_requests_share_pages(gpu):
+    """Two requests whose tables name the same pages (a shared prefix), and a mask
+    with more words than the tokens need."""
+    b = Batch(gpu, [100, 90], [3, 4], seed=14, tree=True)
+    b.indices = b.indices.copy()
+    b.indices[b.indptr[1]:b.indptr[1] + 5] = b.indices[:5]
+    b.seen_rows[1] = np.concatenate([b.seen_rows[0][:80], b.seen_rows[1][80:]])
+    b.mask = np.concatenate([b.mask, np.full((7, 2), 2 ** 64 - 1, np.uint64)], 1)
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    b.check(out, lse)
+
+
+@pytest.mark.parametrize("fmt", [None, "mxfp8"])
+def test_offsets_past_32_bits(gpu, fmt):
+    """A layer's cache of more than 4 GiB, its last pages in use: appended to,
+    converted, attended to."""
+    H, D, P = 8, 128, 64
+    width = D if fmt is None else mx.row_width(D, fmt)
+    pages = (9 << 29) // (2 * P * H * width * (2 if fmt is None else 1)) + 8
+    b = Batch(gpu, [150, 70], [4, 2], H=H, G=2, D=D, P=P, fmt=fmt, seed=15)
+    cache = torch.zeros((pages, 2, P, H, width), dtype=b.cache.dtype, device=gpu)
+    assert cache.numel() * cache.element_size() > 1 << 32
+    move = pages - b.num_pages
+    cache[move:] = b.cache
+    small, b.cache = b.cache, cache
+    b.indices = b.indices + move
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    b.check(out, lse)
+    if fmt is not None:
+        plain = [torch.zeros((b.num_pages, 2, P, H, D), dtype=BF16, device=gpu) for _ in range(2)]
+        every = list(range(b.num_pages))
+        mx.dequantize_pages([cache], [move + i for i in every], plain[:1], every)
+        mx.dequantize_pages([small], every, plain[1:], every)
+        assert torch.equal(plain[0].view(torch.int16), plain[1].view(torch.int16))
+        mx.quantize_pages(plain[:1], [2], [cache], [pages - 1])
+        mx.quantize_pages(plain[:1], [2], [small], [b.num_pages - 1])
+        rows = torch.randn(3, H, D, device=gpu, dtype=BF16)
+        for c, at in ((cache, pages - 2), (small, b.num_pages - 2)):
+            mx.append_paged_kv_cache_mx_indptr(rows, rows, i32([0, 3], gpu), c, i32([at], gpu), i32([0, 1], gpu),
+                                               i32([7], gpu))
+        assert torch.equal(cache[move:], small) and not cache[:move].any()
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_batches(gpu, seed):
+    rng = np.random.default_rng(1000 + seed)
+    R = int(rng.integers(1, 9))
+    D = int(rng.choice([64, 128, 256]))
+    fmt = [None, "mxfp8", "mxfp4"][int(rng.integers(3))]
+    kv = rng.integers(0, int(rng.choice([20, 200, 2500])) + 1, R)
+    new = np.minimum(rng.integers(0, int(rng.choice([1, 6, 80])) + 1, R), np.maximum(kv, 0))
+    new[0] = max(new[0], 1)
+    kv[0] = max(kv[0], 1)
+    case = dict(H=int(rng.integers(1, 4)), G=int(rng.choice([1, 2, 3, 5, 8])), D=D, P=int(rng.choice([16, 16, 32, 48])),
+                dtype=[BF16, FP16][int(rng.integers(2))], fmt=fmt, tree=bool(rng.integers(2)), seed=seed)
+    print(f"random batch {kv.tolist()} {new.tolist()} {case}", flush=True)
+    b = Batch(gpu, kv, new, **case)
+    cap = float(rng.choice([0.0, 15.0]))
+    out, lse = b.run(cap)
+    torch.cuda.synchronize()
+    b.check(out, lse, cap)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("chunks", [2, 3, 5, 17, 18, 63, 64, 65, 66, 67, 69, 71, 127, 130])
+def test_every_count_of_chunks(gpu, D, chunks):
+    """A long context over few pages, named again and again: as many chunks of 512
+    tokens, the last one short, as the joining waves may get, alone and split."""
+    b = Batch(gpu, [8 * 16], [1], H=1, G=1, D=D, seed=chunks)
+    n = 512 * (chunks - 1) + 17
+    table = np.arange(-(-n // 16)) % 8
+    rows = b.seen_rows[0].reshape(8, 16, 2, 1, D)
+    b.seen_rows[0] = np.ascontiguousarray(rows[table].reshape(-1, 2, 1, D)[:n])
+    b.indices, b.indptr, b.last = b.indices[table], np.array([0, len(table)]), np.array([(n - 1) % 16 + 1])
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    b.check(out, lse)
