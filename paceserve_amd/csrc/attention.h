@@ -18,11 +18,12 @@
 // type for the product (within 2^-8 of each weight in bfloat16, 2^-11 in float16,
 // errors that average out over the row); l sums the unrounded weights.
 //
-// Work split: a request's pages in chunks of C; chunk k of request b is work
-// item floor(kv_indptr[b] / C) + b + k, which a workgroup inverts by counting
-// the requests that start at or before its item, so a launch needs no plan and
-// a captured one follows the tables.  A request of one chunk is written
-// directly; the others leave (o, m, l) in a workspace for combine_kernel.
+// Work split: a request's pages in chunks of C, the chunks of all requests numbered
+// through.  A workgroup finds the request of its number in the tables themselves,
+// so a launch needs no plan and a captured one follows them; the grid has room for
+// the most chunks there can be, floor(pages / C) + requests.  A request of one chunk
+// is written directly; the others leave (o, m, l) in a workspace for
+// combine_kernel.
 #pragma once
 
 #include <type_traits>
@@ -90,16 +91,12 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 
 // A request and the part of it that a work item covers.
 struct Request {
-  uint32_t b, chunk, chunks;
+  uint32_t chunk, chunks;
   int32_t first_page;          // in kv_indices
   uint32_t pages;
   uint32_t kv_len;
   uint32_t q0, q_len;
 };
-
-__device__ __forceinline__ uint32_t item_of(const AttnParams& p, uint32_t b, int32_t first) {
-  return over(p.by_chunk, static_cast<uint32_t>(max(first, 0))) + b;
-}
 
 // What the tables say of a request.
 struct Tables {
@@ -120,56 +117,86 @@ __device__ __forceinline__ Tables tables_of(const AttnParams& p, uint32_t b) {
   return t;
 }
 
+__device__ __forceinline__ uint32_t pages_of(const AttnParams& p, const Tables& t) {
+  const uint32_t first = static_cast<uint32_t>(max(t.k0, 0));
+  const uint32_t n = t.k1 > t.k0 && t.k1 > 0 ? static_cast<uint32_t>(t.k1) - first : 0u;
+  return min(n, p.num_indices - min(first, p.num_indices));
+}
+
+// Chunks of a request of n pages; one without pages still has its rows to write.
+__device__ __forceinline__ uint32_t chunks_of(const AttnParams& p, uint32_t n) {
+  const uint32_t c = over(p.by_chunk, n);
+  return max(c * p.chunk_pages < n ? c + 1 : c, 1u);
+}
+
 // The sizes of request b; false where its queries are not among nnz or exceed
 // max_q.
-__device__ __forceinline__ bool request_of(const AttnParams& p, uint32_t b, const Tables& t, Request* r) {
-  const int32_t k0 = max(t.k0, 0);
-  r->b = b;
-  r->first_page = k0;
-  r->pages = t.k1 > k0 ? static_cast<uint32_t>(t.k1 - k0) : 0u;
-  r->pages = min(r->pages, p.num_indices - min(static_cast<uint32_t>(k0), p.num_indices));
+__device__ __forceinline__ bool request_of(const AttnParams& p, const Tables& t, Request* r) {
+  r->first_page = max(t.k0, 0);
+  r->pages = pages_of(p, t);
   const int64_t most = static_cast<int64_t>(r->pages) * p.page_size;
   const int64_t len = (most > p.page_size ? most - p.page_size : 0) + t.last;
   r->kv_len = static_cast<uint32_t>(min(max(len, int64_t(0)), most));
-  const uint32_t n = over(p.by_chunk, r->pages);
-  r->chunks = max(n * p.chunk_pages < r->pages ? n + 1 : n, 1u);
+  r->chunks = chunks_of(p, r->pages);
   r->q0 = static_cast<uint32_t>(t.a0);
   r->q_len = static_cast<uint32_t>(t.a1 - t.a0);
   return t.a0 >= 0 && t.a1 >= t.a0 && static_cast<uint32_t>(t.a1) <= p.nnz && r->q_len <= p.max_q;
 }
 
-// The last request whose key is at most x, keys not decreasing, and what the
-// tables say of it; false if there is none.  The wave looks at 256 requests a
-// round, and holds what it loads of each, so up to 256 cost one load latency.
+// The last request whose key is at most x, keys not decreasing: what the tables say
+// of it, and its first work item (the chunks of the requests before it); false if
+// there is none.  The wave looks at 256 requests a round, four neighbours to a
+// lane, and holds what it loads of each, so up to 256 cost one load latency.
 template <class Key>
-__device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Key key, uint32_t* b, Tables* t) {
+__device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Key key, Tables* t, uint32_t* first_item) {
+  const uint32_t lane = threadIdx.x % 64;
   bool found = false;
+  uint32_t before = 0;                                   // chunks of the rounds before
   for (uint32_t e0 = 0; e0 < p.batch; e0 += 256) {
     Tables mine[4] = {};
-    uint64_t pass[4];
+    uint32_t start[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t e = e0 + k * 64 + threadIdx.x % 64;
-      if (e < p.batch) mine[k] = tables_of(p, e);
+    for (uint32_t k = 0; k < 4; ++k)
+      if (e0 + lane * 4 + k < p.batch) mine[k] = tables_of(p, e0 + lane * 4 + k);
+    uint32_t sum = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      start[k] = sum;
+      if (e0 + lane * 4 + k < p.batch) sum += chunks_of(p, pages_of(p, mine[k]));
     }
+    uint32_t upto = sum;                                 // over the lanes up to this one
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t e = e0 + k * 64 + threadIdx.x % 64;
-      pass[k] = __ballot(e < p.batch && key(e, mine[k]) <= x);
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t left = __shfl_up(upto, d);
+      if (lane >= static_cast<uint32_t>(d)) upto += left;
     }
+    int best = -1;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (pass[k] == 0) continue;
-      const int at = 63 - __builtin_clzll(pass[k]);
+      start[k] += before + upto - sum;
+      if (e0 + lane * 4 + k < p.batch && key(mine[k], start[k]) <= x) best = k;
+    }
+    const uint64_t pass = __ballot(best >= 0);
+    if (pass != 0) {
       found = true;
-      *b = e0 + k * 64 + at;
-      t->k0 = __builtin_amdgcn_readlane(mine[k].k0, at);
-      t->k1 = __builtin_amdgcn_readlane(mine[k].k1, at);
-      t->last = __builtin_amdgcn_readlane(mine[k].last, at);
-      t->a0 = __builtin_amdgcn_readlane(mine[k].a0, at);
-      t->a1 = __builtin_amdgcn_readlane(mine[k].a1, at);
+      const int at = 63 - __builtin_clzll(pass);
+      Tables of = mine[0];
+      uint32_t item = start[0];
+#pragma unroll
+      for (int k = 1; k < 4; ++k)
+        if (best == k) {
+          of = mine[k];
+          item = start[k];
+        }
+      t->k0 = __builtin_amdgcn_readlane(of.k0, at);
+      t->k1 = __builtin_amdgcn_readlane(of.k1, at);
+      t->last = __builtin_amdgcn_readlane(of.last, at);
+      t->a0 = __builtin_amdgcn_readlane(of.a0, at);
+      t->a1 = __builtin_amdgcn_readlane(of.a1, at);
+      *first_item = __builtin_amdgcn_readlane(item, at);
     }
-    if (pass[3] != ~0ull) break;
+    if (__builtin_amdgcn_readlane(best, 63) != 3) break;
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
   return found;
 }
@@ -269,12 +296,12 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   const uint32_t item = nth * kXcds + blockIdx.x % kXcds;
   if (item >= p.items) return;
   const uint32_t in_unit = at - nth * unit, head = over(p.by_tiles, in_unit), tile = in_unit - head * p.row_tiles;
-  uint32_t b;
+  uint32_t first_item;
   Tables tables;
-  if (!find_request(p, item, [&](uint32_t e, const Tables& t) { return item_of(p, e, t.k0); }, &b, &tables)) return;
+  if (!find_request(p, item, [](const Tables&, uint32_t start) { return start; }, &tables, &first_item)) return;
   Request r;
-  const bool valid_request = request_of(p, b, tables, &r);
-  r.chunk = item - item_of(p, r.b, r.first_page);
+  const bool valid_request = request_of(p, tables, &r);
+  r.chunk = item - first_item;
   if (r.chunk >= r.chunks) return;
   if (!valid_request) {
     if (r.chunk == 0 && in_unit == 0 && threadIdx.x == 0 && p.err != nullptr) atomicAdd(p.err, 1);
@@ -603,17 +630,10 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
       load_values();
       load_id(t0 + 2 * step);
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (decltype(full)::value) {
-        weigh(full, t0, 0, 0);
-        gather(full, 0);
-        weigh(full, t0 + 32, 32, 0);
-        gather(full, 32);
-      } else {
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          weigh(full, t0 + 32 * h, 32 * h, static_cast<uint32_t>(ok >> (32 * h)));
-          gather(full, 32 * h);
-        }
+      for (int h = 0; h < 2 && wave_row0 < rows; ++h) {  // a wave of padding only loads
+        weigh(full, t0 + 32 * h, 32 * h, static_cast<uint32_t>(ok >> (32 * h)));
+        gather(full, 32 * h);
       }
     }
     t0 += step;

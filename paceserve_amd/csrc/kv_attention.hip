@@ -19,21 +19,17 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(const AttnParams p) {
   const uint32_t row_id = WAVES == 1 ? blockIdx.x * kWaves + w : blockIdx.x;
   const uint32_t token = over(p.by_heads, row_id), qh = row_id - token * all_heads;
   if (token >= p.nnz) return;
-  uint32_t b = token;
   Tables tables;
-  if (p.qo_indptr == nullptr) {
-    if (b >= p.batch) return;
-    tables = tables_of(p, b);
-  } else if (!find_request(p, token, [](uint32_t, const Tables& t) { return static_cast<uint32_t>(max(t.a0, 0)); }, &b,
-                           &tables)) {
+  uint32_t first_item;
+  if (!find_request(p, token, [](const Tables& t, uint32_t) { return static_cast<uint32_t>(max(t.a0, 0)); }, &tables,
+                    &first_item))
     return;
-  }
   Request r;
-  if (!request_of(p, b, tables, &r) || token < r.q0 || token - r.q0 >= r.q_len || r.chunks == 1) return;
+  if (!request_of(p, tables, &r) || token < r.q0 || token - r.q0 >= r.q_len || r.chunks == 1) return;
   const uint32_t head = over(p.by_group, qh), row = (token - r.q0) * p.group + (qh - head * p.group);
   const uint32_t tile = row / p.tile_rows;
   const int64_t unit = static_cast<int64_t>(p.heads) * p.row_tiles;
-  const int64_t first = (static_cast<int64_t>(item_of(p, b, r.first_page)) * unit +
+  const int64_t first = (static_cast<int64_t>(first_item) * unit +
                          static_cast<int64_t>(head) * p.row_tiles + tile) * p.tile_rows + row % p.tile_rows;
   const int64_t step = unit * p.tile_rows;
   const uint32_t col = lane % kCols, group = lane / kCols;
