@@ -58,6 +58,7 @@ struct AttnParams {
   int32_t* err;
   uint32_t num_indices, batch, nnz, heads, group, num_pages, page_size, max_q, mask_words;
   uint32_t chunk_pages, items, row_tiles, tile_rows;
+  uint32_t join_rows;          // rows that a wave of the joining kernel takes
   uint32_t page16, half16, row16;  // page, half page and token row, in 16-byte units
   uint32_t scale_at, scale_row;    // scales within a half page, scale bytes of a token
   FastDiv by_page, by_chunk, by_group, by_unit, by_tiles, by_heads;
@@ -143,6 +144,18 @@ __device__ __forceinline__ bool request_of(const AttnParams& p, const Tables& t,
   return t.a0 >= 0 && t.a1 >= t.a0 && static_cast<uint32_t>(t.a1) <= p.nnz && r->q_len <= p.max_q;
 }
 
+// Sum over the lanes up to this one: within rows of 16 lanes by shifts, then each
+// row's total to the rows behind it.
+__device__ __forceinline__ uint32_t sum_upto(uint32_t x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
 // The last request whose key is at most x, keys not decreasing: what the tables say
 // of it, and its first work item (the chunks of the requests before it); false if
 // there is none.  The wave looks at 256 requests a round, four neighbours to a
@@ -164,12 +177,7 @@ __device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Ke
       start[k] = sum;
       if (e0 + lane * 4 + k < p.batch) sum += chunks_of(p, pages_of(p, mine[k]));
     }
-    uint32_t upto = sum;                                 // over the lanes up to this one
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const uint32_t left = __shfl_up(upto, d);
-      if (lane >= static_cast<uint32_t>(d)) upto += left;
-    }
+    const uint32_t upto = sum_upto(sum);                 // over the lanes up to this one
     int best = -1;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -275,9 +283,11 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   constexpr uint32_t kLoads = (kLoadRows * kPieces + 63) / 64;
   constexpr uint32_t kLdsRows = WR == 1 ? 128 : 64;
   constexpr int kDT = D / 16, kKS = D / 32;
-  // Rows that no other workgroup reads are loaded nontemporally.  MI355X, reading
-  // 2 GiB of pages in this pattern: 6.3 to 6.8 TB/s against 5.7 to 6.1.
-  constexpr bool kReadOnce = WR == 1 || R == 1;
+  // Rows that no other workgroup reads are loaded nontemporally, unless two heads
+  // share a 128-byte line.  MI355X, reading 2 GiB of pages of 8 heads in this pattern:
+  // 256-byte rows 6.4 TB/s against 5.8, 128-byte ones 6.3 against 5.6, 64-byte ones
+  // 4.8 against 5.9 (and 3.5 with the heads of a page on different XCDs).
+  constexpr bool kReadOnce = (WR == 1 || R == 1) && D * kBits / 8 >= 128;
 
   constexpr uint32_t kRowBytes = WR == 1 ? kStride<D> : 2 * kStride<D>;
   constexpr uint32_t kJoinBytes = WR == 1 ? kWaves * 16 * D * 4 : 0;
