@@ -58,10 +58,10 @@ struct AttnParams {
   int32_t* err;
   uint32_t num_indices, batch, nnz, heads, group, num_pages, page_size, max_q, mask_words;
   uint32_t chunk_pages, items, row_tiles, tile_rows;
-  uint32_t join_rows;          // rows that a wave of the joining kernel takes
+  uint32_t join_turns, token_waves;  // of the joining kernel
   uint32_t page16, half16, row16;  // page, half page and token row, in 16-byte units
   uint32_t scale_at, scale_row;    // scales within a half page, scale bytes of a token
-  FastDiv by_page, by_chunk, by_group, by_unit, by_tiles, by_heads;
+  FastDiv by_page, by_chunk, by_group, by_unit, by_tiles, by_heads, by_token_waves;
   float scale_log2;            // scale * log2(e); with a cap: scale / cap * 2 * log2(e)
   float cap_log2;              // cap * log2(e), or 0
 };

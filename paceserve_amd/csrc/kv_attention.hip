@@ -7,26 +7,62 @@
 namespace pace_kv {
 namespace {
 
-// Joins the chunks of one row (query head qh of a token) of request r.  WAVES waves
-// take a row; within a wave D / 4 lanes take four columns each of a chunk, and the
-// wave as many chunks at a time as fit.  The chunks' weights come first, 64 at a
-// time, so that the loads of their outputs do not wait for one another.
-template <int D, int TYPE, int WAVES>
-__device__ __forceinline__ void combine_row(const AttnParams& p, const Request& r, uint32_t first_item, uint32_t token,
-                                            uint32_t qh, uint32_t lane, uint32_t w) {
-  constexpr uint32_t kCols = D / 4, kGroups = 64 / kCols;
-  __shared__ f32x4 lds_o[WAVES][kCols];
-  __shared__ float lds_m[WAVES], lds_l[WAVES];
+// A row (query head qh of a token) whose chunks are joined: where its parts are.
+struct Parts {
+  int64_t first, step;
+  uint32_t chunks;
+};
+
+// The parts of rows of `token`; false where its request is not split.
+__device__ __forceinline__ bool parts_of(const AttnParams& p, uint32_t token, Request* r, uint32_t* first_item) {
+  Tables t;
+  return find_request(p, token, [](const Tables& x, uint32_t) { return static_cast<uint32_t>(max(x.a0, 0)); }, &t,
+                      first_item) &&
+         request_of(p, t, r) && token >= r->q0 && token - r->q0 < r->q_len && r->chunks > 1;
+}
+
+__device__ __forceinline__ Parts parts_of_row(const AttnParams& p, const Request& r, uint32_t first_item, uint32_t token,
+                                              uint32_t qh) {
   const uint32_t head = over(p.by_group, qh), row = (token - r.q0) * p.group + (qh - head * p.group);
   const uint32_t tile = row / p.tile_rows;
   const int64_t unit = static_cast<int64_t>(p.heads) * p.row_tiles;
-  const int64_t first = (static_cast<int64_t>(first_item) * unit +
-                         static_cast<int64_t>(head) * p.row_tiles + tile) * p.tile_rows + row % p.tile_rows;
-  const int64_t step = unit * p.tile_rows;
+  return {(static_cast<int64_t>(first_item) * unit + static_cast<int64_t>(head) * p.row_tiles + tile) * p.tile_rows +
+              row % p.tile_rows,
+          unit * p.tile_rows, r.chunks};
+}
+
+// Four columns of a row, of its weighted sum o and the sum l of weights over 2^m.
+template <int TYPE>
+__device__ __forceinline__ void write_row(const AttnParams& p, uint32_t token, uint32_t qh, int D, uint32_t col, f32x4 o,
+                                          float m, float l) {
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const u32x2 x = {pair_of<TYPE>(o[0] * inv, o[1] * inv), pair_of<TYPE>(o[2] * inv, o[3] * inv)};
+  *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(token) * p.out_stride +
+                            (static_cast<int64_t>(qh) * D + col * 4) * 2) = x;
+  if (col == 0 && p.lse != nullptr)
+    p.lse[static_cast<int64_t>(token) * (p.heads * p.group) + qh] =
+        l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+}
+
+// Few rows of many chunks: a workgroup joins a row.  D / 4 lanes take four columns
+// each of a chunk, a wave as many chunks at a time as fit, and the waves a quarter of
+// the chunks each.  The chunks' weights come first, 64 at a time, so that the loads
+// of their outputs do not wait for one another.
+template <int D, int TYPE>
+__global__ __launch_bounds__(kThreads) void combine_few_kernel(const AttnParams p) {
+  constexpr uint32_t kCols = D / 4, kGroups = 64 / kCols;
+  __shared__ f32x4 lds_o[kWaves][kCols];
+  __shared__ float lds_m[kWaves], lds_l[kWaves];
+  const uint32_t lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t token = over(p.by_heads, blockIdx.x), qh = blockIdx.x - token * p.heads * p.group;
+  Request r;
+  uint32_t first_item;
+  if (!parts_of(p, token, &r, &first_item)) return;
+  const auto [first, step, chunks] = parts_of_row(p, r, first_item, token, qh);
   const uint32_t col = lane % kCols, group = lane / kCols;
   // The wave's part of the chunks.
-  const uint32_t per_wave = (r.chunks + WAVES - 1) / WAVES;
-  const uint32_t c_begin = WAVES == 1 ? 0 : w * per_wave, c_end = min(c_begin + per_wave, r.chunks);
+  const uint32_t per_wave = (chunks + kWaves - 1) / kWaves;
+  const uint32_t c_begin = w * per_wave, c_end = min(c_begin + per_wave, chunks);
   float m = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   for (uint32_t c0 = c_begin; c0 < c_end; c0 += 64) {
@@ -62,60 +98,62 @@ __device__ __forceinline__ void combine_row(const AttnParams& p, const Request& 
   for (int k = kCols; k < 64; k *= 2)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], k);
-  if constexpr (WAVES > 1) {
-    if (group == 0) lds_o[w][col] = o;
-    if (lane == 0) {
-      lds_m[w] = m;
-      lds_l[w] = l;
-    }
-    __syncthreads();
-    if (w != 0) return;
-    m = -INFINITY;
-#pragma unroll
-    for (int v = 0; v < WAVES; ++v) m = fmaxf(m, lds_m[v]);
-    const float from = m == -INFINITY ? 0.f : m;
-    l = 0.f;
-    o = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int v = 0; v < WAVES; ++v) {
-      const float weight = exp2_of(lds_m[v] - from);
-      l += weight * lds_l[v];
-      o += weight * lds_o[v][col];
-    }
+  if (group == 0) lds_o[w][col] = o;
+  if (lane == 0) {
+    lds_m[w] = m;
+    lds_l[w] = l;
   }
-  if (group != 0) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const u32x2 x = {pair_of<TYPE>(o[0] * inv, o[1] * inv), pair_of<TYPE>(o[2] * inv, o[3] * inv)};
-  *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(token) * p.out_stride +
-                            (static_cast<int64_t>(qh) * D + col * 4) * 2) = x;
-  if (col == 0 && p.lse != nullptr)
-    p.lse[static_cast<int64_t>(token) * (p.heads * p.group) + qh] =
-        l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+  __syncthreads();
+  if (w != 0) return;
+  m = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) m = fmaxf(m, lds_m[v]);
+  const float from = m == -INFINITY ? 0.f : m;
+  l = 0.f;
+  o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) {
+    const float weight = exp2_of(lds_m[v] - from);
+    l += weight * lds_l[v];
+    o += weight * lds_o[v][col];
+  }
+  if (group == 0) write_row<TYPE>(p, token, qh, D, col, o, m, l);
 }
 
-// Finding a token's request costs about as much as joining a row's chunks, so where
-// there are more rows than waves fit the GPU a wave takes p.join_rows neighbours and
-// searches once.  MI355X, 32256 rows of 8 requests: 23 us with a wave for each, 19
-// with four rows a wave; 2688 rows of 16: 6 and 16.
-template <int D, int TYPE, int WAVES>
-__global__ __launch_bounds__(kThreads) void combine_kernel(const AttnParams p) {
-  const uint32_t rows = WAVES == 1 ? p.join_rows : 1;
+// Many rows of few chunks: D / 4 lanes join a row by themselves, and a wave takes
+// p.join_turns times as many rows of a token as fit into it; finding the token's
+// request costs as much as joining a row.  MI355X, 32256 rows of two chunks: 13 us,
+// where a wave per row takes 23 and four rows a wave 19.
+template <int D, int TYPE>
+__global__ __launch_bounds__(kThreads) void combine_many_kernel(const AttnParams p) {
+  constexpr uint32_t kCols = D / 4, kGroups = 64 / kCols;
   const uint32_t lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const uint32_t row0 = (WAVES == 1 ? blockIdx.x * kWaves + w : blockIdx.x) * rows;
-  uint32_t of = UINT32_MAX, first_item = 0;              // the token whose request r is
-  Request r = {};
-  bool split = false;
-  for (uint32_t row = row0; row < row0 + rows; ++row) {
-    const uint32_t token = over(p.by_heads, row);
-    if (token >= p.nnz) return;
-    if (token != of) {
-      Tables tables;
-      split = find_request(p, token, [](const Tables& t, uint32_t) { return static_cast<uint32_t>(max(t.a0, 0)); },
-                           &tables, &first_item) &&
-              request_of(p, tables, &r) && token >= r.q0 && token - r.q0 < r.q_len && r.chunks > 1;
-      of = token;
+  const uint32_t wave = blockIdx.x * kWaves + w;
+  const uint32_t token = over(p.by_token_waves, wave);
+  if (token >= p.nnz) return;
+  Request r;
+  uint32_t first_item;
+  if (!parts_of(p, token, &r, &first_item)) return;
+  const uint32_t col = lane % kCols, heads = p.heads * p.group;
+  const uint32_t qh0 = (wave - token * p.token_waves) * p.join_turns * kGroups + lane / kCols;
+  for (uint32_t turn = 0; turn < p.join_turns; ++turn) {
+    const uint32_t qh = qh0 + turn * kGroups;
+    if (qh >= heads) return;
+    const auto [first, step, chunks] = parts_of_row(p, r, first_item, token, qh);
+    float m = -INFINITY;
+#pragma unroll 4
+    for (uint32_t c = 0; c < chunks; ++c) m = fmaxf(m, p.part_ml[(first + c * step) * 2]);
+    const float from = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (uint32_t c = 0; c < chunks; ++c) {
+      const int64_t at = first + c * step;
+      const float weight = exp2_of(p.part_ml[at * 2] - from);
+      l += weight * p.part_ml[at * 2 + 1];
+      o += weight * *reinterpret_cast<const f32x4*>(p.part_o + at * D + col * 4);
     }
-    if (split) combine_row<D, TYPE, WAVES>(p, r, first_item, token, row - token * p.heads * p.group, lane, w);
+    write_row<TYPE>(p, token, qh, D, col, o, m, l);
   }
 }
 
@@ -156,16 +194,15 @@ Split split_of(int64_t batch, int64_t heads, int64_t group, int head_dim, int64_
   return s;
 }
 
-// Calls of at least this many rows give each row one wave to join its chunks,
-// smaller ones a workgroup.
+// Rows of a call from which on they are joined several to a wave.
 constexpr int64_t kManyRows = 2048;
 // Waves that the GPU holds at once: 256 CUs, eight waves on each of their four SIMDs.
 constexpr int64_t kWavesHeld = 8192;
 
 template <int D, int TYPE>
 const void* pick_combine(bool many) {
-  return many ? reinterpret_cast<const void*>(&combine_kernel<D, TYPE, 1>)
-              : reinterpret_cast<const void*>(&combine_kernel<D, TYPE, kWaves>);
+  return many ? reinterpret_cast<const void*>(&combine_many_kernel<D, TYPE>)
+              : reinterpret_cast<const void*>(&combine_few_kernel<D, TYPE>);
 }
 
 template <int D>
@@ -285,7 +322,14 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   p.scale_row = static_cast<uint32_t>(row / kMxBlock);
   const int64_t out_rows = nnz * num_kv_heads * group;
   const bool many = out_rows >= kManyRows;
-  p.join_rows = static_cast<uint32_t>(many ? std::min<int64_t>((out_rows + kWavesHeld - 1) / kWavesHeld, 8) : 1);
+  // Rows that one turn of a wave joins, turns so that the GPU holds all waves, and
+  // waves that a token's rows take.
+  const int64_t turn_rows = 256 / head_dim, token_rows = static_cast<int64_t>(num_kv_heads) * group;
+  const int64_t turns = std::min((out_rows + turn_rows * kWavesHeld - 1) / (turn_rows * kWavesHeld),
+                                 (token_rows + turn_rows - 1) / turn_rows);
+  p.join_turns = static_cast<uint32_t>(turns);
+  p.token_waves = static_cast<uint32_t>((token_rows + turn_rows * turns - 1) / (turn_rows * turns));
+  p.by_token_waves = fast_div(p.token_waves);
   p.by_page = fast_div(p.page_size);
   p.by_chunk = fast_div(p.chunk_pages);
   p.by_group = fast_div(p.group);
@@ -306,8 +350,7 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   PACE_KV_TRY(hip_status(hipLaunchKernel(attention, dim3(items * p.heads * p.row_tiles), dim3(kThreads), args, 0,
                                          static_cast<hipStream_t>(stream)), "attention launch"));
   if (need == 0) return PACE_KV_OK;
-  const int64_t per_group = many ? kWaves * p.join_rows : 1;
-  const uint32_t groups = static_cast<uint32_t>((out_rows + per_group - 1) / per_group);
+  const uint32_t groups = static_cast<uint32_t>(many ? (nnz * p.token_waves + kWaves - 1) / kWaves : out_rows);
   return hip_status(hipLaunchKernel(combine, dim3(groups), dim3(kThreads), args, 0, static_cast<hipStream_t>(stream)),
                     "attention combine launch");
 }
