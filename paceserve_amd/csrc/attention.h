@@ -323,7 +323,10 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   // Without a mask no row of the tile sees past its last query.
   const int32_t first_q = static_cast<int32_t>(over(p.by_group, row0));
   const int32_t last_q = static_cast<int32_t>(over(p.by_group, min(row0 + kTileRows, rows) - 1));
-  const int32_t chunk_tokens = static_cast<int32_t>(p.chunk_pages * p.page_size);
+  // A request's chunks are of one length, at most chunk_pages, and none is empty:
+  // (chunks - 1) * ceil(pages / chunks) < pages.  A short last one would leave its XCD
+  // idle where all requests have as many chunks.
+  const int32_t chunk_tokens = static_cast<int32_t>((r.pages + r.chunks - 1) / r.chunks * p.page_size);
   const int32_t t_begin = static_cast<int32_t>(r.chunk) * chunk_tokens;
   int32_t t_end = static_cast<int32_t>(min(static_cast<int64_t>(t_begin) + chunk_tokens, static_cast<int64_t>(r.kv_len)));
   if (p.mask == nullptr) t_end = min(t_end, base + last_q + 1);
