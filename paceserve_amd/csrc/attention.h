@@ -57,7 +57,7 @@ struct AttnParams {
   float* part_ml;              // [items, heads, row_tiles, rows of a tile, 2]
   int32_t* err;
   uint32_t num_indices, batch, nnz, heads, group, num_pages, page_size, max_q, mask_words;
-  uint32_t chunk_pages, items, row_tiles, tile_rows;
+  uint32_t chunk_pages, step_pages, items, row_tiles, tile_rows;
   uint32_t join_turns, token_waves;  // of the joining kernel
   uint32_t page16, half16, row16;  // page, half page and token row, in 16-byte units
   uint32_t scale_at, scale_row;    // scales within a half page, scale bytes of a token
@@ -131,7 +131,8 @@ __device__ __forceinline__ uint32_t chunks_of(const AttnParams& p, uint32_t n) {
 }
 
 // The sizes of request b; false where its queries are not among nnz or exceed
-// max_q.
+// max_q.  (Offsets that run backwards can count pages twice: a request whose items
+// do not fit p.items is refused as well.)
 __device__ __forceinline__ bool request_of(const AttnParams& p, const Tables& t, Request* r) {
   r->first_page = max(t.k0, 0);
   r->pages = pages_of(p, t);
@@ -310,7 +311,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   Tables tables;
   if (!find_request(p, item, [](const Tables&, uint32_t start) { return start; }, &tables, &first_item)) return;
   Request r;
-  const bool valid_request = request_of(p, tables, &r);
+  const bool valid_request = request_of(p, tables, &r) && first_item + r.chunks <= p.items;
   r.chunk = item - first_item;
   if (r.chunk >= r.chunks) return;
   if (!valid_request) {
@@ -323,10 +324,12 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   // Without a mask no row of the tile sees past its last query.
   const int32_t first_q = static_cast<int32_t>(over(p.by_group, row0));
   const int32_t last_q = static_cast<int32_t>(over(p.by_group, min(row0 + kTileRows, rows) - 1));
-  // A request's chunks are of one length, at most chunk_pages, and none is empty:
-  // (chunks - 1) * ceil(pages / chunks) < pages.  A short last one would leave its XCD
-  // idle where all requests have as many chunks.
-  const int32_t chunk_tokens = static_cast<int32_t>((r.pages + r.chunks - 1) / r.chunks * p.page_size);
+  // A request's chunks are of one length, in whole steps and at most chunk_pages, and
+  // none is empty: (chunks - 1) * chunk_pages < pages.  A short last one would leave
+  // its XCD idle where all requests have as many chunks.
+  const uint32_t even = (r.pages + r.chunks - 1) / r.chunks;
+  const uint32_t length = min((even + p.step_pages - 1) / p.step_pages * p.step_pages, p.chunk_pages);
+  const int32_t chunk_tokens = static_cast<int32_t>(length * p.page_size);
   const int32_t t_begin = static_cast<int32_t>(r.chunk) * chunk_tokens;
   int32_t t_end = static_cast<int32_t>(min(static_cast<int64_t>(t_begin) + chunk_tokens, static_cast<int64_t>(r.kv_len)));
   if (p.mask == nullptr) t_end = min(t_end, base + last_q + 1);

@@ -18,7 +18,8 @@ __device__ __forceinline__ bool parts_of(const AttnParams& p, uint32_t token, Re
   Tables t;
   return find_request(p, token, [](const Tables& x, uint32_t) { return static_cast<uint32_t>(max(x.a0, 0)); }, &t,
                       first_item) &&
-         request_of(p, t, r) && token >= r->q0 && token - r->q0 < r->q_len && r->chunks > 1;
+         request_of(p, t, r) && token >= r->q0 && token - r->q0 < r->q_len && r->chunks > 1 &&
+         *first_item + r->chunks <= p.items;
 }
 
 __device__ __forceinline__ Parts parts_of_row(const AttnParams& p, const Request& r, uint32_t first_item, uint32_t token,
@@ -159,22 +160,22 @@ __global__ __launch_bounds__(kThreads) void combine_many_kernel(const AttnParams
 
 // How a call is cut up.
 struct Split {
-  uint32_t tile_rows, row_tiles, chunk_pages, items;
+  uint32_t tile_rows, row_tiles, chunk_pages, step_pages, items;
   int64_t part_rows() const { return static_cast<int64_t>(items) * row_tiles * tile_rows; }  // times the KV heads
 };
 
-// Workgroups that a call's contexts are split over: about what the CUs hold at once
-// (three, or of 128 rows two, each); more pay for their starts and for joining
-// their parts.  MI355X, kernel and joining, at 512, 768 and 1024 workgroups:
-//   a decode step of 256 ragged requests    204, 204, 205 us
-//   12 rows over 32768 tokens               101,  99, 105
-//   36 rows over 16 ragged 4-bit contexts    63,  63,  53 (rounds of unequal length)
-//   504 rows over 8 x 4096 8-bit tokens     130, 193, 143
-constexpr int64_t target_groups(uint32_t tile_rows) { return tile_rows <= 32 ? 768 : tile_rows == 64 ? 1024 : 512; }
-// Tokens that a chunk has at least: four steps of a workgroup that splits the tokens,
-// two of one that splits the rows, whose steps are longer.  MI355X, 4 rows over 512
-// tokens: 13 us in one launch, 7 + 4 in two, which take the host 3 us more.
-constexpr int64_t min_chunk_tokens(uint32_t tile_rows) { return tile_rows <= 32 ? 512 : 128; }
+// A call's contexts are split so that every CU gets as many workgroups of about one
+// length: a request's work items go round the XCDs, and an item's heads and row tiles
+// to the CUs of its XCD.  With w workgroups for the fullest CU, of n tokens, the call
+// takes about (w + idle) * (n + start): `start` is what a workgroup's start and the
+// joining of its part cost, in tokens, and `idle` what a CU loses while it holds too
+// few waves to hide its loads: two thirds and a third of a workgroup of 16 or 32 rows
+// with one and two of them, half a larger one alone.  The fewest turns win; of the
+// requests' lengths the host knows only the sum, so they are taken as equal.
+// MI355X, against 768 (512 of 128 rows) workgroups whatever the sizes: 129 calls of 1
+// to 112 rows 4 % faster as a whole, 81 calls of 72 to 504 rows 11 %; 504 rows over
+// 3 x 9000 bf16 tokens 131 -> 98 us, 1 row of 32 heads over 5 x 20000 300 -> 262 us.
+constexpr int64_t kXcdCus = 32, kMostTurns = 6;
 
 Split split_of(int64_t batch, int64_t heads, int64_t group, int head_dim, int64_t max_q, int64_t num_indices,
                int64_t page_size) {
@@ -182,13 +183,35 @@ Split split_of(int64_t batch, int64_t heads, int64_t group, int head_dim, int64_
   const int64_t rows = max_q * group;
   s.tile_rows = tile_rows_of(head_dim, rows);
   s.row_tiles = static_cast<uint32_t>((rows + s.tile_rows - 1) / s.tile_rows);
-  const int64_t units = heads * s.row_tiles;
-  const int64_t target = target_groups(s.tile_rows);
-  int64_t chunk = (num_indices * units + target - 1) / target;
-  const int64_t least = (min_chunk_tokens(s.tile_rows) + page_size - 1) / page_size;
-  if (chunk < least) chunk = least;
-  if (num_indices <= least + least / 2) chunk = num_indices;  // no short second chunk
-  if (chunk < 1) chunk = 1;
+  const bool by_tokens = s.tile_rows <= 32;
+  // A chunk is whole steps of a wave, and long enough to be worth a part: MI355X, 4
+  // rows over 512 tokens, 13 us in one launch, 7 + 4 in two, which take the host 3 more.
+  const int64_t step = by_tokens ? 32 : 64, start = by_tokens ? 128 : 512, least = by_tokens ? 512 : 128;
+  s.step_pages = static_cast<uint32_t>(step % page_size ? 1 : step / page_size);
+  const int64_t unit = heads * s.row_tiles, requests = std::max<int64_t>(batch, 1);
+  const int64_t pages = std::max<int64_t>((num_indices + requests - 1) / requests, 1);
+  const int64_t most_chunks = std::max<int64_t>(pages * page_size / least, 1);
+  int64_t chunk = pages, best = INT64_MAX;
+  for (int64_t turns = 0; turns <= kMostTurns; ++turns) {
+    // The most chunks a request that keep to so many turns; first of all one.
+    const int64_t k = turns == 0 ? 1 : std::min(kXcds * (kXcdCus * turns / unit) / requests, most_chunks);
+    if (k < 1) continue;
+    const int64_t length = ((pages + k - 1) / k + s.step_pages - 1) / s.step_pages * s.step_pages;
+    const int64_t groups = (requests * k + kXcds - 1) / kXcds * unit, each = (groups + kXcdCus - 1) / kXcdCus;
+    const int64_t idle = by_tokens ? std::max<int64_t>(6 - 2 * each, 0) : each == 1 ? 3 : 0;   // in sixths
+    const int64_t cost = (6 * each + idle) * (length * page_size + start);
+    if (cost < best) {
+      best = cost;
+      chunk = length;
+    }
+  }
+  // Without a split only requests far longer than the others are cut: past the length
+  // that would give 768 workgroups, which for large tiles is at least the mean.  (200
+  // ragged requests of 56 rows: 47 us, 54 with those past the mean cut.)
+  if (chunk >= pages) chunk = std::max((num_indices * unit + 767) / 768, by_tokens ? 1 : pages);
+  const int64_t least_pages = (least + page_size - 1) / page_size;
+  chunk = std::max(chunk, least_pages);
+  if (num_indices <= least_pages + least_pages / 2) chunk = std::max<int64_t>(num_indices, 1);  // no short second chunk
   s.chunk_pages = static_cast<uint32_t>(chunk);
   s.items = static_cast<uint32_t>(num_indices / chunk + batch);
   return s;
@@ -312,6 +335,7 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   p.page_size = static_cast<uint32_t>(page_size);
   p.max_q = static_cast<uint32_t>(qo_indptr ? max_q_len : 1);
   p.chunk_pages = s.chunk_pages;
+  p.step_pages = s.step_pages;
   p.items = s.items;
   p.row_tiles = s.row_tiles;
   p.tile_rows = s.tile_rows;

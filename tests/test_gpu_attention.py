@@ -511,3 +511,16 @@ def test_every_count_of_chunks(gpu, D, chunks):
     out, lse = b.run()
     torch.cuda.synchronize()
     b.check(out, lse)
+
+
+def test_offsets_that_run_backwards(gpu):
+    """kv_indptr [0, 200, 0, 200] counts every page twice: more work items than the call has room for.  The
+    first request is whole, the second has no pages, the third is refused."""
+    b = Batch(gpu, [3200, 0, 0], [1, 0, 0], H=2, G=1, seed=8)
+    q = torch.cat([b.q, b.q, b.q])
+    out = torch.full_like(q, 7.0)
+    err = torch.zeros(1, dtype=torch.int32, device=gpu)
+    _, lse = paged_attention(q, b.cache, i32(b.indices, gpu), i32([0, 200, 0, 200], gpu), i32([16, 16, 16], gpu), out=out,
+                             err=err, return_lse=True)
+    b.check(out[:1], lse[:1])
+    assert (out[1] == 0).all() and (out[2] == 7).all() and err.item() == 1
