@@ -1,6 +1,7 @@
 // Attention over a paged cache: how a call is cut up, the kernel that joins the
 // parts, and the entry points.  The attention itself: attention.h.
 #include <algorithm>
+#include <cmath>
 
 #include "attention.h"
 
@@ -211,7 +212,8 @@ Split split_of(int64_t batch, int64_t heads, int64_t group, int head_dim, int64_
   if (chunk >= pages) chunk = std::max((num_indices * unit + 767) / 768, by_tokens ? 1 : pages);
   const int64_t least_pages = (least + page_size - 1) / page_size;
   chunk = std::max(chunk, least_pages);
-  if (num_indices <= least_pages + least_pages / 2) chunk = std::max<int64_t>(num_indices, 1);  // no short second chunk
+  if (num_indices <= least_pages + least_pages / 2) chunk = num_indices;  // no short second chunk
+  chunk = std::max<int64_t>(std::min(chunk, num_indices), 1);
   s.chunk_pages = static_cast<uint32_t>(chunk);
   s.items = static_cast<uint32_t>(num_indices / chunk + batch);
   return s;
@@ -283,8 +285,10 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   if (format != PACE_KV_PLAIN && !is_mx_format(format)) return fail(PACE_KV_EINVAL, "attention: unknown format %d", format);
   if (num_pages < 0 || num_pages > INT32_MAX || nnz > INT32_MAX / 2)
     return fail(PACE_KV_ERANGE, "attention: too many pages or tokens");
-  if (!(soft_cap >= 0.f) || !(soft_cap <= 3e38f) || !(scale == scale))
-    return fail(PACE_KV_EINVAL, "attention: soft_cap must be finite and >= 0, scale a number");
+  const float log2e = 1.44269504088896341f;
+  const float scale_log2 = soft_cap > 0.f ? scale / soft_cap * (2.f * log2e) : scale * log2e;
+  if (!(soft_cap >= 0.f) || !std::isfinite(soft_cap * log2e) || !std::isfinite(scale_log2))
+    return fail(PACE_KV_EINVAL, "attention: soft_cap must be >= 0, and it, scale and scale / soft_cap within float's range");
   if (nnz * num_kv_heads * group >= (int64_t(1) << 24))
     return fail(PACE_KV_ERANGE, "attention: 2^24 query rows or more");
   if (nnz == 0 || batch_size == 0) return PACE_KV_OK;
@@ -360,8 +364,7 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   p.by_heads = fast_div(p.heads * p.group);
   p.by_unit = fast_div(p.heads * p.row_tiles);
   p.by_tiles = fast_div(p.row_tiles);
-  const float log2e = 1.44269504088896341f;
-  p.scale_log2 = soft_cap > 0.f ? scale / soft_cap * (2.f * log2e) : scale * log2e;
+  p.scale_log2 = scale_log2;
   p.cap_log2 = soft_cap * log2e;
   const void* attention = head_dim == 64    ? attention_kernel_d64(elem_type, format, s.tile_rows)
                           : head_dim == 128 ? attention_kernel_d128(elem_type, format, s.tile_rows)

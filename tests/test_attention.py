@@ -57,6 +57,17 @@ def test_workspace_size():
     assert LIB.pace_kv_attention_workspace(1, 8, 4, 100, 1, 8192, 16, ctypes.byref(out)) == EINVAL
 
 
+def test_scales_past_float32_are_refused():
+    assert call(scale=math.inf) == EINVAL and call(scale=math.nan) == EINVAL
+    assert call(cap=1e-44) == EINVAL and "soft_cap" in LIB.pace_kv_last_error().decode()   # scale / soft_cap
+
+
+def test_sizes_whose_products_pass_32_bits():
+    """3 * 2^27 pages times 2^13 heads, a request of which is never cut: no parts are kept."""
+    out = ctypes.c_int64(-1)
+    assert LIB.pace_kv_attention_workspace(1, 1 << 13, 1, 128, 1, 3 << 27, 1, ctypes.byref(out)) == 0 and out.value == 0
+
+
 def test_oracle_against_torch():
     rng = np.random.default_rng(0)
     q, k, v = rng.standard_normal((3, 4, 64)), rng.standard_normal((20, 2, 64)), rng.standard_normal((20, 2, 64))

@@ -524,3 +524,21 @@ def test_offsets_that_run_backwards(gpu):
                              err=err, return_lse=True)
     b.check(out[:1], lse[:1])
     assert (out[1] == 0).all() and (out[2] == 7).all() and err.item() == 1
+
+
+def test_hundreds_of_chunks(gpu):
+    """Some 580 chunks of a request: a joining wave weighs its share 64 at a time."""
+    b = Batch(gpu, [300000], [1], H=1, G=2, D=64, seed=21)
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    b.check(out, lse)
+
+
+@pytest.mark.parametrize("D,kv,new", [(64, [2000, 700, 5], [60, 41, 1]), (128, [2000, 700, 5], [60, 41, 1]),
+                                      (256, [2000, 90], [400, 80])])
+def test_many_rows_are_joined(gpu, D, kv, new):
+    """2142 and 10080 rows of 21 heads, a count that the rows which a joining wave takes do not divide."""
+    b = Batch(gpu, kv, new, H=3, G=7, D=D, seed=22, tree=True)
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    b.check(out, lse)
