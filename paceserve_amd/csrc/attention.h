@@ -424,18 +424,23 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   const auto load_values = [&]() {
     if (valid != 0) fetch(vr, p.half16);
   };
+  // The 16-byte pieces that a lane expands one load to are two (or four) apart from
+  // its neighbour's, half the banks: every other group of lanes starts at its second.
+  const uint32_t turn = lane >> (FORMAT == PACE_KV_MXFP8 || D == 64 ? 2 : 1) & 1;
   const auto store_piece = [&](char* row, uint32_t c, const u32x4& x, uint64_t bytes) {
     u32x4* to = reinterpret_cast<u32x4*>(row);
     if constexpr (FORMAT == PACE_KV_PLAIN) {
       to[c] = x;
     } else if constexpr (FORMAT == PACE_KV_MXFP8) {      // 16 elements: half a block
       const float s = scale_of(static_cast<uint32_t>(bytes >> (c / 2 * 8)) & 255u);
-      to[2 * c] = run_up<TYPE, FORMAT>(u32x2{x[0], x[1]}, s);
-      to[2 * c + 1] = run_up<TYPE, FORMAT>(u32x2{x[2], x[3]}, s);
+      const u32x2 lo = {x[0], x[1]}, hi = {x[2], x[3]};
+      to[2 * c + turn] = run_up<TYPE, FORMAT>(turn ? hi : lo, s);
+      to[2 * c + 1 - turn] = run_up<TYPE, FORMAT>(turn ? lo : hi, s);
     } else {                                             // 32 elements: a block
       const float s = scale_of(static_cast<uint32_t>(bytes >> (c * 8)) & 255u);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) to[4 * c + k] = run_up<TYPE, FORMAT>(u32x2{x[k], 0}, s);
+      for (int k = 0; k < 4; ++k)
+        to[4 * c + (k + turn) % 4] = run_up<TYPE, FORMAT>(u32x2{turn ? x[(k + 1) % 4] : x[k], 0}, s);
     }
   };
   // Loaded rows into LDS; unless WHOLE, those of tokens outside `exist` as zeros.
@@ -568,28 +573,29 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
     if constexpr (!decltype(full)::value) {
       bool found = false;
 #pragma unroll 1
-      for (uint32_t c = lane; c < 32 * D / 8; c += 64) {
+      for (uint32_t c0 = 0; c0 < 32 * D / 8; c0 += 64) {
+        const uint32_t c = c0 + lane;
         const u32x4 x = *reinterpret_cast<const u32x4*>(value_at + c / (D / 8) * kStride<D> + c % (D / 8) * 16);
 #pragma unroll
         for (int e = 0; e < 4; ++e) found |= odd_word<TYPE>(x[e]);
       }
       odd = __ballot(found) != 0;
     }
-    if (!odd) {
 #pragma unroll
-      for (int d = 0; d < kDT; ++d) {
-        // Lane: row 4 g + n / 4 of each 16 tokens, four columns; transposed over
-        // 16 lanes: four tokens of column n.
-        const char* at = value_at + (4 * g + n / 4) * kStride<D> + n % 4 * 8 + d * 32;
-        typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 16 * kStride<D>));
-        const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
-        const u32x4 vf = {lo2[0], lo2[1], hi2[0], hi2[1]};
+    for (int d = 0; d < kDT; ++d) {
+      // Lane: row 4 g + n / 4 of each 16 tokens, four columns; transposed over
+      // 16 lanes: four tokens of column n.
+      const char* at = value_at + (4 * g + n / 4) * kStride<D> + n % 4 * 8 + d * 32;
+      typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 16 * kStride<D>));
+      const u32x2 lo2 = __builtin_bit_cast(u32x2, lo), hi2 = __builtin_bit_cast(u32x2, hi);
+      u32x4 vf = {lo2[0], lo2[1], hi2[0], hi2[1]};
+      if (odd) vf = u32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int a = 0; a < R; ++a) acc[a][d] = mfma<TYPE>(vf, pf[a], acc[a][d]);
-      }
-    } else {
+      for (int a = 0; a < R; ++a) acc[a][d] = mfma<TYPE>(vf, pf[a], acc[a][d]);
+    }
+    if constexpr (!decltype(full)::value) if (odd) {
       // A product with weight zero would spread an infinity or a NaN to rows
       // that do not see its token: the same sum, token by token, over those seen.
 #pragma unroll
