@@ -245,6 +245,11 @@ __device__ __forceinline__ uint32_t opaque(uint32_t x) {
   return x;
 }
 
+template <bool HIDE>
+__device__ __forceinline__ uint32_t opaque_if(uint32_t x) {
+  return HIDE ? opaque(x) : x;
+}
+
 template <int TYPE>
 __device__ __forceinline__ float value_of(uint32_t word, int half) {
   const unsigned short h = static_cast<unsigned short>(word >> (16 * half));
@@ -262,10 +267,13 @@ __device__ __forceinline__ bool odd_word(uint32_t w) {
 // Waves per SIMD that the registers are held to.  Two workgroups a CU fit the
 // accumulators and loads of 32 rows of 128 (and of 16 rows of 256, with a few spills
 // outside the loops: MI355X, 24 rows over 8 x 4096 bf16 tokens, 93 us against 114
-// with one); a decode step over a quantised cache leaves room for a third, whose
-// loads in flight count.
+// with one).  A quantised cache, whose loads in flight take fewer registers, leaves room
+// for a third: for a decode step its loads count; where a wave takes 32 of 128 rows
+// it computes while the others wait (320 rows over 24 x 2000 tokens, 8 bits 156 -> 137 us,
+// 4 bits 153 -> 130), if addresses are derived anew in each step.  A 16-bit cache
+// would spill there (33 registers: 152 -> 157 us).
 constexpr int min_waves(int D, int format, int R, int WR) {
-  return D != 256 && R == 1 && WR == 1 && format != PACE_KV_PLAIN ? 3 : 2;
+  return D != 256 && format != PACE_KV_PLAIN && (R == 1 ? WR == 1 : WR == 4) ? 3 : 2;
 }
 
 // TYPE: of queries and output, and what a quantised cache is expanded to.
@@ -284,6 +292,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   constexpr uint32_t kLoads = (kLoadRows * kPieces + 63) / 64;
   constexpr uint32_t kLdsRows = WR == 1 ? 128 : 64;
   constexpr int kDT = D / 16, kKS = D / 32;
+  constexpr bool kTight = R == 2 && WR == 4 && D == 128 && FORMAT != PACE_KV_PLAIN;  // three waves fill the registers
   // Rows that no other workgroup reads are loaded nontemporally, unless two heads
   // share a 128-byte line.  MI355X, reading 2 GiB of pages of 8 heads in this pattern:
   // 256-byte rows 6.4 TB/s against 5.8, 128-byte ones 6.3 against 5.6, 64-byte ones
@@ -343,11 +352,9 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
            (static_cast<int64_t>(head) * p.group + (row - i * p.group)) * (D * 2);
   };
   u32x4 qf[R][kKS];
-  int32_t qi[R];
 #pragma unroll
   for (int a = 0; a < R; ++a) {
     const uint32_t row = wave_row0 + a * 16 + n;
-    qi[a] = static_cast<int32_t>(over(p.by_group, row));
     if constexpr (WR != 1) {
 #pragma unroll
       for (int k = 0; k < kKS; ++k) {
@@ -363,7 +370,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
 #pragma unroll
   for (int a = 0; a < R; ++a) {
     m[a] = -INFINITY;
-    from[a] = 0.f;
+    from[a] = 0.f;                                       // m, or 0 while nothing is seen: weights of 2^-inf = 0
     l[a] = 0.f;
 #pragma unroll
     for (int d = 0; d < kDT; ++d) acc[a][d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -384,13 +391,13 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   };
   // Load j of a lane: column lane % kPieces of row j * kRowStep + lane / kPieces.
   constexpr uint32_t kRowStep = 64 / kPieces;
-  const uint32_t my_row = lane / kPieces, my_col = lane % kPieces;
   u32x4 kr[kLoads] = {}, vr[kLoads] = {};
   uint32_t row_at = 0;                                   // the lane's token's row, in 16-byte units
   uint64_t k_bytes = 0, v_bytes = 0;                     // the scales of the lane's token
   uint64_t valid = 0;
   const auto fetch = [&](u32x4* to, int64_t from) {
-    const uint32_t first_row = opaque((WR == 1 ? 0 : w * kLoadRows) + my_row % kLoadRows);
+    const uint32_t ln = opaque_if<kTight>(lane), my_row = ln / kPieces, my_col = ln % kPieces;
+    const uint32_t first_row = opaque_if<!kTight>((WR == 1 ? 0 : w * kLoadRows) + my_row % kLoadRows);
 #pragma unroll
     for (uint32_t j = 0; j < kLoads; ++j) {
       const int64_t at = static_cast<int64_t>(static_cast<uint32_t>(__shfl(row_at, first_row + j * kRowStep))) + from;
@@ -426,8 +433,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   };
   // The 16-byte pieces that a lane expands one load to are two (or four) apart from
   // its neighbour's, half the banks: every other group of lanes starts at its second.
-  const uint32_t turn = lane >> (FORMAT == PACE_KV_MXFP8 || D == 64 ? 2 : 1) & 1;
-  const auto store_piece = [&](char* row, uint32_t c, const u32x4& x, uint64_t bytes) {
+  const auto store_piece = [&](char* row, uint32_t c, uint32_t turn, const u32x4& x, uint64_t bytes) {
     u32x4* to = reinterpret_cast<u32x4*>(row);
     if constexpr (FORMAT == PACE_KV_PLAIN) {
       to[c] = x;
@@ -445,7 +451,9 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   };
   // Loaded rows into LDS; unless WHOLE, those of tokens outside `exist` as zeros.
   const auto store = [&](auto whole, char* to, u32x4* x, uint64_t bytes, uint64_t exist) {
-    const uint32_t from = opaque((WR == 1 ? 0 : w * kLoadRows) + my_row % kLoadRows);
+    const uint32_t ln = opaque_if<kTight>(lane), my_row = ln / kPieces, my_col = ln % kPieces;
+    const uint32_t turn = ln >> (FORMAT == PACE_KV_MXFP8 || D == 64 ? 2 : 1) & 1;
+    const uint32_t from = opaque_if<!kTight>((WR == 1 ? 0 : w * kLoadRows) + my_row % kLoadRows);
     if constexpr (!decltype(whole)::value) {
 #pragma unroll
       for (uint32_t j = 0; j < kLoads; ++j)
@@ -460,7 +468,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
         if constexpr (D == 256)
           b |= static_cast<uint64_t>(__shfl(static_cast<uint32_t>(bytes >> 32), from + j * kRowStep)) << 32;
       }
-      if (kRowStep <= kLoadRows || my_row < kLoadRows) store_piece(row + j * kRowStep * kStride<D>, my_col, x[j], b);
+      if (kRowStep <= kLoadRows || my_row < kLoadRows) store_piece(row + j * kRowStep * kStride<D>, my_col, turn, x[j], b);
     }
   };
 
@@ -487,7 +495,8 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   uint32_t sees[R];
   const float per_score = p.cap_log2 > 0.f || p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
   const auto weigh = [&](auto full, int32_t t0, uint32_t lds_row, uint32_t ok) {
-    const char* key_at = lds_k + (lds_row + n) * kStride<D> + g * 16;
+    const uint32_t ln = opaque_if<kTight>(lane);
+    const char* key_at = lds_k + (lds_row + ln % 16) * kStride<D> + ln / 16 * 16;
     f32x4 s[R][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -529,7 +538,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
     if constexpr (!decltype(full)::value) {
 #pragma unroll
       for (int a = 0; a < R; ++a) {
-        sees[a] = seen(t0, qi[a]) & ok;
+        sees[a] = seen(t0, static_cast<int32_t>(over(p.by_group, wave_row0 + a * 16 + opaque_if<kTight>(n)))) & ok;
         const uint32_t mine = sees[a] >> opaque(4 * g);
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -548,13 +557,14 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
       // their sums within float32), and most steps need no joint maximum.
       if (__ballot(top > m[a] + 8.f) != 0) {
         top = fmaxf(m[a], across_groups(top, max_of));
-        from[a] = top == -INFINITY ? 0.f : top;          // nothing seen yet: weights of 2^-inf = 0
+        from[a] = top == -INFINITY ? 0.f : top;
         const float shrink = exp2_of(m[a] - from[a]);
         m[a] = top;
         l[a] *= shrink;
 #pragma unroll
         for (int d = 0; d < kDT; ++d) acc[a][d] *= shrink;
       }
+      if (kTight) from[a] = m[a] == -INFINITY ? 0.f : m[a];
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -569,6 +579,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   // Adds the weighted values of those tokens, at lds_row.
   const auto gather = [&](auto full, uint32_t lds_row) {
     const char* value_at = lds_v + lds_row * kStride<D>;
+    const uint32_t ln = opaque_if<kTight>(lane);
     bool odd = false;                                    // an infinite or NaN value that some row must not see
     if constexpr (!decltype(full)::value) {
       bool found = false;
@@ -585,7 +596,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
     for (int d = 0; d < kDT; ++d) {
       // Lane: row 4 g + n / 4 of each 16 tokens, four columns; transposed over
       // 16 lanes: four tokens of column n.
-      const char* at = value_at + (4 * g + n / 4) * kStride<D> + n % 4 * 8 + d * 32;
+      const char* at = value_at + ln / 4 * kStride<D> + ln % 4 * 8 + d * 32;
       typedef __attribute__((address_space(3))) s16x4* lds_ptr;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)at);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + 16 * kStride<D>));

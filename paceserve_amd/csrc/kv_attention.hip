@@ -170,8 +170,8 @@ struct Split {
 // to the CUs of its XCD.  With w workgroups for the fullest CU, of n tokens, the call
 // takes about (w + idle) * (n + start): `start` is what a workgroup's start and the
 // joining of its part cost, in tokens, and `idle` what a CU loses while it holds too
-// few waves to hide its loads: two thirds and a third of a workgroup of 16 or 32 rows
-// with one and two of them, half a larger one alone.  The fewest turns win; of the
+// few waves to hide its loads: two thirds and a third of a workgroup with one and two
+// of those that fit it by threes, half of one alone of others.  The fewest turns win; of the
 // requests' lengths the host knows only the sum, so they are taken as equal.
 // MI355X, against 768 (512 of 128 rows) workgroups whatever the sizes: 129 calls of 1
 // to 112 rows 4 % faster as a whole, 81 calls of 72 to 504 rows 11 %; 504 rows over
@@ -179,12 +179,13 @@ struct Split {
 constexpr int64_t kXcdCus = 32, kMostTurns = 6;
 
 Split split_of(int64_t batch, int64_t heads, int64_t group, int head_dim, int64_t max_q, int64_t num_indices,
-               int64_t page_size) {
+               int64_t page_size, bool quantised) {
   Split s = {};
   const int64_t rows = max_q * group;
   s.tile_rows = tile_rows_of(head_dim, rows);
   s.row_tiles = static_cast<uint32_t>((rows + s.tile_rows - 1) / s.tile_rows);
   const bool by_tokens = s.tile_rows <= 32;
+  const bool three = by_tokens || (head_dim != 256 && (quantised || (head_dim == 64 && s.tile_rows == 128)));
   // A chunk is whole steps of a wave, and long enough to be worth a part: MI355X, 4
   // rows over 512 tokens, 13 us in one launch, 7 + 4 in two, which take the host 3 more.
   const int64_t step = by_tokens ? 32 : 64, start = by_tokens ? 128 : 512, least = by_tokens ? 512 : 128;
@@ -199,7 +200,7 @@ Split split_of(int64_t batch, int64_t heads, int64_t group, int head_dim, int64_
     if (k < 1) continue;
     const int64_t length = ((pages + k - 1) / k + s.step_pages - 1) / s.step_pages * s.step_pages;
     const int64_t groups = (requests * k + kXcds - 1) / kXcds * unit, each = (groups + kXcdCus - 1) / kXcdCus;
-    const int64_t idle = by_tokens ? std::max<int64_t>(6 - 2 * each, 0) : each == 1 ? 3 : 0;   // in sixths
+    const int64_t idle = three ? std::max<int64_t>(6 - 2 * each, 0) : each == 1 ? 3 : 0;   // in sixths
     const int64_t cost = (6 * each + idle) * (length * page_size + start);
     if (cost < best) {
       best = cost;
@@ -244,9 +245,11 @@ int check_sizes(int batch_size, int num_kv_heads, int group, int head_dim, int m
   const int64_t rows = static_cast<int64_t>(max_q_len) * group;
   if (num_indices * page_size > INT32_MAX / 2 || rows > INT32_MAX / 2)
     return fail(PACE_KV_ERANGE, "attention: more than 2^30 tokens or query rows");
-  const Split s = split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size);
-  if ((static_cast<int64_t>(s.items) + kXcds) * num_kv_heads * s.row_tiles >= (int64_t(1) << 24))
-    return fail(PACE_KV_ERANGE, "attention: too many requests, heads or query rows for one call");
+  for (bool quantised : {false, true}) {
+    const Split s = split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size, quantised);
+    if ((static_cast<int64_t>(s.items) + kXcds) * num_kv_heads * s.row_tiles >= (int64_t(1) << 24))
+      return fail(PACE_KV_ERANGE, "attention: too many requests, heads or query rows for one call");
+  }
   return PACE_KV_OK;
 }
 
@@ -265,8 +268,10 @@ int pace_kv_attention_workspace(int batch_size, int num_kv_heads, int group, int
   using namespace pace_kv;
   if (!bytes) return fail(PACE_KV_EINVAL, "attention: NULL argument");
   PACE_KV_TRY(check_sizes(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size));
-  *bytes = workspace_bytes(split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size), num_kv_heads,
-                           head_dim, num_indices);
+  *bytes = 0;                                            // of either kind of cache
+  for (bool quantised : {false, true})
+    *bytes = std::max(*bytes, workspace_bytes(split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices,
+                                                       page_size, quantised), num_kv_heads, head_dim, num_indices));
   return PACE_KV_OK;
 }
 
@@ -310,7 +315,8 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   if (half_bytes % 16) return fail(PACE_KV_EINVAL, "attention: half a page must be a multiple of 16 bytes");
   if (num_pages * 2 * half_bytes / 16 >= UINT32_MAX)
     return fail(PACE_KV_ERANGE, "attention: a layer's cache must be smaller than 64 GiB");
-  const Split s = split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size);
+  const Split s = split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size,
+                           format != PACE_KV_PLAIN);
   const int64_t need = workspace_bytes(s, num_kv_heads, head_dim, num_indices);
   if (need > 0 && (!workspace || workspace_size < need || reinterpret_cast<uintptr_t>(workspace) & 15u))
     return fail(PACE_KV_EINVAL, "attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
