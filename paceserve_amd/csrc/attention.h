@@ -22,8 +22,18 @@
 // through.  A workgroup finds the request of its number in the tables themselves,
 // so a launch needs no plan and a captured one follows them; the grid has room for
 // the most chunks there can be, floor(pages / C) + requests.  A request of one chunk
-// is written directly; the others leave (o, m, l) in a workspace for
-// combine_kernel.
+// is written directly; the others leave (o, m, l) in a workspace for the joining
+// kernels.
+//
+// Bounds on MI355X (kernel alone): up to 32 rows over a 16-bit cache HBM, 5.3 to 5.7
+// TB/s (256 ragged requests of 2048 tokens with 8 heads of 128, 4 rows each, 191 to 204
+// us; 12 rows of 32 heads over 32768 tokens 94 to 96 us).  Over a quantised cache, and
+// with more rows, expansion, exponentials and matrix instructions take about the same
+// issue time each and overlap only in part: 504 rows over 8 x 4096 8-bit tokens 105 us,
+// where the products alone take 27 at the matrix peak (counters: matrix instructions
+// 30% of the time, vector ones 50%, LDS 30%; leaving out any one of them saves 10 to 20
+// us, all of them 70).  A single short request is a chain of latencies: 12.5 us over
+// 512 tokens, of which the four steps of a wave take six.
 #pragma once
 
 #include <type_traits>
@@ -764,8 +774,11 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
 // Rows that a workgroup takes, of `rows` that a request has for one KV head: up to 32
 // the waves split the tokens, past that the rows.  (48 or 64 rows with the tokens
 // split fill 256 registers and spill: MI355X, 36 rows over a 4-bit cache, 48 us
-// either way.)  With head_dim 256 a wave has registers for 16 rows: 320 rows over 8 x
-// 4096 8-bit tokens 235 us, 561 with 32.
+// either way.)  Eight waves on 256 rows took 188 us for 252 rows over 32 x 4096 8-bit
+// tokens where four on 128 take 203, but up to 60% longer where their workgroups do not
+// divide evenly among the CUs.  With head_dim 256 a wave has registers for 16 rows: 320
+// rows over 8 x 4096 8-bit tokens 235 us against 561 with 32 (and
+// 190 since requests are split evenly).
 inline uint32_t tile_rows_of(int head_dim, int64_t rows) {
   if (rows <= 16) return 16;
   if (head_dim == 256) return 64;
