@@ -236,6 +236,18 @@ const void* pick_combine(int type, bool many) {
   return type == PACE_KV_BF16 ? pick_combine<D, PACE_KV_BF16>(many) : pick_combine<D, PACE_KV_FP16>(many);
 }
 
+// LDS that a workgroup asks for beyond its own.  16 rows of 128 columns over a 16-bit
+// cache fit a CU by threes, which long contexts read more slowly than by twos: MI355X,
+// ragged requests of up to 4096 tokens, 64 of 32 heads 402 us by threes, 393 by twos, up
+// to 2048 tokens, 256 of 8 heads 207 and 200, up to 1500, 100 of 32 heads 230 and 227; but
+// up to 1000, 256 of 32 heads 361 and 373, up to 300, 300 of 32 heads 158 and 191.  (Half
+// of those lengths on the mean.)
+uint32_t spare_lds(int head_dim, uint32_t tile_rows, bool quantised, int64_t batch, int64_t num_indices,
+                   int64_t page_size) {
+  const bool by_twos = head_dim == 128 && tile_rows == 16 && !quantised && num_indices * page_size >= 768 * batch;
+  return by_twos ? 14 << 10 : 0;                         // 41 KiB of its own; 160 KiB a CU
+}
+
 int check_sizes(int batch_size, int num_kv_heads, int group, int head_dim, int max_q_len, int64_t num_indices,
                 int page_size) {
   if (batch_size < 0 || num_kv_heads <= 0 || group <= 0 || max_q_len <= 0 || num_indices < 0 || page_size <= 0)
@@ -380,7 +392,9 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
                                           : pick_combine<256>(elem_type, many);
   const uint32_t items = (s.items + kXcds - 1) / kXcds * kXcds;
   void* args[] = {&p};
-  PACE_KV_TRY(hip_status(hipLaunchKernel(attention, dim3(items * p.heads * p.row_tiles), dim3(kThreads), args, 0,
+  PACE_KV_TRY(hip_status(hipLaunchKernel(attention, dim3(items * p.heads * p.row_tiles), dim3(kThreads), args,
+                                         spare_lds(head_dim, s.tile_rows, format != PACE_KV_PLAIN, batch_size,
+                                                   num_indices, page_size),
                                          static_cast<hipStream_t>(stream)), "attention launch"));
   if (need == 0) return PACE_KV_OK;
   const uint32_t groups = static_cast<uint32_t>(many ? (nnz * p.token_waves + kWaves - 1) / kWaves : out_rows);
