@@ -26,13 +26,13 @@
 // kernels.
 //
 // Bounds on MI355X (kernel alone): up to 32 rows over a 16-bit cache HBM, 5.3 to 5.7
-// TB/s (256 ragged requests of 2048 tokens with 8 heads of 128, 4 rows each, 191 to 204
-// us; 12 rows of 32 heads over 32768 tokens 94 to 96 us).  Over a quantised cache, and
+// TB/s (256 ragged requests of up to 2048 tokens with 8 heads of 128, 8 rows each, 191 to
+// 198 us; 12 rows of 32 heads over 32768 tokens 94 to 96 us).  Over a quantised cache, and
 // with more rows, expansion, exponentials and matrix instructions take about the same
 // issue time each and overlap only in part: 504 rows over 8 x 4096 8-bit tokens 105 us,
 // where the products alone take 27 at the matrix peak (counters: matrix instructions
-// 30% of the time, vector ones 50%, LDS 30%; leaving out any one of them saves 10 to 20
-// us, all of them 70).  A single short request is a chain of latencies: 12.5 us over
+// 32% of the time, vector ones 55%, LDS 28%; of an earlier 119 us leaving out any one of
+// them saved 4 to 18, all of them 68).  A single short request is a chain of latencies: 12.5 us over
 // 512 tokens, of which the four steps of a wave take six.
 #pragma once
 
