@@ -173,8 +173,8 @@ struct Split {
 // few waves to hide its loads: two thirds and a third of a workgroup with one and two
 // of those that fit it by threes, half of one alone of others.  The fewest turns win; of the
 // requests' lengths the host knows only the sum, so they are taken as equal.
-// MI355X, against 768 (512 of 128 rows) workgroups whatever the sizes: 129 calls of 1
-// to 112 rows 4 % faster as a whole, 81 calls of 72 to 504 rows 11 %; 504 rows over
+// MI355X, against 768 (512 of 128 rows) workgroups whatever the sizes: 144 calls of 1
+// to 112 rows 4 % faster as a whole, 126 calls of 72 to 504 rows 11 %; 504 rows over
 // 3 x 9000 bf16 tokens 131 -> 98 us, 1 row of 32 heads over 5 x 20000 300 -> 262 us.
 constexpr int64_t kXcdCus = 32, kMostTurns = 6;
 
