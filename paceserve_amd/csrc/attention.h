@@ -248,6 +248,18 @@ __device__ __forceinline__ uint32_t pair_of(float a, float b) {
   }
 }
 
+// Two results.  A weighted mean of finite values is none larger than they are, but
+// rounded weights can carry one past float16's largest number by 2^-11 of it.
+template <int TYPE>
+__device__ __forceinline__ uint32_t result_pair(float a, float b) {
+  if constexpr (TYPE == PACE_KV_FP16) {
+    constexpr float kMost = 65504.f;
+    if (fabsf(a) < INFINITY) a = fminf(fmaxf(a, -kMost), kMost);
+    if (fabsf(b) < INFINITY) b = fminf(fmaxf(b, -kMost), kMost);
+  }
+  return pair_of<TYPE>(a, b);
+}
+
 // Hides where x comes from, so that what a loop derives from it is derived anew
 // each time (an add) instead of being held in a register throughout.
 __device__ __forceinline__ uint32_t opaque(uint32_t x) {
@@ -720,7 +732,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const uint32_t i = over(p.by_group, row);
     const uint32_t qh = head * p.group + (row - i * p.group);
-    const u32x2 x = {pair_of<TYPE>(o[0] * inv, o[1] * inv), pair_of<TYPE>(o[2] * inv, o[3] * inv)};
+    const u32x2 x = {result_pair<TYPE>(o[0] * inv, o[1] * inv), result_pair<TYPE>(o[2] * inv, o[3] * inv)};
     *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(r.q0 + i) * p.out_stride +
                               (static_cast<int64_t>(qh) * D + d) * 2) = x;
     if (first && p.lse != nullptr)

@@ -38,7 +38,7 @@ template <int TYPE>
 __device__ __forceinline__ void write_row(const AttnParams& p, uint32_t token, uint32_t qh, int D, uint32_t col, f32x4 o,
                                           float m, float l) {
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const u32x2 x = {pair_of<TYPE>(o[0] * inv, o[1] * inv), pair_of<TYPE>(o[2] * inv, o[3] * inv)};
+  const u32x2 x = {result_pair<TYPE>(o[0] * inv, o[1] * inv), result_pair<TYPE>(o[2] * inv, o[3] * inv)};
   *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(token) * p.out_stride +
                             (static_cast<int64_t>(qh) * D + col * 4) * 2) = x;
   if (col == 0 && p.lse != nullptr)

@@ -1,0 +1,42 @@
+"""paged_attention (HIP) at the limits of its numbers: values, weights, scores
+and caps where the arithmetic could leave the type, and infinities, each
+against the 64-bit oracle."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_attention import FP16, Batch
+
+pytestmark = pytest.mark.gpu
+
+
+def one_dominant(b, score, key=4.0):
+    """Every key zero but the middle token's of each request, whose score is
+    `score`; all queries alike."""
+    b.q.zero_()
+    b.q[:, :, 0] = score * math.sqrt(b.D) / key
+    at = []
+    for x, n, t in zip(b.rows, b.kv, b.new):
+        x[:, 0] = 0
+        at.append((n - t) // 2)
+        x[at[-1], 0, :, 0] = key
+    return at
+
+
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("rising", [False, True])
+def test_values_of_float16s_largest_stay_finite(gpu, rising, T):
+    """A weighted mean of one value is that value: weights rounded up must not push
+    65504 past the type.  Tokens of equal scores have equal roundings."""
+    for k in range(24):
+        b = Batch(gpu, [600], [T], H=1, G=1, D=64, dtype=FP16, seed=k)
+        one_dominant(b, 0.5 + k / 16)
+        if rising:                                      # the larger scores come late
+            b.rows[0][200:, 0] = 4.0
+        b.rows[0][:, 1] = torch.tensor([65504.0, -65504.0] * 32, dtype=torch.float64)
+        b.fill()
+        out, lse = b.run()
+        torch.cuda.synchronize()
+        assert torch.isfinite(out).all(), f"score {0.5 + k / 16}"
+        b.check(out, lse)
