@@ -24,6 +24,24 @@ def one_dominant(b, score, key=4.0):
     return at
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("T,G,fmt", [(1, 1, None), (20, 1, None), (10, 8, None), (1, 2, "mxfp8"), (10, 8, "mxfp8")])
+def test_a_value_at_the_types_limit(gpu, T, G, fmt, D):
+    """The row's largest score belongs to a value of 2^127: any weight of more than
+    2 on it passes float32, whose largest number is below 2^128."""
+    b = Batch(gpu, [700, 90], [T, T], H=1, G=G, D=D, fmt=fmt, seed=T + G)
+    for x, at in zip(b.rows, one_dominant(b, 5.0)):
+        x[:, 1, :, 3] = 0
+        x[at, 1, :, 3] = 2.0 ** 127
+        # the block that shares the value's scale: as small a number as it holds is large
+        x[at, 1, :, :3] = x[at, 1, :, 4:32] = 0
+    b.fill()
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    assert (out[:, :, 3].float() > 1e37).all() and torch.isfinite(out).all()
+    b.check(out, lse)
+
+
 @pytest.mark.parametrize("T", [1, 40])
 @pytest.mark.parametrize("rising", [False, True])
 def test_values_of_float16s_largest_stay_finite(gpu, rising, T):
