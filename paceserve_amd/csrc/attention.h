@@ -16,7 +16,11 @@
 // consecutive entries of the product's k, for which V's rows are read in the
 // same order through the transposing LDS read.  P is rounded to the values'
 // type for the product (within 2^-8 of each weight in bfloat16, 2^-11 in float16,
-// errors that average out over the row); l sums the unrounded weights.
+// errors that average out over the row); l sums the unrounded weights.  Weights are
+// 2^(score - m) of at most 1; in float16 they are of at most 2^15 (m lies 15 below the
+// largest score), which leaves those down to 2^-29 of the largest their 2^-11, and the
+// least 2^-40 of it: with 1 as the most, a long tail of weights below 2^-14 lost up to
+// all of its mass in the output, though not in l.
 //
 // Work split: a request's pages in chunks of C, the chunks of all requests numbered
 // through.  A workgroup finds the request of its number in the tables themselves,
@@ -236,6 +240,10 @@ __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                   0);
 }
+
+// log2 of a row's largest weight.
+template <int TYPE>
+constexpr float kTopWeight = TYPE == PACE_KV_FP16 ? 15.f : 0.f;
 
 template <int TYPE>
 __device__ __forceinline__ uint32_t pair_of(float a, float b) {
@@ -574,8 +582,8 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
       float top = max3_of(s[a][0][0], s[a][0][1], s[a][0][2]);
       top = max3_of(top, s[a][0][3], s[a][1][0]);
       top = max3_of(top, s[a][1][1], s[a][1][2]);
-      top = max3_of(top, s[a][1][3], s[a][1][3]) * per_score;
-      // m is the largest score so far, exactly: its weight is 1 and is not rounded, and a
+      top = __builtin_fmaf(max3_of(top, s[a][1][3], s[a][1][3]), per_score, -kTopWeight<TYPE>);
+      // m follows the largest score so far exactly: its weight is not rounded, and a
       // weighted value is no larger than the value.  (Raising m only past 2^8 of it spares
       // most steps the joint maximum, MI355X: 3 % over 70 calls, 11 % of 320 rows; but
       // the largest weight is then rounded as the others are, bfloat16 outputs are off by

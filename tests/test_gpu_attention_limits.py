@@ -3,9 +3,11 @@ and caps where the arithmetic could leave the type, and infinities, each
 against the 64-bit oracle."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
+from oracle import attention_oracle as ao
 from test_gpu_attention import FP16, Batch
 
 pytestmark = pytest.mark.gpu
@@ -40,6 +42,32 @@ def test_a_value_at_the_types_limit(gpu, T, G, fmt, D):
     torch.cuda.synchronize()
     assert (out[:, :, 3].float() > 1e37).all() and torch.isfinite(out).all()
     b.check(out, lse)
+
+
+@pytest.mark.parametrize("fmt", [None, "mxfp8", "mxfp4"])
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("nats", [9, 16, 18, 22])
+def test_float16_keeps_many_small_weights(gpu, nats, T, fmt):
+    """A dominant token whose value is zero before a long flat tail, whose weights are
+    below float16's smallest normal number and whose sum makes the output."""
+    b = Batch(gpu, [30000, 200], [T, T], H=1, G=1, D=64, dtype=FP16, fmt=fmt, seed=nats)
+    for x, at in zip(b.rows, one_dominant(b, float(nats))):
+        x[at, 1] = 0
+    b.fill()
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    b.check(out, lse)
+    # The bound of check() grants each weight float16's subnormal half step, 2^-25 of
+    # the largest weight.  Weights of up to 2^15 leave 2^-40 of it.
+    got = out.double().cpu().numpy()
+    for r, x in enumerate(b.seen_rows):
+        s = slice(b.qo[r], b.qo[r + 1])
+        o, l, mean, dots, spread = ao.attend(b.q[s].double().cpu().numpy(), x[:, 0], x[:, 1], 1 / math.sqrt(b.D), 0.0,
+                                             ao.visible(len(x), T, None))
+        bo, _ = ao.bounds(b.D, torch.finfo(FP16).eps, o, l, mean, dots, spread, 0.0, len(x), 2.0 ** -40)
+        # the result is itself rounded to float16, whose subnormals are 2^-24 apart
+        assert (np.abs(got[s] - o) <= bo + 2.0 ** -25).all(), \
+            f"request {r}: off by {np.max(np.abs(got[s] - o) / (bo + 2.0 ** -25)):.3g} of the bound"
 
 
 @pytest.mark.parametrize("T", [1, 40])
