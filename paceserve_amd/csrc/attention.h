@@ -397,8 +397,10 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
 
   f32x4 acc[R][kDT];
   float m[R], from[R], l[R];
+  bool wide[R];                                          // some row's |m| is past 2^20
 #pragma unroll
   for (int a = 0; a < R; ++a) {
+    wide[a] = false;
     m[a] = -INFINITY;
     from[a] = 0.f;                                       // m, or 0 while nothing is seen: weights of 2^-inf = 0
     l[a] = 0.f;
@@ -593,17 +595,34 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
         from[a] = top == -INFINITY ? 0.f : top;
         const float shrink = exp2_of(m[a] - from[a]);
         m[a] = top;
+        wide[a] = __ballot(fabsf(from[a]) > 0x1p20f) != 0;
         l[a] *= shrink;
 #pragma unroll
         for (int d = 0; d < kDT; ++d) acc[a][d] *= shrink;
       }
       if (kTight) from[a] = m[a] == -INFINITY ? 0.f : m[a];
+      // The fused difference holds what m lost when it was rounded: less than a tenth up
+      // to 2^20, but past 2^27 enough to make the largest weight an infinity or a zero.
+      if (wide[a]) {
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float scaled = s[a][t][e] * per_score, x = scaled - from[a];
+            s[a][t][e] = x > kTopWeight<TYPE> ? kTopWeight<TYPE> : x;
+          }
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[a][t][e] = __builtin_fmaf(s[a][t][e], per_score, -from[a]);
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
-          const float x = exp2_of(__builtin_fmaf(s[a][t][e], per_score, -from[a]));
-          const float y = exp2_of(__builtin_fmaf(s[a][t][e + 1], per_score, -from[a]));
+          const float x = exp2_of(s[a][t][e]), y = exp2_of(s[a][t][e + 1]);
           l[a] += x + y;
           pf[a][t * 2 + e / 2] = pair_of<TYPE>(x, y);
         }

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import attention_oracle as ao
-from test_gpu_attention import FP16, Batch
+from test_gpu_attention import BF16, FP16, Batch
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,34 @@ def test_values_of_float16s_largest_stay_finite(gpu, rising, T):
         torch.cuda.synchronize()
         assert torch.isfinite(out).all(), f"score {0.5 + k / 16}"
         b.check(out, lse)
+
+
+@pytest.mark.parametrize("fmt", [None, "mxfp8"])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("T,G", [(1, 1), (20, 1), (10, 8)])
+@pytest.mark.parametrize("size", [10, 12, 13, 14, 15])
+def test_scores_far_past_any_exponential(gpu, size, T, G, dtype, fmt):
+    """Queries and keys of powers of two, whose scores (up to 2^34) are exact sums: all
+    the weight goes to the token with the largest, and the mean of two equal ones."""
+    D = 128
+    b = Batch(gpu, [700, 90], [T, T], H=1, G=G, D=D, dtype=dtype, fmt=fmt, seed=size)
+    b.q.fill_(2.0 ** size)
+    want, top = [], []
+    for x, n, t in zip(b.rows, b.kv, b.new):
+        x[:, 0] = 2.0 ** (size - 1) * torch.where(torch.arange(n) % 3 == 0, 1, -1)[:, None, None]
+        for at in (n // 2, n // 5):
+            x[at, 0] = 2.0 ** size
+            x[at, 0, :, 5] = 2.0 ** (size - 1) * 1.5    # and a sum that is no power of two
+        x[:, 1] = torch.round(x[:, 1] * 4).clamp(-6, 6)
+        x[n // 5, 1] = x[n // 2, 1] + 2
+    b.fill()
+    for scale in (None, 0.1, 0.3):
+        out, lse = b.run(**({} if scale is None else dict(sm_scale=scale)))
+        torch.cuda.synchronize()
+        for r, x in enumerate(b.seen_rows):
+            n, t, s = len(x), int(b.new[r]), slice(b.qo[r], b.qo[r + 1])
+            mean = torch.from_numpy((x[n // 5, 1] + x[n // 2, 1]) / 2).to(gpu)
+            assert (out[s].double() - mean).abs().max() <= torch.finfo(dtype).eps * 8, f"scale {scale} request {r}"
+            score = (127 * 4.0 ** size + 0.75 * 4.0 ** size) * (scale or 1 / math.sqrt(D))
+            # the scale as float32, times log2(e) and back: a few roundings of the score
+            assert (lse[s].double() - score - math.log(2)).abs().max() <= 8 * 2.0 ** -24 * score
