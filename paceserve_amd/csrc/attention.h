@@ -78,6 +78,8 @@ struct AttnParams {
   FastDiv by_page, by_chunk, by_group, by_unit, by_tiles, by_heads, by_token_waves;
   float scale_log2;            // scale * log2(e); with a cap: scale / cap * 2 * log2(e)
   float cap_log2;              // cap * log2(e), or 0
+  float uncapped_log2;         // scale * log2(e)
+  uint32_t large_cap;          // the cap is past kLargeCap
 };
 
 // Swaps of half a wave and of neighbouring rows of 16 lanes bring the four
@@ -549,8 +551,8 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
       }
     }
     // The weights are 2^(per_score * s - m).
-    if (p.cap_log2 > 0.f) {
-      // tanh(z) = 1 - 2 / (1 + 2^(2 log2(e) z)), times the cap
+    if (p.cap_log2 > 0.f && !p.large_cap) {
+      // x = 2 log2(e) z: tanh(z) = 1 - 2 / (1 + 2^x), times the cap: off by 2^-22 of the cap
 #pragma unroll
       for (int a = 0; a < R; ++a)
 #pragma unroll
@@ -559,6 +561,28 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
           for (int e = 0; e < 4; ++e) {
             const float half = __builtin_amdgcn_rcpf(1.f + exp2_of(s[a][t][e] * p.scale_log2));
             s[a][t][e] = __builtin_fmaf(half, -2.f * p.cap_log2, p.cap_log2);
+          }
+    } else if (p.cap_log2 > 0.f) {
+      // The same where |x| >= 0.8: off by 2^-20 of itself.  Below, the series z (1 - z^2/3 +
+      // 2 z^4/15 - 17 z^6/315 + 62 z^8/2835), in x, times the score: off by a few 2^-24 of
+      // itself, however large the cap; the next term is below 2^-25.
+      constexpr float kSq = 0.12011325f;                 // (ln(2) / 2)^2: z^2 = kSq x^2
+      constexpr float c1 = -1.f / 3 * kSq, c2 = 2.f / 15 * kSq * kSq, c3 = -17.f / 315 * kSq * kSq * kSq,
+                      c4 = 62.f / 2835 * kSq * kSq * kSq * kSq;
+#pragma unroll
+      for (int a = 0; a < R; ++a)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = s[a][t][e] * p.scale_log2, x2 = x * x;
+            const float half = __builtin_amdgcn_rcpf(1.f + exp2_of(x));
+            float f = __builtin_fmaf(x2, c4, c3);
+            f = __builtin_fmaf(x2, f, c2);
+            f = __builtin_fmaf(x2, f, c1);
+            f = __builtin_fmaf(x2, f, 1.f);
+            const float near = s[a][t][e] * p.uncapped_log2 * f;
+            s[a][t][e] = fabsf(x) < 0.8f ? near : __builtin_fmaf(half, -2.f * p.cap_log2, p.cap_log2);
           }
     } else if (p.scale_log2 <= 0.f) {
       const float sign = p.scale_log2 < 0.f ? -1.f : 0.f;

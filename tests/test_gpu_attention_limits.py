@@ -88,6 +88,28 @@ def test_values_of_float16s_largest_stay_finite(gpu, rising, T):
         b.check(out, lse)
 
 
+@pytest.mark.parametrize("dtype,fmt", [(BF16, None), (FP16, None), (BF16, "mxfp4")])
+@pytest.mark.parametrize("T,G", [(1, 4), (20, 8)])
+@pytest.mark.parametrize("cap", [0.25, 3.0, 64.0, 65.0, 1e3, 1e5, 1e6, 1e8, 1e12, 1e30])
+def test_soft_caps_of_every_size(gpu, cap, T, G, dtype, fmt):
+    """cap * tanh(s / cap): as the cap grows it is s itself."""
+    b = Batch(gpu, [500, 70], [T, T], G=G, dtype=dtype, fmt=fmt, seed=T)
+    out, lse = b.run(cap)
+    torch.cuda.synchronize()
+    got, got_l = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    for r, x in enumerate(b.seen_rows):
+        s = slice(b.qo[r], b.qo[r + 1])
+        o, l, mean, dots, spread = ao.attend(b.q[s].double().cpu().numpy(), x[:, 0], x[:, 1], 1 / math.sqrt(b.D), cap,
+                                             ao.visible(len(x), T, None))
+        # bounds() takes 2^-21 of what it is given for the cap: past 64 a capped score is
+        # right to 2^-20 of itself, and it is at most |s| and at most cap
+        term = cap if cap <= 64 else 2 * np.minimum(dots, cap)
+        bo, bs = ao.bounds(b.D, torch.finfo(dtype).eps, o, l, mean, dots, spread, term, len(x),
+                           2.0 ** -25 if dtype is FP16 else 0.0)
+        assert (np.abs(got[s] - o) <= bo).all(), f"request {r}: off by {np.max(np.abs(got[s] - o) / bo):.3g} of its bound"
+        assert (np.abs(got_l[s] - l) <= bs).all(), f"request {r}: lse off by {np.max(np.abs(got_l[s] - l) / bs):.3g}"
+
+
 @pytest.mark.parametrize("fmt", [None, "mxfp8"])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("T,G", [(1, 1), (20, 1), (10, 8)])
