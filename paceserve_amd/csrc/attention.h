@@ -27,7 +27,9 @@
 // so a launch needs no plan and a captured one follows them; the grid has room for
 // the most chunks there can be, floor(pages / C) + requests.  A request of one chunk
 // is written directly; the others leave (o, m, l) in a workspace for the joining
-// kernels.
+// kernels: their chunks are numbered through once more, as parts.  A request of n > C
+// pages has at most ceil(n / C) <= 2 floor(n / C) chunks, so 2 floor(pages / C) parts are
+// enough, however many requests there are beside the split ones.
 //
 // Bounds on MI355X (kernel alone): up to 32 rows over a 16-bit cache HBM, 5.3 to 5.7
 // TB/s (256 ragged requests of up to 2048 tokens with 8 heads of 128, 8 rows each, 191 to
@@ -67,11 +69,11 @@ struct AttnParams {
   char* out;
   int64_t out_stride;
   float* lse;                  // [nnz, heads * group], or nullptr
-  float* part_o;               // [items, heads, row_tiles, rows of a tile, D]
-  float* part_ml;              // [items, heads, row_tiles, rows of a tile, 2]
+  float* part_o;               // [parts, heads, row_tiles, rows of a tile, D]
+  float* part_ml;              // [parts, heads, row_tiles, rows of a tile, 2]
   int32_t* err;
   uint32_t num_indices, batch, nnz, heads, group, num_pages, page_size, max_q, mask_words;
-  uint32_t chunk_pages, step_pages, items, row_tiles, tile_rows;
+  uint32_t chunk_pages, step_pages, items, parts, row_tiles, tile_rows;
   uint32_t join_turns, token_waves;  // of the joining kernel
   uint32_t page16, half16, row16;  // page, half page and token row, in 16-byte units
   uint32_t scale_at, scale_row;    // scales within a half page, scale bytes of a token
@@ -147,8 +149,7 @@ __device__ __forceinline__ uint32_t chunks_of(const AttnParams& p, uint32_t n) {
 }
 
 // The sizes of request b; false where its queries are not among nnz or exceed
-// max_q.  (Offsets that run backwards can count pages twice: a request whose items
-// do not fit p.items is refused as well.)
+// max_q.
 __device__ __forceinline__ bool request_of(const AttnParams& p, const Tables& t, Request* r) {
   r->first_page = max(t.k0, 0);
   r->pages = pages_of(p, t);
@@ -159,6 +160,13 @@ __device__ __forceinline__ bool request_of(const AttnParams& p, const Tables& t,
   r->q0 = static_cast<uint32_t>(t.a0);
   r->q_len = static_cast<uint32_t>(t.a1 - t.a0);
   return t.a0 >= 0 && t.a1 >= t.a0 && static_cast<uint32_t>(t.a1) <= p.nnz && r->q_len <= p.max_q;
+}
+
+// Whether a request's items and parts are among the call's: offsets that run backwards
+// can count pages twice.
+__device__ __forceinline__ bool has_room(const AttnParams& p, const Request& r, uint32_t first_item,
+                                         uint32_t first_part) {
+  return first_item + r.chunks <= p.items && (r.chunks == 1 || first_part + r.chunks <= p.parts);
 }
 
 // Sum over the lanes up to this one: within rows of 16 lanes by shifts, then each
@@ -174,17 +182,19 @@ __device__ __forceinline__ uint32_t sum_upto(uint32_t x) {
 }
 
 // The last request whose key is at most x, keys not decreasing: what the tables say
-// of it, and its first work item (the chunks of the requests before it); false if
-// there is none.  The wave looks at 256 requests a round, four neighbours to a
+// of it, its first work item (the chunks of the requests before it) and, where it is
+// split, its first part (those of the split ones before it); false if there is none.  The wave looks at 256 requests a round, four neighbours to a
 // lane, and holds what it loads of each, so up to 256 cost one load latency.
 template <class Key>
-__device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Key key, Tables* t, uint32_t* first_item) {
+__device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Key key, Tables* t, uint32_t* first_item,
+                                             uint32_t* first_part) {
   const uint32_t lane = threadIdx.x % 64;
   bool found = false;
-  uint32_t before = 0;                                   // chunks of the rounds before
+  uint32_t before = 0, whole_before = 0;                 // chunks, and requests of one, of the rounds before
   for (uint32_t e0 = 0; e0 < p.batch; e0 += 256) {
     Tables mine[4] = {};
     uint32_t start[4];
+    uint64_t whole[4];                                   // lanes whose k-th request has one chunk
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k)
       if (e0 + lane * 4 + k < p.batch) mine[k] = tables_of(p, e0 + lane * 4 + k);
@@ -192,7 +202,9 @@ __device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Ke
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
       start[k] = sum;
-      if (e0 + lane * 4 + k < p.batch) sum += chunks_of(p, pages_of(p, mine[k]));
+      const uint32_t n = e0 + lane * 4 + k < p.batch ? chunks_of(p, pages_of(p, mine[k])) : 0;
+      sum += n;
+      whole[k] = __ballot(n == 1);
     }
     const uint32_t upto = sum_upto(sum);                 // over the lanes up to this one
     int best = -1;
@@ -219,9 +231,18 @@ __device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Ke
       t->a0 = __builtin_amdgcn_readlane(of.a0, at);
       t->a1 = __builtin_amdgcn_readlane(of.a1, at);
       *first_item = __builtin_amdgcn_readlane(item, at);
+      // Its parts follow those of the split requests before it: all items but the whole ones'.
+      const uint64_t lanes = (uint64_t(1) << at) - 1;
+      const int kth = __builtin_amdgcn_readlane(best, at);
+      *first_part = *first_item - whole_before;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        *first_part -= static_cast<uint32_t>(__popcll(whole[k] & (k < kth ? lanes | uint64_t(1) << at : lanes)));
     }
     if (__builtin_amdgcn_readlane(best, 63) != 3) break;
     before += __builtin_amdgcn_readlane(upto, 63);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) whole_before += static_cast<uint32_t>(__popcll(whole[k]));
   }
   return found;
 }
@@ -348,11 +369,12 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   const uint32_t item = nth * kXcds + blockIdx.x % kXcds;
   if (item >= p.items) return;
   const uint32_t in_unit = at - nth * unit, head = over(p.by_tiles, in_unit), tile = in_unit - head * p.row_tiles;
-  uint32_t first_item;
+  uint32_t first_item, first_part;
   Tables tables;
-  if (!find_request(p, item, [](const Tables&, uint32_t start) { return start; }, &tables, &first_item)) return;
+  if (!find_request(p, item, [](const Tables&, uint32_t start) { return start; }, &tables, &first_item, &first_part))
+    return;
   Request r;
-  const bool valid_request = request_of(p, tables, &r) && first_item + r.chunks <= p.items;
+  const bool valid_request = request_of(p, tables, &r) && has_room(p, r, first_item, first_part);
   r.chunk = item - first_item;
   if (r.chunk >= r.chunks) return;
   if (!valid_request) {
@@ -770,7 +792,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   for (int a = 0; a < R; ++a) l[a] = across_groups(l[a], sum_of);
 
   const bool direct = r.chunks == 1;
-  const int64_t part_row0 = (static_cast<int64_t>(item) * unit + in_unit) * kTileRows;
+  const int64_t part_row0 = (static_cast<int64_t>(first_part + r.chunk) * unit + in_unit) * kTileRows;
   // Row `in_tile` of the tile: four output columns from d, and its m and l.
   const auto write = [&](uint32_t in_tile, uint32_t d, f32x4 o, float top, float sum, bool first) {
     const uint32_t row = row0 + in_tile;

@@ -15,20 +15,21 @@ struct Parts {
 };
 
 // The parts of rows of `token`; false where its request is not split.
-__device__ __forceinline__ bool parts_of(const AttnParams& p, uint32_t token, Request* r, uint32_t* first_item) {
+__device__ __forceinline__ bool parts_of(const AttnParams& p, uint32_t token, Request* r, uint32_t* first_part) {
   Tables t;
+  uint32_t first_item;
   return find_request(p, token, [](const Tables& x, uint32_t) { return static_cast<uint32_t>(max(x.a0, 0)); }, &t,
-                      first_item) &&
+                      &first_item, first_part) &&
          request_of(p, t, r) && token >= r->q0 && token - r->q0 < r->q_len && r->chunks > 1 &&
-         *first_item + r->chunks <= p.items;
+         has_room(p, *r, first_item, *first_part);
 }
 
-__device__ __forceinline__ Parts parts_of_row(const AttnParams& p, const Request& r, uint32_t first_item, uint32_t token,
+__device__ __forceinline__ Parts parts_of_row(const AttnParams& p, const Request& r, uint32_t first_part, uint32_t token,
                                               uint32_t qh) {
   const uint32_t head = over(p.by_group, qh), row = (token - r.q0) * p.group + (qh - head * p.group);
   const uint32_t tile = row / p.tile_rows;
   const int64_t unit = static_cast<int64_t>(p.heads) * p.row_tiles;
-  return {(static_cast<int64_t>(first_item) * unit + static_cast<int64_t>(head) * p.row_tiles + tile) * p.tile_rows +
+  return {(static_cast<int64_t>(first_part) * unit + static_cast<int64_t>(head) * p.row_tiles + tile) * p.tile_rows +
               row % p.tile_rows,
           unit * p.tile_rows, r.chunks};
 }
@@ -58,9 +59,9 @@ __global__ __launch_bounds__(kThreads) void combine_few_kernel(const AttnParams 
   const uint32_t lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t token = over(p.by_heads, blockIdx.x), qh = blockIdx.x - token * p.heads * p.group;
   Request r;
-  uint32_t first_item;
-  if (!parts_of(p, token, &r, &first_item)) return;
-  const auto [first, step, chunks] = parts_of_row(p, r, first_item, token, qh);
+  uint32_t first_part;
+  if (!parts_of(p, token, &r, &first_part)) return;
+  const auto [first, step, chunks] = parts_of_row(p, r, first_part, token, qh);
   const uint32_t col = lane % kCols, group = lane / kCols;
   // The wave's part of the chunks.
   const uint32_t per_wave = (chunks + kWaves - 1) / kWaves;
@@ -134,14 +135,14 @@ __global__ __launch_bounds__(kThreads) void combine_many_kernel(const AttnParams
   const uint32_t token = over(p.by_token_waves, wave);
   if (token >= p.nnz) return;
   Request r;
-  uint32_t first_item;
-  if (!parts_of(p, token, &r, &first_item)) return;
+  uint32_t first_part;
+  if (!parts_of(p, token, &r, &first_part)) return;
   const uint32_t col = lane % kCols, heads = p.heads * p.group;
   const uint32_t qh0 = (wave - token * p.token_waves) * p.join_turns * kGroups + lane / kCols;
   for (uint32_t turn = 0; turn < p.join_turns; ++turn) {
     const uint32_t qh = qh0 + turn * kGroups;
     if (qh >= heads) return;
-    const auto [first, step, chunks] = parts_of_row(p, r, first_item, token, qh);
+    const auto [first, step, chunks] = parts_of_row(p, r, first_part, token, qh);
     float m = -INFINITY;
 #pragma unroll 4
     for (uint32_t c = 0; c < chunks; ++c) m = fmaxf(m, p.part_ml[(first + c * step) * 2]);
@@ -161,8 +162,8 @@ __global__ __launch_bounds__(kThreads) void combine_many_kernel(const AttnParams
 
 // How a call is cut up.
 struct Split {
-  uint32_t tile_rows, row_tiles, chunk_pages, step_pages, items;
-  int64_t part_rows() const { return static_cast<int64_t>(items) * row_tiles * tile_rows; }  // times the KV heads
+  uint32_t tile_rows, row_tiles, chunk_pages, step_pages, items, parts;
+  int64_t part_rows() const { return static_cast<int64_t>(parts) * row_tiles * tile_rows; }  // times the KV heads
 };
 
 // A call's contexts are split so that every CU gets as many workgroups of about one
@@ -217,6 +218,7 @@ Split split_of(int64_t batch, int64_t heads, int64_t group, int head_dim, int64_
   chunk = std::max<int64_t>(std::min(chunk, num_indices), 1);
   s.chunk_pages = static_cast<uint32_t>(chunk);
   s.items = static_cast<uint32_t>(num_indices / chunk + batch);
+  s.parts = chunk >= num_indices ? 0 : std::min(s.items, static_cast<uint32_t>(2 * (num_indices / chunk)));
   return s;
 }
 
@@ -271,8 +273,7 @@ int check_sizes(int batch_size, int num_kv_heads, int group, int head_dim, int m
   return PACE_KV_OK;
 }
 
-int64_t workspace_bytes(const Split& s, int heads, int head_dim, int64_t num_indices) {
-  if (s.chunk_pages >= num_indices) return 0;            // no request has more than one chunk
+int64_t workspace_bytes(const Split& s, int heads, int head_dim) {
   return s.part_rows() * heads * (head_dim + 2) * 4;
 }
 
@@ -289,7 +290,7 @@ int pace_kv_attention_workspace(int batch_size, int num_kv_heads, int group, int
   *bytes = 0;                                            // of either kind of cache
   for (bool quantised : {false, true})
     *bytes = std::max(*bytes, workspace_bytes(split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices,
-                                                       page_size, quantised), num_kv_heads, head_dim, num_indices));
+                                                       page_size, quantised), num_kv_heads, head_dim));
   return PACE_KV_OK;
 }
 
@@ -336,7 +337,7 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
     return fail(PACE_KV_ERANGE, "attention: a layer's cache must be smaller than 64 GiB");
   const Split s = split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size,
                            format != PACE_KV_PLAIN);
-  const int64_t need = workspace_bytes(s, num_kv_heads, head_dim, num_indices);
+  const int64_t need = workspace_bytes(s, num_kv_heads, head_dim);
   if (need > 0 && (!workspace || workspace_size < need || reinterpret_cast<uintptr_t>(workspace) & 15u))
     return fail(PACE_KV_EINVAL, "attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
   AttnParams p = {};
@@ -366,6 +367,7 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   p.chunk_pages = s.chunk_pages;
   p.step_pages = s.step_pages;
   p.items = s.items;
+  p.parts = s.parts;
   p.row_tiles = s.row_tiles;
   p.tile_rows = s.tile_rows;
   p.half16 = static_cast<uint32_t>(half_bytes / 16);

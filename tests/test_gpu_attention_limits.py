@@ -139,3 +139,16 @@ def test_scores_far_past_any_exponential(gpu, size, T, G, dtype, fmt):
             score = (127 * 4.0 ** size + 0.75 * 4.0 ** size) * (scale or 1 / math.sqrt(D))
             # the scale as float32, times log2(e) and back: a few roundings of the score
             assert (lse[s].double() - score - math.log(2)).abs().max() <= 8 * 2.0 ** -24 * score
+
+
+def test_a_split_request_among_many_that_are_not(gpu):
+    """Parts are kept for split requests alone: their numbers skip the others'."""
+    rng = np.random.default_rng(31)
+    kv = rng.integers(1, 60, 600)
+    kv[[0, 3, 255, 256, 257, 300, 599]] = [9000, 12000, 0, 9500, 20000, 8800, 15000]
+    new = np.minimum(rng.integers(0, 3, 600), kv)
+    for H, G in ((1, 2), (4, 4)):
+        b = Batch(gpu, kv, new, H=H, G=G, D=64, seed=31)
+        out, lse = b.run()
+        torch.cuda.synchronize()
+        b.check(out, lse)
