@@ -256,6 +256,9 @@ uint32_t spare_lds(int head_dim, uint32_t tile_rows, bool quantised, int64_t bat
   return by_twos ? 14 << 10 : 0;                         // 41 KiB of its own; 160 KiB a CU
 }
 
+// Workgroups of a launch, whose threads are counted in 32 bits.
+constexpr int64_t kMostGroups = int64_t(1) << 24;
+
 int check_sizes(int batch_size, int num_kv_heads, int group, int head_dim, int max_q_len, int64_t num_indices,
                 int page_size) {
   if (batch_size < 0 || num_kv_heads <= 0 || group <= 0 || max_q_len <= 0 || num_indices < 0 || page_size <= 0)
@@ -263,13 +266,18 @@ int check_sizes(int batch_size, int num_kv_heads, int group, int head_dim, int m
   if (head_dim != 64 && head_dim != 128 && head_dim != 256)
     return fail(PACE_KV_EINVAL, "attention: head_dim must be 64, 128 or 256, got %d", head_dim);
   const int64_t rows = static_cast<int64_t>(max_q_len) * group;
-  if (num_indices * page_size > INT32_MAX / 2 || rows > INT32_MAX / 2)
+  if (num_indices > INT32_MAX / 2 / page_size || rows > INT32_MAX / 2)
     return fail(PACE_KV_ERANGE, "attention: more than 2^30 tokens or query rows");
+  // No product below passes 64 bits, and no divisor of the kernel 32: each factor is
+  // bounded before it is multiplied.
+  const int64_t tile = tile_rows_of(head_dim, rows), unit = num_kv_heads * ((rows + tile - 1) / tile);
+  bool fits = batch_size < kMostGroups && unit < kMostGroups && (batch_size + kXcds) * unit < kMostGroups;
   for (bool quantised : {false, true}) {
+    if (!fits) break;
     const Split s = split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size, quantised);
-    if ((static_cast<int64_t>(s.items) + kXcds) * num_kv_heads * s.row_tiles >= (int64_t(1) << 24))
-      return fail(PACE_KV_ERANGE, "attention: too many requests, heads or query rows for one call");
+    fits = (static_cast<int64_t>(s.items) + kXcds) * unit < kMostGroups;
   }
+  if (!fits) return fail(PACE_KV_ERANGE, "attention: too many requests, heads or query rows for one call");
   return PACE_KV_OK;
 }
 
@@ -333,7 +341,7 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   const int bits = format == PACE_KV_PLAIN ? 16 : mx_bits(format);
   const int64_t half_bytes = format == PACE_KV_PLAIN ? half * 2 : mx_half_bytes(half, format);
   if (half_bytes % 16) return fail(PACE_KV_EINVAL, "attention: half a page must be a multiple of 16 bytes");
-  if (num_pages * 2 * half_bytes / 16 >= UINT32_MAX)
+  if (half_bytes >= int64_t(1) << 36 || num_pages * (2 * half_bytes / 16) >= UINT32_MAX)
     return fail(PACE_KV_ERANGE, "attention: a layer's cache must be smaller than 64 GiB");
   const Split s = split_of(batch_size, num_kv_heads, group, head_dim, max_q_len, num_indices, page_size,
                            format != PACE_KV_PLAIN);

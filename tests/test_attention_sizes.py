@@ -6,11 +6,33 @@ import pytest
 from paceserve_amd import _native
 
 LIB = _native.load()
+ERANGE = _native.PACE_KV_ERANGE
 
 
 def workspace(batch=1, heads=8, group=4, D=128, max_q=1, num_indices=8192, page=16):
     out = ctypes.c_int64(-1)
     return LIB.pace_kv_attention_workspace(batch, heads, group, D, max_q, num_indices, page, ctypes.byref(out)), out.value
+
+
+@pytest.mark.parametrize("sizes", [
+    # (requests + 8) * heads * row tiles = 2^10 * 2^30 * 2^24 = 2^64
+    dict(batch=1016, heads=1 << 30, group=1, D=256, max_q=(1 << 30) - 1, num_indices=0),
+    # 2^20 * 2^20 * 2^24
+    dict(batch=(1 << 20) - 8, heads=1 << 20, group=1, D=256, max_q=(1 << 30) - 1, num_indices=0),
+    # pages * heads * row tiles past 2^63
+    dict(heads=1 << 30, group=1, D=256, max_q=(1 << 30) - 1, num_indices=1 << 26),
+    # tokens past 2^63
+    dict(num_indices=1 << 60, page=16), dict(num_indices=(1 << 62) + 1, page=4),
+    dict(batch=1 << 24, heads=1, num_indices=0), dict(batch=(1 << 31) - 1, num_indices=0)])
+def test_products_past_64_bits_are_refused(sizes):
+    assert workspace(**sizes)[0] == ERANGE
+    assert "too many" in LIB.pace_kv_last_error().decode() or "more than" in LIB.pace_kv_last_error().decode()
+
+
+def test_a_call_of_such_sizes_is_refused():
+    assert LIB.pace_kv_attention(0x1000, 1 << 30, 0, 1, 0x100, (1 << 20) - 8, 1 << 20, 1, 256, 0x2000, 0, 1, 1, 0x100, 0,
+                                 0x100, 0x100, (1 << 30) - 1, None, 0, 0.1, 0.0, 0x3000, 1 << 30, None, None, 0, None,
+                                 None) == ERANGE
 
 
 @pytest.mark.parametrize("batch,num_indices,max_q", [(256, 33024, 512), (256, 33024, 1024), (1024, 132096, 512)])
