@@ -517,10 +517,14 @@ int pace_kv_dequantize_pages(const void* const* src_layers,
  *
  * A query that sees nothing gets zeros and lse = -infinity.  A token that a
  * query does not see, and a slot past a request's last token, never affect it,
- * whatever they hold.  Rows of q outside every request are not written, and a
- * request with more than max_q_len tokens, or tokens outside [0, nnz), is
- * skipped and counted in err_count.  Tokens on a page whose id is outside
- * [0, num_pages) are not read and count as not seen.
+ * whatever they hold.  Rows of q outside every request are not written.
+ * err_count goes up by one for each token on a page whose id is outside
+ * [0, num_pages), which is not read and not seen by any query; for each request
+ * whose offsets lie outside [0, num_indices] or whose kv_last_page_len lies
+ * outside [0, page_size], which are cut to them (without pages the length is
+ * not looked at); and for each request that is skipped, its rows not written:
+ * one with more than max_q_len tokens, with tokens outside [0, nnz), or past
+ * the num_indices pages in all that the call has room for.
  *
  * Contexts are split over workgroups by the sizes here alone, so a captured
  * call follows tables that change between replays.  workspace (device,

@@ -122,6 +122,12 @@ struct Tables {
   int32_t k0, k1, last, a0, a1;
 };
 
+// Where a request stands among the call's: its number, its first work item and, where it
+// is split, its first part.
+struct Place {
+  uint32_t index, item, part;
+};
+
 __device__ __forceinline__ Tables tables_of(const AttnParams& p, uint32_t b) {
   Tables t;
   t.k0 = p.kv_indptr[b];
@@ -164,9 +170,14 @@ __device__ __forceinline__ bool request_of(const AttnParams& p, const Tables& t,
 
 // Whether a request's items and parts are among the call's: offsets that run backwards
 // can count pages twice.
-__device__ __forceinline__ bool has_room(const AttnParams& p, const Request& r, uint32_t first_item,
-                                         uint32_t first_part) {
-  return first_item + r.chunks <= p.items && (r.chunks == 1 || first_part + r.chunks <= p.parts);
+__device__ __forceinline__ bool has_room(const AttnParams& p, const Request& r, const Place& place) {
+  return place.item + r.chunks <= p.items && (r.chunks == 1 || place.part + r.chunks <= p.parts);
+}
+
+// Whether the tables name entries that do not exist, which pages_of and request_of cut off.
+__device__ __forceinline__ bool is_cut(const AttnParams& p, const Tables& t, const Request& r) {
+  return t.k0 < 0 || (t.k1 > 0 && static_cast<uint32_t>(t.k1) > p.num_indices) ||
+         (r.pages > 0 && static_cast<uint32_t>(t.last) > p.page_size);
 }
 
 // Sum over the lanes up to this one: within rows of 16 lanes by shifts, then each
@@ -182,12 +193,11 @@ __device__ __forceinline__ uint32_t sum_upto(uint32_t x) {
 }
 
 // The last request whose key is at most x, keys not decreasing: what the tables say
-// of it, its first work item (the chunks of the requests before it) and, where it is
-// split, its first part (those of the split ones before it); false if there is none.  The wave looks at 256 requests a round, four neighbours to a
+// of it, and its place (items: the chunks of the requests before it, parts: those of
+// the split ones before it); false if there is none.  The wave looks at 256 requests a round, four neighbours to a
 // lane, and holds what it loads of each, so up to 256 cost one load latency.
 template <class Key>
-__device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Key key, Tables* t, uint32_t* first_item,
-                                             uint32_t* first_part) {
+__device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Key key, Tables* t, Place* place) {
   const uint32_t lane = threadIdx.x % 64;
   bool found = false;
   uint32_t before = 0, whole_before = 0;                 // chunks, and requests of one, of the rounds before
@@ -230,14 +240,15 @@ __device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Ke
       t->last = __builtin_amdgcn_readlane(of.last, at);
       t->a0 = __builtin_amdgcn_readlane(of.a0, at);
       t->a1 = __builtin_amdgcn_readlane(of.a1, at);
-      *first_item = __builtin_amdgcn_readlane(item, at);
+      place->item = __builtin_amdgcn_readlane(item, at);
       // Its parts follow those of the split requests before it: all items but the whole ones'.
       const uint64_t lanes = (uint64_t(1) << at) - 1;
       const int kth = __builtin_amdgcn_readlane(best, at);
-      *first_part = *first_item - whole_before;
+      place->index = e0 + at * 4 + kth;
+      place->part = place->item - whole_before;
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        *first_part -= static_cast<uint32_t>(__popcll(whole[k] & (k < kth ? lanes | uint64_t(1) << at : lanes)));
+        place->part -= static_cast<uint32_t>(__popcll(whole[k] & (k < kth ? lanes | uint64_t(1) << at : lanes)));
     }
     if (__builtin_amdgcn_readlane(best, 63) != 3) break;
     before += __builtin_amdgcn_readlane(upto, 63);
@@ -369,18 +380,20 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   const uint32_t item = nth * kXcds + blockIdx.x % kXcds;
   if (item >= p.items) return;
   const uint32_t in_unit = at - nth * unit, head = over(p.by_tiles, in_unit), tile = in_unit - head * p.row_tiles;
-  uint32_t first_item, first_part;
+  Place place;
   Tables tables;
-  if (!find_request(p, item, [](const Tables&, uint32_t start) { return start; }, &tables, &first_item, &first_part))
-    return;
+  if (!find_request(p, item, [](const Tables&, uint32_t start) { return start; }, &tables, &place)) return;
   Request r;
-  const bool valid_request = request_of(p, tables, &r) && has_room(p, r, first_item, first_part);
-  r.chunk = item - first_item;
+  const bool valid_request = request_of(p, tables, &r) && has_room(p, r, place);
+  r.chunk = item - place.item;
   if (r.chunk >= r.chunks) return;
-  if (!valid_request) {
-    if (r.chunk == 0 && in_unit == 0 && threadIdx.x == 0 && p.err != nullptr) atomicAdd(p.err, 1);
-    return;
+  if (p.err != nullptr && in_unit == 0 && threadIdx.x == 0) {
+    if (r.chunk == 0 && (!valid_request || is_cut(p, tables, r))) atomicAdd(p.err, 1);
+    // Behind the last item lie requests that no workgroup looks at.
+    if (item + 1 == p.items && place.index + 1 < p.batch)
+      atomicAdd(p.err, static_cast<int32_t>(p.batch - 1 - place.index));
   }
+  if (!valid_request) return;
   const uint32_t rows = r.q_len * p.group, row0 = tile * kTileRows;
   if (row0 >= rows) return;
   const int32_t base = static_cast<int32_t>(r.kv_len) - static_cast<int32_t>(r.q_len);
@@ -396,6 +409,15 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   const int32_t t_begin = static_cast<int32_t>(r.chunk) * chunk_tokens;
   int32_t t_end = static_cast<int32_t>(min(static_cast<int64_t>(t_begin) + chunk_tokens, static_cast<int64_t>(r.kv_len)));
   if (p.mask == nullptr) t_end = min(t_end, base + last_q + 1);
+  // Tokens on pages that do not exist are counted by one workgroup of those over a chunk,
+  // the last row tile's: it sees all of the chunk.  A look at the pages of its own, that
+  // calls without a counter do not take, and no registers in the steps below.
+  if (p.err != nullptr && head == 0 && row0 + kTileRows >= rows) {
+    const int32_t page = static_cast<int32_t>(p.page_size), first = static_cast<int32_t>(r.chunk * length);
+    for (int32_t i = static_cast<int32_t>(threadIdx.x); static_cast<int64_t>(i) * page < t_end - t_begin; i += kThreads)
+      if (static_cast<uint32_t>(p.kv_indices[r.first_page + first + i]) >= p.num_pages)
+        atomicAdd(p.err, min(page, t_end - t_begin - i * page));
+  }
 
   // Query fragments: row n of each tile, eight elements from 32 * k + 8 * g.  In
   // registers, or (WR = 1, whose registers hold more loads in flight) in LDS.
@@ -792,7 +814,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   for (int a = 0; a < R; ++a) l[a] = across_groups(l[a], sum_of);
 
   const bool direct = r.chunks == 1;
-  const int64_t part_row0 = (static_cast<int64_t>(first_part + r.chunk) * unit + in_unit) * kTileRows;
+  const int64_t part_row0 = (static_cast<int64_t>(place.part + r.chunk) * unit + in_unit) * kTileRows;
   // Row `in_tile` of the tile: four output columns from d, and its m and l.
   const auto write = [&](uint32_t in_tile, uint32_t d, f32x4 o, float top, float sum, bool first) {
     const uint32_t row = row0 + in_tile;

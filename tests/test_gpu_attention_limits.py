@@ -8,7 +8,8 @@ import pytest
 import torch
 
 from oracle import attention_oracle as ao
-from test_gpu_attention import BF16, FP16, Batch
+from paceserve_amd.kv_transfer.attention import paged_attention
+from test_gpu_attention import BF16, FP16, Batch, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -139,6 +140,66 @@ def test_scores_far_past_any_exponential(gpu, size, T, G, dtype, fmt):
             score = (127 * 4.0 ** size + 0.75 * 4.0 ** size) * (scale or 1 / math.sqrt(D))
             # the scale as float32, times log2(e) and back: a few roundings of the score
             assert (lse[s].double() - score - math.log(2)).abs().max() <= 8 * 2.0 ** -24 * score
+
+
+@pytest.mark.parametrize("T,G,kv", [(1, 1, 100), (1, 4, 9000), (20, 2, 100), (30, 8, 5000)])
+@pytest.mark.parametrize("fmt", [None, "mxfp4"])
+def test_tokens_on_bad_pages_are_counted(gpu, T, G, kv, fmt):
+    """Each token that lies on a page outside the pool once, however many heads, row
+    tiles, waves and chunks look at it."""
+    b = Batch(gpu, [kv, 90, 64], [T, T, T], G=G, fmt=fmt, seed=4, tree=G == 2)
+    b.indices = b.indices.copy()
+    last = b.indptr[1] - 1
+    b.indices[2], b.indices[last], b.indices[b.indptr[1]] = b.num_pages, 1 << 30, -5
+    err = torch.zeros(1, dtype=torch.int32, device=gpu)
+    out, lse = b.run(err=err)
+    torch.cuda.synchronize()
+    b.check(out, lse, hidden=lambda r, p: ((p // 16 == 2) | (p // 16 == last)) if r == 0 else (p // 16 == 0) if r == 1
+            else p < 0)
+    assert err.item() == 32 + (kv - 1) % 16 + 1
+
+
+def test_lengths_outside_the_pages_are_counted(gpu):
+    b = Batch(gpu, [100, 90, 64, 20], [3, 5, 2, 1], seed=4)
+    idx, ip, last = b.tables()
+    qo = i32(b.qo, gpu)
+    want, _ = b.run()
+    for at, bad in ((0, 17), (1, -1), (3, 1 << 30), (3, -(1 << 31))):
+        err = torch.zeros(1, dtype=torch.int32, device=gpu)
+        l2 = last.clone()
+        l2[at] = bad
+        out = paged_attention(b.q, b.cache, idx, ip, l2, qo, max_q_len=5, err=err)
+        assert err.item() == 1
+        for r in range(4):
+            if r != at:
+                assert torch.equal(out[b.qo[r]:b.qo[r + 1]], want[b.qo[r]:b.qo[r + 1]])
+    err = torch.zeros(1, dtype=torch.int32, device=gpu)
+    none = paged_attention(b.q, b.cache, idx, i32([0] * 5, gpu), last, qo, max_q_len=5, err=err)
+    assert err.item() == 0 and (none == 0).all()            # without pages the last one's length means nothing
+    # offsets past the table: cut to it, and counted
+    ip2 = ip.clone()
+    ip2[4] += 3
+    out = paged_attention(b.q, b.cache, idx, ip2, last, qo, max_q_len=5, err=err)
+    assert err.item() == 1 and torch.equal(out, want)
+    err.zero_()
+    ip2 = ip.clone()
+    ip2[0] = -2
+    out = paged_attention(b.q, b.cache, idx, ip2, last, qo, max_q_len=5, err=err)
+    assert err.item() == 1 and torch.equal(out, want)
+
+
+def test_requests_past_the_work_items_are_counted(gpu):
+    """kv_indptr [0, 200, 0, 200, 0, 200, 200]: pages counted three times over.  The last requests' items lie
+    past those that the call has room for: none of them is lost without a count."""
+    b = Batch(gpu, [3200, 0, 0, 0, 0, 0], [1, 0, 0, 0, 0, 0], H=2, G=1, seed=8)
+    q = b.q.repeat(6, 1, 1)
+    out = torch.full_like(q, 7.0)
+    err = torch.zeros(1, dtype=torch.int32, device=gpu)
+    paged_attention(q, b.cache, i32(b.indices, gpu), i32([0, 200, 0, 200, 0, 200, 200], gpu), i32([16] * 6, gpu), out=out,
+                    err=err)
+    left = [(out[r] == 7).all().item() for r in range(6)]
+    assert left[:3] == [False, False, True] and (out[1] == 0).all()
+    assert err.item() == sum(left)
 
 
 def test_a_split_request_among_many_that_are_not(gpu):
