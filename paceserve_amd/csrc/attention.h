@@ -122,10 +122,9 @@ struct Tables {
   int32_t k0, k1, last, a0, a1;
 };
 
-// Where a request stands among the call's: its number, its first work item and, where it
-// is split, its first part.
+// Where a request stands among the call's: its number and its first work item.
 struct Place {
-  uint32_t index, item, part;
+  uint32_t index, item;
 };
 
 __device__ __forceinline__ Tables tables_of(const AttnParams& p, uint32_t b) {
@@ -170,8 +169,8 @@ __device__ __forceinline__ bool request_of(const AttnParams& p, const Tables& t,
 
 // Whether a request's items and parts are among the call's: offsets that run backwards
 // can count pages twice.
-__device__ __forceinline__ bool has_room(const AttnParams& p, const Request& r, const Place& place) {
-  return place.item + r.chunks <= p.items && (r.chunks == 1 || place.part + r.chunks <= p.parts);
+__device__ __forceinline__ bool has_room(const AttnParams& p, const Request& r, const Place& place, uint32_t part) {
+  return place.item + r.chunks <= p.items && (r.chunks == 1 || part + r.chunks <= p.parts);
 }
 
 // Whether the tables name entries that do not exist, which pages_of and request_of cut off.
@@ -193,18 +192,17 @@ __device__ __forceinline__ uint32_t sum_upto(uint32_t x) {
 }
 
 // The last request whose key is at most x, keys not decreasing: what the tables say
-// of it, and its place (items: the chunks of the requests before it, parts: those of
-// the split ones before it); false if there is none.  The wave looks at 256 requests a round, four neighbours to a
+// of it, and its place (items: the chunks of the requests before it); false if there
+// is none.  The wave looks at 256 requests a round, four neighbours to a
 // lane, and holds what it loads of each, so up to 256 cost one load latency.
 template <class Key>
 __device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Key key, Tables* t, Place* place) {
   const uint32_t lane = threadIdx.x % 64;
   bool found = false;
-  uint32_t before = 0, whole_before = 0;                 // chunks, and requests of one, of the rounds before
+  uint32_t before = 0;                                   // chunks of the rounds before
   for (uint32_t e0 = 0; e0 < p.batch; e0 += 256) {
     Tables mine[4] = {};
     uint32_t start[4];
-    uint64_t whole[4];                                   // lanes whose k-th request has one chunk
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k)
       if (e0 + lane * 4 + k < p.batch) mine[k] = tables_of(p, e0 + lane * 4 + k);
@@ -212,9 +210,7 @@ __device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Ke
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
       start[k] = sum;
-      const uint32_t n = e0 + lane * 4 + k < p.batch ? chunks_of(p, pages_of(p, mine[k])) : 0;
-      sum += n;
-      whole[k] = __ballot(n == 1);
+      if (e0 + lane * 4 + k < p.batch) sum += chunks_of(p, pages_of(p, mine[k]));
     }
     const uint32_t upto = sum_upto(sum);                 // over the lanes up to this one
     int best = -1;
@@ -241,21 +237,32 @@ __device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Ke
       t->a0 = __builtin_amdgcn_readlane(of.a0, at);
       t->a1 = __builtin_amdgcn_readlane(of.a1, at);
       place->item = __builtin_amdgcn_readlane(item, at);
-      // Its parts follow those of the split requests before it: all items but the whole ones'.
-      const uint64_t lanes = (uint64_t(1) << at) - 1;
-      const int kth = __builtin_amdgcn_readlane(best, at);
-      place->index = e0 + at * 4 + kth;
-      place->part = place->item - whole_before;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        place->part -= static_cast<uint32_t>(__popcll(whole[k] & (k < kth ? lanes | uint64_t(1) << at : lanes)));
+      place->index = e0 + at * 4 + __builtin_amdgcn_readlane(best, at);
     }
     if (__builtin_amdgcn_readlane(best, 63) != 3) break;
     before += __builtin_amdgcn_readlane(upto, 63);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) whole_before += static_cast<uint32_t>(__popcll(whole[k]));
   }
   return found;
+}
+
+// The first part of a split request: its items but for those before it of requests that
+// are not split, one each.  Read apart from the search, which every workgroup makes:
+// there it costs calls that split nothing 5 % (MI355X, 1000 requests of 100 tokens, 134
+// to 140 us).
+__device__ __forceinline__ uint32_t first_part_of(const AttnParams& p, const Place& place) {
+  uint32_t whole = 0;
+  for (uint32_t e0 = 0; e0 < place.index; e0 += 64) {
+    const uint32_t e = e0 + threadIdx.x % 64;
+    bool one = false;
+    if (e < place.index) {
+      Tables t = {};
+      t.k0 = p.kv_indptr[e];
+      t.k1 = p.kv_indptr[e + 1];
+      one = chunks_of(p, pages_of(p, t)) == 1;
+    }
+    whole += static_cast<uint32_t>(__popcll(__ballot(one)));
+  }
+  return place.item - whole;
 }
 
 // Rows in LDS are padded by 32 bytes, so that 8 rows' 32 bytes of a transposing
@@ -384,7 +391,9 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   Tables tables;
   if (!find_request(p, item, [](const Tables&, uint32_t start) { return start; }, &tables, &place)) return;
   Request r;
-  const bool valid_request = request_of(p, tables, &r) && has_room(p, r, place);
+  const bool of_call = request_of(p, tables, &r);
+  const uint32_t first_part = r.chunks == 1 ? 0 : first_part_of(p, place);
+  const bool valid_request = of_call && has_room(p, r, place, first_part);
   r.chunk = item - place.item;
   if (r.chunk >= r.chunks) return;
   if (p.err != nullptr && in_unit == 0 && threadIdx.x == 0) {
@@ -814,7 +823,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   for (int a = 0; a < R; ++a) l[a] = across_groups(l[a], sum_of);
 
   const bool direct = r.chunks == 1;
-  const int64_t part_row0 = (static_cast<int64_t>(place.part + r.chunk) * unit + in_unit) * kTileRows;
+  const int64_t part_row0 = (static_cast<int64_t>(first_part + r.chunk) * unit + in_unit) * kTileRows;
   // Row `in_tile` of the tile: four output columns from d, and its m and l.
   const auto write = [&](uint32_t in_tile, uint32_t d, f32x4 o, float top, float sum, bool first) {
     const uint32_t row = row0 + in_tile;

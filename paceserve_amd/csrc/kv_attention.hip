@@ -15,20 +15,22 @@ struct Parts {
 };
 
 // The parts of rows of `token`; false where its request is not split.
-__device__ __forceinline__ bool parts_of(const AttnParams& p, uint32_t token, Request* r, Place* place) {
+__device__ __forceinline__ bool parts_of(const AttnParams& p, uint32_t token, Request* r, uint32_t* first_part) {
   Tables t;
-  return find_request(p, token, [](const Tables& x, uint32_t) { return static_cast<uint32_t>(max(x.a0, 0)); }, &t,
-                      place) &&
-         request_of(p, t, r) && token >= r->q0 && token - r->q0 < r->q_len && r->chunks > 1 &&
-         has_room(p, *r, *place);
+  Place place;
+  if (!find_request(p, token, [](const Tables& x, uint32_t) { return static_cast<uint32_t>(max(x.a0, 0)); }, &t, &place) ||
+      !request_of(p, t, r) || token < r->q0 || token - r->q0 >= r->q_len || r->chunks == 1)
+    return false;
+  *first_part = first_part_of(p, place);
+  return has_room(p, *r, place, *first_part);
 }
 
-__device__ __forceinline__ Parts parts_of_row(const AttnParams& p, const Request& r, const Place& place, uint32_t token,
+__device__ __forceinline__ Parts parts_of_row(const AttnParams& p, const Request& r, uint32_t first_part, uint32_t token,
                                               uint32_t qh) {
   const uint32_t head = over(p.by_group, qh), row = (token - r.q0) * p.group + (qh - head * p.group);
   const uint32_t tile = row / p.tile_rows;
   const int64_t unit = static_cast<int64_t>(p.heads) * p.row_tiles;
-  return {(static_cast<int64_t>(place.part) * unit + static_cast<int64_t>(head) * p.row_tiles + tile) * p.tile_rows +
+  return {(static_cast<int64_t>(first_part) * unit + static_cast<int64_t>(head) * p.row_tiles + tile) * p.tile_rows +
               row % p.tile_rows,
           unit * p.tile_rows, r.chunks};
 }
@@ -58,9 +60,9 @@ __global__ __launch_bounds__(kThreads) void combine_few_kernel(const AttnParams 
   const uint32_t lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t token = over(p.by_heads, blockIdx.x), qh = blockIdx.x - token * p.heads * p.group;
   Request r;
-  Place place;
-  if (!parts_of(p, token, &r, &place)) return;
-  const auto [first, step, chunks] = parts_of_row(p, r, place, token, qh);
+  uint32_t first_part;
+  if (!parts_of(p, token, &r, &first_part)) return;
+  const auto [first, step, chunks] = parts_of_row(p, r, first_part, token, qh);
   const uint32_t col = lane % kCols, group = lane / kCols;
   // The wave's part of the chunks.
   const uint32_t per_wave = (chunks + kWaves - 1) / kWaves;
@@ -134,14 +136,14 @@ __global__ __launch_bounds__(kThreads) void combine_many_kernel(const AttnParams
   const uint32_t token = over(p.by_token_waves, wave);
   if (token >= p.nnz) return;
   Request r;
-  Place place;
-  if (!parts_of(p, token, &r, &place)) return;
+  uint32_t first_part;
+  if (!parts_of(p, token, &r, &first_part)) return;
   const uint32_t col = lane % kCols, heads = p.heads * p.group;
   const uint32_t qh0 = (wave - token * p.token_waves) * p.join_turns * kGroups + lane / kCols;
   for (uint32_t turn = 0; turn < p.join_turns; ++turn) {
     const uint32_t qh = qh0 + turn * kGroups;
     if (qh >= heads) return;
-    const auto [first, step, chunks] = parts_of_row(p, r, place, token, qh);
+    const auto [first, step, chunks] = parts_of_row(p, r, first_part, token, qh);
     float m = -INFINITY;
 #pragma unroll 4
     for (uint32_t c = 0; c < chunks; ++c) m = fmaxf(m, p.part_ml[(first + c * step) * 2]);
