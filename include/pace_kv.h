@@ -513,7 +513,7 @@ int pace_kv_dequantize_pages(const void* const* src_layers,
  * head h / group; lse is [nnz, num_kv_heads * group] float or NULL.
  * head_dim is 64, 128 or 256.  The cache is one layer's, of elem_type
  * (format PACE_KV_PLAIN) or quantised, whose values are those that
- * pace_kv_dequantize_pages gives in elem_type.
+ * pace_kv_dequantize_pages gives in elem_type; NULL if num_pages is 0.
  *
  * A query that sees nothing gets zeros and lse = -infinity.  A token that a
  * query does not see, and a slot past a request's last token, never affect it,

@@ -326,7 +326,8 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type, int6
   if (nnz * num_kv_heads * group >= (int64_t(1) << 24))
     return fail(PACE_KV_ERANGE, "attention: 2^24 query rows or more");
   if (nnz == 0 || batch_size == 0) return PACE_KV_OK;
-  if (!q || !cache || !kv_indptr || !kv_last_page_len || !out || (num_indices > 0 && !kv_indices))
+  // A pool without pages has no memory, and none of its pages is read.
+  if (!q || (num_pages > 0 && !cache) || !kv_indptr || !kv_last_page_len || !out || (num_indices > 0 && !kv_indices))
     return fail(PACE_KV_EINVAL, "attention: NULL argument");
   if (!qo_indptr && nnz != batch_size)
     return fail(PACE_KV_EINVAL, "attention: without qo_indptr each request has one token");

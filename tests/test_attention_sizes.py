@@ -6,7 +6,7 @@ import pytest
 from paceserve_amd import _native
 
 LIB = _native.load()
-ERANGE = _native.PACE_KV_ERANGE
+EINVAL, ERANGE = _native.PACE_KV_EINVAL, _native.PACE_KV_ERANGE
 
 
 def workspace(batch=1, heads=8, group=4, D=128, max_q=1, num_indices=8192, page=16):
@@ -43,3 +43,12 @@ def test_requests_that_are_not_split_take_no_workspace(batch, num_indices, max_q
     rows = 8 * max_q * 8                                   # of all heads
     # rows enough to fill the CUs: chunks of a third of all pages, or more
     assert rc == 0 and size <= 2 * 3 * rows * (128 + 2) * 4
+
+
+def test_a_pool_without_pages_needs_no_memory():
+    def call(pages, space):
+        return LIB.pace_kv_attention(0x1000, 8192, 0, 8, 0x100, 2, 8, 4, 128, None, 0, pages, 16, 0x100, 4096, 0x100,
+                                     0x100, 4, None, 0, 0.1, 0.0, 0x3000, 8192, None, space, 0, None, None)
+
+    assert call(9, None) == EINVAL and "NULL" in LIB.pace_kv_last_error().decode()
+    assert call(0, None) == EINVAL and "workspace" in LIB.pace_kv_last_error().decode()  # the next thing it lacks

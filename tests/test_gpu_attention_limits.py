@@ -202,6 +202,19 @@ def test_requests_past_the_work_items_are_counted(gpu):
     assert err.item() == sum(left)
 
 
+def test_a_pool_without_pages(gpu):
+    q = torch.randn(3, 8, 64, dtype=BF16, device=gpu)
+    for cache in (torch.zeros(0, 2, 16, 2, 64, dtype=BF16, device=gpu),
+                  torch.zeros(0, 2, 16, 2, 66, dtype=torch.uint8, device=gpu)):
+        idx, err = i32([], gpu), torch.zeros(1, dtype=torch.int32, device=gpu)
+        out, lse = paged_attention(q, cache, idx, i32([0] * 4, gpu), i32([0] * 3, gpu), return_lse=True, err=err)
+        assert (out == 0).all() and torch.isneginf(lse).all() and err.item() == 0
+        # pages named all the same are outside the pool
+        out, lse = paged_attention(q, cache, i32([0, 1, 2], gpu), i32([0, 1, 2, 3], gpu), i32([16, 2, 1], gpu),
+                                   return_lse=True, err=err)
+        assert (out == 0).all() and torch.isneginf(lse).all()
+
+
 def test_a_split_request_among_many_that_are_not(gpu):
     """Parts are kept for split requests alone: their numbers skip the others'."""
     rng = np.random.default_rng(31)
