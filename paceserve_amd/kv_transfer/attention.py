@@ -71,13 +71,21 @@ def paged_attention(q: torch.Tensor, paged_kv_cache: torch.Tensor, kv_indices: t
     j // 64 of its row is set, else itself and those before it.  One that sees
     nothing gets zeros and a log-sum-exp of -inf.
 
-    Scores are float32 sums: a key whose products with a query pass its range
-    makes that query's row NaN.
+    Scores and weighted sums are float32: a key whose products with a query
+    pass its range upwards makes that query's row NaN, and values whose weighted
+    sum passes it make the output infinite or NaN.  There is no backward pass:
+    tensors that require gradients are refused while gradients are enabled.
+
+    `err` goes up by one for each token on a page whose id is out of range (not
+    read, not seen), each request whose offsets or last page's length are (cut),
+    and each that is skipped, its rows not written.
 
     logits_soft_cap > 0 replaces scores s by cap * tanh(s / cap).  sm_scale is
     1 / sqrt(head_dim) by default.  Returns out ([nnz, num_qo_heads, head_dim],
     `out` if given; rows outside every request are not written), and with
     return_lse also the natural log-sum-exp [nnz, num_qo_heads] float32."""
+    if torch.is_grad_enabled() and (q.requires_grad or paged_kv_cache.requires_grad):
+        raise ValueError("paged_attention has no backward pass: call it under torch.no_grad() or with detached tensors")
     fmt = _check(q, paged_kv_cache)
     cache = paged_kv_cache
     dev, at = cache.device, cache.get_device()
