@@ -111,6 +111,34 @@ def test_soft_caps_of_every_size(gpu, cap, T, G, dtype, fmt):
         assert (np.abs(got_l[s] - l) <= bs).all(), f"request {r}: lse off by {np.max(np.abs(got_l[s] - l) / bs):.3g}"
 
 
+@pytest.mark.parametrize("dtype,fmt", [(BF16, None), (FP16, None), (BF16, "mxfp8")])
+@pytest.mark.parametrize("T,G", [(6, 2), (20, 8)])
+def test_infinite_values_reach_those_that_see_them(gpu, dtype, fmt, T, G):
+    """An infinity makes an output infinite, of its sign, exactly where its token is
+    seen; two of opposite signs make it NaN.  (In a quantised cache its block is NaN.)"""
+    b = Batch(gpu, [50, 200], [T, T], dtype=dtype, fmt=fmt, tree=True, G=G, seed=3)
+    for x, n in zip(b.rows, b.kv):
+        x[n - T + 2, 1, 0, 5] = math.inf
+        x[n - T + 3, 1, 1, 7] = -math.inf
+        x[n - T + 4, 1, 0, 5] = -math.inf
+    for r in range(2):
+        for i in range(T):
+            b.mask[b.qo[r] + i, 0] = np.uint64(1 << i | (4 if i % 3 == 0 else 0) | (8 if i % 2 else 0))
+    b.fill()
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    b.check(out, lse)
+    got = out.double().cpu().numpy()
+    infinite = 0
+    for r, x in enumerate(b.seen_rows):
+        s = slice(b.qo[r], b.qo[r + 1])
+        o = ao.attend(b.q[s].double().cpu().numpy(), x[:, 0], x[:, 1], 1 / math.sqrt(b.D), 0.0,
+                      ao.visible(len(x), T, b.mask[s]))[0]
+        assert np.array_equal(np.isposinf(got[s]), np.isposinf(o)) and np.array_equal(np.isneginf(got[s]), np.isneginf(o))
+        infinite += int(np.isinf(o).sum())
+    assert infinite > 0 or fmt is not None
+
+
 @pytest.mark.parametrize("fmt", [None, "mxfp8"])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 @pytest.mark.parametrize("T,G", [(1, 1), (20, 1), (10, 8)])
