@@ -309,6 +309,14 @@ __device__ __forceinline__ uint32_t result_pair(float a, float b) {
   return pair_of<TYPE>(a, b);
 }
 
+// Natural logarithm of a row's sum of exponentials, l over 2^m.  The 15 that m lies below
+// the largest score in float16 go back first: both terms would lose bits to them.
+template <int TYPE>
+__device__ __forceinline__ float log_sum(float m, float l) {
+  constexpr float kTop = kTopWeight<TYPE>, kScale = TYPE == PACE_KV_FP16 ? 0x1p-15f : 1.f;
+  return l == 0.f ? -INFINITY : (m + kTop + __log2f(l * kScale)) * 0.69314718055994531f;
+}
+
 // Hides where x comes from, so that what a loop derives from it is derived anew
 // each time (an add) instead of being held in a register throughout.
 __device__ __forceinline__ uint32_t opaque(uint32_t x) {
@@ -365,7 +373,10 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   constexpr int kDT = D / 16, kKS = D / 32;
   constexpr bool kTight = R == 2 && WR == 4 && D == 128 && FORMAT != PACE_KV_PLAIN;  // three waves fill the registers
   // Rows that no other workgroup reads are loaded nontemporally, unless two heads
-  // share a 128-byte line.  MI355X, reading 2 GiB of pages of 8 heads in this pattern:
+  // share a 128-byte line; with head_dim 256 past 64 rows, whose tiles share them, as
+  // well: one kernel serves one tile and several (bf16, 36 to 64 rows over 8 x 4096 to
+  // 24 x 2000 tokens 5 to 16% faster so, 128 and 320 rows up to 7% slower; 8 and 4 bits
+  // the same within 5%).  MI355X, reading 2 GiB of pages of 8 heads in this pattern:
   // 256-byte rows 6.4 TB/s against 5.8, 128-byte ones 6.3 against 5.6, 64-byte ones
   // 4.8 against 5.9 (and 3.5 with the heads of a page on different XCDs).
   constexpr bool kReadOnce = (WR == 1 || R == 1) && D * kBits / 8 >= 128;
@@ -843,8 +854,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
     *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(r.q0 + i) * p.out_stride +
                               (static_cast<int64_t>(qh) * D + d) * 2) = x;
     if (first && p.lse != nullptr)
-      p.lse[static_cast<int64_t>(r.q0 + i) * p.heads * p.group + qh] =
-          sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.69314718055994531f;
+      p.lse[static_cast<int64_t>(r.q0 + i) * p.heads * p.group + qh] = log_sum<TYPE>(top, sum);
   };
   if (WR != 1) {
 #pragma unroll

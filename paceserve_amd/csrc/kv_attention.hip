@@ -44,8 +44,7 @@ __device__ __forceinline__ void write_row(const AttnParams& p, uint32_t token, u
   *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(token) * p.out_stride +
                             (static_cast<int64_t>(qh) * D + col * 4) * 2) = x;
   if (col == 0 && p.lse != nullptr)
-    p.lse[static_cast<int64_t>(token) * (p.heads * p.group) + qh] =
-        l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+    p.lse[static_cast<int64_t>(token) * (p.heads * p.group) + qh] = log_sum<TYPE>(m, l);
 }
 
 // Few rows of many chunks: a workgroup joins a row.  D / 4 lanes take four columns

@@ -71,6 +71,27 @@ def test_float16_keeps_many_small_weights(gpu, nats, T, fmt):
             f"request {r}: off by {np.max(np.abs(got[s] - o) / (bo + 2.0 ** -25)):.3g} of the bound"
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("kv,T", [([1, 2, 3, 4], 1), ([24, 21], 20), ([9000], 2)])
+def test_log_sums_near_zero(gpu, kv, T, dtype):
+    """Small scores: a log-sum-exp to a few float32 roundings of its own terms.  Bound: the
+    scores' D + 4 roundings of sum |q k|; an exponential's 2^-23 and its argument's 2^-24;
+    sums of n / 4 of a lane, then of 4 lanes, and of waves and chunks; the logarithm's 2^-23 of
+    itself, at most log2(n); three roundings of the result's terms."""
+    b = Batch(gpu, kv, [T] * len(kv), D=64, dtype=dtype, seed=len(kv), q_gain=0.001)
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    for r, x in enumerate(b.seen_rows):
+        s = slice(b.qo[r], b.qo[r + 1])
+        o, l, mean, dots, spread = ao.attend(b.q[s].double().cpu().numpy(), x[:, 0], x[:, 1], 1 / math.sqrt(b.D), 0.0,
+                                             ao.visible(len(x), T, None))
+        n, unit = len(x), 2.0 ** -24
+        terms = math.log2(n) + dots * math.log2(math.e)
+        bound = (b.D + 4) * unit * dots + (3 + min(n, 512) / 4 + (16 if n > 32 else 2)) * unit + 5 * terms * unit
+        assert (np.abs(lse[s].double().cpu().numpy() - l) <= bound).all(), \
+            f"request {r}: off by {np.max(np.abs(lse[s].double().cpu().numpy() - l) / bound):.3g} of the bound"
+
+
 @pytest.mark.parametrize("T", [1, 40])
 @pytest.mark.parametrize("rising", [False, True])
 def test_values_of_float16s_largest_stay_finite(gpu, rising, T):
