@@ -275,3 +275,13 @@ def test_a_split_request_among_many_that_are_not(gpu):
         out, lse = b.run()
         torch.cuda.synchronize()
         b.check(out, lse)
+
+
+@pytest.mark.parametrize("dtype,fmt", [(BF16, None), (FP16, "mxfp8")])
+def test_prompts_over_the_pages(gpu, dtype, fmt):
+    """More than a thousand causal queries of a request, beside a short one and a
+    single token, whose row tiles then are as large."""
+    b = Batch(gpu, [1500, 700, 40], [1100, 1, 40], H=1, G=2, D=64, dtype=dtype, fmt=fmt, seed=41)
+    out, lse = b.run()
+    torch.cuda.synchronize()
+    b.check(out, lse)
