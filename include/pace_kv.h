@@ -472,10 +472,13 @@ int pace_kv_append_mx_indptr(const void* keys, const void* values,
  * Pages from a pool of elem_type into a quantised pool, and back, all layers
  * in one call: page dst_ids[j] of layer l becomes the quantised page src_ids[j]
  * of layer l (every slot of it, stale ones included), or its values rounded to
- * elem_type (a value past the type's range reads as infinity).  half_elems =
- * page_size * H * D.  Ids are device arrays of n_pages; a page whose id is out
- * of range on either side is skipped and counted once per layer in err_count.
- * Destination ids must be distinct, and the pools must not share memory.
+ * elem_type.  A value past the type's range reads as infinity: what float16
+ * pages held from 57344 (4 bits) or 63488 (8 bits) on is rounded to 65536 and
+ * read so.
+ * half_elems = page_size * H * D.  Ids are device arrays of n_pages; a page
+ * whose id is out of range on either side is skipped and counted once per layer
+ * in err_count.  Destination ids must be distinct, and the pools must not share
+ * memory.
  */
 int pace_kv_quantize_pages(const void* const* src_layers,
                            int64_t src_pool_pages, const int32_t* src_ids,

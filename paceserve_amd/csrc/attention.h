@@ -33,13 +33,13 @@
 //
 // Bounds on MI355X (kernel alone): up to 32 rows over a 16-bit cache HBM, 5.3 to 5.7
 // TB/s (256 ragged requests of up to 2048 tokens with 8 heads of 128, 8 rows each, 191 to
-// 198 us; 12 rows of 32 heads over 32768 tokens 94 to 96 us).  Over a quantised cache, and
-// with more rows, expansion, exponentials and matrix instructions take about the same
-// issue time each and overlap only in part: 504 rows over 8 x 4096 8-bit tokens 105 us,
-// where the products alone take 27 at the matrix peak (counters: matrix instructions
-// 32% of the time, vector ones 55%, LDS 28%; of an earlier 119 us leaving out any one of
-// them saved 4 to 18, all of them 68).  A single short request is a chain of latencies: 12.5 us over
-// 512 tokens, of which the four steps of a wave take six.
+// 198 us; 12 rows of 32 heads over 32768 tokens 94 to 96 us); less over short ones (33 x
+// 2000 tokens 65 us a call for 270 MB), whose chunks do not divide evenly among the CUs.  Over a
+// quantised cache, and with more rows, expansion, exponentials and matrix instructions
+// take about the same issue time each and overlap only in part: 504 rows over 8 x 4096
+// 8-bit tokens 118 us, where the products alone take 27 at the matrix peak (counters:
+// matrix instructions 28% of the time, vector ones 59%, LDS 25%).  A single short request
+// is a chain of latencies: 13 us over 512 tokens, of which the four steps of a wave take six.
 #pragma once
 
 #include <type_traits>

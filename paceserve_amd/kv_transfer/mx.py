@@ -5,7 +5,9 @@ quantised one.
 Format.  Blocks of 32 elements along head_dim share one power-of-two scale, the
 smallest 2^e that brings the block's largest magnitude within the element type:
 e4m3 up to 448 ("mxfp8") or e2m1 up to 6 ("mxfp4").  An element is the value
-times 2^-e, rounded to nearest even.  A block with an infinity or a NaN reads
+times 2^-e, rounded to nearest even, and stands for its value whatever type it
+is read as: float16 numbers from 57344 (mxfp4) or 63488 (mxfp8) on round to
+65536, which float16 reads as infinity.  A block with an infinity or a NaN reads
 as NaN.
 
 A layer's cache is a contiguous uint8 tensor [num_pages, 2, page_size, H, R]
