@@ -27,9 +27,11 @@
 // so a launch needs no plan and a captured one follows them; the grid has room for
 // the most chunks there can be, floor(pages / C) + requests.  A request of one chunk
 // is written directly; the others leave (o, m, l) in a workspace for the joining
-// kernels: their chunks are numbered through once more, as parts.  A request of n > C
-// pages has at most ceil(n / C) <= 2 floor(n / C) chunks, so 2 floor(pages / C) parts are
-// enough, however many requests there are beside the split ones.
+// kernels.  With e its chunks past the first and E those of all requests before it (its
+// first item less its number), its parts are 2 E .. 2 E + e: the next split request's E
+// is E + e, and 2 e >= e + 1.  A request of n pages has e <= floor(n / C), so
+// 2 floor(pages / C) parts are enough, however many requests there are beside the split
+// ones, and no search of their own.
 //
 // Bounds on MI355X (kernel alone): up to 32 rows over a 16-bit cache HBM, 5.3 to 5.7
 // TB/s (256 ragged requests of up to 2048 tokens with 8 heads of 128, 8 rows each, 191 to
@@ -122,9 +124,11 @@ struct Tables {
   int32_t k0, k1, last, a0, a1;
 };
 
-// Where a request stands among the call's: its number and its first work item.
+// Where a request stands among the call's: its number, its first work item and, if it is
+// split, its first part.
 struct Place {
   uint32_t index, item;
+  __device__ __forceinline__ uint32_t part() const { return 2 * (item - index); }
 };
 
 __device__ __forceinline__ Tables tables_of(const AttnParams& p, uint32_t b) {
@@ -169,8 +173,8 @@ __device__ __forceinline__ bool request_of(const AttnParams& p, const Tables& t,
 
 // Whether a request's items and parts are among the call's: offsets that run backwards
 // can count pages twice.
-__device__ __forceinline__ bool has_room(const AttnParams& p, const Request& r, const Place& place, uint32_t part) {
-  return place.item + r.chunks <= p.items && (r.chunks == 1 || part + r.chunks <= p.parts);
+__device__ __forceinline__ bool has_room(const AttnParams& p, const Request& r, const Place& place) {
+  return place.item + r.chunks <= p.items && (r.chunks == 1 || place.part() + r.chunks <= p.parts);
 }
 
 // Whether the tables name entries that do not exist, which pages_of and request_of cut off.
@@ -243,26 +247,6 @@ __device__ __forceinline__ bool find_request(const AttnParams& p, uint32_t x, Ke
     before += __builtin_amdgcn_readlane(upto, 63);
   }
   return found;
-}
-
-// The first part of a split request: its items but for those before it of requests that
-// are not split, one each.  Read apart from the search, which every workgroup makes:
-// there it costs calls that split nothing 5 % (MI355X, 1000 requests of 100 tokens, 134
-// to 140 us).
-__device__ __forceinline__ uint32_t first_part_of(const AttnParams& p, const Place& place) {
-  uint32_t whole = 0;
-  for (uint32_t e0 = 0; e0 < place.index; e0 += 64) {
-    const uint32_t e = e0 + threadIdx.x % 64;
-    bool one = false;
-    if (e < place.index) {
-      Tables t = {};
-      t.k0 = p.kv_indptr[e];
-      t.k1 = p.kv_indptr[e + 1];
-      one = chunks_of(p, pages_of(p, t)) == 1;
-    }
-    whole += static_cast<uint32_t>(__popcll(__ballot(one)));
-  }
-  return place.item - whole;
 }
 
 // Rows in LDS are padded by 32 bytes, so that 8 rows' 32 bytes of a transposing
@@ -402,9 +386,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   Tables tables;
   if (!find_request(p, item, [](const Tables&, uint32_t start) { return start; }, &tables, &place)) return;
   Request r;
-  const bool of_call = request_of(p, tables, &r);
-  const uint32_t first_part = r.chunks == 1 ? 0 : first_part_of(p, place);
-  const bool valid_request = of_call && has_room(p, r, place, first_part);
+  const bool valid_request = request_of(p, tables, &r) && has_room(p, r, place);
   r.chunk = item - place.item;
   if (r.chunk >= r.chunks) return;
   if (p.err != nullptr && in_unit == 0 && threadIdx.x == 0) {
@@ -834,7 +816,7 @@ __global__ __launch_bounds__(kThreads, min_waves(D, FORMAT, R, WR)) void attenti
   for (int a = 0; a < R; ++a) l[a] = across_groups(l[a], sum_of);
 
   const bool direct = r.chunks == 1;
-  const int64_t part_row0 = (static_cast<int64_t>(first_part + r.chunk) * unit + in_unit) * kTileRows;
+  const int64_t part_row0 = (static_cast<int64_t>(place.part() + r.chunk) * unit + in_unit) * kTileRows;
   // Row `in_tile` of the tile: four output columns from d, and its m and l.
   const auto write = [&](uint32_t in_tile, uint32_t d, f32x4 o, float top, float sum, bool first) {
     const uint32_t row = row0 + in_tile;

@@ -18,11 +18,10 @@ struct Parts {
 __device__ __forceinline__ bool parts_of(const AttnParams& p, uint32_t token, Request* r, uint32_t* first_part) {
   Tables t;
   Place place;
-  if (!find_request(p, token, [](const Tables& x, uint32_t) { return static_cast<uint32_t>(max(x.a0, 0)); }, &t, &place) ||
-      !request_of(p, t, r) || token < r->q0 || token - r->q0 >= r->q_len || r->chunks == 1)
+  if (!find_request(p, token, [](const Tables& x, uint32_t) { return static_cast<uint32_t>(max(x.a0, 0)); }, &t, &place))
     return false;
-  *first_part = first_part_of(p, place);
-  return has_room(p, *r, place, *first_part);
+  *first_part = place.part();
+  return request_of(p, t, r) && token >= r->q0 && token - r->q0 < r->q_len && r->chunks > 1 && has_room(p, *r, place);
 }
 
 __device__ __forceinline__ Parts parts_of_row(const AttnParams& p, const Request& r, uint32_t first_part, uint32_t token,
@@ -218,7 +217,7 @@ Split split_of(int64_t batch, int64_t heads, int64_t group, int head_dim, int64_
   chunk = std::max<int64_t>(std::min(chunk, num_indices), 1);
   s.chunk_pages = static_cast<uint32_t>(chunk);
   s.items = static_cast<uint32_t>(num_indices / chunk + batch);
-  s.parts = chunk >= num_indices ? 0 : std::min(s.items, static_cast<uint32_t>(2 * (num_indices / chunk)));
+  s.parts = chunk >= num_indices ? 0 : batch == 1 ? s.items : static_cast<uint32_t>(2 * (num_indices / chunk));
   return s;
 }
 
