@@ -332,9 +332,9 @@ __device__ __forceinline__ bool odd_word(uint32_t w) {
 // outside the loops: MI355X, 24 rows over 8 x 4096 bf16 tokens, 93 us against 114
 // with one).  A quantised cache, whose loads in flight take fewer registers, leaves room
 // for a third: for a decode step its loads count; where a wave takes 32 of 128 rows
-// it computes while the others wait (320 rows over 24 x 2000 tokens, 8 bits 156 -> 137 us,
-// 4 bits 153 -> 130), if addresses are derived anew in each step.  A 16-bit cache
-// would spill there (33 registers: 152 -> 157 us).
+// it computes while the others wait (320 rows over 24 x 2000 tokens, 8 bits 177 -> 150 us,
+// 4 bits 172 -> 140), if addresses are derived anew in each step.  A 16-bit cache would
+// spill there (504 rows over 8 x 4096 tokens 125 -> 161 us, 320 over 24 x 2000 173 -> 166).
 constexpr int min_waves(int D, int format, int R, int WR) {
   return D != 256 && format != PACE_KV_PLAIN && (R == 1 ? WR == 1 : WR == 4) ? 3 : 2;
 }
