@@ -556,6 +556,168 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type,
                       int32_t* err_count, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Tables of a batch, built on the GPU                                        */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Page lists, positions and slots of requests whose first
+ * n_b = ceil(seq_lens[b] / page_size) pages are page_table[b * table_stride]..:
+ *   kv_indptr [batch + 1]: running sum of n_b;  kv_indices [num_indices]: the
+ *   requests' pages end to end, then -1;  kv_last_page_len [batch];
+ *   positions, slot_mapping [nnz]: token j of the n that request b appends,
+ *   rows append_indptr[b]..append_indptr[b + 1] (NULL: row b, one each):
+ *   pos = seq_lens[b] - n + j, slot = page_table[b][pos / page_size] *
+ *   page_size + pos % page_size; -1 and -1 for rows of no request.
+ * Lengths are cut to [0, width * page_size], page lists to num_indices
+ * (kv_indptr runs on); a token before a request's first or past its pages has
+ * slot -1.  err_count goes up by one for each request of which something is
+ * cut, whose offsets run backwards or leave [0, nnz], or that appends more
+ * tokens than it has (but for length 0 with append_indptr NULL: an unused
+ * place of the batch).
+ *
+ * Stands before the producer's calls in
+ * paceserve/model_executor/attention/flashinfer_attention_wrapper.py:241-255,
+ * whose lists the reference builds on the host.
+ */
+int pace_kv_build_tables(const int32_t* page_table, int64_t table_stride,
+                         int width, const int32_t* seq_lens, int batch_size,
+                         int page_size, const int32_t* append_indptr,
+                         int64_t nnz, int32_t* kv_indices, int64_t num_indices,
+                         int32_t* kv_indptr, int32_t* kv_last_page_len,
+                         int32_t* positions, int64_t* slot_mapping,
+                         int32_t* err_count, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Normalised and rotated rows                                                */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Each head of q [nnz, q_heads, head_dim] and k [nnz, k_heads, head_dim] of
+ * elem_type (PACE_KV_BF16 or PACE_KV_FP16; strides in bytes, multiples of 16)
+ * as x / sqrt(mean(x^2) + eps) * weight where its weight [head_dim] is not
+ * NULL, then rotated: of table [table_rows, rotary_dim] float, row
+ * positions[i], the first half are cosines c, the second sines s, and columns
+ * (a, b) = (j, j + rotary_dim / 2), or (2 j, 2 j + 1) if interleaved, become
+ * (a c_j - b s_j, b c_j + a s_j), j < rotary_dim / 2.  float32, rounded once.
+ * head_dim (up to 1024) and rotary_dim are multiples of 16.  Outputs may be the
+ * inputs.  A token whose position is outside the table is not written, and
+ * counted in err_count.
+ */
+int pace_kv_norm_rotate(const void* q, int64_t q_token_stride,
+                        int64_t q_head_stride, int q_heads, void* q_out,
+                        int64_t q_out_token_stride, int64_t q_out_head_stride,
+                        const void* q_weight, const void* k,
+                        int64_t k_token_stride, int64_t k_head_stride,
+                        int k_heads, void* k_out, int64_t k_out_token_stride,
+                        int64_t k_out_head_stride, const void* k_weight,
+                        int elem_type, int head_dim, int64_t nnz,
+                        const int32_t* positions, const float* table,
+                        int64_t table_rows, int rotary_dim, int interleaved,
+                        float eps, int32_t* err_count, void* stream);
+
+/*
+ * The same with k and v [nnz, kv_heads, head_dim] written to slot
+ * slot_mapping[i] = page * page_size + s of one layer's cache, of elem_type
+ * (format PACE_KV_PLAIN) or quantised (head_dim and rotary_dim then multiples
+ * of 64; elements rounded once, from float32).  Slots of one call are distinct.
+ * Slot -1 is padding: nothing of the token is read or written.  A token with
+ * another slot outside the cache or a position outside the table is not
+ * written, and counted in err_count.
+ *
+ * Replaces the append of
+ * paceserve/model_executor/attention/flashinfer_attention_wrapper.py:245-255
+ * and what runs before it in the layer.
+ */
+int pace_kv_append_rope(const void* q, int64_t q_token_stride,
+                        int64_t q_head_stride, int q_heads, void* q_out,
+                        int64_t q_out_token_stride, int64_t q_out_head_stride,
+                        const void* q_weight, const void* k,
+                        int64_t k_token_stride, int64_t k_head_stride,
+                        const void* k_weight, const void* v,
+                        int64_t v_token_stride, int64_t v_head_stride,
+                        int kv_heads, int elem_type, int head_dim, int64_t nnz,
+                        const int32_t* positions, const int64_t* slot_mapping,
+                        const float* table, int64_t table_rows, int rotary_dim,
+                        int interleaved, float eps, void* cache, int format,
+                        int64_t num_pages, int page_size, int32_t* err_count,
+                        void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Latent cache and attention                                                 */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Rows of a latent cache: [num_pages, page_size, latent_dim + 64] of elem_type,
+ * latent_dim 256 or 512.  Token i's row is latent [nnz, latent_dim], normalised
+ * as above where weight [latent_dim] is not NULL, then rope_key [nnz, 64],
+ * rotated as above (table [table_rows, 64]).  Slots, padding and counting as in
+ * pace_kv_append_rope.
+ */
+int pace_kv_append_latent(const void* latent, int64_t latent_stride,
+                          const void* rope_key, int64_t rope_stride,
+                          const void* weight, int elem_type, int latent_dim,
+                          int64_t nnz, const int32_t* positions,
+                          const int64_t* slot_mapping, const float* table,
+                          int64_t table_rows, int interleaved, float eps,
+                          void* cache, int64_t num_pages, int page_size,
+                          int32_t* err_count, void* stream);
+
+/*
+ * Attention over a latent cache (the absorbed form): for head h of a token
+ *   s = scale * q_h . row,  out_h = softmax(s) latent,  lse_h = log(sum exp(s))
+ * with q [nnz, num_heads, latent_dim + 64] and out [nnz, num_heads, latent_dim]
+ * of elem_type (token strides in bytes), lse [nnz, num_heads] float or NULL.
+ * Tables, masks, what a row sees, counting, the workspace and captured calls
+ * are as in pace_kv_attention.
+ */
+int pace_kv_latent_attention_workspace(int batch_size, int num_heads,
+                                       int latent_dim, int max_q_len,
+                                       int64_t num_indices, int page_size,
+                                       int64_t* bytes);
+int pace_kv_latent_attention(const void* q, int64_t q_stride_bytes,
+                             int elem_type, int64_t nnz,
+                             const int32_t* qo_indptr, int batch_size,
+                             int num_heads, int latent_dim, const void* cache,
+                             int64_t num_pages, int page_size,
+                             const int32_t* kv_indices, int64_t num_indices,
+                             const int32_t* kv_indptr,
+                             const int32_t* kv_last_page_len, int max_q_len,
+                             const uint64_t* tree_mask, int mask_words,
+                             float scale, void* out, int64_t out_stride_bytes,
+                             float* lse, void* workspace,
+                             int64_t workspace_size, int32_t* err_count,
+                             void* stream);
+
+/*
+ * Attention of ragged prompts over expanded keys and values (the expanded
+ * form): for head h
+ *   s = scale * (q[:head_dim] . key_h + q[head_dim:] . rope_key),
+ *   out_h = softmax(s) value_h
+ * with q [nnz, num_heads, head_dim + 64], key and value [num_keys, num_heads,
+ * head_dim], rope_key [num_keys, 64], out [nnz, num_heads, head_dim], head_dim
+ * 64 or 128 (strides in bytes, multiples of 16), lse [nnz, num_heads] float or
+ * NULL.  Request b: queries qo_indptr[b]..qo_indptr[b + 1], keys
+ * kv_indptr[b]..kv_indptr[b + 1]; causal: query i of q_len sees the keys up to
+ * kv_len - q_len + i.  A query that sees nothing gets zeros and -infinity; rows
+ * of no request are not written.  err_count goes up by one for each request
+ * that is skipped (queries outside [0, nnz), more than max_q_len, or past the
+ * row tiles of nnz rows where offsets overlap) or whose keys are cut to
+ * [0, num_keys).
+ */
+int pace_kv_prompt_attention(const void* q, int64_t q_token_stride,
+                             int64_t q_head_stride, const void* key,
+                             int64_t k_token_stride, int64_t k_head_stride,
+                             const void* rope_key, int64_t rope_token_stride,
+                             const void* value, int64_t v_token_stride,
+                             int64_t v_head_stride, int elem_type,
+                             int num_heads, int head_dim, int64_t nnz,
+                             int64_t num_keys, const int32_t* qo_indptr,
+                             const int32_t* kv_indptr, int batch_size,
+                             int max_q_len, float scale, int causal, void* out,
+                             int64_t out_token_stride, int64_t out_head_stride,
+                             float* lse, int32_t* err_count, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Native block allocation, batch planning and single-call promotion          */
 /* ------------------------------------------------------------------------ */
 

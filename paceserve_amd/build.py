@@ -22,8 +22,9 @@ LIB_NAME = "libpace_kv.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 
 SOURCES = ["kv_attention_d128.hip", "kv_attention_d256.hip", "kv_attention_d64.hip", "kv_copy.hip", "kv_stage.hip",
-           "kv_plan.cpp", "kv_append.hip", "kv_mx.hip", "kv_attention.hip", "kv_channel.cpp"]
-HEADERS = ["internal.h", "mx.h", "attention.h"]
+           "kv_plan.cpp", "kv_append.hip", "kv_mx.hip", "kv_attention.hip", "kv_tables.hip", "kv_rope.hip", "kv_latent.hip",
+           "kv_prompt.hip", "kv_channel.cpp"]
+HEADERS = ["internal.h", "mx.h", "attention.h", "latent.h"]
 
 # Packed-FP32 instructions are disabled for every HIP translation unit.
 HIPCC_FLAGS = [
