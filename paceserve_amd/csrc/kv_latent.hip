@@ -32,13 +32,25 @@ __device__ __forceinline__ uint32_t seen_of(const AttnParams& p, const Request& 
   return static_cast<uint32_t>(x);
 }
 
-// A workgroup takes 16 rows and a chunk of tokens, 32 at a time through LDS.  Each of its
-// four waves makes the weights of all rows for itself and sums a quarter of the columns.
-template <int L, int TYPE>
-__global__ __launch_bounds__(kThreads, 1) void latent_kernel(const AttnParams p) {
-  constexpr int kW = L + kRope, kKS = kW / 32, kCT = L / 64;
-  constexpr uint32_t kRow = kStride<kW>, kPieces = kW / 8;
-  __shared__ __attribute__((aligned(16))) char lds[kTile * kRow];
+// RT tiles of 16 rows a workgroup, whose four waves sum a quarter of the columns each, of
+// all rows.  Up to two tiles every wave makes the weights of all rows for itself; past
+// that each makes those of a quarter of the rows, and they share them through LDS.
+//
+// 32 tokens a step go from memory straight to LDS, into one of two buffers while the
+// other is read.  There the latents' 16-byte pieces c of row r lie at c ^ swap(r), within
+// each 256 bytes, so that neither 16 rows of one piece (keys) nor 4 rows of two
+// (transposed values) meet in a bank.
+template <int L, int TYPE, int RT>
+__global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const AttnParams p) {
+  constexpr int kW = L + kRope, kKS = L / 32, kCT = L / 64;
+  constexpr bool kShare = RT >= 4;
+  constexpr int RW = kShare ? RT / kWaves : RT;          // tiles whose weights a wave makes
+  constexpr uint32_t kRow = L * 2, kRopeAt = kTile * kRow, kBuffer = kRopeAt + kTile * kRope * 2;
+  constexpr uint32_t kWeightRow = kTile * 2;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer];
+  __shared__ __attribute__((aligned(256))) char lds_p[kShare ? RT * 16 * kWeightRow : 16];
+  __shared__ float lds_shrink[kShare ? RT * 16 : 1], lds_ml[kShare ? RT * 16 : 1][2];
+  __shared__ __attribute__((aligned(16))) uint32_t lds_raised[kWaves];
   const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t at = blockIdx.x / kXcds, nth = over(p.by_unit, at);
@@ -54,155 +66,366 @@ __global__ __launch_bounds__(kThreads, 1) void latent_kernel(const AttnParams p)
   if (r.chunk >= r.chunks) return;
   if (p.err != nullptr && tile == 0 && threadIdx.x == 0) {
     if (r.chunk == 0 && (!valid_request || is_cut(p, tables, r))) atomicAdd(p.err, 1);
+    // Behind the last item lie requests that no workgroup looks at.
     if (item + 1 == p.items && place.index + 1 < p.batch)
       atomicAdd(p.err, static_cast<int32_t>(p.batch - 1 - place.index));
   }
   if (!valid_request) return;
-  const uint32_t rows = r.q_len * p.group, row0 = tile * 16;
+  const uint32_t rows = r.q_len * p.group, row0 = tile * (16 * RT);
   if (row0 >= rows) return;
   const int32_t base = static_cast<int32_t>(r.kv_len) - static_cast<int32_t>(r.q_len);
-  const int32_t last_q = static_cast<int32_t>(over(p.by_group, min(row0 + 16, rows) - 1));
+  const int32_t first_q = static_cast<int32_t>(over(p.by_group, row0));
+  const int32_t last_q = static_cast<int32_t>(over(p.by_group, min(row0 + 16 * RT, rows) - 1));
+  // A request's chunks are of one length, in whole steps, and none is empty.
   const uint32_t even = (r.pages + r.chunks - 1) / r.chunks;
   const uint32_t length = min((even + p.step_pages - 1) / p.step_pages * p.step_pages, p.chunk_pages);
   const int32_t chunk_tokens = static_cast<int32_t>(length * p.page_size);
   const int32_t t_begin = static_cast<int32_t>(r.chunk) * chunk_tokens;
   int32_t t_end = static_cast<int32_t>(min(static_cast<int64_t>(t_begin) + chunk_tokens, static_cast<int64_t>(r.kv_len)));
   if (p.mask == nullptr) t_end = min(t_end, base + last_q + 1);
-  if (p.err != nullptr && row0 + 16 >= rows) {
+  // Tokens on pages that do not exist are counted by the last row tile's workgroup.
+  if (p.err != nullptr && row0 + 16 * RT >= rows) {
     const int32_t page = static_cast<int32_t>(p.page_size), first = static_cast<int32_t>(r.chunk * length);
     for (int32_t i = static_cast<int32_t>(threadIdx.x); static_cast<int64_t>(i) * page < t_end - t_begin; i += kThreads)
       if (static_cast<uint32_t>(p.kv_indices[r.first_page + first + i]) >= p.num_pages)
         atomicAdd(p.err, min(page, t_end - t_begin - i * page));
   }
-  const uint32_t my_row = row0 + n, my_query = over(p.by_group, my_row);
-  u32x4 qf[kKS];
+
+  // Query fragments: row n of each tile, eight elements from 32 k + 8 g, with the scale's
+  // sign: what follows takes it as positive.  (A scale of zero makes all scores zero.)
+  const uint32_t wave_row0 = row0 + (kShare ? w * RW * 16 : 0);
+  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
+  const float per_score = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  u32x4 qf[RW][kKS + 2];
 #pragma unroll
-  for (int k = 0; k < kKS; ++k) {
-    qf[k] = u32x4{0, 0, 0, 0};
-    if (my_row < rows)
-      qf[k] = *reinterpret_cast<const u32x4*>(p.q + static_cast<int64_t>(r.q0 + my_query) * p.q_stride +
-                                              static_cast<int64_t>(my_row - my_query * p.group) * (kW * 2) + k * 64 + g * 16);
+  for (int a = 0; a < RW; ++a) {
+    const uint32_t row = wave_row0 + a * 16 + n, i = over(p.by_group, row);
+    const char* const q = p.q + static_cast<int64_t>(r.q0 + i) * p.q_stride + static_cast<int64_t>(row - i * p.group) * (kW * 2);
+#pragma unroll
+    for (int k = 0; k < kKS + 2; ++k) {
+      qf[a][k] = u32x4{0, 0, 0, 0};
+      if (row < rows) qf[a][k] = (*reinterpret_cast<const u32x4*>(q + k * 64 + g * 16) ^ flip) & keep;
+    }
   }
-  f32x4 acc[kCT];
+  f32x4 acc[RT][kCT];
 #pragma unroll
-  for (int d = 0; d < kCT; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-  for (int32_t t0 = t_begin; t0 < t_end; t0 += kTile) {
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < kTile * kPieces; e += kThreads) {
-      const uint32_t row = e / kPieces, c = e % kPieces;
-      const int32_t t = t0 + static_cast<int32_t>(row);
-      u32x4 x = {0, 0, 0, 0};
-      if (t < t_end) {
-        const uint32_t pg = over(p.by_page, static_cast<uint32_t>(t));
-        const uint32_t id = static_cast<uint32_t>(p.kv_indices[r.first_page + static_cast<int32_t>(pg)]);
-        if (id < p.num_pages)
-          x = *reinterpret_cast<const u32x4*>(
-              p.cache + (static_cast<int64_t>(id) * p.page_size + (static_cast<uint32_t>(t) - pg * p.page_size)) * (kW * 2) +
-              c * 16);
+  for (int a = 0; a < RT; ++a)
+#pragma unroll
+    for (int d = 0; d < kCT; ++d) acc[a][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m[RW], l[RW];
+  bool wide[RW];                                         // some row's |m| is past 2^20
+#pragma unroll
+  for (int a = 0; a < RW; ++a) {
+    m[a] = -INFINITY;
+    l[a] = 0.f;
+    wide[a] = false;
+  }
+
+  // A step's loads: page ids (a token to a lane, the same in all waves), then rows: each
+  // wave brings eight.
+  int32_t id = -1;
+  uint32_t row_at = 0;                                   // the lane's token's row, in 16-byte units
+  uint32_t valid = 0, next_valid = 0;                    // tokens of this step and the next one that exist
+  const auto load_id = [&](int32_t t0) {
+    const int32_t t = t0 + static_cast<int32_t>(lane % kTile);
+    id = -1;
+    if (t < t_end) id = p.kv_indices[r.first_page + static_cast<int32_t>(over(p.by_page, static_cast<uint32_t>(t)))];
+  };
+  const auto place_rows = [&](int32_t t0) {
+    const uint32_t t = static_cast<uint32_t>(t0) + lane % kTile;
+    const bool ok = static_cast<uint32_t>(id) < p.num_pages;
+    next_valid = static_cast<uint32_t>(__ballot(ok));
+    row_at = ok ? static_cast<uint32_t>(id) * p.page16 + (t - over(p.by_page, t) * p.page_size) * (kW / 8) : 0u;
+  };
+  const auto load_rows = [&](auto whole, uint32_t to) {
+    constexpr uint32_t kRowsOnce = 1024 / kRow, kLanes = 64 / kRowsOnce;
+    const uint32_t ln = opaque(lane), mine = next_valid >> (8 * w) & 255u;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; i += kRowsOnce) {
+      const uint32_t row = i + ln / kLanes;
+      uint32_t from = __builtin_amdgcn_readlane(row_at, 8 * w + i);
+      if constexpr (kRowsOnce == 2) {
+        const uint32_t second = __builtin_amdgcn_readlane(row_at, 8 * w + i + 1);
+        from = ln < kLanes ? from : second;
       }
-      *reinterpret_cast<u32x4*>(lds + row * kRow + c * 16) = x;
+      const char* const x = p.cache + static_cast<int64_t>(from) * 16 + ((ln % kLanes) ^ (row * 2 | (w & 1))) * 16;
+      const uint32_t at = to + (w * 8 + i) * kRow;
+      if (decltype(whole)::value || (mine >> row & 1u)) copy_to_lds(x, at);
+      else lds_put(at + ln * 16, u32x4{0, 0, 0, 0});
     }
-    uint32_t ok = 0;
-    {
-      const int32_t t = t0 + static_cast<int32_t>(lane % 32);
-      bool exists = t < t_end;
-      if (exists)
-        exists = static_cast<uint32_t>(p.kv_indices[r.first_page + static_cast<int32_t>(over(p.by_page, static_cast<uint32_t>(t)))]) <
-                 p.num_pages;
-      ok = static_cast<uint32_t>(__ballot(exists));
-    }
-    __syncthreads();
-    f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    const uint32_t row = ln / 8, from = __shfl(row_at, 8 * w + row), at = to + kRopeAt + w * 1024;
+    const char* const x = p.cache + static_cast<int64_t>(from) * 16 + kRow + ((ln % 8) ^ ((4 * w + row / 2) % 8)) * 16;
+    if (decltype(whole)::value || (mine >> row & 1u)) copy_to_lds(x, at);
+    else lds_put(at + ln * 16, u32x4{0, 0, 0, 0});
+  };
+
+  // Scores of 32 tokens: lane: row n of each tile, tokens 16 t + 4 g + e.
+  f32x4 s[RW][2];
+  const uint32_t swap_n = (n % 8) * 2 | n / 8;
+  const uint32_t key_at = n * kRow + (g ^ swap_n) * 16, rope_at = kRopeAt + n * (kRope * 2) + (g ^ (n / 2)) * 16;
+  const auto score = [&](uint32_t from) {
+    const uint32_t key = opaque(key_at) + from, rope = opaque(rope_at) + from;
 #pragma unroll
-    for (int k = 0; k < kKS; ++k)
+    for (int a = 0; a < RW; ++a)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[a][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kKS + 2; ++k)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const u32x4 kf = *reinterpret_cast<const u32x4*>(lds + (t * 16 + n) * kRow + k * 64 + g * 16);
-        s[t] = mfma<TYPE>(kf, qf[k], s[t]);
+        const u32x4 kf = lds_get<u32x4>(k < kKS ? (key ^ (k % 4 * 64)) + t * 16 * kRow + k / 4 * 256
+                                                : (rope ^ ((k - kKS) * 64)) + t * 16 * (kRope * 2));
+#pragma unroll
+        for (int a = 0; a < RW; ++a) s[a][t] = mfma<TYPE>(kf, qf[a][k], s[a][t]);
       }
-    const uint32_t sees = seen_of(p, r, base, t0, static_cast<int32_t>(my_query)) & ok, mine = sees >> (4 * g);
-    float top = -INFINITY;
+  };
+
+  // Weights of those tokens, packed by twos as they lie in s; raises the maximum where a
+  // score passes it by kSlack, for which shrink is the factor of what was summed before.
+  u32x4 pf[RW];
+  float shrink[RW];
+  uint32_t raised = 0;                                   // tiles whose maximum was raised
+  const auto weigh = [&](auto full, int32_t t0) {
+    if constexpr (!decltype(full)::value) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int a = 0; a < RW; ++a) {
+        const uint32_t sees =
+            seen_of(p, r, base, t0, static_cast<int32_t>(over(p.by_group, wave_row0 + a * 16 + n))) & valid;
+        const uint32_t mine = sees >> (4 * g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[t][e] = (mine & (1u << (t * 16 + e))) ? scaled(s[t][e], p.scale_log2) : -INFINITY;
-        top = fmaxf(top, s[t][e]);
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(mine & (1u << (t * 16 + e)))) s[a][t][e] = -INFINITY;
       }
-    top = fmaxf(m, across_groups(top, max_of));
-    const float from = top == -INFINITY ? 0.f : top, shrink = exp2_of(m - from);
-    m = top;
-    l *= shrink;
-#pragma unroll
-    for (int d = 0; d < kCT; ++d) acc[d] *= shrink;
-    u32x4 pf;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        const float x = weight_of<TYPE>(s[t][e], from), y = weight_of<TYPE>(s[t][e + 1], from);
-        l += x + y;
-        pf[t * 2 + e / 2] = pair_of<TYPE>(x, y);
-      }
-    const bool full = __ballot(sees == ~0u) == ~0ull;
-    bool odd = false;
-    if (!full) {
-      bool found = false;
-      for (uint32_t c = lane; c < kTile * L / 8; c += 64) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(lds + c / (L / 8) * kRow + c % (L / 8) * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) found |= odd_word<TYPE>(x[e]);
-      }
-      odd = __ballot(found) != 0;
     }
+    raised = 0;
+#pragma unroll
+    for (int a = 0; a < RW; ++a) settle(s[a][0], s[a][1]);
+#pragma unroll
+    for (int a = 0; a < RW; ++a) {
+      float top = max3_of(s[a][0][0], s[a][0][1], s[a][0][2]);
+      top = max3_of(top, s[a][0][3], s[a][1][0]);
+      top = max3_of(top, s[a][1][1], s[a][1][2]);
+      top = scaled(max3_of(top, s[a][1][3], s[a][1][3]), per_score);
+      shrink[a] = 1.f;
+      if (__ballot(top > m[a] + kSlack) != 0) {
+        raised |= 1u << a;
+        top = across_groups(top, max_of);
+        const float next = top > m[a] + kSlack ? top : m[a];
+        shrink[a] = exp2_of(m[a] - (next == -INFINITY ? 0.f : next));
+        m[a] = next;
+        l[a] *= shrink[a];
+        wide[a] = __ballot(fabsf(next) > 0x1p20f && next != -INFINITY) != 0;
+      }
+      const float from = m[a] == -INFINITY ? 0.f : m[a];
+      // The fused difference holds what m lost when it was rounded: less than a tenth up
+      // to 2^20, but past 2^27 enough to make the largest weight an infinity or a zero.
+      if (wide[a]) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[a][t][e] = unfused(scaled(s[a][t][e], per_score), from) + kUnit<TYPE>;
+      } else {
+        const float offset = kUnit<TYPE> - from;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[a][t][e] = __builtin_fmaf(s[a][t][e], per_score, offset);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const float x = exp2_of(s[a][t][e]), y = exp2_of(s[a][t][e + 1]);
+          l[a] += x + y;
+          pf[a][t * 2 + e / 2] = pair_of<TYPE>(x, y);
+        }
+    }
+  };
+
+  // Takes infinities and NaN out of the wave's columns of a buffer: a product with weight
+  // zero would spread them to rows that do not see their token.
+  bool odd = false;
+  const auto clean = [&](uint32_t from) {
+    bool found = false;
+#pragma unroll 1
+    for (uint32_t c = lane; c < kTile * kCT * 2; c += 64) {
+      const uint32_t row = c / (kCT * 2), piece = (w * kCT * 2 + c % (kCT * 2)) ^ ((row % 8) * 2 | row / 8 % 2);
+      u32x4 x = lds_get<u32x4>(from + row * kRow + piece * 16);
+      bool here = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) here |= odd_word<TYPE>(x[e]);
+      if (here) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = finite_halves<TYPE>(x[e]);
+        lds_put(from + row * kRow + piece * 16, x);
+        found = true;
+      }
+    }
+    odd |= __ballot(found) != 0;
+  };
+
+  // Adds the weighted values of the tokens in a buffer.  For weights in registers the
+  // tokens of a lane's group of 16 are 4 g .. 4 g + 3 and the same behind 16; through LDS
+  // they are 8 g .. 8 g + 7.
+  const uint32_t v_row = kShare ? 8 * g + n / 4 : 4 * g + n / 4;
+  const uint32_t v_at = v_row * kRow + ((w * kCT * 2 + n % 4 / 2) ^ ((v_row % 8) * 2 | v_row / 8 % 2)) * 16 + n % 2 * 8;
+  const uint32_t p_at = lds_offset(lds_p) + n * kWeightRow + (g ^ (n / 4)) * 16;
+  const auto gather = [&](uint32_t from) {
+    u32x4 weight[RT];
+#pragma unroll
+    for (int a = 0; a < RT; ++a) {
+      if constexpr (kShare) weight[a] = lds_get<u32x4>(p_at + a * 16 * kWeightRow);
+      else weight[a] = pf[a];
+    }
+    const uint32_t v = opaque(v_at) + from;
 #pragma unroll
     for (int d = 0; d < kCT; ++d) {
-      const char* v = lds + lane / 4 * kRow + (w * kCT + d) * 32 + lane % 4 * 8;
-      typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)v));
-      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(v + 16 * kRow)));
-      if (!odd) acc[d] = mfma<TYPE>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, acc[d]);
+      const u32x2 lo = lds_transposed(v ^ (d * 32));
+      const u32x2 hi = lds_transposed(kShare ? (v ^ (d * 32 ^ 128)) + 4 * kRow : (v ^ (d * 32)) + 16 * kRow);
+      const u32x4 vf = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+      for (int a = 0; a < RT; ++a) acc[a][d] = mfma<TYPE>(vf, weight[a], acc[a][d]);
     }
-    if (odd) {
-#pragma unroll 1
-      for (uint32_t token = 0; token < kTile; ++token) {
-        const uint32_t word = token / 16 * 2 + token % 4 / 2;
-        const uint32_t of = word == 0 ? pf[0] : word == 1 ? pf[1] : word == 2 ? pf[2] : pf[3];
-        const float weight = value_of<TYPE>(__shfl(of, token % 16 / 4 * 16 + n), token % 2);
-        if (!((sees >> token) & 1u)) continue;
+  };
+
+  constexpr int32_t kStep = static_cast<int32_t>(kTile);
+  const int32_t seen_by_all = p.mask == nullptr ? base + first_q + 1 : base;
+  int32_t t0 = t_begin;
+  uint32_t now = lds_offset(lds), other = now + kBuffer;
+  const auto load_next = [&](int32_t next, uint32_t to) {
+    if (next_valid == ~0u) load_rows(std::true_type{}, to);
+    else if (next < t_end) load_rows(std::false_type{}, to);
+    load_id(next + kStep);
+  };
+  const auto one_step = [&](auto full) {
+    valid = next_valid;
+    place_rows(t0 + kStep);
+    __builtin_amdgcn_s_waitcnt(0x0f70);                  // vmcnt(0): this step's rows are in LDS
+    __syncthreads();                                     // and the other buffer's readers are done
+    load_next(t0 + kStep, other);
+    score(now);
+    weigh(full, t0);
+    if constexpr (kShare) {
+      const uint32_t to = lds_offset(lds_p) + (w * RW * 16 + n) * kWeightRow + g % 2 * 8;
 #pragma unroll
-        for (int d = 0; d < kCT; ++d) {
-          const u32x2 v = *reinterpret_cast<const u32x2*>(lds + token * kRow + (w * kCT + d) * 32 + g * 8);
+      for (int a = 0; a < RW; ++a) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) acc[d][c] += weight * value_of<TYPE>(v[c / 2], c % 2);
+        for (int t = 0; t < 2; ++t)
+          lds_put(to + a * 16 * kWeightRow + ((2 * t + g / 2) ^ (n / 4)) * 16, u32x2{pf[a][2 * t], pf[a][2 * t + 1]});
+        if (raised != 0 && g == 0) lds_shrink[(w * RW + a) * 16 + n] = shrink[a];
+      }
+      if (lane == 0) lds_raised[w] = raised;
+    }
+    if (kShare || !decltype(full)::value) __syncthreads();
+    if constexpr (!decltype(full)::value) clean(now);
+    if constexpr (kShare) {
+      const u32x4 all = *reinterpret_cast<const u32x4*>(lds_raised);
+      if (__builtin_amdgcn_readfirstlane(all[0] | all[1] | all[2] | all[3]) != 0) {
+#pragma unroll
+        for (int a = 0; a < RT; ++a)
+          if (__builtin_amdgcn_readfirstlane(all[a / RW]) != 0) {
+            const float by = lds_shrink[a * 16 + n];
+#pragma unroll
+            for (int d = 0; d < kCT; ++d) acc[a][d] *= by;
+          }
+      }
+    } else {
+#pragma unroll
+      for (int a = 0; a < RT; ++a)
+        if (raised & (1u << a)) {
+#pragma unroll
+          for (int d = 0; d < kCT; ++d) acc[a][d] *= shrink[a];
         }
+    }
+    gather(now);
+    const uint32_t x = now;
+    now = other;
+    other = x;
+    t0 += kStep;
+  };
+  load_id(t0);
+  place_rows(t0);
+  load_next(t0, now);
+  // The steps whose tokens every row sees, then the others.
+  while (t0 + kStep <= seen_by_all && next_valid == ~0u) one_step(std::true_type{});
+  const int32_t t_masked = t0;
+#pragma unroll 1
+  while (t0 < t_end) one_step(std::false_type{});
+#pragma unroll
+  for (int a = 0; a < RW; ++a) {
+    l[a] = across_groups(l[a], sum_of);
+    if constexpr (kShare)
+      if (g == 0) {
+        lds_ml[(w * RW + a) * 16 + n][0] = m[a];
+        lds_ml[(w * RW + a) * 16 + n][1] = l[a];
+      }
+  }
+  if (kShare) __syncthreads();
+  const bool direct = r.chunks == 1;
+  const int64_t part_row0 = (static_cast<int64_t>(place.part() + r.chunk) * p.row_tiles + tile) * (16 * RT);
+  const auto out_at = [&](uint32_t row) {
+    const uint32_t i = over(p.by_group, row);
+    return p.out + static_cast<int64_t>(r.q0 + i) * p.out_stride + static_cast<int64_t>(row - i * p.group) * (L * 2);
+  };
+  const uint32_t col0 = w * kCT * 16 + g * 4;
+#pragma unroll
+  for (int a = 0; a < RT; ++a) {
+    const uint32_t in_tile = a * 16 + n, row = row0 + in_tile;
+    if (row >= rows) continue;
+    float top, sum;
+    if constexpr (kShare) {
+      top = lds_ml[in_tile][0];
+      sum = lds_ml[in_tile][1];
+    } else {
+      top = m[a];
+      sum = l[a];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    char* const out = out_at(row);
+#pragma unroll
+    for (int d = 0; d < kCT; ++d) {
+      const f32x4 o = acc[a][d];
+      if (!direct) {
+        *reinterpret_cast<f32x4*>(p.part_o + (part_row0 + in_tile) * L + col0 + d * 16) = o;
+      } else {
+        const u32x2 x = {result_pair<TYPE>(o[0] * inv, o[1] * inv), result_pair<TYPE>(o[2] * inv, o[3] * inv)};
+        *reinterpret_cast<u32x2*>(out + (col0 + d * 16) * 2) = x;
+      }
+    }
+    if (w == 0 && g == 0) {
+      if (!direct) {
+        p.part_ml[(part_row0 + in_tile) * 2] = top;
+        p.part_ml[(part_row0 + in_tile) * 2 + 1] = sum;
+      } else if (p.lse != nullptr) {
+        const uint32_t i = over(p.by_group, row);
+        p.lse[static_cast<int64_t>(r.q0 + i) * p.group + (row - i * p.group)] = log_total<TYPE>(top, sum);
       }
     }
   }
-  l = across_groups(l, sum_of);
-  if (my_row >= rows) return;
-  const bool direct = r.chunks == 1;
-  const int64_t part_row = (static_cast<int64_t>(place.part() + r.chunk) * p.row_tiles + tile) * 16 + n;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int d = 0; d < kCT; ++d) {
-    const uint32_t col = (w * kCT + d) * 16 + g * 4;
-    if (!direct) {
-      *reinterpret_cast<f32x4*>(p.part_o + part_row * L + col) = acc[d];
-    } else {
-      const u32x2 x = {result_pair<TYPE>(acc[d][0] * inv, acc[d][1] * inv),
-                       result_pair<TYPE>(acc[d][2] * inv, acc[d][3] * inv)};
-      *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(r.q0 + my_query) * p.out_stride +
-                                (static_cast<int64_t>(my_row - my_query * p.group) * L + col) * 2) = x;
-    }
-  }
-  if (w == 0 && g == 0) {
-    if (!direct) {
-      p.part_ml[part_row * 2] = m;
-      p.part_ml[part_row * 2 + 1] = l;
-    } else if (p.lse != nullptr) {
-      p.lse[static_cast<int64_t>(r.q0 + my_query) * p.group + (my_row - my_query * p.group)] = log_total<TYPE>(m, l);
+  if (!odd) return;
+  // An infinity or a NaN in a latent that a row sees is in its score too: either the row
+  // has no sum (NaN), or the token's weight is zero, and zero times it makes its column NaN.
+#pragma unroll 1
+  for (uint32_t a = 0; a < RT; ++a) {
+    const uint32_t in_tile = a * 16 + n, row = row0 + in_tile;
+    if (row >= rows) continue;
+    char* const out = out_at(row);
+#pragma unroll 1
+    for (int32_t t = t_masked; t < t_end; ++t) {
+      const uint32_t page = over(p.by_page, static_cast<uint32_t>(t));
+      const uint32_t of = static_cast<uint32_t>(p.kv_indices[r.first_page + static_cast<int32_t>(page)]);
+      if (of >= p.num_pages || !(seen_of(p, r, base, t, static_cast<int32_t>(over(p.by_group, row))) & 1u)) continue;
+      const char* const x = p.cache + (static_cast<int64_t>(of) * p.page_size + (static_cast<uint32_t>(t) - page * p.page_size)) *
+                                          (kW * 2) + col0 * 2;
+#pragma unroll 1
+      for (uint32_t c = 0; c < kCT * 4; ++c) {
+        const uint32_t col = c / 4 * 16 + c % 4;
+        if (!odd_word<TYPE>(*reinterpret_cast<const uint16_t*>(x + col * 2))) continue;
+        if (!direct) p.part_o[(part_row0 + in_tile) * L + col0 + col] = NAN;
+        else *reinterpret_cast<uint16_t*>(out + (col0 + col) * 2) = 0x7fffu;
+      }
     }
   }
 }
@@ -250,7 +473,7 @@ struct Split {
 
 Split split_of(int64_t batch, int64_t rows, int64_t num_indices, int64_t page_size) {
   Split s = {};
-  s.tile_rows = 16;
+  s.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   s.row_tiles = static_cast<uint32_t>((rows + s.tile_rows - 1) / s.tile_rows);
   s.step_pages = static_cast<uint32_t>(kTile % page_size ? 1 : kTile / page_size);
   const int64_t requests = std::max<int64_t>(batch, 1), pages = std::max<int64_t>((num_indices + requests - 1) / requests, 1);
@@ -287,10 +510,18 @@ int check_sizes(int batch_size, int heads, int latent_dim, int max_q_len, int64_
 
 int64_t workspace_bytes(const Split& s, int latent_dim) { return s.part_rows() * (latent_dim + 2) * 4; }
 
+template <int L, int TYPE>
+const void* pick_latent(uint32_t tile_rows) {
+  switch (tile_rows) {
+    case 16: return reinterpret_cast<const void*>(&latent_kernel<L, TYPE, 1>);
+    case 32: return reinterpret_cast<const void*>(&latent_kernel<L, TYPE, 2>);
+    default: return reinterpret_cast<const void*>(&latent_kernel<L, TYPE, 4>);
+  }
+}
+
 template <int L>
-const void* pick_latent(int type) {
-  return type == PACE_KV_BF16 ? reinterpret_cast<const void*>(&latent_kernel<L, PACE_KV_BF16>)
-                              : reinterpret_cast<const void*>(&latent_kernel<L, PACE_KV_FP16>);
+const void* pick_latent(int type, uint32_t tile_rows) {
+  return type == PACE_KV_BF16 ? pick_latent<L, PACE_KV_BF16>(tile_rows) : pick_latent<L, PACE_KV_FP16>(tile_rows);
 }
 
 template <int L>
@@ -343,6 +574,8 @@ int pace_kv_latent_attention(const void* q, int64_t q_stride_bytes, int elem_typ
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out)) & 15u ||
       reinterpret_cast<uintptr_t>(tree_mask) & 7u)
     return fail(PACE_KV_EINVAL, "latent attention: q, cache and out must be 16-byte aligned, mask 8-byte");
+  if (page_size > (INT64_C(1) << 36) / (width * 2) || num_pages * (page_size * width / 8) >= UINT32_MAX)
+    return fail(PACE_KV_ERANGE, "latent attention: a layer's cache must be smaller than 64 GiB");
   const Split s = split_of(batch_size, static_cast<int64_t>(max_q_len) * num_heads, num_indices, page_size);
   const int64_t need = workspace_bytes(s, latent_dim);
   if (need > 0 && (!workspace || workspace_size < need || reinterpret_cast<uintptr_t>(workspace) & 15u))
@@ -377,6 +610,7 @@ int pace_kv_latent_attention(const void* q, int64_t q_stride_bytes, int elem_typ
   p.parts = s.parts;
   p.row_tiles = s.row_tiles;
   p.tile_rows = s.tile_rows;
+  p.page16 = static_cast<uint32_t>(page_size * width / 8);
   p.by_page = fast_div(p.page_size);
   p.by_chunk = fast_div(p.chunk_pages);
   p.by_group = fast_div(p.group);
@@ -385,7 +619,8 @@ int pace_kv_latent_attention(const void* q, int64_t q_stride_bytes, int elem_typ
   p.scale_log2 = scale_log2;
   const uint32_t items = (s.items + kXcds - 1) / kXcds * kXcds;
   void* args[] = {&p};
-  PACE_KV_TRY(hip_status(hipLaunchKernel(latent_dim == 512 ? pick_latent<512>(elem_type) : pick_latent<256>(elem_type),
+  PACE_KV_TRY(hip_status(hipLaunchKernel(latent_dim == 512 ? pick_latent<512>(elem_type, s.tile_rows)
+                                                           : pick_latent<256>(elem_type, s.tile_rows),
                                          dim3(items * p.row_tiles), dim3(kThreads), args, 0,
                                          static_cast<hipStream_t>(stream)), "latent attention launch"));
   if (need == 0) return PACE_KV_OK;

@@ -14,18 +14,72 @@ __device__ __forceinline__ float scaled(float s, float scale_log2) {
   return s * scale_log2;
 }
 
-// The weight of a score s over the maximum m: at most 1, in float16 at most 2^15 (whose
-// subnormals then lie below 2^-29 of the largest).
+__device__ __forceinline__ float unfused(float a, float b) {
+#pragma clang fp contract(off)
+  return a - b;
+}
+
+// Log2 of the least by which a score has to pass the running maximum before that is
+// raised, which costs a product of every sum; weights are then 2^kSlack at most.
+constexpr float kSlack = 4.f;
+
+// log2 of the weight of a score that equals the maximum: in float16 the largest weights
+// are 2^15, which leaves those down to 2^-29 of the largest their 2^-11.
+template <int TYPE>
+constexpr float kUnit = TYPE == PACE_KV_FP16 ? 15.f - kSlack : 0.f;
+
+// The weight of a score s over the maximum m.
 template <int TYPE>
 __device__ __forceinline__ float weight_of(float s, float m) {
 #pragma clang fp contract(off)
-  return exp2_of((s - m) + kTopWeight<TYPE>);
+  return exp2_of((s - m) + kUnit<TYPE>);
 }
 
-// Natural logarithm of a row's sum of exponentials: l weights over the maximum m.
+// Matrix instructions' results, waited for: max3_of reads them in assembly, which the
+// compiler does not do for.  20 cycles, more than any such instruction takes to write.
+__device__ __forceinline__ void settle(f32x4& x, f32x4& y) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x), "+v"(y)); }
+
+// LDS by offsets, whose swizzles are xors.
+__device__ __forceinline__ uint32_t lds_offset(const void* x) {
+  return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)x));
+}
+
+template <class T>
+__device__ __forceinline__ T lds_get(uint32_t at) {
+  return *(const __attribute__((address_space(3))) T*)static_cast<uintptr_t>(at);
+}
+
+template <class T>
+__device__ __forceinline__ void lds_put(uint32_t at, T x) {
+  *(__attribute__((address_space(3))) T*)static_cast<uintptr_t>(at) = x;
+}
+
+// Transposing read: lanes of 16 hold four columns each of four rows, and get four rows
+// of a column each.
+__device__ __forceinline__ u32x2 lds_transposed(uint32_t at) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4*)static_cast<uintptr_t>(at)));
+}
+
+// Each lane's 16 bytes at `from` into LDS, at `at` (the same for all lanes) + 16 * lane;
+// there once vmcnt says so.
+__device__ __forceinline__ void copy_to_lds(const char* from, uint32_t at) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                   (__attribute__((address_space(3))) void*)static_cast<uintptr_t>(at), 16, 0, 0);
+}
+
+// A word with its infinite and NaN halves as zeros.
+template <int TYPE>
+__device__ __forceinline__ uint32_t finite_halves(uint32_t x) {
+  if (odd_word<TYPE>(x & 0xffffu)) x &= 0xffff0000u;
+  if (odd_word<TYPE>(x >> 16)) x &= 0xffffu;
+  return x;
+}
+
+// Natural logarithm of a row's sum of exponentials: l, its weights over the maximum m.
 template <int TYPE>
 __device__ __forceinline__ float log_total(float m, float l) {
-  constexpr float kScale = TYPE == PACE_KV_FP16 ? 0x1p-15f : 1.f;
+  constexpr float kScale = TYPE == PACE_KV_FP16 ? 0x1p-11f : 1.f;  // 2^-kUnit
   return l == 0.f ? -INFINITY : (m + __log2f(l * kScale)) * 0.69314718055994531f;
 }
 
