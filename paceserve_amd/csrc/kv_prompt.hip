@@ -15,8 +15,9 @@
 namespace pace_kv {
 namespace {
 
-constexpr uint32_t kTile = 32;                           // keys of a step
-constexpr uint32_t kRows = 64;                           // query rows of a workgroup
+constexpr uint32_t kTile = 64;                           // keys of a step
+constexpr int kRT = 2;                                   // tiles of 16 query rows of a wave
+constexpr uint32_t kRows = 16 * kRT * kWaves;            // query rows of a workgroup
 
 struct PromptParams {
   const char* q;
@@ -39,6 +40,15 @@ struct PromptRequest {
   int32_t q0, q1, k0, k1;
 };
 
+// Whether a request's queries are among the rows, and not too many.
+__device__ __forceinline__ bool has_rows(const PromptParams& p, int32_t q0, int32_t q1) {
+  return q0 >= 0 && q1 > q0 && static_cast<uint32_t>(q1) <= p.nnz && static_cast<uint32_t>(q1 - q0) <= p.max_q;
+}
+
+__device__ __forceinline__ uint32_t tiles_of(int32_t q0, int32_t q1) {
+  return (static_cast<uint32_t>(q1 - q0) + kRows - 1) / kRows;
+}
+
 // The request whose row tiles (ceil(q_len / kRows) each) hold number x; false past the
 // last.  The wave looks at 64 requests a round.
 __device__ __forceinline__ bool find_tile(const PromptParams& p, uint32_t x, PromptRequest* r) {
@@ -51,9 +61,7 @@ __device__ __forceinline__ bool find_tile(const PromptParams& p, uint32_t x, Pro
       q0 = p.qo_indptr[b];
       q1 = p.qo_indptr[b + 1];
     }
-    // Offsets outside the rows leave the request without tiles.
-    const bool fine = q0 >= 0 && q1 > q0 && static_cast<uint32_t>(q1) <= p.nnz && static_cast<uint32_t>(q1 - q0) <= p.max_q;
-    const uint32_t n = fine ? (static_cast<uint32_t>(q1 - q0) + kRows - 1) / kRows : 0u;
+    const uint32_t n = has_rows(p, q0, q1) ? tiles_of(q0, q1) : 0u;
     const uint32_t upto = before + sum_upto(n);
     const uint64_t mine = __ballot(x < upto);
     if (mine != 0) {
@@ -69,143 +77,301 @@ __device__ __forceinline__ bool find_tile(const PromptParams& p, uint32_t x, Pro
   return false;
 }
 
+// Counts the requests that are skipped or cut; by one wave.
+__device__ __forceinline__ void count_bad(const PromptParams& p) {
+  const uint32_t lane = threadIdx.x % 64;
+  uint32_t before = 0;
+  for (uint32_t b0 = 0; b0 < p.batch; b0 += 64) {
+    const uint32_t b = b0 + lane;
+    uint32_t n = 0;
+    bool fine = true;
+    if (b < p.batch) {
+      const int32_t q0 = p.qo_indptr[b], q1 = p.qo_indptr[b + 1], k0 = p.kv_indptr[b], k1 = p.kv_indptr[b + 1];
+      const bool rows = has_rows(p, q0, q1);
+      n = rows ? tiles_of(q0, q1) : 0u;
+      fine = (rows || q0 == q1) && q0 >= 0 && static_cast<uint32_t>(q1) <= p.nnz && k0 >= 0 && k1 >= k0 &&
+             static_cast<uint32_t>(k1) <= p.keys;
+    }
+    const uint32_t upto = before + sum_upto(n);
+    if (upto > p.tiles && n > 0) fine = false;           // offsets that overlap: more tiles than nnz rows have
+    if (!fine) atomicAdd(p.err, 1);
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+}
+
+// How far the 16-byte pieces of row r of a tile are xored, within 256 bytes (rows of 128
+// columns) or 128 (of 64, two rows to 256): neither 16 rows of one piece (keys) nor 4 rows
+// of two (transposed values) meet in a bank.
+template <int D>
+__device__ __forceinline__ uint32_t swap_of(uint32_t r) {
+  return D == 128 ? (r % 8) * 2 | r / 8 % 2 : (r / 2 % 4) * 2 | r / 8 % 2;
+}
+
+// A workgroup takes 128 query rows of a head, 32 a wave, and passes over the keys they see,
+// 64 at a time: rows go from memory straight to LDS, into one of two buffers while the
+// other is read.
 template <int DN, int TYPE>
-__global__ __launch_bounds__(kThreads, 1) void prompt_kernel(const PromptParams p) {
-  constexpr int kW = DN + kRope, kKS = kW / 32, kCT = DN / 16;
-  constexpr uint32_t kKeyRow = kStride<kW>, kValRow = kStride<DN>;
-  __shared__ __attribute__((aligned(16))) char lds_k[kTile * kKeyRow];
-  __shared__ __attribute__((aligned(16))) char lds_v[kTile * kValRow];
+__global__ __launch_bounds__(kThreads, 2) void prompt_kernel(const PromptParams p) {
+  constexpr int kNS = DN / 32, kCT = DN / 16;
+  constexpr uint32_t kRow = DN * 2, kRopeRow = kRope * 2;
+  constexpr uint32_t kRopeAt = kTile * kRow, kValueAt = kRopeAt + kTile * kRopeRow, kBuffer = kValueAt + kTile * kRow;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer];
   const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t head = blockIdx.x;
-  // One workgroup counts the requests that are cut or skipped.
-  if (p.err != nullptr && blockIdx.x == 0 && blockIdx.y == 0) {
-    for (uint32_t b = threadIdx.x; b < p.batch; b += kThreads) {
-      const int32_t q0 = p.qo_indptr[b], q1 = p.qo_indptr[b + 1], k0 = p.kv_indptr[b], k1 = p.kv_indptr[b + 1];
-      const bool fine = q0 >= 0 && q1 >= q0 && static_cast<uint32_t>(q1) <= p.nnz &&
-                        static_cast<uint32_t>(q1 - q0) <= p.max_q && k0 >= 0 && k1 >= k0 &&
-                        static_cast<uint32_t>(k1) <= p.keys;
-      if (!fine) atomicAdd(p.err, 1);
-    }
-  }
+  if (p.err != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && w == 0) count_bad(p);
   PromptRequest r;
-  if (!find_tile(p, blockIdx.y, &r)) return;
+  // The last tiles first: they see the most keys.
+  if (!find_tile(p, gridDim.y - 1 - blockIdx.y, &r)) return;
   const int32_t k0 = min(max(p.kv_indptr[r.index], 0), static_cast<int32_t>(p.keys));
   const int32_t k1 = min(max(p.kv_indptr[r.index + 1], k0), static_cast<int32_t>(p.keys));
   const int32_t q_len = r.q1 - r.q0, kv_len = k1 - k0, base = kv_len - q_len;
-  const int32_t row0 = static_cast<int32_t>(r.tile * kRows), my_row = row0 + static_cast<int32_t>(w * 16 + n);
+  const int32_t row0 = static_cast<int32_t>(r.tile * kRows), wave_row0 = row0 + static_cast<int32_t>(w * 16 * kRT);
   int32_t t_end = kv_len;
   if (p.causal) t_end = min(t_end, base + min(row0 + static_cast<int32_t>(kRows), q_len));
-  u32x4 qf[kKS];
+  // Keys that a row sees: those before `seen_by`.
+  const auto seen_by = [&](int32_t row) { return p.causal ? base + row + 1 : kv_len; };
+
+  // Query fragments with the scale's sign: what follows takes it as positive.  (A scale
+  // of zero makes all scores zero.)
+  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
+  const float per_score = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  u32x4 qf[kRT][kNS + 2];
 #pragma unroll
-  for (int k = 0; k < kKS; ++k) {
-    qf[k] = u32x4{0, 0, 0, 0};
-    if (my_row < q_len)
-      qf[k] = *reinterpret_cast<const u32x4*>(p.q + static_cast<int64_t>(r.q0 + my_row) * p.q_token + head * p.q_head +
-                                              k * 64 + g * 16);
+  for (int a = 0; a < kRT; ++a) {
+    const int32_t row = wave_row0 + a * 16 + static_cast<int32_t>(n);
+    const char* const q = p.q + static_cast<int64_t>(r.q0 + row) * p.q_token + head * p.q_head;
+#pragma unroll
+    for (int k = 0; k < kNS + 2; ++k) {
+      qf[a][k] = u32x4{0, 0, 0, 0};
+      if (row < q_len) qf[a][k] = (*reinterpret_cast<const u32x4*>(q + k * 64 + g * 16) ^ flip) & keep;
+    }
   }
-  f32x4 acc[kCT];
+  f32x4 acc[kRT][kCT];
+  float m[kRT], l[kRT];
+  bool wide[kRT];                                        // some row's |m| is past 2^20
 #pragma unroll
-  for (int d = 0; d < kCT; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-  for (int32_t t0 = 0; t0 < t_end; t0 += kTile) {
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < kTile * (kW / 8); e += kThreads) {
-      const uint32_t row = e / (kW / 8), c = e % (kW / 8);
-      const int64_t t = k0 + t0 + static_cast<int64_t>(row);
-      u32x4 x = {0, 0, 0, 0};
-      if (t0 + static_cast<int32_t>(row) < t_end)
-        x = c < DN / 8 ? *reinterpret_cast<const u32x4*>(p.key + t * p.k_token + head * p.k_head + c * 16)
-                       : *reinterpret_cast<const u32x4*>(p.rope_key + t * p.r_token + (c - DN / 8) * 16);
-      *reinterpret_cast<u32x4*>(lds_k + row * kKeyRow + c * 16) = x;
-    }
-    for (uint32_t e = threadIdx.x; e < kTile * (DN / 8); e += kThreads) {
-      const uint32_t row = e / (DN / 8), c = e % (DN / 8);
-      const int64_t t = k0 + t0 + static_cast<int64_t>(row);
-      u32x4 x = {0, 0, 0, 0};
-      if (t0 + static_cast<int32_t>(row) < t_end)
-        x = *reinterpret_cast<const u32x4*>(p.value + t * p.v_token + head * p.v_head + c * 16);
-      *reinterpret_cast<u32x4*>(lds_v + row * kValRow + c * 16) = x;
-    }
-    __syncthreads();
-    f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  for (int a = 0; a < kRT; ++a) {
+    m[a] = -INFINITY;
+    l[a] = 0.f;
+    wide[a] = false;
 #pragma unroll
-    for (int k = 0; k < kKS; ++k)
+    for (int d = 0; d < kCT; ++d) acc[a][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // A step's loads: 16 rows of keys, rotated parts and values a wave, 1 KiB an instruction.
+  const char* const key0 = p.key + k0 * p.k_token + head * p.k_head;
+  const char* const value0 = p.value + k0 * p.v_token + head * p.v_head;
+  const char* const rope0 = p.rope_key + k0 * p.r_token;
+  const auto load_part = [&](auto whole, auto dim, const char* from, int64_t stride, int32_t t0, uint32_t to) {
+    constexpr uint32_t kD = decltype(dim)::value, kLanes = kD / 8, kAtOnce = 64 / kLanes;
+    const uint32_t ln = opaque(lane), in = ln / kLanes;
+#pragma unroll
+    for (uint32_t i = 0; i < 16; i += kAtOnce) {
+      const uint32_t row = w * 16 + i;                   // and `in` more
+      const char* const rows = from + (static_cast<int64_t>(t0) + row) * stride;
+      const uint32_t piece = (ln % kLanes) ^ swap_of<kD>(i + in);
+      const char* const x = rows + static_cast<uint64_t>(in * static_cast<uint32_t>(stride) + piece * 16);
+      const uint32_t at = to + row * (kD * 2);
+      if (decltype(whole)::value || t0 + static_cast<int32_t>(row + in) < t_end) copy_to_lds(x, at);
+      else lds_put(at + ln * 16, u32x4{0, 0, 0, 0});
+    }
+  };
+  const auto load_step = [&](auto whole, int32_t t0, uint32_t to) {
+    load_part(whole, std::integral_constant<int, DN>{}, key0, p.k_token, t0, to);
+    load_part(whole, std::integral_constant<int, kRope>{}, rope0, p.r_token, t0, to + kRopeAt);
+    load_part(whole, std::integral_constant<int, DN>{}, value0, p.v_token, t0, to + kValueAt);
+  };
+  const auto load_next = [&](int32_t t0, uint32_t to) {
+    if (t0 + static_cast<int32_t>(kTile) <= t_end) load_step(std::true_type{}, t0, to);
+    else if (t0 < t_end) load_step(std::false_type{}, t0, to);
+  };
+
+  // Scores of 32 keys from row `key` on: lane: row n of each tile, keys 16 t + 4 g + e.
+  f32x4 s[kRT][2];
+  const uint32_t key_at = n * kRow + (g ^ swap_of<DN>(n)) * 16, rope_at = kRopeAt + n * kRopeRow + (g ^ swap_of<kRope>(n)) * 16;
+  const auto score = [&](uint32_t from, uint32_t first) {
+    const uint32_t key = opaque(key_at) + from, rope = opaque(rope_at) + from;
+#pragma unroll
+    for (int a = 0; a < kRT; ++a)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[a][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kNS + 2; ++k)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const u32x4 kf = *reinterpret_cast<const u32x4*>(lds_k + (t * 16 + n) * kKeyRow + k * 64 + g * 16);
-        s[t] = mfma<TYPE>(kf, qf[k], s[t]);
+        const u32x4 kf = lds_get<u32x4>(k < kNS ? (key ^ (k * 64)) + (first + t * 16) * kRow
+                                                : (rope ^ ((k - kNS) * 64)) + (first + t * 16) * kRopeRow);
+#pragma unroll
+        for (int a = 0; a < kRT; ++a) s[a][t] = mfma<TYPE>(kf, qf[a][k], s[a][t]);
       }
-    const int32_t upto = min((p.causal ? base + my_row + 1 : kv_len) - t0, t_end - t0);
-    const uint32_t sees = upto >= 32 ? ~0u : upto <= 0 ? 0u : (1u << upto) - 1u, mine = sees >> (4 * g);
-    float top = -INFINITY;
+  };
+  // Weights of those keys, the first of which is t0, packed by twos as they lie in s.
+  u32x4 pf[kRT];
+  const auto weigh = [&](auto full, int32_t t0) {
+    if constexpr (!decltype(full)::value) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int a = 0; a < kRT; ++a) {
+        const int32_t upto = min(seen_by(wave_row0 + a * 16 + static_cast<int32_t>(n)), t_end) - t0 - 4 * static_cast<int32_t>(g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[t][e] = (mine & (1u << (t * 16 + e))) ? scaled(s[t][e], p.scale_log2) : -INFINITY;
-        top = fmaxf(top, s[t][e]);
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (t * 16 + e >= upto) s[a][t][e] = -INFINITY;
       }
-    top = fmaxf(m, across_groups(top, max_of));
-    const float from = top == -INFINITY ? 0.f : top, shrink = exp2_of(m - from);
-    m = top;
-    l *= shrink;
-#pragma unroll
-    for (int d = 0; d < kCT; ++d) acc[d] *= shrink;
-    u32x4 pf;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        const float x = weight_of<TYPE>(s[t][e], from), y = weight_of<TYPE>(s[t][e + 1], from);
-        l += x + y;
-        pf[t * 2 + e / 2] = pair_of<TYPE>(x, y);
-      }
-    bool odd = false;
-    if (__ballot(sees == ~0u) != ~0ull) {
-      bool found = false;
-      for (uint32_t c = lane; c < kTile * DN / 8; c += 64) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(lds_v + c / (DN / 8) * kValRow + c % (DN / 8) * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) found |= odd_word<TYPE>(x[e]);
-      }
-      odd = __ballot(found) != 0;
     }
+#pragma unroll
+    for (int a = 0; a < kRT; ++a) settle(s[a][0], s[a][1]);
+#pragma unroll
+    for (int a = 0; a < kRT; ++a) {
+      float top = max3_of(s[a][0][0], s[a][0][1], s[a][0][2]);
+      top = max3_of(top, s[a][0][3], s[a][1][0]);
+      top = max3_of(top, s[a][1][1], s[a][1][2]);
+      top = scaled(max3_of(top, s[a][1][3], s[a][1][3]), per_score);
+      if (__ballot(top > m[a] + kSlack) != 0) {
+        top = across_groups(top, max_of);
+        const float next = top > m[a] + kSlack ? top : m[a];
+        const float shrink = exp2_of(m[a] - (next == -INFINITY ? 0.f : next));
+        m[a] = next;
+        l[a] *= shrink;
+        wide[a] = __ballot(fabsf(next) > 0x1p20f && next != -INFINITY) != 0;
+#pragma unroll
+        for (int d = 0; d < kCT; ++d) acc[a][d] *= shrink;
+      }
+      const float from = m[a] == -INFINITY ? 0.f : m[a];
+      // The fused difference holds what m lost when it was rounded: less than a tenth up
+      // to 2^20, but past 2^27 enough to make the largest weight an infinity or a zero.
+      if (wide[a]) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[a][t][e] = unfused(scaled(s[a][t][e], per_score), from) + kUnit<TYPE>;
+      } else {
+        const float offset = kUnit<TYPE> - from;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[a][t][e] = __builtin_fmaf(s[a][t][e], per_score, offset);
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const float x = exp2_of(s[a][t][e]), y = exp2_of(s[a][t][e + 1]);
+          l[a] += x + y;
+          pf[a][t * 2 + e / 2] = pair_of<TYPE>(x, y);
+        }
+    }
+  };
+  // Adds the weighted values of those keys: a lane's group holds those of rows 4 g .. 4 g + 3
+  // and the same behind 16.
+  const uint32_t v_row = 4 * g + n / 4;
+  const uint32_t v_at = kValueAt + v_row * kRow + (n % 4 / 2 ^ swap_of<DN>(v_row)) * 16 + n % 2 * 8;
+  const auto gather = [&](uint32_t from, uint32_t first) {
+    const uint32_t v = opaque(v_at) + from;
 #pragma unroll
     for (int d = 0; d < kCT; ++d) {
-      const char* v = lds_v + lane / 4 * kValRow + d * 32 + lane % 4 * 8;
-      typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-      const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)v));
-      const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(v + 16 * kValRow)));
-      if (!odd) acc[d] = mfma<TYPE>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf, acc[d]);
+      const uint32_t x = (v ^ (d * 32)) + first * kRow;
+      const u32x2 lo = lds_transposed(x), hi = lds_transposed(x + 16 * kRow);
+      const u32x4 vf = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+      for (int a = 0; a < kRT; ++a) acc[a][d] = mfma<TYPE>(vf, pf[a], acc[a][d]);
     }
-    if (odd) {
+  };
+  // Takes infinities and NaN out of the values that the wave loaded: a product with weight
+  // zero would spread them to rows that do not see their key.
+  bool odd = false;
+  const auto clean = [&](uint32_t from) {
+    bool found = false;
 #pragma unroll 1
-      for (uint32_t token = 0; token < kTile; ++token) {
-        const uint32_t word = token / 16 * 2 + token % 4 / 2;
-        const uint32_t of = word == 0 ? pf[0] : word == 1 ? pf[1] : word == 2 ? pf[2] : pf[3];
-        const float weight = value_of<TYPE>(__shfl(of, token % 16 / 4 * 16 + n), token % 2);
-        if (!((sees >> token) & 1u)) continue;
+    for (uint32_t c = lane; c < 16 * DN / 8; c += 64) {
+      const uint32_t at = from + kValueAt + w * 16 * kRow + c * 16;
+      u32x4 x = lds_get<u32x4>(at);
+      bool here = false;
 #pragma unroll
-        for (int d = 0; d < kCT; ++d) {
-          const u32x2 v = *reinterpret_cast<const u32x2*>(lds_v + token * kValRow + d * 32 + g * 8);
+      for (int e = 0; e < 4; ++e) here |= odd_word<TYPE>(x[e]);
+      if (here) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) acc[d][c] += weight * value_of<TYPE>(v[c / 2], c % 2);
-        }
+        for (int e = 0; e < 4; ++e) x[e] = finite_halves<TYPE>(x[e]);
+        lds_put(at, x);
+        found = true;
+      }
+    }
+    odd |= found;
+  };
+
+  constexpr int32_t kStep = static_cast<int32_t>(kTile);
+  uint32_t now = lds_offset(lds), other = now + kBuffer;
+  int32_t t0 = 0;
+  const auto one_step = [&](auto full) {
+    __builtin_amdgcn_s_waitcnt(0x0f70);                  // vmcnt(0): this step's rows are in LDS
+    __syncthreads();                                     // and the other buffer's readers are done
+    load_next(t0 + kStep, other);
+    if constexpr (!decltype(full)::value) {
+      clean(now);
+      __syncthreads();
+    }
+#pragma unroll
+    for (uint32_t h = 0; h < kTile; h += 32) {
+      if constexpr (!decltype(full)::value)
+        if (t0 + static_cast<int32_t>(h) >= seen_by(wave_row0 + 16 * kRT - 1)) break;  // no row of the wave sees any
+      score(now, h);
+      weigh(full, t0 + static_cast<int32_t>(h));
+      gather(now, h);
+    }
+    const uint32_t x = now;
+    now = other;
+    other = x;
+    t0 += kStep;
+  };
+  load_next(0, now);
+  // The steps whose keys every row sees, then the others.
+  while (t0 + kStep <= min(seen_by(row0), t_end)) one_step(std::true_type{});
+  const int32_t t_masked = t0;
+#pragma unroll 1
+  while (t0 < t_end) one_step(std::false_type{});
+#pragma unroll
+  for (int a = 0; a < kRT; ++a) {
+    l[a] = across_groups(l[a], sum_of);
+    const int32_t row = wave_row0 + a * 16 + static_cast<int32_t>(n);
+    if (row >= q_len) continue;
+    const float inv = l[a] == 0.f ? 0.f : 1.f / l[a];
+    char* const out = p.out + static_cast<int64_t>(r.q0 + row) * p.o_token + head * p.o_head;
+#pragma unroll
+    for (int d = 0; d < kCT; ++d) {
+      const u32x2 x = {result_pair<TYPE>(acc[a][d][0] * inv, acc[a][d][1] * inv),
+                       result_pair<TYPE>(acc[a][d][2] * inv, acc[a][d][3] * inv)};
+      *reinterpret_cast<u32x2*>(out + (d * 16 + g * 4) * 2) = x;
+    }
+    if (g == 0 && p.lse != nullptr) p.lse[static_cast<int64_t>(r.q0 + row) * p.heads + head] = log_total<TYPE>(m[a], l[a]);
+  }
+  if (t_masked >= t_end) return;
+  // What any wave took out reaches the rows that see it.  (LDS is full: two workgroups' buffers
+  // take all of a CU's.)
+  __syncthreads();
+  const bool found = __ballot(odd) != 0;
+  if (lane == 0) lds_put(lds_offset(lds) + w * 4, found ? 1u : 0u);
+  __syncthreads();
+  const u32x4 any = lds_get<u32x4>(lds_offset(lds));
+  if ((any[0] | any[1] | any[2] | any[3]) == 0) return;
+#pragma unroll 1
+  for (int a = 0; a < kRT; ++a) {
+    const int32_t row = wave_row0 + a * 16 + static_cast<int32_t>(n);
+    if (row >= q_len) continue;
+    char* const out = p.out + static_cast<int64_t>(r.q0 + row) * p.o_token + head * p.o_head;
+#pragma unroll 1
+    for (int32_t t = t_masked; t < min(seen_by(row), t_end); ++t) {
+      const char* const x = value0 + static_cast<int64_t>(t) * p.v_token;
+#pragma unroll 1
+      for (uint32_t c = 0; c < kCT * 4; ++c) {
+        const uint32_t at = (c / 4 * 16 + g * 4 + c % 4) * 2;
+        const uint32_t v = *reinterpret_cast<const uint16_t*>(x + at);
+        if (!odd_word<TYPE>(v)) continue;
+        uint16_t* const o = reinterpret_cast<uint16_t*>(out + at);
+        *o = static_cast<uint16_t>(pair_of<TYPE>(value_of<TYPE>(*o, 0) + value_of<TYPE>(v, 0), 0.f));
       }
     }
   }
-  l = across_groups(l, sum_of);
-  if (my_row >= q_len) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int d = 0; d < kCT; ++d) {
-    const u32x2 x = {result_pair<TYPE>(acc[d][0] * inv, acc[d][1] * inv),
-                     result_pair<TYPE>(acc[d][2] * inv, acc[d][3] * inv)};
-    *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(r.q0 + my_row) * p.o_token + head * p.o_head +
-                              (d * 16 + g * 4) * 2) = x;
-  }
-  if (g == 0 && p.lse != nullptr) p.lse[static_cast<int64_t>(r.q0 + my_row) * p.heads + head] = log_total<TYPE>(m, l);
 }
 
 template <int DN>
@@ -245,6 +411,9 @@ int pace_kv_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_he
        static_cast<uintptr_t>(q_token_stride | q_head_stride | k_token_stride | k_head_stride | rope_token_stride |
                               v_token_stride | v_head_stride | out_token_stride | out_head_stride)) & 15u)
     return fail(PACE_KV_EINVAL, "prompt attention: rows and strides must be multiples of 16 bytes");
+  const int64_t longest = std::max({k_token_stride, rope_token_stride, v_token_stride});
+  if (longest >= int64_t(1) << 26 || std::min({k_token_stride, rope_token_stride, v_token_stride}) < 0)
+    return fail(PACE_KV_EINVAL, "prompt attention: token strides of keys and values must be in [0, 2^26)");
   // As many tiles as there can be: a short last one for each request.
   const int64_t tiles = std::min<int64_t>(nnz, nnz / kRows + batch_size);
   if (tiles > 65535 || num_heads > (1 << 20) || tiles * num_heads >= (int64_t(1) << 24))
