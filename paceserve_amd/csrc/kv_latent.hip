@@ -33,8 +33,10 @@ __device__ __forceinline__ uint32_t seen_of(const AttnParams& p, const Request& 
 }
 
 // RT tiles of 16 rows a workgroup, whose four waves sum a quarter of the columns each, of
-// all rows.  Up to two tiles every wave makes the weights of all rows for itself; past
-// that each makes those of a quarter of the rows, and they share them through LDS.
+// all rows.  Up to two tiles every wave makes the weights of all rows for itself.  Of four
+// tiles a wave multiplies two by every other 32 columns of the keys, swaps halves of the
+// sums with its neighbour, so that each has the scores of one tile, and the waves share the
+// weights through LDS: a key that is read from there serves two products.
 //
 // 32 tokens a step go from memory straight to LDS, into one of two buffers while the
 // other is read.  There the latents' 16-byte pieces c of row r lie at c ^ swap(r), within
@@ -44,13 +46,16 @@ template <int L, int TYPE, int RT>
 __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const AttnParams p) {
   constexpr int kW = L + kRope, kKS = L / 32, kCT = L / 64;
   constexpr bool kShare = RT >= 4;
-  constexpr int RW = kShare ? RT / kWaves : RT;          // tiles whose weights a wave makes
+  constexpr int RW = kShare ? 1 : RT;                    // tiles whose weights a wave makes
+  constexpr int RQ = kShare ? 2 : RT, kQS = kShare ? kKS / 2 + 1 : kKS + 2;  // tiles and steps of its products
   constexpr uint32_t kRow = L * 2, kRopeAt = kTile * kRow, kBuffer = kRopeAt + kTile * kRope * 2;
   constexpr uint32_t kWeightRow = kTile * 2;
   __shared__ __attribute__((aligned(1024))) char lds[2 * kBuffer];
-  __shared__ __attribute__((aligned(256))) char lds_p[kShare ? RT * 16 * kWeightRow : 16];
-  __shared__ float lds_shrink[kShare ? RT * 16 : 1], lds_ml[kShare ? RT * 16 : 1][2];
-  __shared__ __attribute__((aligned(16))) uint32_t lds_raised[kWaves];
+  // What the waves share, 2 KiB each: first sums for the neighbour, then, in the place of
+  // those it has read, a wave's weights, the factors of its rows, whether any is not 1, and
+  // in the end their maxima and sums.  (Two workgroups fill a CU's LDS.)
+  constexpr uint32_t kShared = 2048, kShrinkAt = 1024, kRaisedAt = 1088, kMlAt = 1152;
+  __shared__ __attribute__((aligned(1024))) char lds_p[kShare ? kWaves * kShared : 16];
   const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t at = blockIdx.x / kXcds, nth = over(p.by_unit, at);
@@ -93,18 +98,19 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
 
   // Query fragments: row n of each tile, eight elements from 32 k + 8 g, with the scale's
   // sign: what follows takes it as positive.  (A scale of zero makes all scores zero.)
-  const uint32_t wave_row0 = row0 + (kShare ? w * RW * 16 : 0);
+  const uint32_t wave_row0 = row0 + (kShare ? w * 16 : 0), query_row0 = row0 + (kShare ? w / 2 * 32 : 0);
   const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
   const float per_score = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
-  u32x4 qf[RW][kKS + 2];
+  u32x4 qf[RQ][kQS];
 #pragma unroll
-  for (int a = 0; a < RW; ++a) {
-    const uint32_t row = wave_row0 + a * 16 + n, i = over(p.by_group, row);
+  for (int a = 0; a < RQ; ++a) {
+    const uint32_t row = query_row0 + a * 16 + n, i = over(p.by_group, row);
     const char* const q = p.q + static_cast<int64_t>(r.q0 + i) * p.q_stride + static_cast<int64_t>(row - i * p.group) * (kW * 2);
 #pragma unroll
-    for (int k = 0; k < kKS + 2; ++k) {
+    for (int k = 0; k < kQS; ++k) {
       qf[a][k] = u32x4{0, 0, 0, 0};
-      if (row < rows) qf[a][k] = (*reinterpret_cast<const u32x4*>(q + k * 64 + g * 16) ^ flip) & keep;
+      const uint32_t of = kShare ? 2 * k + w % 2 : k;
+      if (row < rows) qf[a][k] = (*reinterpret_cast<const u32x4*>(q + of * 64 + g * 16) ^ flip) & keep;
     }
   }
   f32x4 acc[RT][kCT];
@@ -161,25 +167,46 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
 
   // Scores of 32 tokens: lane: row n of each tile, tokens 16 t + 4 g + e.
   f32x4 s[RW][2];
-  const uint32_t swap_n = (n % 8) * 2 | n / 8;
-  const uint32_t key_at = n * kRow + (g ^ swap_n) * 16, rope_at = kRopeAt + n * (kRope * 2) + (g ^ (n / 2)) * 16;
+  const uint32_t swap_n = (n % 8) * 2 | n / 8, odd_step = kShare ? w % 2 * 64 : 0;
+  const uint32_t key_at = (n * kRow + (g ^ swap_n) * 16) ^ odd_step;
+  const uint32_t rope_at = kRopeAt + ((n * (kRope * 2) + (g ^ (n / 2)) * 16) ^ odd_step);
+  const uint32_t my_sums = lds_offset(lds_p) + w * kShared, other_sums = lds_offset(lds_p) + (w ^ 1) * kShared;
   const auto score = [&](uint32_t from) {
     const uint32_t key = opaque(key_at) + from, rope = opaque(rope_at) + from;
+    constexpr int kMain = kShare ? kKS / 2 : kKS;
+    f32x4 x[RQ][2];
 #pragma unroll
-    for (int a = 0; a < RW; ++a)
+    for (int a = 0; a < RQ; ++a)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) s[a][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < 2; ++t) x[a][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < kKS + 2; ++k)
+    for (int k = 0; k < kQS; ++k)
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const u32x4 kf = lds_get<u32x4>(k < kKS ? (key ^ (k % 4 * 64)) + t * 16 * kRow + k / 4 * 256
-                                                : (rope ^ ((k - kKS) * 64)) + t * 16 * (kRope * 2));
+        u32x4 kf;
+        if (k >= kMain) kf = lds_get<u32x4>((rope ^ ((k - kMain) * 64)) + t * 16 * (kRope * 2));
+        else if (kShare) kf = lds_get<u32x4>((key ^ (k % 2 * 128)) + t * 16 * kRow + k / 2 * 256);
+        else kf = lds_get<u32x4>((key ^ (k % 4 * 64)) + t * 16 * kRow + k / 4 * 256);
 #pragma unroll
-        for (int a = 0; a < RW; ++a) s[a][t] = mfma<TYPE>(kf, qf[a][k], s[a][t]);
+        for (int a = 0; a < RQ; ++a) x[a][t] = mfma<TYPE>(kf, qf[a][k], x[a][t]);
       }
+    if constexpr (kShare) {
+      const bool second = w % 2 != 0;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        lds_put(my_sums + t * 1024 + lane * 16, second ? x[0][t] : x[1][t]);
+        s[0][t] = second ? x[1][t] : x[0][t];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < 2; ++t) s[0][t] += lds_get<f32x4>(other_sums + t * 1024 + lane * 16);
+    } else {
+#pragma unroll
+      for (int a = 0; a < RW; ++a)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) s[a][t] = x[a][t];
+    }
   };
-
   // Weights of those tokens, packed by twos as they lie in s; raises the maximum where a
   // score passes it by kSlack, for which shrink is the factor of what was summed before.
   u32x4 pf[RW];
@@ -271,12 +298,12 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   // they are 8 g .. 8 g + 7.
   const uint32_t v_row = kShare ? 8 * g + n / 4 : 4 * g + n / 4;
   const uint32_t v_at = v_row * kRow + ((w * kCT * 2 + n % 4 / 2) ^ ((v_row % 8) * 2 | v_row / 8 % 2)) * 16 + n % 2 * 8;
-  const uint32_t p_at = lds_offset(lds_p) + n * kWeightRow + (g ^ (n / 4)) * 16;
+  const uint32_t p_at = lds_offset(lds_p) + n * kWeightRow + (g ^ (n / 4)) * 16;  // tile a's are at (a ^ 1) * kShared
   const auto gather = [&](uint32_t from) {
     u32x4 weight[RT];
 #pragma unroll
     for (int a = 0; a < RT; ++a) {
-      if constexpr (kShare) weight[a] = lds_get<u32x4>(p_at + a * 16 * kWeightRow);
+      if constexpr (kShare) weight[a] = lds_get<u32x4>(p_at + (a ^ 1) * kShared);
       else weight[a] = pf[a];
     }
     const uint32_t v = opaque(v_at) + from;
@@ -308,25 +335,23 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
     score(now);
     weigh(full, t0);
     if constexpr (kShare) {
-      const uint32_t to = lds_offset(lds_p) + (w * RW * 16 + n) * kWeightRow + g % 2 * 8;
 #pragma unroll
-      for (int a = 0; a < RW; ++a) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          lds_put(to + a * 16 * kWeightRow + ((2 * t + g / 2) ^ (n / 4)) * 16, u32x2{pf[a][2 * t], pf[a][2 * t + 1]});
-        if (raised != 0 && g == 0) lds_shrink[(w * RW + a) * 16 + n] = shrink[a];
-      }
-      if (lane == 0) lds_raised[w] = raised;
+      for (int t = 0; t < 2; ++t)
+        lds_put(other_sums + n * kWeightRow + ((2 * t + g / 2) ^ (n / 4)) * 16 + g % 2 * 8,
+                u32x2{pf[0][2 * t], pf[0][2 * t + 1]});
+      if (g == 0) lds_put(other_sums + kShrinkAt + n * 4, shrink[0]);
+      if (lane == 0) lds_put(other_sums + kRaisedAt, raised);
     }
     if (kShare || !decltype(full)::value) __syncthreads();
     if constexpr (!decltype(full)::value) clean(now);
     if constexpr (kShare) {
-      const u32x4 all = *reinterpret_cast<const u32x4*>(lds_raised);
-      if (__builtin_amdgcn_readfirstlane(all[0] | all[1] | all[2] | all[3]) != 0) {
+      const uint32_t any = lds_get<uint32_t>(lds_offset(lds_p) + lane % kWaves * kShared + kRaisedAt);
+      const uint64_t which = __ballot(any != 0);         // bit a: tile a ^ 1
+      if (which != 0) {
 #pragma unroll
         for (int a = 0; a < RT; ++a)
-          if (__builtin_amdgcn_readfirstlane(all[a / RW]) != 0) {
-            const float by = lds_shrink[a * 16 + n];
+          if (which >> (a ^ 1) & 1u) {
+            const float by = lds_get<float>(lds_offset(lds_p) + (a ^ 1) * kShared + kShrinkAt + n * 4);
 #pragma unroll
             for (int d = 0; d < kCT; ++d) acc[a][d] *= by;
           }
@@ -357,10 +382,7 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   for (int a = 0; a < RW; ++a) {
     l[a] = across_groups(l[a], sum_of);
     if constexpr (kShare)
-      if (g == 0) {
-        lds_ml[(w * RW + a) * 16 + n][0] = m[a];
-        lds_ml[(w * RW + a) * 16 + n][1] = l[a];
-      }
+      if (g == 0) lds_put(other_sums + kMlAt + n * 8, f32x2{m[a], l[a]});
   }
   if (kShare) __syncthreads();
   const bool direct = r.chunks == 1;
@@ -376,8 +398,9 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
     if (row >= rows) continue;
     float top, sum;
     if constexpr (kShare) {
-      top = lds_ml[in_tile][0];
-      sum = lds_ml[in_tile][1];
+      const f32x2 ml = lds_get<f32x2>(lds_offset(lds_p) + (a ^ 1) * kShared + kMlAt + n * 8);
+      top = ml[0];
+      sum = ml[1];
     } else {
       top = m[a];
       sum = l[a];
