@@ -197,7 +197,7 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
         lds_put(my_sums + t * 1024 + lane * 16, second ? x[0][t] : x[1][t]);
         s[0][t] = second ? x[1][t] : x[0][t];
       }
-      __syncthreads();
+      lds_barrier();
 #pragma unroll
       for (int t = 0; t < 2; ++t) s[0][t] += lds_get<f32x4>(other_sums + t * 1024 + lane * 16);
     } else {
@@ -329,8 +329,7 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   const auto one_step = [&](auto full) {
     valid = next_valid;
     place_rows(t0 + kStep);
-    __builtin_amdgcn_s_waitcnt(0x0f70);                  // vmcnt(0): this step's rows are in LDS
-    __syncthreads();                                     // and the other buffer's readers are done
+    rows_barrier();                                      // this step's rows are in LDS, the other buffer's readers done
     load_next(t0 + kStep, other);
     score(now);
     weigh(full, t0);
@@ -342,7 +341,7 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
       if (g == 0) lds_put(other_sums + kShrinkAt + n * 4, shrink[0]);
       if (lane == 0) lds_put(other_sums + kRaisedAt, raised);
     }
-    if (kShare || !decltype(full)::value) __syncthreads();
+    if (kShare || !decltype(full)::value) lds_barrier();
     if constexpr (!decltype(full)::value) clean(now);
     if constexpr (kShare) {
       const uint32_t any = lds_get<uint32_t>(lds_offset(lds_p) + lane % kWaves * kShared + kRaisedAt);
@@ -453,13 +452,17 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   }
 }
 
-// Joins the parts of split requests' rows, a wave a row.
-template <int L, int TYPE>
+// Joins the parts of split requests' rows, WAVES waves a row (four where the rows alone do
+// not fill the GPU): the chunks' maxima and sums come first, 64 at a time, so that the loads
+// of their outputs do not wait for one another.
+template <int L, int TYPE, uint32_t WAVES>
 __global__ __launch_bounds__(kThreads) void latent_join_kernel(const AttnParams p) {
   constexpr uint32_t kVec = L / 64;                      // columns of a lane
   typedef float vec __attribute__((ext_vector_type(kVec)));
+  __shared__ vec lds_o[WAVES == 1 ? 1 : WAVES][WAVES == 1 ? 1 : 64];
   const uint32_t lane = threadIdx.x % 64, w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const uint32_t id = blockIdx.x * kWaves + w, token = over(p.by_heads, id), head = id - token * p.group;
+  const uint32_t id = WAVES == 1 ? blockIdx.x * kWaves + w : blockIdx.x;
+  const uint32_t token = over(p.by_heads, id), head = id - token * p.group, part = WAVES == 1 ? 0 : w;
   if (token >= p.nnz) return;
   Tables t;
   Place place;
@@ -470,16 +473,34 @@ __global__ __launch_bounds__(kThreads) void latent_join_kernel(const AttnParams 
   const uint32_t row = (token - r.q0) * p.group + head, tile = row / p.tile_rows;
   const int64_t first = (static_cast<int64_t>(place.part()) * p.row_tiles + tile) * p.tile_rows + row % p.tile_rows;
   const int64_t step = static_cast<int64_t>(p.row_tiles) * p.tile_rows;
+  // The maximum over all chunks, which every wave finds for itself.
   float m = -INFINITY;
-  for (uint32_t c = 0; c < r.chunks; ++c) m = fmaxf(m, p.part_ml[(first + c * step) * 2]);
+  for (uint32_t c = lane; c < r.chunks; c += 64) m = fmaxf(m, p.part_ml[(first + c * step) * 2]);
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) m = fmaxf(m, __shfl_xor(m, k));
   const float from = m == -INFINITY ? 0.f : m;
   float l = 0.f;
   vec o = {};
-  for (uint32_t c = 0; c < r.chunks; ++c) {
-    const int64_t at = first + c * step;
-    const float weight = exp2_of(p.part_ml[at * 2] - from);
-    l += weight * p.part_ml[at * 2 + 1];
-    o += weight * *reinterpret_cast<const vec*>(p.part_o + at * L + lane * kVec);
+  for (uint32_t c0 = 0; c0 < r.chunks; c0 += 64) {
+    float weight = 0.f;
+    if (c0 + lane < r.chunks) {
+      const int64_t at = (first + (c0 + lane) * step) * 2;
+      weight = exp2_of(p.part_ml[at] - from);
+      l += weight * p.part_ml[at + 1];
+    }
+    const uint32_t n = min(r.chunks - c0, 64u);
+#pragma unroll 4
+    for (uint32_t c = part; c < n; c += WAVES)
+      o += __shfl(weight, c) * *reinterpret_cast<const vec*>(p.part_o + (first + (c0 + c) * step) * L + lane * kVec);
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) l += __shfl_xor(l, k);
+  if constexpr (WAVES > 1) {
+    if (w != 0) lds_o[w][lane] = o;
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (uint32_t v = 1; v < WAVES; ++v) o += lds_o[v][lane];
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   char* const out = p.out + static_cast<int64_t>(token) * p.out_stride + (static_cast<int64_t>(head) * L + lane * kVec) * 2;
@@ -494,16 +515,38 @@ struct Split {
   int64_t part_rows() const { return static_cast<int64_t>(parts) * row_tiles * tile_rows; }
 };
 
-Split split_of(int64_t batch, int64_t rows, int64_t num_indices, int64_t page_size) {
+// A call's contexts are cut so that the CUs' 512 places for workgroups (two a CU) are filled
+// evenly.  With w workgroups of n steps a call takes about ceil(w / 512) (n + kStart) steps,
+// and, where requests are cut, the joining kernel: its launch, and the parts written and
+// read.  Of the requests' lengths the host knows only the sum: w is taken as the mean of
+// what equal lengths give and what lengths spread evenly give, whose last chunks are half
+// empty.
+constexpr int64_t kPlaces = 512, kStart = 3, kJoin = 2, kPartBytes = int64_t(8) << 20;
+
+Split split_of(int64_t batch, int64_t rows, int latent_dim, int64_t num_indices, int64_t page_size) {
   Split s = {};
   s.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
   s.row_tiles = static_cast<uint32_t>((rows + s.tile_rows - 1) / s.tile_rows);
   s.step_pages = static_cast<uint32_t>(kTile % page_size ? 1 : kTile / page_size);
   const int64_t requests = std::max<int64_t>(batch, 1), pages = std::max<int64_t>((num_indices + requests - 1) / requests, 1);
-  const int64_t least = 256;
-  const int64_t k = std::max<int64_t>(std::min<int64_t>(512 / (requests * s.row_tiles), pages * page_size / least), 1);
-  int64_t chunk = ((pages + k - 1) / k + s.step_pages - 1) / s.step_pages * s.step_pages;
-  chunk = std::max<int64_t>(chunk, (least + page_size - 1) / page_size);
+  const auto steps_of = [&](int64_t chunk) { return (chunk * page_size + kTile - 1) / kTile; };
+  const auto turns_of = [&](int64_t items) { return (items * s.row_tiles + kPlaces - 1) / kPlaces; };
+  const int64_t part_bytes = requests * rows * latent_dim * 8;
+  int64_t chunk = pages, best = INT64_MAX, before = 0;
+  const int64_t most = std::min<int64_t>(std::max<int64_t>(steps_of(pages), 1), 256);
+  for (int64_t k = 1; k <= most; ++k) {
+    const int64_t length = ((pages + k - 1) / k + s.step_pages - 1) / s.step_pages * s.step_pages;
+    if (length == before) continue;
+    before = length;
+    const int64_t even = requests * ((pages + length - 1) / length);
+    const int64_t spread = batch > 1 ? num_indices / length + requests / 2 : even;
+    const int64_t join = k == 1 ? 0 : 2 * kJoin + 2 * part_bytes * k / kPartBytes;
+    const int64_t cost = (turns_of(even) + turns_of(spread)) * (steps_of(length) + kStart) + join;
+    if (cost < best) {
+      best = cost;
+      chunk = length;
+    }
+  }
   chunk = std::max<int64_t>(std::min(chunk, num_indices), 1);
   s.chunk_pages = static_cast<uint32_t>(chunk);
   s.items = static_cast<uint32_t>(num_indices / chunk + batch);
@@ -524,7 +567,7 @@ int check_sizes(int batch_size, int heads, int latent_dim, int max_q_len, int64_
     return fail(PACE_KV_ERANGE, "latent attention: more than 2^30 tokens or query rows");
   bool fits = batch_size < kMostGroups;
   if (fits) {
-    const Split s = split_of(batch_size, rows, num_indices, page_size);
+    const Split s = split_of(batch_size, rows, latent_dim, num_indices, page_size);
     fits = s.row_tiles < kMostGroups && (static_cast<int64_t>(s.items) + kXcds) * s.row_tiles < kMostGroups;
   }
   if (!fits) return fail(PACE_KV_ERANGE, "latent attention: too many requests, heads or query rows for one call");
@@ -547,10 +590,18 @@ const void* pick_latent(int type, uint32_t tile_rows) {
   return type == PACE_KV_BF16 ? pick_latent<L, PACE_KV_BF16>(tile_rows) : pick_latent<L, PACE_KV_FP16>(tile_rows);
 }
 
+// Rows of a call from which on a wave joins one by itself.
+constexpr int64_t kManyRows = 4096;
+
+template <int L, int TYPE>
+const void* pick_join(bool many) {
+  return many ? reinterpret_cast<const void*>(&latent_join_kernel<L, TYPE, 1>)
+              : reinterpret_cast<const void*>(&latent_join_kernel<L, TYPE, kWaves>);
+}
+
 template <int L>
-const void* pick_join(int type) {
-  return type == PACE_KV_BF16 ? reinterpret_cast<const void*>(&latent_join_kernel<L, PACE_KV_BF16>)
-                              : reinterpret_cast<const void*>(&latent_join_kernel<L, PACE_KV_FP16>);
+const void* pick_join(int type, bool many) {
+  return type == PACE_KV_BF16 ? pick_join<L, PACE_KV_BF16>(many) : pick_join<L, PACE_KV_FP16>(many);
 }
 
 }  // namespace
@@ -563,7 +614,7 @@ int pace_kv_latent_attention_workspace(int batch_size, int num_heads, int latent
   using namespace pace_kv;
   if (!bytes) return fail(PACE_KV_EINVAL, "latent attention: NULL argument");
   PACE_KV_TRY(check_sizes(batch_size, num_heads, latent_dim, max_q_len, num_indices, page_size));
-  *bytes = workspace_bytes(split_of(batch_size, static_cast<int64_t>(max_q_len) * num_heads, num_indices, page_size),
+  *bytes = workspace_bytes(split_of(batch_size, static_cast<int64_t>(max_q_len) * num_heads, latent_dim, num_indices, page_size),
                            latent_dim);
   return PACE_KV_OK;
 }
@@ -599,7 +650,7 @@ int pace_kv_latent_attention(const void* q, int64_t q_stride_bytes, int elem_typ
     return fail(PACE_KV_EINVAL, "latent attention: q, cache and out must be 16-byte aligned, mask 8-byte");
   if (page_size > (INT64_C(1) << 36) / (width * 2) || num_pages * (page_size * width / 8) >= UINT32_MAX)
     return fail(PACE_KV_ERANGE, "latent attention: a layer's cache must be smaller than 64 GiB");
-  const Split s = split_of(batch_size, static_cast<int64_t>(max_q_len) * num_heads, num_indices, page_size);
+  const Split s = split_of(batch_size, static_cast<int64_t>(max_q_len) * num_heads, latent_dim, num_indices, page_size);
   const int64_t need = workspace_bytes(s, latent_dim);
   if (need > 0 && (!workspace || workspace_size < need || reinterpret_cast<uintptr_t>(workspace) & 15u))
     return fail(PACE_KV_EINVAL, "latent attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
@@ -647,9 +698,12 @@ int pace_kv_latent_attention(const void* q, int64_t q_stride_bytes, int elem_typ
                                          dim3(items * p.row_tiles), dim3(kThreads), args, 0,
                                          static_cast<hipStream_t>(stream)), "latent attention launch"));
   if (need == 0) return PACE_KV_OK;
-  return hip_status(hipLaunchKernel(latent_dim == 512 ? pick_join<512>(elem_type) : pick_join<256>(elem_type),
-                                    dim3(static_cast<uint32_t>((nnz * num_heads + kWaves - 1) / kWaves)), dim3(kThreads),
-                                    args, 0, static_cast<hipStream_t>(stream)), "latent attention join launch");
+  const int64_t out_rows = nnz * num_heads;
+  const bool many = out_rows >= kManyRows;
+  return hip_status(hipLaunchKernel(latent_dim == 512 ? pick_join<512>(elem_type, many) : pick_join<256>(elem_type, many),
+                                    dim3(static_cast<uint32_t>(many ? (out_rows + kWaves - 1) / kWaves : out_rows)),
+                                    dim3(kThreads), args, 0, static_cast<hipStream_t>(stream)),
+                    "latent attention join launch");
 }
 
 }  // extern "C"

@@ -304,12 +304,11 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(const PromptParams 
   uint32_t now = lds_offset(lds), other = now + kBuffer;
   int32_t t0 = 0;
   const auto one_step = [&](auto full) {
-    __builtin_amdgcn_s_waitcnt(0x0f70);                  // vmcnt(0): this step's rows are in LDS
-    __syncthreads();                                     // and the other buffer's readers are done
+    rows_barrier();                                      // this step's rows are in LDS, the other buffer's readers done
     load_next(t0 + kStep, other);
     if constexpr (!decltype(full)::value) {
       clean(now);
-      __syncthreads();
+      lds_barrier();
     }
 #pragma unroll
     for (uint32_t h = 0; h < kTile; h += 32) {

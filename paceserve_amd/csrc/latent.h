@@ -39,6 +39,15 @@ __device__ __forceinline__ float weight_of(float s, float m) {
 // compiler does not do for.  20 cycles, more than any such instruction takes to write.
 __device__ __forceinline__ void settle(f32x4& x, f32x4& y) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x), "+v"(y)); }
 
+// A workgroup's barrier that waits for its LDS operations alone, not for rows on their way
+// into LDS as __syncthreads does.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// One that waits for those rows too.
+__device__ __forceinline__ void rows_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 // LDS by offsets, whose swizzles are xors.
 __device__ __forceinline__ uint32_t lds_offset(const void* x) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)x));
