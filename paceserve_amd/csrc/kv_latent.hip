@@ -32,6 +32,9 @@ __device__ __forceinline__ uint32_t seen_of(const AttnParams& p, const Request& 
   return static_cast<uint32_t>(x);
 }
 
+// How far the 16-byte pieces of row r of a tile are xored within 256 bytes.
+__device__ __forceinline__ uint32_t swap_of_row(uint32_t r) { return (r % 8) * 2 | r / 8 % 2; }
+
 // RT tiles of 16 rows a workgroup, whose four waves sum a quarter of the columns each, of
 // all rows.  Up to two tiles every wave makes the weights of all rows for itself.  Of four
 // tiles a wave multiplies two by every other 32 columns of the keys, swaps halves of the
@@ -56,7 +59,7 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   // in the end their maxima and sums.  (Two workgroups fill a CU's LDS.)
   constexpr uint32_t kShared = 2048, kShrinkAt = 1024, kRaisedAt = 1088, kMlAt = 1152;
   __shared__ __attribute__((aligned(1024))) char lds_p[kShare ? kWaves * kShared : 16];
-  const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
+  const uint32_t lane = threadIdx.x % 64;
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t at = blockIdx.x / kXcds, nth = over(p.by_unit, at);
   const uint32_t item = nth * kXcds + blockIdx.x % kXcds;
@@ -104,7 +107,7 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   u32x4 qf[RQ][kQS];
 #pragma unroll
   for (int a = 0; a < RQ; ++a) {
-    const uint32_t row = query_row0 + a * 16 + n, i = over(p.by_group, row);
+    const uint32_t n = lane % 16, g = lane / 16, row = query_row0 + a * 16 + n, i = over(p.by_group, row);
     const char* const q = p.q + static_cast<int64_t>(r.q0 + i) * p.q_stride + static_cast<int64_t>(row - i * p.group) * (kW * 2);
 #pragma unroll
     for (int k = 0; k < kQS; ++k) {
@@ -133,73 +136,87 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   uint32_t row_at = 0;                                   // the lane's token's row, in 16-byte units
   uint32_t valid = 0, next_valid = 0;                    // tokens of this step and the next one that exist
   const auto load_id = [&](int32_t t0) {
-    const int32_t t = t0 + static_cast<int32_t>(lane % kTile);
+    const int32_t t = t0 + static_cast<int32_t>(opaque(lane) % kTile);
     id = -1;
     if (t < t_end) id = p.kv_indices[r.first_page + static_cast<int32_t>(over(p.by_page, static_cast<uint32_t>(t)))];
   };
   const auto place_rows = [&](int32_t t0) {
-    const uint32_t t = static_cast<uint32_t>(t0) + lane % kTile;
+    const uint32_t t = static_cast<uint32_t>(t0) + opaque(lane) % kTile;
     const bool ok = static_cast<uint32_t>(id) < p.num_pages;
     next_valid = static_cast<uint32_t>(__ballot(ok));
     row_at = ok ? static_cast<uint32_t>(id) * p.page16 + (t - over(p.by_page, t) * p.page_size) * (kW / 8) : 0u;
   };
-  const auto load_rows = [&](auto whole, uint32_t to) {
-    constexpr uint32_t kRowsOnce = 1024 / kRow, kLanes = 64 / kRowsOnce;
-    const uint32_t ln = opaque(lane), mine = next_valid >> (8 * w) & 255u;
-#pragma unroll
-    for (uint32_t i = 0; i < 8; i += kRowsOnce) {
-      const uint32_t row = i + ln / kLanes;
-      uint32_t from = __builtin_amdgcn_readlane(row_at, 8 * w + i);
+  // The wave's part of a step's rows, 1 KiB at a time: piece i, rows that exist alone unless WHOLE.
+  constexpr int kRowsOnce = 1024 / kRow, kPieces = 8 / kRowsOnce + 1;
+  const auto load_piece = [&](auto whole, uint32_t ln, int i, uint32_t to) {
+    constexpr uint32_t kLanes = 64 / kRowsOnce;
+    uint32_t row, from, at, piece;
+    if (i < kPieces - 1) {
+      row = 8 * w + i * kRowsOnce;
+      from = __builtin_amdgcn_readlane(row_at, 8 * w + i * kRowsOnce);
       if constexpr (kRowsOnce == 2) {
-        const uint32_t second = __builtin_amdgcn_readlane(row_at, 8 * w + i + 1);
+        const uint32_t second = __builtin_amdgcn_readlane(row_at, 8 * w + i * kRowsOnce + 1);
         from = ln < kLanes ? from : second;
+        row += ln / kLanes;
       }
-      const char* const x = p.cache + static_cast<int64_t>(from) * 16 + ((ln % kLanes) ^ (row * 2 | (w & 1))) * 16;
-      const uint32_t at = to + (w * 8 + i) * kRow;
-      if (decltype(whole)::value || (mine >> row & 1u)) copy_to_lds(x, at);
-      else lds_put(at + ln * 16, u32x4{0, 0, 0, 0});
+      at = to + (8 * w + i * kRowsOnce) * kRow;
+      piece = (kRowsOnce == 2 ? ln % kLanes : ln) ^ swap_of_row(row);
+    } else {
+      row = 8 * w + ln / 8;
+      from = __shfl(row_at, row);
+      at = to + kRopeAt + w * 1024;
+      piece = kRow / 16 + ((ln % 8) ^ (row / 2 % 8));
     }
-    const uint32_t row = ln / 8, from = __shfl(row_at, 8 * w + row), at = to + kRopeAt + w * 1024;
-    const char* const x = p.cache + static_cast<int64_t>(from) * 16 + kRow + ((ln % 8) ^ ((4 * w + row / 2) % 8)) * 16;
-    if (decltype(whole)::value || (mine >> row & 1u)) copy_to_lds(x, at);
-    else lds_put(at + ln * 16, u32x4{0, 0, 0, 0});
+    if (decltype(whole)::value || (next_valid >> row & 1u))
+      copy_to_lds(p.cache + static_cast<int64_t>(from) * 16 + piece * 16, at);
+    else
+      lds_put(at + ln * 16, u32x4{0, 0, 0, 0});
   };
 
   // Scores of 32 tokens: lane: row n of each tile, tokens 16 t + 4 g + e.
   f32x4 s[RW][2];
-  const uint32_t swap_n = (n % 8) * 2 | n / 8, odd_step = kShare ? w % 2 * 64 : 0;
-  const uint32_t key_at = (n * kRow + (g ^ swap_n) * 16) ^ odd_step;
-  const uint32_t rope_at = kRopeAt + ((n * (kRope * 2) + (g ^ (n / 2)) * 16) ^ odd_step);
+  const uint32_t odd_step = kShare ? w % 2 * 64 : 0;
   const uint32_t my_sums = lds_offset(lds_p) + w * kShared, other_sums = lds_offset(lds_p) + (w ^ 1) * kShared;
-  const auto score = [&](uint32_t from) {
-    const uint32_t key = opaque(key_at) + from, rope = opaque(rope_at) + from;
+  const auto score = [&](auto loads, uint32_t from, uint32_t to) {
+    const uint32_t ln = opaque(lane), n = ln % 16, g = ln / 16;
+    const uint32_t key = from + ((n * kRow + (g ^ swap_of_row(n)) * 16) ^ odd_step);
+    const uint32_t rope = from + kRopeAt + ((n * (kRope * 2) + (g ^ (n / 2)) * 16) ^ odd_step);
     constexpr int kMain = kShare ? kKS / 2 : kKS;
     f32x4 x[RQ][2];
 #pragma unroll
     for (int a = 0; a < RQ; ++a)
 #pragma unroll
       for (int t = 0; t < 2; ++t) x[a][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto read = [&](int i) {
+      const int k = i / 2, t = i % 2;
+      if (k >= kMain) return lds_get<u32x4>((rope ^ ((k - kMain) * 64)) + t * 16 * (kRope * 2));
+      if (kShare) return lds_get<u32x4>((key ^ (k % 2 * 128)) + t * 16 * kRow + k / 2 * 256);
+      return lds_get<u32x4>((key ^ (k % 4 * 64)) + t * 16 * kRow + k / 4 * 256);
+    };
+    // Reads stay kAhead before their products: left to itself the compiler waits for each.
+    constexpr int kReads = 2 * kQS, kEach = kReads / kPieces, kAhead = RT == 4 ? 4 : RT == 2 ? 1 : 8;
+    u32x4 kf[kReads];
 #pragma unroll
-    for (int k = 0; k < kQS; ++k)
+    for (int i = 0; i < kAhead; ++i) kf[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        u32x4 kf;
-        if (k >= kMain) kf = lds_get<u32x4>((rope ^ ((k - kMain) * 64)) + t * 16 * (kRope * 2));
-        else if (kShare) kf = lds_get<u32x4>((key ^ (k % 2 * 128)) + t * 16 * kRow + k / 2 * 256);
-        else kf = lds_get<u32x4>((key ^ (k % 4 * 64)) + t * 16 * kRow + k / 4 * 256);
+    for (int i = 0; i < kReads; ++i) {
+      if (i + kAhead < kReads) kf[i + kAhead] = read(i + kAhead);
+      if (decltype(loads)::value && i % kEach == 0 && i / kEach < kPieces) load_piece(std::true_type{}, ln, i / kEach, to);
 #pragma unroll
-        for (int a = 0; a < RQ; ++a) x[a][t] = mfma<TYPE>(kf, qf[a][k], x[a][t]);
-      }
+      for (int a = 0; a < RQ; ++a) x[a][i % 2] = mfma<TYPE>(kf[i], qf[a][i / 2], x[a][i % 2]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     if constexpr (kShare) {
       const bool second = w % 2 != 0;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        lds_put(my_sums + t * 1024 + lane * 16, second ? x[0][t] : x[1][t]);
+        lds_put(my_sums + t * 1024 + ln * 16, second ? x[0][t] : x[1][t]);
         s[0][t] = second ? x[1][t] : x[0][t];
       }
       lds_barrier();
 #pragma unroll
-      for (int t = 0; t < 2; ++t) s[0][t] += lds_get<f32x4>(other_sums + t * 1024 + lane * 16);
+      for (int t = 0; t < 2; ++t) s[0][t] += lds_get<f32x4>(other_sums + t * 1024 + ln * 16);
     } else {
 #pragma unroll
       for (int a = 0; a < RW; ++a)
@@ -214,6 +231,7 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   uint32_t raised = 0;                                   // tiles whose maximum was raised
   const auto weigh = [&](auto full, int32_t t0) {
     if constexpr (!decltype(full)::value) {
+      const uint32_t ln = opaque(lane), n = ln % 16, g = ln / 16;
 #pragma unroll
       for (int a = 0; a < RW; ++a) {
         const uint32_t sees =
@@ -278,7 +296,7 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
     bool found = false;
 #pragma unroll 1
     for (uint32_t c = lane; c < kTile * kCT * 2; c += 64) {
-      const uint32_t row = c / (kCT * 2), piece = (w * kCT * 2 + c % (kCT * 2)) ^ ((row % 8) * 2 | row / 8 % 2);
+      const uint32_t row = c / (kCT * 2), piece = (w * kCT * 2 + c % (kCT * 2)) ^ swap_of_row(row);
       u32x4 x = lds_get<u32x4>(from + row * kRow + piece * 16);
       bool here = false;
 #pragma unroll
@@ -296,24 +314,33 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   // Adds the weighted values of the tokens in a buffer.  For weights in registers the
   // tokens of a lane's group of 16 are 4 g .. 4 g + 3 and the same behind 16; through LDS
   // they are 8 g .. 8 g + 7.
-  const uint32_t v_row = kShare ? 8 * g + n / 4 : 4 * g + n / 4;
-  const uint32_t v_at = v_row * kRow + ((w * kCT * 2 + n % 4 / 2) ^ ((v_row % 8) * 2 | v_row / 8 % 2)) * 16 + n % 2 * 8;
-  const uint32_t p_at = lds_offset(lds_p) + n * kWeightRow + (g ^ (n / 4)) * 16;  // tile a's are at (a ^ 1) * kShared
   const auto gather = [&](uint32_t from) {
+    const uint32_t ln = opaque(lane), n = ln % 16, g = ln / 16;
+    const uint32_t v_row = kShare ? 8 * g + n / 4 : 4 * g + n / 4;
+    const uint32_t v = from + v_row * kRow + ((w * kCT * 2 + n % 4 / 2) ^ swap_of_row(v_row)) * 16 + n % 2 * 8;
+    const uint32_t p_at = lds_offset(lds_p) + n * kWeightRow + (g ^ (n / 4)) * 16;  // tile a's are at (a ^ 1) * kShared
     u32x4 weight[RT];
 #pragma unroll
     for (int a = 0; a < RT; ++a) {
       if constexpr (kShare) weight[a] = lds_get<u32x4>(p_at + (a ^ 1) * kShared);
       else weight[a] = pf[a];
     }
-    const uint32_t v = opaque(v_at) + from;
-#pragma unroll
-    for (int d = 0; d < kCT; ++d) {
+    const auto read = [&](int d) {
       const u32x2 lo = lds_transposed(v ^ (d * 32));
       const u32x2 hi = lds_transposed(kShare ? (v ^ (d * 32 ^ 128)) + 4 * kRow : (v ^ (d * 32)) + 16 * kRow);
-      const u32x4 vf = {lo[0], lo[1], hi[0], hi[1]};
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    constexpr int kAhead = RT == 2 ? 1 : 3;
+    u32x4 vf[kCT];
 #pragma unroll
-      for (int a = 0; a < RT; ++a) acc[a][d] = mfma<TYPE>(vf, weight[a], acc[a][d]);
+    for (int d = 0; d < kAhead; ++d) vf[d] = read(d);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int d = 0; d < kCT; ++d) {
+      if (d + kAhead < kCT) vf[d + kAhead] = read(d + kAhead);
+#pragma unroll
+      for (int a = 0; a < RT; ++a) acc[a][d] = mfma<TYPE>(vf[d], weight[a], acc[a][d]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -322,29 +349,39 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   int32_t t0 = t_begin;
   uint32_t now = lds_offset(lds), other = now + kBuffer;
   const auto load_next = [&](int32_t next, uint32_t to) {
-    if (next_valid == ~0u) load_rows(std::true_type{}, to);
-    else if (next < t_end) load_rows(std::false_type{}, to);
-    load_id(next + kStep);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      if (next_valid == ~0u) load_piece(std::true_type{}, opaque(lane), i, to);
+      else if (next < t_end) load_piece(std::false_type{}, opaque(lane), i, to);
+    }
   };
   const auto one_step = [&](auto full) {
     valid = next_valid;
     place_rows(t0 + kStep);
     rows_barrier();                                      // this step's rows are in LDS, the other buffer's readers done
-    load_next(t0 + kStep, other);
-    score(now);
+    // The next step's rows are asked for between the products.
+    if (next_valid == ~0u) {
+      score(std::true_type{}, now, other);
+    } else {
+      load_next(t0 + kStep, other);
+      score(std::false_type{}, now, other);
+    }
+    load_id(t0 + 2 * kStep);
     weigh(full, t0);
     if constexpr (kShare) {
+      const uint32_t ln = opaque(lane), n = ln % 16, g = ln / 16;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
         lds_put(other_sums + n * kWeightRow + ((2 * t + g / 2) ^ (n / 4)) * 16 + g % 2 * 8,
                 u32x2{pf[0][2 * t], pf[0][2 * t + 1]});
       if (g == 0) lds_put(other_sums + kShrinkAt + n * 4, shrink[0]);
-      if (lane == 0) lds_put(other_sums + kRaisedAt, raised);
+      if (ln == 0) lds_put(other_sums + kRaisedAt, raised);
     }
     if (kShare || !decltype(full)::value) lds_barrier();
     if constexpr (!decltype(full)::value) clean(now);
     if constexpr (kShare) {
-      const uint32_t any = lds_get<uint32_t>(lds_offset(lds_p) + lane % kWaves * kShared + kRaisedAt);
+      const uint32_t ln = opaque(lane), n = ln % 16;
+      const uint32_t any = lds_get<uint32_t>(lds_offset(lds_p) + ln % kWaves * kShared + kRaisedAt);
       const uint64_t which = __ballot(any != 0);         // bit a: tile a ^ 1
       if (which != 0) {
 #pragma unroll
@@ -372,11 +409,13 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   load_id(t0);
   place_rows(t0);
   load_next(t0, now);
+  load_id(t0 + kStep);
   // The steps whose tokens every row sees, then the others.
   while (t0 + kStep <= seen_by_all && next_valid == ~0u) one_step(std::true_type{});
   const int32_t t_masked = t0;
 #pragma unroll 1
   while (t0 < t_end) one_step(std::false_type{});
+  const uint32_t ln = opaque(lane), n = ln % 16, g = ln / 16;
 #pragma unroll
   for (int a = 0; a < RW; ++a) {
     l[a] = across_groups(l[a], sum_of);
