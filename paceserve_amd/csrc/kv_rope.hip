@@ -16,6 +16,7 @@
 // against 32 of its rows: a lane loads them once and goes on over the token's heads.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "mx.h"
 
@@ -25,6 +26,13 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int64_t kMaxGroupsPerLaunch = int64_t(1) << 24;
+// Rows of more bytes than this are loaded nontemporally: what a projection has just written
+// is still in the memory-side cache where it is smaller.  MI355X, 40 heads of 128: 40 MiB
+// 17.2 us plain, 18.6 so, 160 MiB 71 and 61.
+constexpr int64_t kStreamBytes = int64_t(64) << 20;
+// Latent rows of a call from which on a lane group takes two.  MI355X, 65536 rows of 576 numbers
+// 45 us by one, 39 by two, 16384 10.4 and 10.0, 2000 3.4 and 3.8.
+constexpr int64_t kManyRows = 8192;
 
 struct Rows {
   const char* in;
@@ -49,7 +57,7 @@ struct RopeParams {
   uint32_t parts, part_heads;  // waves that a token's heads are dealt to, and heads of each
   uint32_t page_size;
   float eps, inv_dim;
-  FastDiv by_page;
+  FastDiv by_page, by_parts;
 };
 
 template <int TYPE>
@@ -130,13 +138,39 @@ __device__ __forceinline__ Run<PACE_KV_FP32> float_run(const float* x) {
   return r;
 }
 
-// FORMAT: of the cache, or -1 without one.
-template <int TYPE, int FORMAT, bool INTERLEAVED>
+// The sum over aligned groups of `lanes` lanes, in each of them: within rows of 16 by
+// exchanges that need no LDS.
+__device__ __forceinline__ float sum_of_group(float x, uint32_t lanes) {
+  const auto moved = [](float v, auto control) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), decltype(control)::value, 0xf, 0xf, true));
+  };
+  if (lanes >= 2) x += moved(x, std::integral_constant<int, 0xB1>{});    // lane ^ 1
+  if (lanes >= 4) x += moved(x, std::integral_constant<int, 0x4E>{});    // lane ^ 2
+  if (lanes >= 8) x += moved(x, std::integral_constant<int, 0x141>{});   // the other four of eight
+  if (lanes >= 16) x += moved(x, std::integral_constant<int, 0x140>{});  // the other eight of sixteen
+  for (uint32_t k = 16; k < lanes; k *= 2) x += __shfl_xor(x, k);
+  return x;
+}
+
+// Written through the L2 at device scope.  The asm carries the wait states that a store of
+// more than 64 bits needs before its data registers change.
+__device__ __forceinline__ void put_vec(char* to, u32x4 v) {
+  asm volatile("global_store_dwordx4 %0, %1, off sc1\n\ts_nop 1" : : "v"(to), "v"(v) : "memory");
+}
+
+template <bool STREAM>
+__device__ __forceinline__ u32x4 load_vec(const char* x) {
+  const u32x4* const at = reinterpret_cast<const u32x4*>(x);
+  return STREAM ? __builtin_nontemporal_load(at) : *at;
+}
+
+// FORMAT: of the cache, or -1 without one.  STREAM: rows are loaded and stored nontemporally.
+template <int TYPE, int FORMAT, bool INTERLEAVED, bool STREAM>
 __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeParams p) {
   const uint32_t lane = threadIdx.x % 64;
-  const int64_t wave = static_cast<int64_t>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int64_t token = wave / p.parts;
-  const uint32_t part = static_cast<uint32_t>(wave - token * p.parts);
+  const uint32_t wave = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t whole = over(p.by_parts, wave), part = wave - whole * p.parts;
+  const int64_t token = whole;
   if (token >= p.nnz) return;
   int64_t page_at = 0, slot = 0;
   if constexpr (FORMAT >= 0) {
@@ -146,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeParams p) {
       if (p.err != nullptr && part == 0 && lane == 0) atomicAdd(p.err, 1);
       return;
     }
-    const int64_t page = s / p.page_size;
+    const int64_t page = s <= UINT32_MAX ? over(p.by_page, static_cast<uint32_t>(s)) : s / p.page_size;
     slot = s - page * p.page_size;
     page_at = page * p.page_bytes;
   }
@@ -165,14 +199,15 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeParams p) {
   if (rotates) load_angles(p.table + position * p.rotary, p.rotary, INTERLEAVED, u, cos, sin);
   const uint32_t qk = p.q.heads + p.k.heads, heads = qk + (FORMAT >= 0 ? p.v.heads : 0u);
   const uint32_t end = min((part + 1) * p.part_heads, heads);
-  for (uint32_t h = part * p.part_heads + (lane >> p.group_log2); h < end; h += 64u >> p.group_log2) {
+  const uint32_t turn = 64u >> p.group_log2;
+  for (uint32_t h = part * p.part_heads + (lane >> p.group_log2); h < end; h += turn) {
     const Rows& rows = h < p.q.heads ? p.q : h < qk ? p.k : p.v;
     const uint32_t head = h < p.q.heads ? h : h < qk ? h - p.q.heads : h - qk;
     const char* const in = rows.in + token * rows.in_token + head * rows.in_head;
     u32x4 ra = {0, 0, 0, 0}, rb = {0, 0, 0, 0};
     if (active) {
-      ra = *reinterpret_cast<const u32x4*>(in + ea * 2);
-      rb = *reinterpret_cast<const u32x4*>(in + eb * 2);
+      ra = load_vec<STREAM>(in + ea * 2);
+      rb = load_vec<STREAM>(in + eb * 2);
     }
     float a[8], b[8];
     if (h < qk) {
@@ -182,8 +217,8 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeParams p) {
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum += a[j] * a[j] + b[j] * b[j];
-        for (uint32_t k = 1; k < group; k *= 2) sum += __shfl_xor(sum, k);
-        const float inv = 1.f / sqrtf(sum * p.inv_dim + p.eps);
+        sum = sum_of_group(sum, group);
+        const float inv = __builtin_amdgcn_rsqf(sum * p.inv_dim + p.eps);
         if (active) {
           float wa[8], wb[8];
           widen<TYPE>(*reinterpret_cast<const u32x4*>(rows.weight + ea * 2), wa);
@@ -200,27 +235,28 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeParams p) {
     if (!active) continue;
     if (FORMAT < 0 || h < p.q.heads) {
       char* const out = rows.out + token * rows.out_token + head * rows.out_head;
-      *reinterpret_cast<u32x4*>(out + ea * 2) = narrow<TYPE>(a);
-      *reinterpret_cast<u32x4*>(out + eb * 2) = narrow<TYPE>(b);
+      put_vec(out + ea * 2, narrow<TYPE>(a));
+      put_vec(out + eb * 2, narrow<TYPE>(b));
     } else if constexpr (FORMAT >= 0) {
       const int64_t element = (slot * p.k.heads + head) * p.head_dim;
       char* const half = p.cache + page_at + (h < qk ? 0 : p.half_bytes);
       if constexpr (FORMAT == PACE_KV_PLAIN) {
-        *reinterpret_cast<u32x4*>(half + (element + ea) * 2) = h < qk ? narrow<TYPE>(a) : ra;
-        *reinterpret_cast<u32x4*>(half + (element + eb) * 2) = h < qk ? narrow<TYPE>(b) : rb;
+        put_vec(half + (element + ea) * 2, h < qk ? narrow<TYPE>(a) : ra);
+        put_vec(half + (element + eb) * 2, h < qk ? narrow<TYPE>(b) : rb);
       } else {
         // Blocks of 32 are four neighbouring lanes' runs: rotary and tail are multiples of 64.
         constexpr int kBits = mx_bits(FORMAT);
-        const auto put_run = [&](const float* x, const u32x4& raw, uint32_t e) {
-          Run<PACE_KV_FP32> r = float_run(x);
-          if (h >= qk) {
-            float f[8];
-            widen<TYPE>(raw, f);
-            r = float_run(f);
+        const auto put_run = [&](const float* x, const u32x4& v, uint32_t e) {
+          char* const data = half + (element + e) * kBits / 8;
+          char* const scale = half + p.scale_at + (element + e) / kMxBlock;
+          if (h < qk) {
+            const Run<PACE_KV_FP32> r = float_run(x);
+            store_run<PACE_KV_FP32, FORMAT, false>(r, scale_byte<FORMAT>(block_amax<PACE_KV_FP32>(r)), data, scale);
+          } else {
+            Run<TYPE> r;
+            r.v[0] = v;
+            store_run<TYPE, FORMAT, false>(r, scale_byte<FORMAT>(block_amax<TYPE>(r)), data, scale);
           }
-          const uint32_t byte = scale_byte<FORMAT>(block_amax<PACE_KV_FP32>(r));
-          store_run<PACE_KV_FP32, FORMAT, false>(r, byte, half + (element + e) * kBits / 8,
-                                                 half + p.scale_at + (element + e) / kMxBlock);
         };
         put_run(a, ra, ea);
         put_run(b, rb, eb);
@@ -245,79 +281,108 @@ struct LatentParams {
 
 constexpr int kRope = 64;      // columns of a latent row's rotated part
 
-// L / 8 lanes take a token: eight elements of the latent each, and the first four two
-// runs of the rotated part.
-template <int L, int TYPE, bool INTERLEAVED>
+// L / 8 lanes take ROWS tokens: eight elements of each latent a lane, and four lanes
+// a token two runs of its rotated part.
+template <int L, int TYPE, bool INTERLEAVED, uint32_t ROWS>
 __global__ __launch_bounds__(kThreads) void latent_rows_kernel(const LatentParams p) {
-  constexpr uint32_t kLanes = L / 8, kTokens = kThreads / kLanes;
+  constexpr uint32_t kLanes = L / 8, kTokens = kThreads / kLanes * ROWS;
   const uint32_t u = threadIdx.x % kLanes;
-  const int64_t token = static_cast<int64_t>(blockIdx.x) * kTokens + threadIdx.x / kLanes;
-  if (token >= p.nnz) return;
-  const int64_t slot = p.slots[token];
-  if (slot == -1) return;                                // padding
-  const int64_t position = p.positions[token];
-  if (slot < 0 || slot >= p.num_slots || position < 0 || position >= p.table_rows) {
-    if (p.err != nullptr && u == 0) atomicAdd(p.err, 1);
-    return;
-  }
-  u32x4 raw = *reinterpret_cast<const u32x4*>(p.latent + token * p.latent_stride + u * 16);
-  u32x4 ra, rb;
-  float cos[8], sin[8];
-  if (u < kRope / 16) {
-    const char* const in = p.rope_key + token * p.rope_stride;
-    ra = *reinterpret_cast<const u32x4*>(in + u * 16);
-    rb = *reinterpret_cast<const u32x4*>(in + u * 16 + kRope);
-    load_angles(p.table + position * kRope, kRope, INTERLEAVED, u, cos, sin);
-  }
-  char* const row = p.cache + slot * ((L + kRope) * 2);
-  if (p.weight != nullptr) {
-    float x[8], w[8];
-    widen<TYPE>(raw, x);
-    widen<TYPE>(*reinterpret_cast<const u32x4*>(p.weight + u * 16), w);
-    float sum = 0.f;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kTokens + threadIdx.x / kLanes * ROWS;
+  // Everything that does not wait for a slot or a position is asked for first.
+  const int64_t rope_token = first + u / 4;
+  const bool ropes = u < 4 * ROWS && rope_token < p.nnz;
+  u32x4 raw[ROWS], ra, rb;
+  int64_t slot[ROWS], rope_slot = -1;
+  int32_t position[ROWS], rope_position = -1;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum += x[j] * x[j];
-#pragma unroll
-    for (uint32_t k = 1; k < kLanes; k *= 2) sum += __shfl_xor(sum, k);
-    const float inv = 1.f / sqrtf(sum * (1.f / L) + p.eps);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = x[j] * inv * w[j];
-    raw = narrow<TYPE>(x);
+  for (uint32_t k = 0; k < ROWS; ++k) {
+    slot[k] = -1;
+    position[k] = -1;
+    raw[k] = u32x4{0, 0, 0, 0};
+    const int64_t token = first + k;
+    if (token >= p.nnz) continue;
+    slot[k] = p.slots[token];
+    position[k] = p.positions[token];
+    raw[k] = *reinterpret_cast<const u32x4*>(p.latent + token * p.latent_stride + u * 16);
   }
-  *reinterpret_cast<u32x4*>(row + u * 16) = raw;
-  if (u < kRope / 16) {
-    float a[8], b[8];
+  if (ropes) {
+    const char* const in = p.rope_key + rope_token * p.rope_stride + u % 4 * 16;
+    ra = *reinterpret_cast<const u32x4*>(in);
+    rb = *reinterpret_cast<const u32x4*>(in + kRope);
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < ROWS; ++k) {
+    if (slot[k] == -1) continue;                         // padding
+    if (slot[k] < 0 || slot[k] >= p.num_slots || position[k] < 0 || position[k] >= p.table_rows) {
+      if (p.err != nullptr && u == 0) atomicAdd(p.err, 1);
+      slot[k] = -1;
+    } else if (u / 4 == k) {
+      rope_slot = slot[k];
+      rope_position = position[k];
+    }
+  }
+  if (rope_slot >= 0) {
+    float a[8], b[8], cos[8], sin[8];
+    load_angles(p.table + static_cast<int64_t>(rope_position) * kRope, kRope, INTERLEAVED, u % 4, cos, sin);
     widen<TYPE>(ra, a);
     widen<TYPE>(rb, b);
     rotate(INTERLEAVED, a, b, cos, sin);
-    *reinterpret_cast<u32x4*>(row + L * 2 + u * 16) = narrow<TYPE>(a);
-    *reinterpret_cast<u32x4*>(row + L * 2 + u * 16 + kRope) = narrow<TYPE>(b);
+    char* const row = p.cache + rope_slot * ((L + kRope) * 2) + L * 2 + u % 4 * 16;
+    put_vec(row, narrow<TYPE>(a));
+    put_vec(row + kRope, narrow<TYPE>(b));
+  }
+  float w[8];
+  if (p.weight != nullptr) widen<TYPE>(*reinterpret_cast<const u32x4*>(p.weight + u * 16), w);
+#pragma unroll
+  for (uint32_t k = 0; k < ROWS; ++k) {
+    if (p.weight != nullptr) {
+      float x[8], sum = 0.f;
+      widen<TYPE>(raw[k], x);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += x[j] * x[j];
+      sum = sum_of_group(sum, kLanes);
+      const float inv = __builtin_amdgcn_rsqf(sum * (1.f / L) + p.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = x[j] * inv * w[j];
+      raw[k] = narrow<TYPE>(x);
+    }
+    if (slot[k] >= 0) put_vec(p.cache + slot[k] * ((L + kRope) * 2) + u * 16, raw[k]);
   }
 }
 
-template <int TYPE, int FORMAT>
+template <int TYPE, int FORMAT, bool STREAM>
 const void* pick_rope(bool interleaved) {
-  return interleaved ? reinterpret_cast<const void*>(&rope_kernel<TYPE, FORMAT, true>)
-                     : reinterpret_cast<const void*>(&rope_kernel<TYPE, FORMAT, false>);
+  return interleaved ? reinterpret_cast<const void*>(&rope_kernel<TYPE, FORMAT, true, STREAM>)
+                     : reinterpret_cast<const void*>(&rope_kernel<TYPE, FORMAT, false, STREAM>);
 }
 
-template <int TYPE>
+template <int TYPE, bool STREAM>
 const void* pick_rope(int format, bool interleaved) {
   switch (format) {
-    case -1: return pick_rope<TYPE, -1>(interleaved);
-    case PACE_KV_PLAIN: return pick_rope<TYPE, PACE_KV_PLAIN>(interleaved);
-    case PACE_KV_MXFP8: return pick_rope<TYPE, PACE_KV_MXFP8>(interleaved);
-    default: return pick_rope<TYPE, PACE_KV_MXFP4>(interleaved);
+    case -1: return pick_rope<TYPE, -1, STREAM>(interleaved);
+    case PACE_KV_PLAIN: return pick_rope<TYPE, PACE_KV_PLAIN, STREAM>(interleaved);
+    case PACE_KV_MXFP8: return pick_rope<TYPE, PACE_KV_MXFP8, STREAM>(interleaved);
+    default: return pick_rope<TYPE, PACE_KV_MXFP4, STREAM>(interleaved);
   }
+}
+
+template <bool STREAM>
+const void* pick_rope(int type, int format, bool interleaved) {
+  return type == PACE_KV_BF16 ? pick_rope<PACE_KV_BF16, STREAM>(format, interleaved)
+                              : pick_rope<PACE_KV_FP16, STREAM>(format, interleaved);
+}
+
+template <int L, int TYPE, uint32_t ROWS>
+const void* pick_latent(bool interleaved) {
+  return interleaved ? reinterpret_cast<const void*>(&latent_rows_kernel<L, TYPE, true, ROWS>)
+                     : reinterpret_cast<const void*>(&latent_rows_kernel<L, TYPE, false, ROWS>);
 }
 
 template <int L>
-const void* pick_latent(int type, bool interleaved) {
+const void* pick_latent(int type, bool interleaved, bool many) {
   if (type == PACE_KV_BF16)
-    return interleaved ? reinterpret_cast<const void*>(&latent_rows_kernel<L, PACE_KV_BF16, true>)
-                       : reinterpret_cast<const void*>(&latent_rows_kernel<L, PACE_KV_BF16, false>);
-  return interleaved ? reinterpret_cast<const void*>(&latent_rows_kernel<L, PACE_KV_FP16, true>)
-                     : reinterpret_cast<const void*>(&latent_rows_kernel<L, PACE_KV_FP16, false>);
+    return many ? pick_latent<L, PACE_KV_BF16, 2>(interleaved) : pick_latent<L, PACE_KV_BF16, 1>(interleaved);
+  return many ? pick_latent<L, PACE_KV_FP16, 2>(interleaved) : pick_latent<L, PACE_KV_FP16, 1>(interleaved);
 }
 
 int check_rows(const char* call, const Rows& r, bool writes, uint32_t head_dim) {
@@ -364,8 +429,11 @@ int launch_rope(RopeParams& p, int elem_type, int format, int head_dim, int rota
   const int64_t groups = (p.nnz * p.parts + kWaves - 1) / kWaves;
   if (groups > kMaxGroupsPerLaunch) return fail(PACE_KV_ERANGE, "rope: too many tokens for one call");
   void* args[] = {&p};
-  const void* kernel = elem_type == PACE_KV_BF16 ? pick_rope<PACE_KV_BF16>(format, interleaved != 0)
-                                                 : pick_rope<PACE_KV_FP16>(format, interleaved != 0);
+  p.by_parts = fast_div(p.parts);
+  p.by_page = fast_div(p.page_size);
+  const bool streams = p.nnz * heads * head_dim * 2 > kStreamBytes;
+  const void* kernel = streams ? pick_rope<true>(elem_type, format, interleaved != 0)
+                              : pick_rope<false>(elem_type, format, interleaved != 0);
   return hip_status(hipLaunchKernel(kernel, dim3(static_cast<uint32_t>(groups)), dim3(kThreads), args, 0, stream),
                     "rope launch");
 }
@@ -480,7 +548,8 @@ int pace_kv_append_latent(const void* latent, int64_t latent_stride, const void*
         reinterpret_cast<uintptr_t>(weight) | static_cast<uintptr_t>(latent_stride | rope_stride)) & 15u) ||
       (reinterpret_cast<uintptr_t>(slot_mapping) & 7u))
     return fail(PACE_KV_EINVAL, "%s: rows, strides, weight and cache must be multiples of 16 bytes, slot_mapping of 8", call);
-  const int64_t tokens = kThreads / (latent_dim / 8), groups = (nnz + tokens - 1) / tokens;
+  const bool many = nnz >= kManyRows;
+  const int64_t tokens = kThreads / (latent_dim / 8) * (many ? 2 : 1), groups = (nnz + tokens - 1) / tokens;
   if (groups > kMaxGroupsPerLaunch) return fail(PACE_KV_ERANGE, "%s: too many tokens for one call", call);
   LatentParams p = {};
   p.latent = static_cast<const char*>(latent);
@@ -498,8 +567,8 @@ int pace_kv_append_latent(const void* latent, int64_t latent_stride, const void*
   p.num_slots = num_pages * page_size;
   p.eps = eps;
   void* args[] = {&p};
-  const void* kernel = latent_dim == 512 ? pick_latent<512>(elem_type, interleaved != 0)
-                                         : pick_latent<256>(elem_type, interleaved != 0);
+  const void* kernel = latent_dim == 512 ? pick_latent<512>(elem_type, interleaved != 0, many)
+                                         : pick_latent<256>(elem_type, interleaved != 0, many);
   return hip_status(hipLaunchKernel(kernel, dim3(static_cast<uint32_t>(groups)), dim3(kThreads), args, 0,
                                     static_cast<hipStream_t>(stream)), "append_latent launch");
 }
