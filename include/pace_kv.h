@@ -702,8 +702,13 @@ int pace_kv_latent_attention(const void* q, int64_t q_stride_bytes,
  * of no request are not written.  err_count goes up by one for each request
  * that is skipped (queries outside [0, nnz), more than max_q_len, or past the
  * row tiles of nnz rows where offsets overlap) or whose keys are cut to
- * [0, num_keys).
+ * [0, num_keys).  The keys of few rows are cut up by the sizes here alone;
+ * workspace as in pace_kv_attention.
  */
+int pace_kv_prompt_attention_workspace(int64_t nnz, int64_t num_keys,
+                                       int batch_size, int num_heads,
+                                       int head_dim, int causal,
+                                       int64_t* bytes);
 int pace_kv_prompt_attention(const void* q, int64_t q_token_stride,
                              int64_t q_head_stride, const void* key,
                              int64_t k_token_stride, int64_t k_head_stride,
@@ -715,7 +720,9 @@ int pace_kv_prompt_attention(const void* q, int64_t q_token_stride,
                              const int32_t* kv_indptr, int batch_size,
                              int max_q_len, float scale, int causal, void* out,
                              int64_t out_token_stride, int64_t out_head_stride,
-                             float* lse, int32_t* err_count, void* stream);
+                             float* lse, void* workspace,
+                             int64_t workspace_size, int32_t* err_count,
+                             void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Native block allocation, batch planning and single-call promotion          */

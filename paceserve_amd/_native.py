@@ -94,9 +94,12 @@ SIGNATURES = {
     "pace_kv_latent_attention": (
         c_int, [_VP, c_int64, c_int, c_int64, _VP, c_int, c_int, c_int, _VP, c_int64, c_int, _VP, c_int64, _VP, _VP,
                 c_int, _VP, c_int, c_float, _VP, c_int64, _VP, _VP, c_int64, _VP, _VP]),
+    "pace_kv_prompt_attention_workspace": (
+        c_int, [c_int64, c_int64, c_int, c_int, c_int, c_int, POINTER(c_int64)]),
     "pace_kv_prompt_attention": (
         c_int, [_VP, c_int64, c_int64, _VP, c_int64, c_int64, _VP, c_int64, _VP, c_int64, c_int64, c_int, c_int, c_int,
-                c_int64, c_int64, _VP, _VP, c_int, c_int, c_float, c_int, _VP, c_int64, c_int64, _VP, _VP, _VP]),
+                c_int64, c_int64, _VP, _VP, c_int, c_int, c_float, c_int, _VP, c_int64, c_int64, _VP, _VP, c_int64, _VP,
+                _VP]),
     "pace_kv_seq_lens": (c_int, [_VP, _VP, c_int, c_int, _VP, _VP]),
     "pace_kv_batch_indices_positions": (c_int, [_VP, _VP, c_int, c_int64, _VP, _VP, _VP]),
     "pace_kv_allocator_create": (c_int, [c_int64, _VP, c_int64, POINTER(c_void_p)]),

@@ -100,21 +100,26 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
   }
 
   // Query fragments: row n of each tile, eight elements from 32 k + 8 g, with the scale's
-  // sign: what follows takes it as positive.  (A scale of zero makes all scores zero.)
+  // sign: what follows takes it as positive.  (A scale of zero makes all scores zero.)  Rows
+  // behind the last read it and become zeros: loads under a condition would wait for one
+  // another (MI355X: 9 us).
   const uint32_t wave_row0 = row0 + (kShare ? w * 16 : 0), query_row0 = row0 + (kShare ? w / 2 * 32 : 0);
   const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
   const float per_score = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
   u32x4 qf[RQ][kQS];
 #pragma unroll
   for (int a = 0; a < RQ; ++a) {
-    const uint32_t n = lane % 16, g = lane / 16, row = query_row0 + a * 16 + n, i = over(p.by_group, row);
+    const uint32_t row = min(query_row0 + a * 16 + lane % 16, rows - 1), i = over(p.by_group, row);
     const char* const q = p.q + static_cast<int64_t>(r.q0 + i) * p.q_stride + static_cast<int64_t>(row - i * p.group) * (kW * 2);
 #pragma unroll
-    for (int k = 0; k < kQS; ++k) {
-      qf[a][k] = u32x4{0, 0, 0, 0};
-      const uint32_t of = kShare ? 2 * k + w % 2 : k;
-      if (row < rows) qf[a][k] = (*reinterpret_cast<const u32x4*>(q + of * 64 + g * 16) ^ flip) & keep;
-    }
+    for (int k = 0; k < kQS; ++k)
+      qf[a][k] = *reinterpret_cast<const u32x4*>(q + (kShare ? 2 * k + w % 2 : k) * 64 + lane / 16 * 16);
+  }
+#pragma unroll
+  for (int a = 0; a < RQ; ++a) {
+    const uint32_t mask = query_row0 + a * 16 + lane % 16 < rows ? keep : 0u;
+#pragma unroll
+    for (int k = 0; k < kQS; ++k) qf[a][k] = (qf[a][k] ^ flip) & mask;
   }
   f32x4 acc[RT][kCT];
 #pragma unroll

@@ -29,8 +29,10 @@ struct PromptParams {
   const int32_t* qo_indptr;
   const int32_t* kv_indptr;
   int32_t* err;
+  float* part_o;               // [parts, nnz, heads, DN], of more than one
+  float* part_ml;              // [parts, nnz, heads, 2]
   int64_t q_token, q_head, k_token, k_head, r_token, v_token, v_head, o_token, o_head;  // strides in bytes
-  uint32_t batch, nnz, keys, heads, max_q, tiles;
+  uint32_t batch, nnz, keys, heads, max_q, tiles, parts;
   float scale_log2;
   uint32_t causal;
 };
@@ -119,7 +121,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(const PromptParams 
   const uint32_t lane = threadIdx.x % 64, g = lane / 16, n = lane % 16;
   const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t head = blockIdx.x;
-  if (p.err != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && w == 0) count_bad(p);
+  if (p.err != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && w == 0) count_bad(p);
   PromptRequest r;
   // The last tiles first: they see the most keys.
   if (!find_tile(p, gridDim.y - 1 - blockIdx.y, &r)) return;
@@ -129,23 +131,35 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(const PromptParams 
   const int32_t row0 = static_cast<int32_t>(r.tile * kRows), wave_row0 = row0 + static_cast<int32_t>(w * 16 * kRT);
   int32_t t_end = kv_len;
   if (p.causal) t_end = min(t_end, base + min(row0 + static_cast<int32_t>(kRows), q_len));
+  // The keys that the tile sees are dealt to its workgroups in whole steps.
+  int32_t t_begin = 0;
+  if (p.parts > 1) {
+    const uint32_t steps = (static_cast<uint32_t>(max(t_end, 0)) + kTile - 1) / kTile;
+    const uint32_t each = (steps + p.parts - 1) / p.parts * kTile;
+    t_begin = static_cast<int32_t>(blockIdx.z * each);
+    t_end = min(t_end, t_begin + static_cast<int32_t>(each));
+  }
   // Keys that a row sees: those before `seen_by`.
   const auto seen_by = [&](int32_t row) { return p.causal ? base + row + 1 : kv_len; };
 
   // Query fragments with the scale's sign: what follows takes it as positive.  (A scale
-  // of zero makes all scores zero.)
+  // of zero makes all scores zero.)  Rows behind the last read it and become zeros: loads
+  // under a condition would wait for one another (MI355X: 6 us).
   const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
   const float per_score = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
   u32x4 qf[kRT][kNS + 2];
 #pragma unroll
   for (int a = 0; a < kRT; ++a) {
-    const int32_t row = wave_row0 + a * 16 + static_cast<int32_t>(n);
+    const int32_t row = min(wave_row0 + a * 16 + static_cast<int32_t>(n), q_len - 1);
     const char* const q = p.q + static_cast<int64_t>(r.q0 + row) * p.q_token + head * p.q_head;
 #pragma unroll
-    for (int k = 0; k < kNS + 2; ++k) {
-      qf[a][k] = u32x4{0, 0, 0, 0};
-      if (row < q_len) qf[a][k] = (*reinterpret_cast<const u32x4*>(q + k * 64 + g * 16) ^ flip) & keep;
-    }
+    for (int k = 0; k < kNS + 2; ++k) qf[a][k] = *reinterpret_cast<const u32x4*>(q + k * 64 + g * 16);
+  }
+#pragma unroll
+  for (int a = 0; a < kRT; ++a) {
+    const uint32_t mask = wave_row0 + a * 16 + static_cast<int32_t>(n) < q_len ? keep : 0u;
+#pragma unroll
+    for (int k = 0; k < kNS + 2; ++k) qf[a][k] = (qf[a][k] ^ flip) & mask;
   }
   f32x4 acc[kRT][kCT];
   float m[kRT], l[kRT];
@@ -302,7 +316,7 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(const PromptParams 
 
   constexpr int32_t kStep = static_cast<int32_t>(kTile);
   uint32_t now = lds_offset(lds), other = now + kBuffer;
-  int32_t t0 = 0;
+  int32_t t0 = t_begin;
   const auto one_step = [&](auto full) {
     rows_barrier();                                      // this step's rows are in LDS, the other buffer's readers done
     load_next(t0 + kStep, other);
@@ -323,18 +337,28 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(const PromptParams 
     other = x;
     t0 += kStep;
   };
-  load_next(0, now);
+  load_next(t0, now);
   // The steps whose keys every row sees, then the others.
   while (t0 + kStep <= min(seen_by(row0), t_end)) one_step(std::true_type{});
   const int32_t t_masked = t0;
 #pragma unroll 1
   while (t0 < t_end) one_step(std::false_type{});
+  const auto part_at = [&](int32_t row) {
+    return (static_cast<int64_t>(blockIdx.z) * p.nnz + static_cast<uint32_t>(r.q0 + row)) * p.heads + head;
+  };
 #pragma unroll
   for (int a = 0; a < kRT; ++a) {
     l[a] = across_groups(l[a], sum_of);
     const int32_t row = wave_row0 + a * 16 + static_cast<int32_t>(n);
     if (row >= q_len) continue;
     const float inv = l[a] == 0.f ? 0.f : 1.f / l[a];
+    if (p.parts > 1) {
+      const int64_t at = part_at(row);
+#pragma unroll
+      for (int d = 0; d < kCT; ++d) *reinterpret_cast<f32x4*>(p.part_o + at * DN + d * 16 + g * 4) = acc[a][d];
+      if (g == 0) *reinterpret_cast<f32x2*>(p.part_ml + at * 2) = f32x2{m[a], l[a]};
+      continue;
+    }
     char* const out = p.out + static_cast<int64_t>(r.q0 + row) * p.o_token + head * p.o_head;
 #pragma unroll
     for (int d = 0; d < kCT; ++d) {
@@ -366,11 +390,96 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(const PromptParams 
         const uint32_t at = (c / 4 * 16 + g * 4 + c % 4) * 2;
         const uint32_t v = *reinterpret_cast<const uint16_t*>(x + at);
         if (!odd_word<TYPE>(v)) continue;
+        if (p.parts > 1) {
+          p.part_o[part_at(row) * DN + at / 2] += value_of<TYPE>(v, 0);
+          continue;
+        }
         uint16_t* const o = reinterpret_cast<uint16_t*>(out + at);
         *o = static_cast<uint16_t>(pair_of<TYPE>(value_of<TYPE>(*o, 0) + value_of<TYPE>(v, 0), 0.f));
       }
     }
   }
+}
+
+// Joins the parts of a tile's rows, as many at a time as DN / 4 lanes a row leave room for:
+// a lane takes four columns.
+template <int DN, int TYPE>
+__global__ __launch_bounds__(kThreads) void prompt_join_kernel(const PromptParams p) {
+  constexpr uint32_t kLanes = DN / 4, kAtOnce = kThreads / kLanes;
+  const uint32_t head = blockIdx.x, col = threadIdx.x % kLanes * 4;
+  PromptRequest r;
+  if (!find_tile(p, blockIdx.y, &r)) return;
+  const int32_t token = r.q0 + static_cast<int32_t>(r.tile * kRows + blockIdx.z * kAtOnce + threadIdx.x / kLanes);
+  if (token < r.q1) {
+    const int64_t at = static_cast<int64_t>(token) * p.heads + head, step = static_cast<int64_t>(p.nnz) * p.heads;
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 4
+    for (uint32_t k = 0; k < p.parts; ++k) m = fmaxf(m, p.part_ml[(at + k * step) * 2]);
+    const float from = m == -INFINITY ? 0.f : m;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (uint32_t k = 0; k < p.parts; ++k) {
+      const f32x2 ml = *reinterpret_cast<const f32x2*>(p.part_ml + (at + k * step) * 2);
+      const float weight = exp2_of(ml[0] - from);
+      l += weight * ml[1];
+      o += weight * *reinterpret_cast<const f32x4*>(p.part_o + (at + k * step) * DN + col);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const u32x2 x = {result_pair<TYPE>(o[0] * inv, o[1] * inv), result_pair<TYPE>(o[2] * inv, o[3] * inv)};
+    *reinterpret_cast<u32x2*>(p.out + static_cast<int64_t>(token) * p.o_token + head * p.o_head + col * 2) = x;
+    if (col == 0 && p.lse != nullptr) p.lse[at] = log_total<TYPE>(m, l);
+  }
+}
+
+template <int DN>
+const void* pick_join(int type) {
+  return type == PACE_KV_BF16 ? reinterpret_cast<const void*>(&prompt_join_kernel<DN, PACE_KV_BF16>)
+                              : reinterpret_cast<const void*>(&prompt_join_kernel<DN, PACE_KV_FP16>);
+}
+
+// Workgroups that a call's row tiles and heads can be, a short last tile for each request.
+int64_t tiles_of_call(int64_t nnz, int64_t batch) { return std::min<int64_t>(nnz, nnz / kRows + batch); }
+
+// Parts that the keys of each row tile are cut into.  The CUs have 512 places for workgroups
+// (two a CU); a call takes as long as its longest workgroup, or as all of them dealt to the
+// places, kStart steps more each; the joining kernel costs kJoin steps and what it reads.
+// The host knows the mean lengths alone.
+constexpr int64_t kPlaces = 512, kStart = 2, kJoin = 2, kMostParts = 32, kStepBytes = int64_t(8) << 20;
+
+int64_t parts_of_call(int64_t nnz, int64_t keys, int64_t batch, int64_t heads, int64_t head_dim, bool causal) {
+  if (batch == 0 || nnz == 0) return 1;
+  const int64_t groups = tiles_of_call(nnz, batch) * heads;
+  const int64_t longest = (keys / batch + kTile - 1) / kTile;
+  const int64_t mean = causal ? std::max<int64_t>(longest - nnz / batch / 2 / kTile, 1) : longest;
+  int64_t best = INT64_MAX, parts = 1;
+  for (int64_t k = 1; k <= std::min(kMostParts, std::max<int64_t>(longest, 1)); ++k) {
+    const int64_t each = (longest + k - 1) / k;
+    const int64_t dealt = (groups * (mean + k * kStart) + kPlaces - 1) / kPlaces + each / 2;
+    const int64_t join = k == 1 ? 0 : kJoin + 2 * k * nnz * heads * head_dim * 4 / kStepBytes;
+    const int64_t cost = std::max(each + kStart, dealt) + join;
+    if (cost < best) {
+      best = cost;
+      parts = k;
+    }
+  }
+  return parts;
+}
+
+int64_t workspace_of_call(int64_t parts, int64_t nnz, int64_t heads, int64_t head_dim) {
+  return parts == 1 ? 0 : parts * nnz * heads * (head_dim + 2) * 4;
+}
+
+int check_sizes(int64_t nnz, int64_t num_keys, int batch_size, int num_heads, int head_dim) {
+  if (nnz < 0 || num_keys < 0 || batch_size < 0 || num_heads <= 0)
+    return fail(PACE_KV_EINVAL, "prompt attention: sizes must be positive");
+  if (head_dim != 64 && head_dim != 128)
+    return fail(PACE_KV_EINVAL, "prompt attention: head_dim must be 64 or 128, got %d", head_dim);
+  if (nnz > INT32_MAX / 2 || num_keys > INT32_MAX / 2)
+    return fail(PACE_KV_ERANGE, "prompt attention: more than 2^30 queries or keys");
+  const int64_t tiles = tiles_of_call(nnz, batch_size);
+  if (tiles > 65535 || num_heads > (1 << 20) || tiles * num_heads >= (int64_t(1) << 24))
+    return fail(PACE_KV_ERANGE, "prompt attention: too many requests, heads or queries for one call");
+  return PACE_KV_OK;
 }
 
 template <int DN>
@@ -384,22 +493,29 @@ const void* pick_prompt(int type) {
 
 extern "C" {
 
+int pace_kv_prompt_attention_workspace(int64_t nnz, int64_t num_keys, int batch_size, int num_heads, int head_dim,
+                                       int causal, int64_t* bytes) {
+  using namespace pace_kv;
+  if (!bytes) return fail(PACE_KV_EINVAL, "prompt attention: NULL argument");
+  PACE_KV_TRY(check_sizes(nnz, num_keys, batch_size, num_heads, head_dim));
+  *bytes = workspace_of_call(parts_of_call(nnz, num_keys, batch_size, num_heads, head_dim, causal != 0), nnz, num_heads,
+                             head_dim);
+  return PACE_KV_OK;
+}
+
+
 int pace_kv_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* key,
                              int64_t k_token_stride, int64_t k_head_stride, const void* rope_key,
                              int64_t rope_token_stride, const void* value, int64_t v_token_stride, int64_t v_head_stride,
                              int elem_type, int num_heads, int head_dim, int64_t nnz, int64_t num_keys,
                              const int32_t* qo_indptr, const int32_t* kv_indptr, int batch_size, int max_q_len,
                              float scale, int causal, void* out, int64_t out_token_stride, int64_t out_head_stride,
-                             float* lse, int32_t* err_count, void* stream) {
+                             float* lse, void* workspace, int64_t workspace_size, int32_t* err_count, void* stream) {
   using namespace pace_kv;
-  if (nnz < 0 || num_keys < 0 || batch_size < 0 || num_heads <= 0 || max_q_len <= 0)
-    return fail(PACE_KV_EINVAL, "prompt attention: sizes must be positive");
-  if (head_dim != 64 && head_dim != 128)
-    return fail(PACE_KV_EINVAL, "prompt attention: head_dim must be 64 or 128, got %d", head_dim);
+  PACE_KV_TRY(check_sizes(nnz, num_keys, batch_size, num_heads, head_dim));
+  if (max_q_len <= 0) return fail(PACE_KV_EINVAL, "prompt attention: sizes must be positive");
   if (elem_type != PACE_KV_BF16 && elem_type != PACE_KV_FP16)
     return fail(PACE_KV_EINVAL, "prompt attention: queries must be bfloat16 or float16");
-  if (nnz > INT32_MAX / 2 || num_keys > INT32_MAX / 2)
-    return fail(PACE_KV_ERANGE, "prompt attention: more than 2^30 queries or keys");
   const float scale_log2 = scale * 1.44269504088896341f;
   if (!std::isfinite(scale_log2)) return fail(PACE_KV_EINVAL, "prompt attention: scale must be within float's range");
   if (nnz == 0 || batch_size == 0) return PACE_KV_OK;
@@ -413,10 +529,10 @@ int pace_kv_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_he
   const int64_t longest = std::max({k_token_stride, rope_token_stride, v_token_stride});
   if (longest >= int64_t(1) << 26 || std::min({k_token_stride, rope_token_stride, v_token_stride}) < 0)
     return fail(PACE_KV_EINVAL, "prompt attention: token strides of keys and values must be in [0, 2^26)");
-  // As many tiles as there can be: a short last one for each request.
-  const int64_t tiles = std::min<int64_t>(nnz, nnz / kRows + batch_size);
-  if (tiles > 65535 || num_heads > (1 << 20) || tiles * num_heads >= (int64_t(1) << 24))
-    return fail(PACE_KV_ERANGE, "prompt attention: too many requests, heads or queries for one call");
+  const int64_t parts = parts_of_call(nnz, num_keys, batch_size, num_heads, head_dim, causal != 0);
+  const int64_t need = workspace_of_call(parts, nnz, num_heads, head_dim);
+  if (need > 0 && (!workspace || workspace_size < need || reinterpret_cast<uintptr_t>(workspace) & 15u))
+    return fail(PACE_KV_EINVAL, "prompt attention: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
   PromptParams p = {};
   p.q = static_cast<const char*>(q);
   p.key = static_cast<const char*>(key);
@@ -437,13 +553,20 @@ int pace_kv_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_he
   p.keys = static_cast<uint32_t>(num_keys);
   p.heads = static_cast<uint32_t>(num_heads);
   p.max_q = static_cast<uint32_t>(max_q_len);
-  p.tiles = static_cast<uint32_t>(tiles);
+  p.tiles = static_cast<uint32_t>(tiles_of_call(nnz, batch_size));
+  p.parts = static_cast<uint32_t>(parts);
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + parts * nnz * num_heads * head_dim;
   p.scale_log2 = scale_log2;
   p.causal = causal != 0;
   void* args[] = {&p};
-  return hip_status(hipLaunchKernel(head_dim == 128 ? pick_prompt<128>(elem_type) : pick_prompt<64>(elem_type),
-                                    dim3(p.heads, p.tiles), dim3(kThreads), args, 0, static_cast<hipStream_t>(stream)),
-                    "prompt attention launch");
+  PACE_KV_TRY(hip_status(hipLaunchKernel(head_dim == 128 ? pick_prompt<128>(elem_type) : pick_prompt<64>(elem_type),
+                                         dim3(p.heads, p.tiles, p.parts), dim3(kThreads), args, 0,
+                                         static_cast<hipStream_t>(stream)), "prompt attention launch"));
+  if (parts == 1) return PACE_KV_OK;
+  return hip_status(hipLaunchKernel(head_dim == 128 ? pick_join<128>(elem_type) : pick_join<64>(elem_type),
+                                    dim3(p.heads, p.tiles, kRows * head_dim / 4 / kThreads), dim3(kThreads), args, 0,
+                                    static_cast<hipStream_t>(stream)), "prompt attention join launch");
 }
 
 }  // extern "C"

@@ -178,6 +178,13 @@ def paged_latent_attention(q: torch.Tensor, latent_cache: torch.Tensor, kv_indic
     return (out, lse) if return_lse else out
 
 
+@functools.lru_cache(maxsize=4096)
+def _prompt_workspace_bytes(*sizes: int) -> int:
+    out = ctypes.c_int64()
+    _native.check(_native.load().pace_kv_prompt_attention_workspace(*sizes, ctypes.byref(out)))
+    return out.value
+
+
 def latent_prompt_attention(q: torch.Tensor, key: torch.Tensor, rope_key: torch.Tensor, value: torch.Tensor,
                             qo_indptr: torch.Tensor, kv_indptr: torch.Tensor, *, sm_scale: Optional[float] = None,
                             max_q_len: Optional[int] = None, causal: bool = True, out: Optional[torch.Tensor] = None,
@@ -240,9 +247,11 @@ def latent_prompt_attention(q: torch.Tensor, key: torch.Tensor, rope_key: torch.
         return x.stride(0) * 2 if x.shape[0] > 1 else 0, x.stride(1) * 2 if heads > 1 else 0
 
     if nnz:
+        need = _prompt_workspace_bytes(nnz, n, batch, heads, D, int(causal))
+        space = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _call(dev, "pace_kv_prompt_attention", q.data_ptr(), *strides(q), key.data_ptr(), *strides(key),
               rope_key.data_ptr(), rope_key.stride(0) * 2 if n > 1 else 0, value.data_ptr(), *strides(value),
               _native.ELEM_TYPES[q.dtype], heads, D, nnz, n, qo.data_ptr(), ip.data_ptr(), batch,
               min(int(max_q_len), max(nnz, 1)), sm_scale, causal, out.data_ptr(), *strides(out),
-              None if lse is None else lse.data_ptr(), _err_ptr(err))
+              None if lse is None else lse.data_ptr(), None if space is None else space.data_ptr(), need, _err_ptr(err))
     return (out, lse) if return_lse else out
