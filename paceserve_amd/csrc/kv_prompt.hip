@@ -15,7 +15,8 @@
 namespace pace_kv {
 namespace {
 
-constexpr uint32_t kTile = 64;                           // keys of a step
+constexpr uint32_t kTile = 32;                           // keys of a step
+constexpr uint32_t kLoadRows = kTile / kWaves;           // of which a wave loads so many
 constexpr int kRT = 2;                                   // tiles of 16 query rows of a wave
 constexpr uint32_t kRows = 16 * kRT * kWaves;            // query rows of a workgroup
 
@@ -38,8 +39,8 @@ struct PromptParams {
 };
 
 struct PromptRequest {
-  uint32_t index, tile;        // the request, and the tile of it
-  int32_t q0, q1, k0, k1;
+  uint32_t tile;
+  int32_t q0, q1, k0, k1;      // its rows of queries and keys
 };
 
 // Whether a request's queries are among the rows, and not too many.
@@ -51,30 +52,63 @@ __device__ __forceinline__ uint32_t tiles_of(int32_t q0, int32_t q1) {
   return (static_cast<uint32_t>(q1 - q0) + kRows - 1) / kRows;
 }
 
-// The request whose row tiles (ceil(q_len / kRows) each) hold number x; false past the
-// last.  The wave looks at 64 requests a round.
+// Row tile x of a call and its request; false past the last.  A request's tiles that see the
+// most keys come first, and of up to 64 requests, a lane each, the one with the most: a long
+// tile that starts last would keep the call waiting.  (MI355X, 16 heads of 8 requests of up
+// to 2000 tokens in order 130 us, so 110; all tiles by their keys 109, but 4 requests of
+// 128 heads, whose keys then share the caches, 826 and 998.)
 __device__ __forceinline__ bool find_tile(const PromptParams& p, uint32_t x, PromptRequest* r) {
   const uint32_t lane = threadIdx.x % 64;
-  uint32_t before = 0;
-  for (uint32_t b0 = 0; b0 < p.batch; b0 += 64) {
-    const uint32_t b = b0 + lane;
-    int32_t q0 = 0, q1 = 0;
+  const auto load = [&](uint32_t b) {
+    PromptRequest mine = {0, 0, 0, 0, 0};
     if (b < p.batch) {
-      q0 = p.qo_indptr[b];
-      q1 = p.qo_indptr[b + 1];
+      mine.q0 = p.qo_indptr[b];
+      mine.q1 = p.qo_indptr[b + 1];
+      mine.k0 = p.kv_indptr[b];
+      mine.k1 = p.kv_indptr[b + 1];
     }
-    const uint32_t n = has_rows(p, q0, q1) ? tiles_of(q0, q1) : 0u;
-    const uint32_t upto = before + sum_upto(n);
-    const uint64_t mine = __ballot(x < upto);
-    if (mine != 0) {
-      const int at = __builtin_ctzll(mine);
-      r->index = b0 + at;
-      r->tile = x - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at));
-      r->q0 = __builtin_amdgcn_readlane(q0, at);
-      r->q1 = __builtin_amdgcn_readlane(q1, at);
-      return true;
+    return mine;
+  };
+  const auto take = [&](const PromptRequest& of, int at, uint32_t tile) {
+    r->q0 = __builtin_amdgcn_readlane(of.q0, at);
+    r->q1 = __builtin_amdgcn_readlane(of.q1, at);
+    r->k0 = min(max(__builtin_amdgcn_readlane(of.k0, at), 0), static_cast<int32_t>(p.keys));
+    r->k1 = min(max(__builtin_amdgcn_readlane(of.k1, at), r->k0), static_cast<int32_t>(p.keys));
+    r->tile = tile;
+    return true;
+  };
+  const auto total_of = [](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(sum_upto(v), 63)); };
+  PromptRequest mine = load(lane);
+  uint32_t n = has_rows(p, mine.q0, mine.q1) ? tiles_of(mine.q0, mine.q1) : 0u;
+  const uint32_t total = total_of(n);
+  if (p.batch <= 64 && total <= p.tiles) {
+    if (x >= total) return false;
+    const int64_t most = n > 0 ? max(static_cast<int64_t>(mine.k1) - mine.k0, int64_t(0)) : -1;
+    const int32_t key = static_cast<int32_t>(min(most, int64_t(INT32_MAX)));
+    uint32_t first = 0;                                  // tiles of the requests before the lane's
+    for (uint32_t j = 0; j < p.batch; ++j) {
+      const int32_t other = __builtin_amdgcn_readlane(key, j);
+      const uint32_t tiles = __builtin_amdgcn_readlane(n, j);
+      if (other > key || (other == key && j < lane)) first += tiles;
     }
-    before = __builtin_amdgcn_readlane(upto, 63);
+    const uint64_t here = __ballot(x >= first && x - first < n);
+    const int at = here != 0 ? __builtin_ctzll(here) : 0;
+    return take(mine, at, __builtin_amdgcn_readlane(n, at) - 1 - (x - __builtin_amdgcn_readlane(first, at)));
+  }
+  const uint32_t y = p.tiles - 1 - x;
+  uint32_t done = 0;
+  for (uint32_t b0 = 0; b0 < p.batch; b0 += 64) {
+    if (b0 != 0) {
+      mine = load(b0 + lane);
+      n = has_rows(p, mine.q0, mine.q1) ? tiles_of(mine.q0, mine.q1) : 0u;
+    }
+    const uint32_t upto = done + sum_upto(n);
+    const uint64_t past = __ballot(y < upto);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      return take(mine, at, y - (__builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(n, at)));
+    }
+    done = __builtin_amdgcn_readlane(upto, 63);
   }
   return false;
 }
@@ -113,7 +147,7 @@ __device__ __forceinline__ uint32_t swap_of(uint32_t r) {
 // 64 at a time: rows go from memory straight to LDS, into one of two buffers while the
 // other is read.
 template <int DN, int TYPE>
-__global__ __launch_bounds__(kThreads, 2) void prompt_kernel(const PromptParams p) {
+__global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams p) {
   constexpr int kNS = DN / 32, kCT = DN / 16;
   constexpr uint32_t kRow = DN * 2, kRopeRow = kRope * 2;
   constexpr uint32_t kRopeAt = kTile * kRow, kValueAt = kRopeAt + kTile * kRopeRow, kBuffer = kValueAt + kTile * kRow;
@@ -123,11 +157,8 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(const PromptParams 
   const uint32_t head = blockIdx.x;
   if (p.err != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && w == 0) count_bad(p);
   PromptRequest r;
-  // The last tiles first: they see the most keys.
-  if (!find_tile(p, gridDim.y - 1 - blockIdx.y, &r)) return;
-  const int32_t k0 = min(max(p.kv_indptr[r.index], 0), static_cast<int32_t>(p.keys));
-  const int32_t k1 = min(max(p.kv_indptr[r.index + 1], k0), static_cast<int32_t>(p.keys));
-  const int32_t q_len = r.q1 - r.q0, kv_len = k1 - k0, base = kv_len - q_len;
+  if (!find_tile(p, blockIdx.y, &r)) return;
+  const int32_t k0 = r.k0, q_len = r.q1 - r.q0, kv_len = r.k1 - r.k0, base = kv_len - q_len;
   const int32_t row0 = static_cast<int32_t>(r.tile * kRows), wave_row0 = row0 + static_cast<int32_t>(w * 16 * kRT);
   int32_t t_end = kv_len;
   if (p.causal) t_end = min(t_end, base + min(row0 + static_cast<int32_t>(kRows), q_len));
@@ -181,10 +212,10 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(const PromptParams 
     constexpr uint32_t kD = decltype(dim)::value, kLanes = kD / 8, kAtOnce = 64 / kLanes;
     const uint32_t ln = opaque(lane), in = ln / kLanes;
 #pragma unroll
-    for (uint32_t i = 0; i < 16; i += kAtOnce) {
-      const uint32_t row = w * 16 + i;                   // and `in` more
+    for (uint32_t i = 0; i < kLoadRows; i += kAtOnce) {
+      const uint32_t row = w * kLoadRows + i;            // and `in` more
       const char* const rows = from + (static_cast<int64_t>(t0) + row) * stride;
-      const uint32_t piece = (ln % kLanes) ^ swap_of<kD>(i + in);
+      const uint32_t piece = (ln % kLanes) ^ swap_of<kD>(row + in);
       const char* const x = rows + static_cast<uint64_t>(in * static_cast<uint32_t>(stride) + piece * 16);
       const uint32_t at = to + row * (kD * 2);
       if (decltype(whole)::value || t0 + static_cast<int32_t>(row + in) < t_end) copy_to_lds(x, at);
@@ -298,8 +329,8 @@ __global__ __launch_bounds__(kThreads, 2) void prompt_kernel(const PromptParams 
   const auto clean = [&](uint32_t from) {
     bool found = false;
 #pragma unroll 1
-    for (uint32_t c = lane; c < 16 * DN / 8; c += 64) {
-      const uint32_t at = from + kValueAt + w * 16 * kRow + c * 16;
+    for (uint32_t c = lane; c < kLoadRows * DN / 8; c += 64) {
+      const uint32_t at = from + kValueAt + w * kLoadRows * kRow + c * 16;
       u32x4 x = lds_get<u32x4>(at);
       bool here = false;
 #pragma unroll
@@ -440,15 +471,18 @@ const void* pick_join(int type) {
 // Workgroups that a call's row tiles and heads can be, a short last tile for each request.
 int64_t tiles_of_call(int64_t nnz, int64_t batch) { return std::min<int64_t>(nnz, nnz / kRows + batch); }
 
-// Parts that the keys of each row tile are cut into.  The CUs have 512 places for workgroups
-// (two a CU); a call takes as long as its longest workgroup, or as all of them dealt to the
+// What they come to if every other request's last tile is half empty.
+int64_t likely_tiles(int64_t nnz, int64_t batch) { return (nnz + kRows - 1) / kRows + (batch - 1) / 2; }
+
+// Parts that the keys of each row tile are cut into.  The CUs have 768 places for workgroups
+// (three a CU); a call takes as long as its longest workgroup, or as all of them dealt to the
 // places, kStart steps more each; the joining kernel costs kJoin steps and what it reads.
 // The host knows the mean lengths alone.
-constexpr int64_t kPlaces = 512, kStart = 2, kJoin = 2, kMostParts = 32, kStepBytes = int64_t(8) << 20;
+constexpr int64_t kPlaces = 768, kStart = 4, kJoin = 4, kMostParts = 32, kStepBytes = int64_t(4) << 20;
 
 int64_t parts_of_call(int64_t nnz, int64_t keys, int64_t batch, int64_t heads, int64_t head_dim, bool causal) {
   if (batch == 0 || nnz == 0) return 1;
-  const int64_t groups = tiles_of_call(nnz, batch) * heads;
+  const int64_t groups = likely_tiles(nnz, batch) * heads;
   const int64_t longest = (keys / batch + kTile - 1) / kTile;
   const int64_t mean = causal ? std::max<int64_t>(longest - nnz / batch / 2 / kTile, 1) : longest;
   int64_t best = INT64_MAX, parts = 1;
@@ -463,6 +497,19 @@ int64_t parts_of_call(int64_t nnz, int64_t keys, int64_t batch, int64_t heads, i
     }
   }
   return parts;
+}
+
+// LDS that a workgroup asks for beyond its own, so that two fit a CU instead of three: the
+// last turn of few workgroups a CU costs more than three at a time gain.  One, two and three
+// workgroups a CU take about 10, 13 and 18 for the same keys (MI355X, 128 columns: 600, 925
+// and 991 TFLOP/s): four a CU take 26 by twos and 28 by threes.
+uint32_t spare_lds(int64_t groups, int head_dim) {
+  constexpr int64_t kCus = 256, kTime[4] = {0, 10, 13, 18};
+  const int64_t each = (groups + kCus - 1) / kCus;
+  const auto time_of = [&](int64_t at_once) { return each / at_once * kTime[at_once] + kTime[each % at_once]; };
+  if (time_of(3) <= time_of(2)) return 0;
+  const uint32_t own = 2 * kTile * (2 * head_dim + kRope) * 2;
+  return (uint32_t(56) << 10) - own;                     // 160 KiB a CU
 }
 
 int64_t workspace_of_call(int64_t parts, int64_t nnz, int64_t heads, int64_t head_dim) {
@@ -561,7 +608,8 @@ int pace_kv_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_he
   p.causal = causal != 0;
   void* args[] = {&p};
   PACE_KV_TRY(hip_status(hipLaunchKernel(head_dim == 128 ? pick_prompt<128>(elem_type) : pick_prompt<64>(elem_type),
-                                         dim3(p.heads, p.tiles, p.parts), dim3(kThreads), args, 0,
+                                         dim3(p.heads, p.tiles, p.parts), dim3(kThreads), args,
+                                         spare_lds(likely_tiles(nnz, batch_size) * num_heads * parts, head_dim),
                                          static_cast<hipStream_t>(stream)), "prompt attention launch"));
   if (parts == 1) return PACE_KV_OK;
   return hip_status(hipLaunchKernel(head_dim == 128 ? pick_join<128>(elem_type) : pick_join<64>(elem_type),
