@@ -99,42 +99,6 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
         atomicAdd(p.err, min(page, t_end - t_begin - i * page));
   }
 
-  // Query fragments: row n of each tile, eight elements from 32 k + 8 g, with the scale's
-  // sign: what follows takes it as positive.  (A scale of zero makes all scores zero.)  Rows
-  // behind the last read it and become zeros: loads under a condition would wait for one
-  // another (MI355X: 9 us).
-  const uint32_t wave_row0 = row0 + (kShare ? w * 16 : 0), query_row0 = row0 + (kShare ? w / 2 * 32 : 0);
-  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
-  const float per_score = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
-  u32x4 qf[RQ][kQS];
-#pragma unroll
-  for (int a = 0; a < RQ; ++a) {
-    const uint32_t row = min(query_row0 + a * 16 + lane % 16, rows - 1), i = over(p.by_group, row);
-    const char* const q = p.q + static_cast<int64_t>(r.q0 + i) * p.q_stride + static_cast<int64_t>(row - i * p.group) * (kW * 2);
-#pragma unroll
-    for (int k = 0; k < kQS; ++k)
-      qf[a][k] = *reinterpret_cast<const u32x4*>(q + (kShare ? 2 * k + w % 2 : k) * 64 + lane / 16 * 16);
-  }
-#pragma unroll
-  for (int a = 0; a < RQ; ++a) {
-    const uint32_t mask = query_row0 + a * 16 + lane % 16 < rows ? keep : 0u;
-#pragma unroll
-    for (int k = 0; k < kQS; ++k) qf[a][k] = (qf[a][k] ^ flip) & mask;
-  }
-  f32x4 acc[RT][kCT];
-#pragma unroll
-  for (int a = 0; a < RT; ++a)
-#pragma unroll
-    for (int d = 0; d < kCT; ++d) acc[a][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m[RW], l[RW];
-  bool wide[RW];                                         // some row's |m| is past 2^20
-#pragma unroll
-  for (int a = 0; a < RW; ++a) {
-    m[a] = -INFINITY;
-    l[a] = 0.f;
-    wide[a] = false;
-  }
-
   // A step's loads: page ids (a token to a lane, the same in all waves), then rows: each
   // wave brings eight.
   int32_t id = -1;
@@ -177,6 +141,59 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
     else
       lds_put(at + ln * 16, u32x4{0, 0, 0, 0});
   };
+
+  constexpr int32_t kStep = static_cast<int32_t>(kTile);
+  const int32_t seen_by_all = p.mask == nullptr ? base + first_q + 1 : base;
+  int32_t t0 = t_begin;
+  uint32_t now = lds_offset(lds), other = now + kBuffer;
+  const auto load_next = [&](int32_t next, uint32_t to) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      if (next_valid == ~0u) load_piece(std::true_type{}, opaque(lane), i, to);
+      else if (next < t_end) load_piece(std::false_type{}, opaque(lane), i, to);
+    }
+  };
+  load_id(t0);
+
+  // Query fragments: row n of each tile, eight elements from 32 k + 8 g, with the scale's
+  // sign: what follows takes it as positive.  (A scale of zero makes all scores zero.)  Rows
+  // behind the last read it and become zeros: loads under a condition would wait for one
+  // another (MI355X: 9 us).
+  const uint32_t wave_row0 = row0 + (kShare ? w * 16 : 0), query_row0 = row0 + (kShare ? w / 2 * 32 : 0);
+  const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
+  const float per_score = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  u32x4 qf[RQ][kQS];
+#pragma unroll
+  for (int a = 0; a < RQ; ++a) {
+    const uint32_t row = min(query_row0 + a * 16 + lane % 16, rows - 1), i = over(p.by_group, row);
+    const char* const q = p.q + static_cast<int64_t>(r.q0 + i) * p.q_stride + static_cast<int64_t>(row - i * p.group) * (kW * 2);
+#pragma unroll
+    for (int k = 0; k < kQS; ++k)
+      qf[a][k] = *reinterpret_cast<const u32x4*>(q + (kShare ? 2 * k + w % 2 : k) * 64 + lane / 16 * 16);
+  }
+  // The first rows are on their way before the queries have come.
+  place_rows(t0);
+  load_next(t0, now);
+  load_id(t0 + kStep);
+#pragma unroll
+  for (int a = 0; a < RQ; ++a) {
+    const uint32_t mask = query_row0 + a * 16 + lane % 16 < rows ? keep : 0u;
+#pragma unroll
+    for (int k = 0; k < kQS; ++k) qf[a][k] = (qf[a][k] ^ flip) & mask;
+  }
+  f32x4 acc[RT][kCT];
+#pragma unroll
+  for (int a = 0; a < RT; ++a)
+#pragma unroll
+    for (int d = 0; d < kCT; ++d) acc[a][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m[RW], l[RW];
+  bool wide[RW];                                         // some row's |m| is past 2^20
+#pragma unroll
+  for (int a = 0; a < RW; ++a) {
+    m[a] = -INFINITY;
+    l[a] = 0.f;
+    wide[a] = false;
+  }
 
   // Scores of 32 tokens: lane: row n of each tile, tokens 16 t + 4 g + e.
   f32x4 s[RW][2];
@@ -349,17 +366,6 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
     }
   };
 
-  constexpr int32_t kStep = static_cast<int32_t>(kTile);
-  const int32_t seen_by_all = p.mask == nullptr ? base + first_q + 1 : base;
-  int32_t t0 = t_begin;
-  uint32_t now = lds_offset(lds), other = now + kBuffer;
-  const auto load_next = [&](int32_t next, uint32_t to) {
-#pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      if (next_valid == ~0u) load_piece(std::true_type{}, opaque(lane), i, to);
-      else if (next < t_end) load_piece(std::false_type{}, opaque(lane), i, to);
-    }
-  };
   const auto one_step = [&](auto full) {
     valid = next_valid;
     place_rows(t0 + kStep);
@@ -411,10 +417,6 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
     other = x;
     t0 += kStep;
   };
-  load_id(t0);
-  place_rows(t0);
-  load_next(t0, now);
-  load_id(t0 + kStep);
   // The steps whose tokens every row sees, then the others.
   while (t0 + kStep <= seen_by_all && next_valid == ~0u) one_step(std::true_type{});
   const int32_t t_masked = t0;

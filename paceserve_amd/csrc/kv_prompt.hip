@@ -173,6 +173,39 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
   // Keys that a row sees: those before `seen_by`.
   const auto seen_by = [&](int32_t row) { return p.causal ? base + row + 1 : kv_len; };
 
+  // A step's loads: kLoadRows rows of keys, rotated parts and values a wave, 1 KiB an instruction.
+  const char* const key0 = p.key + k0 * p.k_token + head * p.k_head;
+  const char* const value0 = p.value + k0 * p.v_token + head * p.v_head;
+  const char* const rope0 = p.rope_key + k0 * p.r_token;
+  const auto load_part = [&](auto whole, auto dim, const char* from, int64_t stride, int32_t t0, uint32_t to) {
+    constexpr uint32_t kD = decltype(dim)::value, kLanes = kD / 8, kAtOnce = 64 / kLanes;
+    const uint32_t ln = opaque(lane), in = ln / kLanes;
+#pragma unroll
+    for (uint32_t i = 0; i < kLoadRows; i += kAtOnce) {
+      const uint32_t row = w * kLoadRows + i;            // and `in` more
+      const char* const rows = from + (static_cast<int64_t>(t0) + row) * stride;
+      const uint32_t piece = (ln % kLanes) ^ swap_of<kD>(row + in);
+      const char* const x = rows + static_cast<uint64_t>(in * static_cast<uint32_t>(stride) + piece * 16);
+      const uint32_t at = to + row * (kD * 2);
+      if (decltype(whole)::value || t0 + static_cast<int32_t>(row + in) < t_end) copy_to_lds(x, at);
+      else lds_put(at + ln * 16, u32x4{0, 0, 0, 0});
+    }
+  };
+  const auto load_step = [&](auto whole, int32_t t0, uint32_t to) {
+    load_part(whole, std::integral_constant<int, DN>{}, key0, p.k_token, t0, to);
+    load_part(whole, std::integral_constant<int, kRope>{}, rope0, p.r_token, t0, to + kRopeAt);
+    load_part(whole, std::integral_constant<int, DN>{}, value0, p.v_token, t0, to + kValueAt);
+  };
+  const auto load_next = [&](int32_t t0, uint32_t to) {
+    if (t0 + static_cast<int32_t>(kTile) <= t_end) load_step(std::true_type{}, t0, to);
+    else if (t0 < t_end) load_step(std::false_type{}, t0, to);
+  };
+
+  constexpr int32_t kStep = static_cast<int32_t>(kTile);
+  uint32_t now = lds_offset(lds), other = now + kBuffer;
+  int32_t t0 = t_begin;
+  load_next(t0, now);
+
   // Query fragments with the scale's sign: what follows takes it as positive.  (A scale
   // of zero makes all scores zero.)  Rows behind the last read it and become zeros: loads
   // under a condition would wait for one another (MI355X: 6 us).
@@ -203,34 +236,6 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
 #pragma unroll
     for (int d = 0; d < kCT; ++d) acc[a][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-
-  // A step's loads: 16 rows of keys, rotated parts and values a wave, 1 KiB an instruction.
-  const char* const key0 = p.key + k0 * p.k_token + head * p.k_head;
-  const char* const value0 = p.value + k0 * p.v_token + head * p.v_head;
-  const char* const rope0 = p.rope_key + k0 * p.r_token;
-  const auto load_part = [&](auto whole, auto dim, const char* from, int64_t stride, int32_t t0, uint32_t to) {
-    constexpr uint32_t kD = decltype(dim)::value, kLanes = kD / 8, kAtOnce = 64 / kLanes;
-    const uint32_t ln = opaque(lane), in = ln / kLanes;
-#pragma unroll
-    for (uint32_t i = 0; i < kLoadRows; i += kAtOnce) {
-      const uint32_t row = w * kLoadRows + i;            // and `in` more
-      const char* const rows = from + (static_cast<int64_t>(t0) + row) * stride;
-      const uint32_t piece = (ln % kLanes) ^ swap_of<kD>(row + in);
-      const char* const x = rows + static_cast<uint64_t>(in * static_cast<uint32_t>(stride) + piece * 16);
-      const uint32_t at = to + row * (kD * 2);
-      if (decltype(whole)::value || t0 + static_cast<int32_t>(row + in) < t_end) copy_to_lds(x, at);
-      else lds_put(at + ln * 16, u32x4{0, 0, 0, 0});
-    }
-  };
-  const auto load_step = [&](auto whole, int32_t t0, uint32_t to) {
-    load_part(whole, std::integral_constant<int, DN>{}, key0, p.k_token, t0, to);
-    load_part(whole, std::integral_constant<int, kRope>{}, rope0, p.r_token, t0, to + kRopeAt);
-    load_part(whole, std::integral_constant<int, DN>{}, value0, p.v_token, t0, to + kValueAt);
-  };
-  const auto load_next = [&](int32_t t0, uint32_t to) {
-    if (t0 + static_cast<int32_t>(kTile) <= t_end) load_step(std::true_type{}, t0, to);
-    else if (t0 < t_end) load_step(std::false_type{}, t0, to);
-  };
 
   // Scores of 32 keys from row `key` on: lane: row n of each tile, keys 16 t + 4 g + e.
   f32x4 s[kRT][2];
@@ -345,9 +350,6 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
     odd |= found;
   };
 
-  constexpr int32_t kStep = static_cast<int32_t>(kTile);
-  uint32_t now = lds_offset(lds), other = now + kBuffer;
-  int32_t t0 = t_begin;
   const auto one_step = [&](auto full) {
     rows_barrier();                                      // this step's rows are in LDS, the other buffer's readers done
     load_next(t0 + kStep, other);
@@ -368,7 +370,6 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
     other = x;
     t0 += kStep;
   };
-  load_next(t0, now);
   // The steps whose keys every row sees, then the others.
   while (t0 + kStep <= min(seen_by(row0), t_end)) one_step(std::true_type{});
   const int32_t t_masked = t0;
