@@ -519,6 +519,15 @@ __global__ __launch_bounds__(kThreads) void latent_join_kernel(const AttnParams 
   const uint32_t row = (token - r.q0) * p.group + head, tile = row / p.tile_rows;
   const int64_t first = (static_cast<int64_t>(place.part()) * p.row_tiles + tile) * p.tile_rows + row % p.tile_rows;
   const int64_t step = static_cast<int64_t>(p.row_tiles) * p.tile_rows;
+  // A wave's parts of 64 chunks; the first ones are asked for before their weights are known.
+  constexpr uint32_t kParts = 4;
+  vec x[kParts];
+  const auto load = [&](uint32_t c0) {
+#pragma unroll
+    for (uint32_t j = 0; j < kParts; ++j)
+      x[j] = *reinterpret_cast<const vec*>(p.part_o + (first + min(c0 + part + j * WAVES, r.chunks - 1) * step) * L + lane * kVec);
+  };
+  load(0);
   // The maximum over all chunks, which every wave finds for itself.
   float m = -INFINITY;
   for (uint32_t c = lane; c < r.chunks; c += 64) m = fmaxf(m, p.part_ml[(first + c * step) * 2]);
@@ -535,9 +544,13 @@ __global__ __launch_bounds__(kThreads) void latent_join_kernel(const AttnParams 
       l += weight * p.part_ml[at + 1];
     }
     const uint32_t n = min(r.chunks - c0, 64u);
-#pragma unroll 4
-    for (uint32_t c = part; c < n; c += WAVES)
-      o += __shfl(weight, c) * *reinterpret_cast<const vec*>(p.part_o + (first + (c0 + c) * step) * L + lane * kVec);
+    for (uint32_t c = part; c < n;) {
+#pragma unroll
+      for (uint32_t j = 0; j < kParts; ++j, c += WAVES)
+        if (c < n) o += __shfl(weight, c) * x[j];
+      const uint32_t after = c < n ? c0 + c - part : c0 + 64;
+      if (after < r.chunks) load(after);
+    }
   }
 #pragma unroll
   for (int k = 1; k < 64; k *= 2) l += __shfl_xor(l, k);
