@@ -620,8 +620,8 @@ int pace_kv_norm_rotate(const void* q, int64_t q_token_stride,
  * slot_mapping[i] = page * page_size + s of one layer's cache, of elem_type
  * (format PACE_KV_PLAIN) or quantised (head_dim and rotary_dim then multiples
  * of 64; elements rounded once, from float32).  Slots of one call are distinct.
- * Slot -1 is padding: nothing of the token is read or written.  A token with
- * another slot outside the cache or a position outside the table is not
+ * Slot -1 is padding: nothing of the token is written.  A token with another
+ * slot outside the cache or a position outside the table is not
  * written, and counted in err_count.
  *
  * Replaces the append of
@@ -702,7 +702,8 @@ int pace_kv_latent_attention(const void* q, int64_t q_stride_bytes,
  * of no request are not written.  err_count goes up by one for each request
  * that is skipped (queries outside [0, nnz), more than max_q_len, or past the
  * row tiles of nnz rows where offsets overlap) or whose keys are cut to
- * [0, num_keys).  The keys of few rows are cut up by the sizes here alone;
+ * [0, num_keys).  Token strides of keys, rotated parts and values lie in
+ * [0, 2^26).  The keys of few rows are cut up by the sizes here alone;
  * workspace as in pace_kv_attention.
  */
 int pace_kv_prompt_attention_workspace(int64_t nnz, int64_t num_keys,

@@ -45,8 +45,17 @@ __device__ __forceinline__ uint32_t swap_of_row(uint32_t r) { return (r % 8) * 2
 // other is read.  There the latents' 16-byte pieces c of row r lie at c ^ swap(r), within
 // each 256 bytes, so that neither 16 rows of one piece (keys) nor 4 rows of two
 // (transposed values) meet in a bank.
+//
+// Bound by memory where a tile is 16 or 32 rows (16 heads read 1152 bytes a token for 35
+// thousand operations): 128 requests of up to 8192 tokens in 126 us, 4.8 TB/s, and 4.2 with
+// the joining kernel; the steps alone reach 6, the rest is the start, where tables, page ids
+// and rows wait for one another, and the last workgroups.  With 64 rows by LDS, whose reads
+// take 63 % of the time against the products' 44: 256 requests of 4096 tokens and 128 heads
+// in 400 us, 730 TFLOP/s.  128 rows, which would halve those reads, need more registers than
+// four waves have (they spill), or two groups of waves that take turns, which wait for each
+// other (560 us where this took 425).
 template <int L, int TYPE, int RT>
-__global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const AttnParams p) {
+__global__ __launch_bounds__(kThreads, 2) void latent_kernel(const AttnParams p) {
   constexpr int kW = L + kRope, kKS = L / 32, kCT = L / 64;
   constexpr bool kShare = RT >= 4;
   constexpr int RW = kShare ? 1 : RT;                    // tiles whose weights a wave makes
@@ -216,7 +225,8 @@ __global__ __launch_bounds__(kThreads, RT == 8 ? 1 : 2) void latent_kernel(const
       return lds_get<u32x4>((key ^ (k % 4 * 64)) + t * 16 * kRow + k / 4 * 256);
     };
     // Reads stay kAhead before their products: left to itself the compiler waits for each.
-    constexpr int kReads = 2 * kQS, kEach = kReads / kPieces, kAhead = RT == 4 ? 4 : RT == 2 ? 1 : 8;
+    // (32 rows have no registers for more than one.)
+    constexpr int kReads = 2 * kQS, kEach = kReads / kPieces, kAhead = kShare ? 4 : RT == 2 ? 1 : 8;
     u32x4 kf[kReads];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) kf[i] = read(i);

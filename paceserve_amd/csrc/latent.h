@@ -28,13 +28,6 @@ constexpr float kSlack = 4.f;
 template <int TYPE>
 constexpr float kUnit = TYPE == PACE_KV_FP16 ? 15.f - kSlack : 0.f;
 
-// The weight of a score s over the maximum m.
-template <int TYPE>
-__device__ __forceinline__ float weight_of(float s, float m) {
-#pragma clang fp contract(off)
-  return exp2_of((s - m) + kUnit<TYPE>);
-}
-
 // Matrix instructions' results, waited for: max3_of reads them in assembly, which the
 // compiler does not do for.  20 cycles, more than any such instruction takes to write.
 __device__ __forceinline__ void settle(f32x4& x, f32x4& y) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x), "+v"(y)); }
