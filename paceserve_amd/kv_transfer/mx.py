@@ -168,6 +168,8 @@ def _pools(plain, small) -> Tuple[PagedPool, PagedPool, int]:
     pp, sp = as_pool(plain), as_pool(small)
     if pp.host or sp.host:
         raise ValueError("quantised pages convert between device pools")
+    if len(pp.page_shape) != 4 or len(sp.page_shape) != 4:
+        raise ValueError("quantised pages are those of keys and values: a latent cache has none")
     if pp.dtype not in _native.ELEM_TYPES:
         raise ValueError(f"pool of {pp.dtype}: bfloat16, float16 or float32 is converted")
     if sp.dtype is not torch.uint8:

@@ -3,7 +3,8 @@
 A *pool* is the per-layer paged KV cache of one instance: a list of L device
 tensors, each contiguous with shape [num_pages, 2, page_size, num_kv_heads,
 head_dim] (the layout of FlashinferAttentionWrapper.gpu_cache,
-paceserve/model_executor/attention/flashinfer_attention_wrapper.py:53-73).
+paceserve/model_executor/attention/flashinfer_attention_wrapper.py:53-73), or
+[num_pages, page_size, width], a latent cache's.
 A *transfer buffer* is one contiguous tensor [L, n, 2, page_size, H, D]: the
 layout KVhelper.get_kv_cache returns (paceserve/kv_transfer/kv_utils.py:44).
 
@@ -58,9 +59,9 @@ class PagedPool:
         if not layers:
             raise ValueError("a pool needs at least one layer tensor")
         first = layers[0]
-        if first.dim() != 5 or first.shape[1] != 2:
-            raise ValueError(
-                f"layer tensors must be [num_pages, 2, page_size, num_kv_heads, head_dim], got {tuple(first.shape)}")
+        if first.dim() != 3 and (first.dim() != 5 or first.shape[1] != 2):
+            raise ValueError("layer tensors must be [num_pages, 2, page_size, num_kv_heads, head_dim] or, latent, "
+                             f"[num_pages, page_size, width], got {tuple(first.shape)}")
         # first's properties are read once: a list of 32 layers, checked at every
         # call that is given one, takes 17 us instead of 29
         shape, dtype, device = first.shape, first.dtype, first.device
@@ -79,6 +80,7 @@ class PagedPool:
         self.num_layers = len(layers)
         self.num_pages = int(first.shape[0])
         self.page_shape: Tuple[int, ...] = tuple(int(s) for s in first.shape[1:])
+        self.page_size = self.page_shape[0 if len(self.page_shape) == 2 else 1]
         self.dtype = first.dtype
         self.device = first.device
         self.page_bytes = int(first[0].numel()) * first.element_size()

@@ -53,7 +53,7 @@ class SwapSpace:
     def __init__(self, dev_pool, num_host_pages: int):
         self.dev = ops.as_pool(dev_pool)
         self.host = ops.HostPagePool.like(self.dev, num_host_pages)
-        self.host_allocator = NativeBlockAllocator(self.dev.page_shape[1], num_host_pages)
+        self.host_allocator = NativeBlockAllocator(self.dev.page_size, num_host_pages)
         self.tables: Dict[str, List[int]] = {}   # seq_id -> host pages
         # seq_id -> event recorded after its swap-out: its swap-in, on any
         # stream, reads the host pages only after they are written.
