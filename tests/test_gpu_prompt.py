@@ -223,3 +223,53 @@ def test_nothing_to_do_and_refusals(gpu):
                 dict(key=torch.zeros((4, 2, 129), dtype=BF16, device=gpu)[..., 1:])):
         with pytest.raises((ValueError, RuntimeError)):
             latent_prompt_attention(**{**good, **bad})
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("heads,D", [(1, 128), (2, 64)])
+def test_keys_dealt_to_many_workgroups(gpu, heads, D, dtype):
+    """Few queries over many keys, one request with fewer keys than there are parts, one
+    with none; infinities and NaN in some parts alone."""
+    b = Prompts(gpu, [5, 3, 2, 130], [20000, 2, 0, 700], heads=heads, D=D, dtype=dtype, seed=11)
+    out, lse = b.run()
+    b.check(out, lse)
+    assert torch.isneginf(lse[5]).all() and torch.isneginf(lse[8:10]).all()
+    wide, _ = b.run(causal=False)
+    b.check(*b.run(causal=False), causal=False)
+    b.value[50, 0, 5], b.value[15000, heads - 1, 6] = math.inf, -math.inf
+    b.value[19998, 0, 7] = math.nan                       # seen by the last two of the five queries
+    b.check(*b.run())
+    b.value[50, 0, 5] = 0
+    b.key[12000, 0, 3] = math.nan
+    b.check(*b.run())
+    assert torch.isfinite(wide[:10]).all()
+
+
+def test_more_requests_than_lanes(gpu):
+    rng = np.random.default_rng(12)
+    q_len = rng.integers(0, 6, 150)
+    q_len[[3, 77, 149]] = [200, 129, 300]
+    b = Prompts(gpu, q_len, q_len + rng.integers(0, 40, 150), heads=1, seed=12)
+    err = torch.zeros(1, dtype=torch.int32, device=gpu)
+    b.check(*b.run(err=err), picks=8)
+    assert err.item() == 0
+    want, _ = b.run()
+    out = torch.full_like(want, 7.0)
+    b.run(max_q_len=150, err=err, out=out)
+    long = np.repeat(q_len > 150, q_len)
+    assert err.item() == 2 and (out[:b.nnz][long] == 7).all() and torch.equal(out[:b.nnz][~long], want[:b.nnz][~long])
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_random_prompts(gpu, seed):
+    rng = np.random.default_rng(100 + seed)
+    batch = int(rng.integers(1, 12))
+    q_len = np.where(rng.random(batch) < 0.3, 1, rng.integers(0, 400, batch))
+    kv = q_len + np.where(rng.random(batch) < 0.5, 0, rng.integers(0, 900, batch))
+    if q_len.sum() == 0:
+        q_len[0] = kv[0] = 9
+    causal = bool(rng.integers(0, 2))
+    print(f"prompts {q_len.tolist()} over {kv.tolist()} causal={causal}", flush=True)
+    b = Prompts(gpu, q_len, kv, heads=int(rng.integers(1, 5)), D=[64, 128][seed % 2], dtype=[BF16, FP16][seed // 2 % 2],
+                seed=seed)
+    b.check(*b.run(causal=causal), causal=causal, picks=12)
