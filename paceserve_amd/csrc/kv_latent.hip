@@ -659,7 +659,8 @@ const void* pick_latent(int type, uint32_t tile_rows) {
   return type == PACE_KV_BF16 ? pick_latent<L, PACE_KV_BF16>(tile_rows) : pick_latent<L, PACE_KV_FP16>(tile_rows);
 }
 
-// Rows of a call from which on a wave joins one by itself.
+// Rows of a call from which on a wave joins one by itself.  (MI355X, calls with four waves a
+// row and with one: 16 rows of 63 parts 16 us and 21, 4096 rows 84 and 79, 12800 124 and 104.)
 constexpr int64_t kManyRows = 4096;
 
 template <int L, int TYPE>
