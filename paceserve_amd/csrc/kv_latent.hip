@@ -286,10 +286,10 @@ __global__ __launch_bounds__(kThreads, 2) void latent_kernel(const AttnParams p)
       top = max3_of(top, s[a][1][1], s[a][1][2]);
       top = scaled(max3_of(top, s[a][1][3], s[a][1][3]), per_score);
       shrink[a] = 1.f;
-      if (__ballot(top > m[a] + kSlack) != 0) {
+      if (__ballot(top > m[a] + kSlack<TYPE>) != 0) {
         raised |= 1u << a;
         top = across_groups(top, max_of);
-        const float next = top > m[a] + kSlack ? top : m[a];
+        const float next = top > m[a] + kSlack<TYPE> ? top : m[a];
         shrink[a] = exp2_of(m[a] - (next == -INFINITY ? 0.f : next));
         m[a] = next;
         l[a] *= shrink[a];

@@ -366,3 +366,40 @@ def test_refusals(gpu):
         latent.empty_cache(1, 16, 128)
     with pytest.raises(ValueError):
         latent.empty_cache(1, 16, 512, torch.float32)
+
+
+@pytest.mark.parametrize("heads", [1, 32, 128])
+def test_values_at_bfloat16s_largest_exponent(gpu, heads):
+    """Weighted means of values of 2^127 are finite, over one token or over thousands, in
+    one part and joined from several."""
+    b = Batch(gpu, [1, 40, 5000], [1, 2, 1], heads=heads, seed=20)
+    for x in b.rows:
+        x[:, 100] = 2.0 ** 127
+        x[:, 101] = 2.0 ** 127 * torch.where(torch.arange(len(x)) % 3 == 0, -1.0, 1.0)
+    b.q[..., 100:102] = 0.0
+    b.fill()
+    out, lse = b.run()
+    assert torch.isfinite(out).all() and (out[..., 100].float() >= 2.0 ** 126).all()
+    b.check(out, lse)
+
+
+@pytest.mark.parametrize("heads", [1, 128])
+@pytest.mark.parametrize("nats", [9, 16, 18, 22])
+def test_float16_keeps_many_small_weights(gpu, nats, heads):
+    """One token far above a flat tail of 6000: the tail's weights are small numbers of
+    float16, and what they add to the columns in which the first token is zero counts."""
+    b = Batch(gpu, [6000], [1], heads=heads, dtype=FP16, seed=21)
+    x = b.rows[0]
+    x[:] = 0.0
+    x[:, 100:164] = torch.from_numpy(b.rng.standard_normal((6000, 64)) * 0.1 + 1.0)
+    x[3000, 100:164] = 0.0
+    x[3000, 0] = 16.0
+    b.q.zero_()
+    b.q[..., 0] = nats / 16.0 / b.scale
+    b.fill()
+    out, lse = b.run()
+    b.check(out, lse)
+    # weights of 2^(15 - nats / ln 2), more than 2^-17: off by 2^-8 at most, as is the result
+    got, p = out[0, 0, 100:164].double().cpu().numpy(), math.exp(-nats)
+    want = p * b.seen[0][:, 100:164].sum(0) / (1 + p * 5999)
+    assert (np.abs(got - want) <= want * 2.0 ** -7 + 2.0 ** -25).all()

@@ -273,3 +273,16 @@ def test_random_prompts(gpu, seed):
     b = Prompts(gpu, q_len, kv, heads=int(rng.integers(1, 5)), D=[64, 128][seed % 2], dtype=[BF16, FP16][seed // 2 % 2],
                 seed=seed)
     b.check(*b.run(causal=causal), causal=causal, picks=12)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_values_at_bfloat16s_largest_exponent(gpu, D):
+    """Weighted means of values of 2^127 are finite, also where the keys are dealt out."""
+    for q_len, kv_len, heads in (([70, 1], [70, 300], 2), ([5], [20000], 1)):
+        b = Prompts(gpu, q_len, kv_len, heads=heads, D=D, seed=13)
+        b.value[..., 3] = 2.0 ** 127
+        b.value[::3, :, 4] = -2.0 ** 127
+        b.value[1::3, :, 4] = 2.0 ** 127
+        out, lse = b.run()
+        assert torch.isfinite(out[:b.nnz]).all() and (out[:b.nnz, :, 3].float() >= 2.0 ** 126).all()
+        b.check(out, lse)
