@@ -65,7 +65,7 @@ def _check_rows(name: str, x: torch.Tensor, like: torch.Tensor, heads: Optional[
     # One look at each property settles a good tensor (a decode step's append 14.1 to 12.5 us
     # on the host, with the others like this).
     if heads is not None or x is like:
-        want = like.shape if x is like else (like.shape[0], heads, like.shape[2])
+        want = like.shape if heads is None else (like.shape[0], heads, like.shape[2])
         if x.shape == want and x.dtype is like.dtype and x.get_device() == like.get_device() and x.stride(2) == 1:
             return
     if x.dim() != 3 or x.shape[0] != like.shape[0] or x.shape[2] != like.shape[2] or x.dtype is not like.dtype \
@@ -164,9 +164,9 @@ def append_paged_kv_cache_rope(query: torch.Tensor, append_key: torch.Tensor, ap
     D and rotary_dim then in multiples of 64): its elements are rounded once,
     from the float32 results.
 
-    A token with slot -1 is padding: nothing of it is read or written.  One with
-    another slot outside the cache, or a position outside the table, is counted
-    in `err` and not written."""
+    A token with slot -1 is padding: nothing of it is written.  One with another
+    slot outside the cache, or a position outside the table, is counted in `err`
+    and not written."""
     cache = paged_kv_cache
     _refuse_gradients("append_paged_kv_cache_rope", query, append_key, append_value, q_weight, k_weight, cache)
     if query.dim() != 3:
