@@ -33,6 +33,11 @@ constexpr int64_t kStreamBytes = int64_t(64) << 20;
 // Latent rows of a call from which on a lane group takes two.  MI355X, 65536 rows of 576 numbers
 // 45 us by one, 39 by two, 16384 10.4 and 10.0, 2000 3.4 and 3.8.
 constexpr int64_t kManyRows = 8192;
+// Waves that a token's heads are dealt to while there are fewer than this: the CUs hold 8192, and
+// a wave's turns wait for their rows one after another.  MI355X, 8190 tokens of 48 heads into
+// an 8-bit cache: by 8190 waves 53 us, by 16380 41, by 49140 42; 16384 tokens of 40 heads,
+// rotated alone, 62 us by as many waves, 65 by four times as many.
+constexpr int64_t kEnoughWaves = 16384;
 
 struct Rows {
   const char* in;
@@ -172,43 +177,55 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeParams p) {
   const uint32_t whole = over(p.by_parts, wave), part = wave - whole * p.parts;
   const int64_t token = whole;
   if (token >= p.nnz) return;
-  int64_t page_at = 0, slot = 0;
-  if constexpr (FORMAT >= 0) {
-    const int64_t s = p.slots[token];
-    if (s == -1) return;                                 // padding
-    if (s < 0 || s >= p.num_slots) {
-      if (p.err != nullptr && part == 0 && lane == 0) atomicAdd(p.err, 1);
-      return;
-    }
-    const int64_t page = s <= UINT32_MAX ? over(p.by_page, static_cast<uint32_t>(s)) : s / p.page_size;
-    slot = s - page * p.page_size;
-    page_at = page * p.page_bytes;
-  }
   const int64_t position = p.positions[token];
-  if (position < 0 || position >= p.table_rows) {
-    if (p.err != nullptr && part == 0 && lane == 0) atomicAdd(p.err, 1);
-    return;
-  }
+  int64_t page_at = 0, slot = 0;
+  if constexpr (FORMAT >= 0) slot = p.slots[token];
   const uint32_t group = 1u << p.group_log2, u = lane & (group - 1);
   const bool rotates = u < p.rotary / 16, active = u < p.units;
   // First elements of the lane's runs.
   const uint32_t tail = p.head_dim - p.rotary;
   const uint32_t ea = rotates ? 8 * u : p.rotary + 8 * (u - p.rotary / 16);
   const uint32_t eb = ea + (rotates ? p.rotary : tail) / 2;
-  float cos[8], sin[8];
-  if (rotates) load_angles(p.table + position * p.rotary, p.rotary, INTERLEAVED, u, cos, sin);
   const uint32_t qk = p.q.heads + p.k.heads, heads = qk + (FORMAT >= 0 ? p.v.heads : 0u);
   const uint32_t end = min((part + 1) * p.part_heads, heads);
   const uint32_t turn = 64u >> p.group_log2;
-  for (uint32_t h = part * p.part_heads + (lane >> p.group_log2); h < end; h += turn) {
+  uint32_t h = part * p.part_heads + (lane >> p.group_log2);
+  const auto load = [&](uint32_t h, u32x4& ra, u32x4& rb) {
+    ra = rb = u32x4{0, 0, 0, 0};
+    if (!active || h >= end) return;
     const Rows& rows = h < p.q.heads ? p.q : h < qk ? p.k : p.v;
     const uint32_t head = h < p.q.heads ? h : h < qk ? h - p.q.heads : h - qk;
     const char* const in = rows.in + token * rows.in_token + head * rows.in_head;
-    u32x4 ra = {0, 0, 0, 0}, rb = {0, 0, 0, 0};
-    if (active) {
-      ra = load_vec<STREAM>(in + ea * 2);
-      rb = load_vec<STREAM>(in + eb * 2);
+    ra = load_vec<STREAM>(in + ea * 2);
+    rb = load_vec<STREAM>(in + eb * 2);
+  };
+  // On the way to a cache the first rows do not wait for the slot.  (MI355X, 8190 tokens of 48
+  // heads into an 8-bit cache 41 us instead of 44; without a cache there is nothing to wait
+  // for but the position, and 16384 tokens took 71 us instead of 62.)
+  constexpr bool kEarly = FORMAT >= 0;
+  u32x4 ra, rb;
+  if (kEarly) load(h, ra, rb);
+  const uint32_t h0 = h;
+  if constexpr (FORMAT >= 0) {
+    if (slot == -1) return;                              // padding
+    if (slot < 0 || slot >= p.num_slots) {
+      if (p.err != nullptr && part == 0 && lane == 0) atomicAdd(p.err, 1);
+      return;
     }
+    const int64_t page = slot <= UINT32_MAX ? over(p.by_page, static_cast<uint32_t>(slot)) : slot / p.page_size;
+    slot -= page * p.page_size;
+    page_at = page * p.page_bytes;
+  }
+  if (position < 0 || position >= p.table_rows) {
+    if (p.err != nullptr && part == 0 && lane == 0) atomicAdd(p.err, 1);
+    return;
+  }
+  float cos[8], sin[8];
+  if (rotates) load_angles(p.table + position * p.rotary, p.rotary, INTERLEAVED, u, cos, sin);
+  for (; h < end; h += turn) {
+    const Rows& rows = h < p.q.heads ? p.q : h < qk ? p.k : p.v;
+    const uint32_t head = h < p.q.heads ? h : h < qk ? h - p.q.heads : h - qk;
+    if (!kEarly || h != h0) load(h, ra, rb);
     float a[8], b[8];
     if (h < qk) {
       widen<TYPE>(ra, a);
@@ -423,7 +440,7 @@ int launch_rope(RopeParams& p, int elem_type, int format, int head_dim, int rota
   // A wave for a token's heads, or several where the tokens are too few for the CUs.
   const uint32_t turns = (heads + turn - 1) / turn;
   uint32_t per = turns;
-  while (per > 1 && p.nnz * ((turns + per - 1) / per) < 4096) per = (per + 1) / 2;
+  while (per > 1 && p.nnz * ((turns + per - 1) / per) < kEnoughWaves) per = (per + 1) / 2;
   p.part_heads = per * turn;
   p.parts = (heads + p.part_heads - 1) / p.part_heads;
   const int64_t groups = (p.nnz * p.parts + kWaves - 1) / kWaves;

@@ -312,3 +312,22 @@ def test_refusals(gpu):
                                                           table=rope.rotary_table(4, 32, device=gpu))):
         with pytest.raises((ValueError, RuntimeError)):
             rope.append_paged_kv_cache_rope(**{**good, **bad})
+
+
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+def test_quantised_blocks_that_are_not_finite(gpu, fmt):
+    """An infinity or a NaN, given or made by the norm, marks its block of 32 and no other;
+    rotated columns spread it to their partner's block."""
+    rng = np.random.default_rng(8)
+    n, H, D, P = 6, 2, 128, 16
+    q, k, v = (rows(rng, (n, H, D), BF16, gpu) for _ in range(3))
+    k[1, 0, 5], k[2, 1, 100], v[3, 0, 40], v[4, 1, 127] = math.inf, math.nan, -math.inf, math.nan
+    table = rope.rotary_table(50, 64, device=gpu)
+    at = torch.arange(n, dtype=torch.int32, device=gpu) + 3
+    cache = torch.zeros((2, 2, P, H, mx.row_width(D, fmt)), dtype=torch.uint8, device=gpu)
+    rope.append_paged_kv_cache_rope(q, k, v, at, torch.arange(n, device=gpu) + 7, cache, table)
+    torch.cuda.synchronize()
+    byte = mx.elements_and_scales(cache, D)[1].cpu().numpy()
+    marked = np.argwhere(byte == 255).tolist()
+    # [page, key or value, place, head, block]
+    assert sorted(marked) == sorted([[0, 0, 8, 0, 0], [0, 0, 8, 0, 1], [0, 0, 9, 1, 3], [0, 1, 10, 0, 1], [0, 1, 11, 1, 3]])
