@@ -33,7 +33,13 @@ __device__ __forceinline__ uint32_t seen_of(const AttnParams& p, const Request& 
 }
 
 // How far the 16-byte pieces of row r of a tile are xored within 256 bytes.
-__device__ __forceinline__ uint32_t swap_of_row(uint32_t r) { return (r % 8) * 2 | r / 8 % 2; }
+__device__ __forceinline__ uint32_t swap_of_row(uint32_t r) {
+  const uint32_t half = r / 8 % 2;
+  return ((r % 8) ^ half * 4) * 2 | half;
+}
+
+// The same of the weights' rows of 64 bytes.
+__device__ __forceinline__ uint32_t swap_of_weights(uint32_t n) { return (0u - n / 4) & 3u; }
 
 // RT tiles of 16 rows a workgroup, whose four waves sum a quarter of the columns each, of
 // all rows.  Up to two tiles every wave makes the weights of all rows for itself.  Of four
@@ -350,7 +356,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_kernel(const AttnParams p)
     const uint32_t ln = opaque(lane), n = ln % 16, g = ln / 16;
     const uint32_t v_row = kShare ? 8 * g + n / 4 : 4 * g + n / 4;
     const uint32_t v = from + v_row * kRow + ((w * kCT * 2 + n % 4 / 2) ^ swap_of_row(v_row)) * 16 + n % 2 * 8;
-    const uint32_t p_at = lds_offset(lds_p) + n * kWeightRow + (g ^ (n / 4)) * 16;  // tile a's are at (a ^ 1) * kShared
+    const uint32_t p_at = lds_offset(lds_p) + n * kWeightRow + (g ^ swap_of_weights(n)) * 16;  // tile a's are at (a ^ 1) * kShared
     u32x4 weight[RT];
 #pragma unroll
     for (int a = 0; a < RT; ++a) {
@@ -393,7 +399,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_kernel(const AttnParams p)
       const uint32_t ln = opaque(lane), n = ln % 16, g = ln / 16;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        lds_put(other_sums + n * kWeightRow + ((2 * t + g / 2) ^ (n / 4)) * 16 + g % 2 * 8,
+        lds_put(other_sums + n * kWeightRow + ((2 * t + g / 2) ^ swap_of_weights(n)) * 16 + g % 2 * 8,
                 u32x2{pf[0][2 * t], pf[0][2 * t + 1]});
       if (g == 0) lds_put(other_sums + kShrinkAt + n * 4, shrink[0]);
       if (ln == 0) lds_put(other_sums + kRaisedAt, raised);

@@ -140,7 +140,8 @@ __device__ __forceinline__ void count_bad(const PromptParams& p) {
 // of two (transposed values) meet in a bank.
 template <int D>
 __device__ __forceinline__ uint32_t swap_of(uint32_t r) {
-  return D == 128 ? (r % 8) * 2 | r / 8 % 2 : (r / 2 % 4) * 2 | r / 8 % 2;
+  const uint32_t half = r / 8 % 2;
+  return D == 128 ? ((r % 8) ^ half * 4) * 2 | half : ((r / 2 % 4) ^ half * 2) * 2 | half;
 }
 
 // A workgroup takes 128 query rows of a head, 32 a wave, and passes over the keys they see,

@@ -46,7 +46,12 @@ __device__ __forceinline__ void rows_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// LDS by offsets, whose swizzles are xors.
+// LDS by offsets, whose swizzles are xors.  Its 64 banks serve 8-byte reads by 32 lanes in
+// order, 16-byte reads by 16: lanes 0-3, 12-15 and 20-27, then 4-11, 16-19 and 28-31, and the
+// upper 32 the same way (measured: the counter of conflicts is 0 for layouts that keep
+// these lanes apart).  Of a fragment read by rows n = lane % 16, rows 0-3 and 12-15 of one
+// 16-byte column thus meet rows 4-11 of the next: the rows whose pieces lie in the same 32
+// bytes are of one set or the other, and, for values, not both of 0-7.
 __device__ __forceinline__ uint32_t lds_offset(const void* x) {
   return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) char*)x));
 }
