@@ -176,7 +176,8 @@ __global__ __launch_bounds__(kThreads, 2) void latent_kernel(const AttnParams p)
   // another (MI355X: 9 us).
   const uint32_t wave_row0 = row0 + (kShare ? w * 16 : 0), query_row0 = row0 + (kShare ? w / 2 * 32 : 0);
   const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
-  const float per_score = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  const float per_score = __uint_as_float(
+      __builtin_amdgcn_readfirstlane(__float_as_uint(p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2))));
   u32x4 qf[RQ][kQS];
 #pragma unroll
   for (int a = 0; a < RQ; ++a) {
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_kernel(const AttnParams p)
   bool wide[RW];                                         // some row's |m| is past 2^20
 #pragma unroll
   for (int a = 0; a < RW; ++a) {
-    m[a] = -INFINITY;
+    m[a] = kLowest;
     l[a] = 0.f;
     wide[a] = false;
   }
@@ -283,8 +284,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_kernel(const AttnParams p)
       }
     }
     raised = 0;
-#pragma unroll
-    for (int a = 0; a < RW; ++a) settle(s[a][0], s[a][1]);
+    settle(s);
 #pragma unroll
     for (int a = 0; a < RW; ++a) {
       float top = max3_of(s[a][0][0], s[a][0][1], s[a][0][2]);
@@ -296,21 +296,20 @@ __global__ __launch_bounds__(kThreads, 2) void latent_kernel(const AttnParams p)
         raised |= 1u << a;
         top = across_groups(top, max_of);
         const float next = top > m[a] + kSlack<TYPE> ? top : m[a];
-        shrink[a] = exp2_of(m[a] - (next == -INFINITY ? 0.f : next));
+        shrink[a] = exp2_of(m[a] - next);
         m[a] = next;
         l[a] *= shrink[a];
-        wide[a] = __ballot(fabsf(next) > 0x1p20f && next != -INFINITY) != 0;
+        wide[a] = __ballot(fabsf(next) > 0x1p20f && next != kLowest) != 0;
       }
-      const float from = m[a] == -INFINITY ? 0.f : m[a];
       // The fused difference holds what m lost when it was rounded: less than a tenth up
       // to 2^20, but past 2^27 enough to make the largest weight an infinity or a zero.
       if (wide[a]) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[a][t][e] = unfused(scaled(s[a][t][e], per_score), from) + kUnit<TYPE>;
+          for (int e = 0; e < 4; ++e) s[a][t][e] = unfused(scaled(s[a][t][e], per_score), m[a]) + kUnit<TYPE>;
       } else {
-        const float offset = kUnit<TYPE> - from;
+        const float offset = kUnit<TYPE> - m[a];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll

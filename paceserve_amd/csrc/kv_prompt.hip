@@ -183,28 +183,46 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
   const char* const key0 = p.key + k0 * p.k_token + head * p.k_head;
   const char* const value0 = p.value + k0 * p.v_token + head * p.v_head;
   const char* const rope0 = p.rope_key + k0 * p.r_token;
-  const auto load_part = [&](auto whole, auto dim, const char* from, int64_t stride, int32_t t0, uint32_t to) {
+  // A lane's place in them: the row within an instruction's, and the piece that belongs at its
+  // place in LDS; four rows further on that is the piece eight away.  Held in registers over
+  // the steps that have no masks (8192 tokens of 32 heads 719 us, so 690), else derived anew.
+  struct Places {
+    uint32_t key, rope, value, four_on;
+  };
+  const auto place_of = [&](uint32_t ln, auto dim, int64_t stride) {
+    constexpr uint32_t kD = decltype(dim)::value, kLanes = kD / 8;
+    const uint32_t in = ln / kLanes;
+    return in * static_cast<uint32_t>(stride) + ((ln % kLanes) ^ swap_of<kD>(w * kLoadRows + in)) * 16;
+  };
+  const auto places_of = [&](uint32_t ln) {
+    return Places{place_of(ln, std::integral_constant<int, DN>{}, p.k_token),
+                  place_of(ln, std::integral_constant<int, kRope>{}, p.r_token),
+                  place_of(ln, std::integral_constant<int, DN>{}, p.v_token),
+                  (ln ^ swap_of<DN>(w * kLoadRows + ln / 16)) & 8u ? 0u - 128u : 128u};
+  };
+  const auto load_part = [&](auto whole, auto dim, const char* from, int64_t stride, uint32_t place, uint32_t four_on,
+                             int32_t t0, uint32_t to) {
     constexpr uint32_t kD = decltype(dim)::value, kLanes = kD / 8, kAtOnce = 64 / kLanes;
-    const uint32_t ln = opaque(lane), in = ln / kLanes;
 #pragma unroll
     for (uint32_t i = 0; i < kLoadRows; i += kAtOnce) {
-      const uint32_t row = w * kLoadRows + i;            // and `in` more
+      const uint32_t row = w * kLoadRows + i, at = to + row * (kD * 2);
       const char* const rows = from + (static_cast<int64_t>(t0) + row) * stride;
-      const uint32_t piece = (ln % kLanes) ^ swap_of<kD>(row + in);
-      const char* const x = rows + static_cast<uint64_t>(in * static_cast<uint32_t>(stride) + piece * 16);
-      const uint32_t at = to + row * (kD * 2);
-      if (decltype(whole)::value || t0 + static_cast<int32_t>(row + in) < t_end) copy_to_lds(x, at);
+      const char* const x = rows + static_cast<uint64_t>(i == 0 ? place : place + four_on);
+      const uint32_t ln = decltype(whole)::value ? 0u : opaque(lane);
+      if (decltype(whole)::value || t0 + static_cast<int32_t>(row + ln / kLanes) < t_end) copy_to_lds(x, at);
       else lds_put(at + ln * 16, u32x4{0, 0, 0, 0});
     }
   };
-  const auto load_step = [&](auto whole, int32_t t0, uint32_t to) {
-    load_part(whole, std::integral_constant<int, DN>{}, key0, p.k_token, t0, to);
-    load_part(whole, std::integral_constant<int, kRope>{}, rope0, p.r_token, t0, to + kRopeAt);
-    load_part(whole, std::integral_constant<int, DN>{}, value0, p.v_token, t0, to + kValueAt);
+  const auto load_step = [&](auto whole, const Places& at, int32_t t0, uint32_t to) {
+    load_part(whole, std::integral_constant<int, DN>{}, key0, p.k_token, at.key, at.four_on, t0, to);
+    load_part(whole, std::integral_constant<int, kRope>{}, rope0, p.r_token, at.rope, 0u, t0, to + kRopeAt);
+    load_part(whole, std::integral_constant<int, DN>{}, value0, p.v_token, at.value, at.four_on, t0, to + kValueAt);
   };
   const auto load_next = [&](int32_t t0, uint32_t to) {
-    if (t0 + static_cast<int32_t>(kTile) <= t_end) load_step(std::true_type{}, t0, to);
-    else if (t0 < t_end) load_step(std::false_type{}, t0, to);
+    if (t0 >= t_end) return;
+    const Places at = places_of(opaque(lane));
+    if (t0 + static_cast<int32_t>(kTile) <= t_end) load_step(std::true_type{}, at, t0, to);
+    else load_step(std::false_type{}, at, t0, to);
   };
 
   constexpr int32_t kStep = static_cast<int32_t>(kTile);
@@ -216,7 +234,8 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
   // of zero makes all scores zero.)  Rows behind the last read it and become zeros: loads
   // under a condition would wait for one another (MI355X: 6 us).
   const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u, keep = p.scale_log2 == 0.f ? 0u : ~0u;
-  const float per_score = p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2);
+  const float per_score = __uint_as_float(
+      __builtin_amdgcn_readfirstlane(__float_as_uint(p.scale_log2 == 0.f ? 1.f : fabsf(p.scale_log2))));
   u32x4 qf[kRT][kNS + 2];
 #pragma unroll
   for (int a = 0; a < kRT; ++a) {
@@ -236,7 +255,7 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
   bool wide[kRT];                                        // some row's |m| is past 2^20
 #pragma unroll
   for (int a = 0; a < kRT; ++a) {
-    m[a] = -INFINITY;
+    m[a] = kLowest;
     l[a] = 0.f;
     wide[a] = false;
 #pragma unroll
@@ -276,8 +295,7 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
             if (t * 16 + e >= upto) s[a][t][e] = -INFINITY;
       }
     }
-#pragma unroll
-    for (int a = 0; a < kRT; ++a) settle(s[a][0], s[a][1]);
+    settle(s);
 #pragma unroll
     for (int a = 0; a < kRT; ++a) {
       float top = max3_of(s[a][0][0], s[a][0][1], s[a][0][2]);
@@ -287,23 +305,22 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
       if (__ballot(top > m[a] + kSlack<TYPE>) != 0) {
         top = across_groups(top, max_of);
         const float next = top > m[a] + kSlack<TYPE> ? top : m[a];
-        const float shrink = exp2_of(m[a] - (next == -INFINITY ? 0.f : next));
+        const float shrink = exp2_of(m[a] - next);
         m[a] = next;
         l[a] *= shrink;
-        wide[a] = __ballot(fabsf(next) > 0x1p20f && next != -INFINITY) != 0;
+        wide[a] = __ballot(fabsf(next) > 0x1p20f && next != kLowest) != 0;
 #pragma unroll
         for (int d = 0; d < kCT; ++d) acc[a][d] *= shrink;
       }
-      const float from = m[a] == -INFINITY ? 0.f : m[a];
       // The fused difference holds what m lost when it was rounded: less than a tenth up
       // to 2^20, but past 2^27 enough to make the largest weight an infinity or a zero.
       if (wide[a]) {
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[a][t][e] = unfused(scaled(s[a][t][e], per_score), from) + kUnit<TYPE>;
+          for (int e = 0; e < 4; ++e) s[a][t][e] = unfused(scaled(s[a][t][e], per_score), m[a]) + kUnit<TYPE>;
       } else {
-        const float offset = kUnit<TYPE> - from;
+        const float offset = kUnit<TYPE> - m[a];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -356,9 +373,11 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
     odd |= found;
   };
 
+  const Places held = places_of(lane);
   const auto one_step = [&](auto full) {
     rows_barrier();                                      // this step's rows are in LDS, the other buffer's readers done
-    load_next(t0 + kStep, other);
+    if constexpr (decltype(full)::value) load_step(std::true_type{}, held, t0 + kStep, other);
+    else load_next(t0 + kStep, other);
     if constexpr (!decltype(full)::value) {
       clean(now);
       lds_barrier();
@@ -376,8 +395,9 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
     other = x;
     t0 += kStep;
   };
-  // The steps whose keys every row sees, then the others.
-  while (t0 + kStep <= min(seen_by(row0), t_end)) one_step(std::true_type{});
+  // The steps whose keys every row sees, if a whole one follows, then the others.
+  const int32_t last_full = min(min(seen_by(row0), t_end) - kStep, t_end - 2 * kStep);
+  while (t0 <= last_full) one_step(std::true_type{});
   const int32_t t_masked = t0;
 #pragma unroll 1
   while (t0 < t_end) one_step(std::false_type{});

@@ -27,6 +27,9 @@ __device__ __forceinline__ float unfused(float a, float b) {
 template <int TYPE>
 constexpr float kSlack = TYPE == PACE_KV_FP16 ? 0.f : 4.f;
 
+// The maximum of no scores: finite, so that differences from it are numbers.
+constexpr float kLowest = -0x1.fffffep127f;
+
 // log2 of the weight of a score that equals the maximum.  In float16 the largest weights are
 // 2^15, which leaves those down to 2^-29 of the largest their 2^-11.  bfloat16 has float32's
 // exponents: 2^-24, so that up to 2^20 values of the largest exponent have a finite sum.
@@ -35,7 +38,12 @@ constexpr float kUnit = TYPE == PACE_KV_FP16 ? 15.f : -24.f;
 
 // Matrix instructions' results, waited for: max3_of reads them in assembly, which the
 // compiler does not do for.  20 cycles, more than any such instruction takes to write.
-__device__ __forceinline__ void settle(f32x4& x, f32x4& y) { asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x), "+v"(y)); }
+template <int N>
+__device__ __forceinline__ void settle(f32x4 (&x)[N][2]) {
+  static_assert(N == 1 || N == 2);
+  if constexpr (N == 1) asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x[0][0]), "+v"(x[0][1]));
+  else asm volatile("s_nop 15\n\ts_nop 3" : "+v"(x[0][0]), "+v"(x[0][1]), "+v"(x[1][0]), "+v"(x[1][1]));
+}
 
 // A workgroup's barrier that waits for its LDS operations alone, not for rows on their way
 // into LDS as __syncthreads does.
