@@ -271,15 +271,25 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
     for (int a = 0; a < kRT; ++a)
 #pragma unroll
       for (int t = 0; t < 2; ++t) s[a][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const auto read = [&](int i) {
+      const int k = i / 2, t = i % 2;
+      return lds_get<u32x4>(k < kNS ? (key ^ (k * 64)) + (first + t * 16) * kRow
+                                    : (rope ^ ((k - kNS) * 64)) + (first + t * 16) * kRopeRow);
+    };
+    // Reads stay two before their products (8192 tokens of 32 heads 640 us to 631; four before,
+    // registers spill).
+    constexpr int kReads = 2 * (kNS + 2), kAhead = 2;
+    u32x4 kf[kReads];
 #pragma unroll
-    for (int k = 0; k < kNS + 2; ++k)
+    for (int i = 0; i < kAhead; ++i) kf[i] = read(i);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const u32x4 kf = lds_get<u32x4>(k < kNS ? (key ^ (k * 64)) + (first + t * 16) * kRow
-                                                : (rope ^ ((k - kNS) * 64)) + (first + t * 16) * kRopeRow);
+    for (int i = 0; i < kReads; ++i) {
+      if (i + kAhead < kReads) kf[i + kAhead] = read(i + kAhead);
 #pragma unroll
-        for (int a = 0; a < kRT; ++a) s[a][t] = mfma<TYPE>(kf, qf[a][k], s[a][t]);
-      }
+      for (int a = 0; a < kRT; ++a) s[a][i % 2] = mfma<TYPE>(kf[i], qf[a][i / 2], s[a][i % 2]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   // Weights of those keys, the first of which is t0, packed by twos as they lie in s.
   u32x4 pf[kRT];
@@ -342,13 +352,22 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
   const uint32_t v_at = kValueAt + v_row * kRow + (n % 4 / 2 ^ swap_of<DN>(v_row)) * 16 + n % 2 * 8;
   const auto gather = [&](uint32_t from, uint32_t first) {
     const uint32_t v = opaque(v_at) + from;
-#pragma unroll
-    for (int d = 0; d < kCT; ++d) {
+    const auto read = [&](int d) {
       const uint32_t x = (v ^ (d * 32)) + first * kRow;
       const u32x2 lo = lds_transposed(x), hi = lds_transposed(x + 16 * kRow);
-      const u32x4 vf = {lo[0], lo[1], hi[0], hi[1]};
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    constexpr int kAhead = 2;
+    u32x4 vf[kCT];
 #pragma unroll
-      for (int a = 0; a < kRT; ++a) acc[a][d] = mfma<TYPE>(vf, pf[a], acc[a][d]);
+    for (int d = 0; d < kAhead; ++d) vf[d] = read(d);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int d = 0; d < kCT; ++d) {
+      if (d + kAhead < kCT) vf[d + kAhead] = read(d + kAhead);
+#pragma unroll
+      for (int a = 0; a < kRT; ++a) acc[a][d] = mfma<TYPE>(vf[d], pf[a], acc[a][d]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // Takes infinities and NaN out of the values that the wave loaded: a product with weight
