@@ -703,8 +703,8 @@ int pace_kv_latent_attention(const void* q, int64_t q_stride_bytes,
  * that is skipped (queries outside [0, nnz), more than max_q_len, or past the
  * row tiles of nnz rows where offsets overlap) or whose keys are cut to
  * [0, num_keys).  Token strides of keys, rotated parts and values lie in
- * [0, 2^26).  The keys of few rows are cut up by the sizes here alone;
- * workspace as in pace_kv_attention.
+ * [0, 2^26), and output rows do not overlap.  The keys of few rows are cut up
+ * by the sizes here alone; workspace as in pace_kv_attention.
  */
 int pace_kv_prompt_attention_workspace(int64_t nnz, int64_t num_keys,
                                        int batch_size, int num_heads,

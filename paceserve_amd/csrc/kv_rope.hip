@@ -16,6 +16,7 @@
 // against 32 of its rows: a lane loads them once and goes on over the token's heads.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <type_traits>
 
 #include "mx.h"
@@ -402,16 +403,16 @@ const void* pick_latent(int type, bool interleaved, bool many) {
   return many ? pick_latent<L, PACE_KV_FP16, 2>(interleaved) : pick_latent<L, PACE_KV_FP16, 1>(interleaved);
 }
 
-int check_rows(const char* call, const Rows& r, bool writes, uint32_t head_dim) {
+int check_rows(const char* call, const Rows& r, bool writes, int64_t nnz, uint32_t head_dim) {
   if (r.heads == 0) return PACE_KV_OK;
   if (!r.in || (writes && !r.out)) return fail(PACE_KV_EINVAL, "%s: NULL rows", call);
   uintptr_t bits = reinterpret_cast<uintptr_t>(r.in) | static_cast<uintptr_t>(r.in_token | r.in_head) |
                    reinterpret_cast<uintptr_t>(r.weight);
   if (writes) bits |= reinterpret_cast<uintptr_t>(r.out) | static_cast<uintptr_t>(r.out_token | r.out_head);
   if (bits & 15u) return fail(PACE_KV_EINVAL, "%s: rows, weights and strides must be multiples of 16 bytes", call);
-  if (writes && r.heads > 1 && r.out_head < static_cast<int64_t>(head_dim) * 2 &&
-      r.out_head > -static_cast<int64_t>(head_dim) * 2)
-    return fail(PACE_KV_EINVAL, "%s: output heads overlap", call);
+  const auto overlaps = [&](int64_t count, int64_t stride) { return count > 1 && std::abs(stride) < int64_t(2) * head_dim; };
+  if (writes && (overlaps(nnz, r.out_token) || overlaps(r.heads, r.out_head)))
+    return fail(PACE_KV_EINVAL, "%s: output rows overlap", call);
   return PACE_KV_OK;
 }
 
@@ -485,8 +486,8 @@ int pace_kv_norm_rotate(const void* q, int64_t q_token_stride, int64_t q_head_st
              q_out_head_stride, static_cast<const char*>(q_weight), static_cast<uint32_t>(q_heads)};
   p.k = Rows{static_cast<const char*>(k), k_token_stride, k_head_stride, static_cast<char*>(k_out), k_out_token_stride,
              k_out_head_stride, static_cast<const char*>(k_weight), static_cast<uint32_t>(k_heads)};
-  PACE_KV_TRY(check_rows(call, p.q, true, static_cast<uint32_t>(head_dim)));
-  PACE_KV_TRY(check_rows(call, p.k, true, static_cast<uint32_t>(head_dim)));
+  PACE_KV_TRY(check_rows(call, p.q, true, nnz, static_cast<uint32_t>(head_dim)));
+  PACE_KV_TRY(check_rows(call, p.k, true, nnz, static_cast<uint32_t>(head_dim)));
   p.positions = positions;
   p.table = table;
   p.table_rows = table_rows;
@@ -525,9 +526,9 @@ int pace_kv_append_rope(const void* q, int64_t q_token_stride, int64_t q_head_st
              static_cast<const char*>(k_weight), static_cast<uint32_t>(kv_heads)};
   p.v = Rows{static_cast<const char*>(v), v_token_stride, v_head_stride, nullptr, 0, 0, nullptr,
              static_cast<uint32_t>(kv_heads)};
-  PACE_KV_TRY(check_rows(call, p.q, true, static_cast<uint32_t>(head_dim)));
-  PACE_KV_TRY(check_rows(call, p.k, false, static_cast<uint32_t>(head_dim)));
-  PACE_KV_TRY(check_rows(call, p.v, false, static_cast<uint32_t>(head_dim)));
+  PACE_KV_TRY(check_rows(call, p.q, true, nnz, static_cast<uint32_t>(head_dim)));
+  PACE_KV_TRY(check_rows(call, p.k, false, nnz, static_cast<uint32_t>(head_dim)));
+  PACE_KV_TRY(check_rows(call, p.v, false, nnz, static_cast<uint32_t>(head_dim)));
   const int64_t half = static_cast<int64_t>(page_size) * kv_heads * head_dim;
   if (half >= int64_t(1) << 36) return fail(PACE_KV_ERANGE, "%s: pages of 2^36 elements or more", call);
   p.half_bytes = format == PACE_KV_PLAIN ? half * 2 : mx_half_bytes(half, format);

@@ -199,7 +199,8 @@ def latent_prompt_attention(q: torch.Tensor, key: torch.Tensor, rope_key: torch.
     kv_indptr[b] .. kv_indptr[b + 1]; its queries are its last tokens.  causal:
     query i of q_len sees the keys up to kv_len - q_len + i; otherwise all of its
     request's.  Tensors may be slices of wider ones (token and head strides of a
-    multiple of 16 bytes): key and value of one projection.
+    multiple of 16 bytes, keys' and values' tokens less than 64 MiB apart): key
+    and value of one projection.
 
     sm_scale is 1 / sqrt(D + 64) by default.  Returns out [nnz, num_heads, D]
     (`out` if given; rows outside every request are not written), and with

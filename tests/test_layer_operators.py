@@ -55,7 +55,8 @@ SHARED = [
     (dict(table=None), EINVAL, "NULL"), (dict(table=0x108), EINVAL, "16-byte"), (dict(q=None), EINVAL, "NULL"),
     (dict(q_out=None), EINVAL, "NULL"), (dict(k=None), EINVAL, "NULL"), (dict(q=0x1008), EINVAL, "16 bytes"),
     (dict(q_token=4104), EINVAL, "16 bytes"), (dict(out_head=264), EINVAL, "16 bytes"), (dict(qw=0x108), EINVAL, "16 bytes"),
-    (dict(kw=0x108), EINVAL, "16 bytes"), (dict(out_head=128), EINVAL, "overlap"), (dict(out_head=-240), EINVAL, "overlap")]
+    (dict(kw=0x108), EINVAL, "16 bytes"), (dict(out_head=128), EINVAL, "overlap"), (dict(out_head=-240), EINVAL, "overlap"),
+    (dict(out_token=0), EINVAL, "overlap"), (dict(out_token=240), EINVAL, "overlap")]
 
 
 @pytest.mark.parametrize("args,code,msg", SHARED + [(dict(k_out=None), EINVAL, "NULL"), (dict(k_out=0x4008), EINVAL, "16 bytes")])
@@ -130,9 +131,9 @@ def test_latent_attention_refuses(args, code, msg):
 
 def prompt(q=0x1000, q_token=16 * 384, q_head=384, k=0x2000, k_token=16 * 512, rk=0x3000, r_token=128, v=0x4000,
            v_token=16 * 512, type=0, heads=16, D=128, nnz=8, keys=40, qo=0x100, kv=0x100, batch=2, max_q=8, scale=0.1,
-           out=0x5000, o_token=16 * 256, space=None, size=0):
+           out=0x5000, o_token=16 * 256, o_head=256, space=None, size=0):
     return LIB.pace_kv_prompt_attention(q, q_token, q_head, k, k_token, 512, rk, r_token, v, v_token, 512, type, heads, D,
-                                        nnz, keys, qo, kv, batch, max_q, scale, 1, out, o_token, 256, None, space, size,
+                                        nnz, keys, qo, kv, batch, max_q, scale, 1, out, o_token, o_head, None, space, size,
                                         None, None)
 
 
@@ -146,6 +147,7 @@ def prompt(q=0x1000, q_token=16 * 384, q_head=384, k=0x2000, k_token=16 * 512, r
     (dict(out=0x5002), EINVAL, "16 bytes"), (dict(q_head=390), EINVAL, "16 bytes"),
     (dict(k_token=1 << 26), EINVAL, "2^26"), (dict(v_token=-8192), EINVAL, "2^26"), (dict(nnz=1 << 31), ERANGE, "2^30"),
     (dict(keys=1 << 31), ERANGE, "2^30"), (dict(nnz=1 << 26), ERANGE, "too many"),
+    (dict(o_token=0), EINVAL, "overlap"), (dict(o_token=240), EINVAL, "overlap"), (dict(o_head=128), EINVAL, "overlap"),
     (dict(heads=(1 << 20) + 1), ERANGE, "too many"), (dict(keys=60000), EINVAL, "workspace"),
     (dict(keys=60000, space=0x1000, size=64), EINVAL, "workspace"),
     (dict(keys=60000, space=0x1008, size=1 << 40), EINVAL, "workspace")])
