@@ -147,12 +147,16 @@ __device__ __forceinline__ uint32_t swap_of(uint32_t r) {
 
 // A workgroup takes 128 query rows of a head, 32 a wave, and passes over the keys they see,
 // 32 at a time: rows go from memory straight to LDS, into one of two buffers while the
-// other is read.  With 128 columns the buffers take 40 KiB, so that three
-// workgroups fit a CU and one's softmax lies under another's products.
+// other is read.  With 128 columns the buffers take 40 KiB, so that three workgroups fit a CU
+// and one's softmax may lie under another's products.
 //
-// Bound by what the three share: LDS is busy 62 % of the time, the matrix units 44, the
-// vector units 42 (MI355X, 8192 tokens of 32 heads: 693 us, 992 TFLOP/s).  Two workgroups
-// with 64 keys a step took 743 us of it.
+// Bound by the SIMDs' issue: of 1290 cycles that a wave's step takes of one, matrix
+// instructions are 640 and vector ones about 600, 256 of them exponentials; LDS is busy a
+// quarter of the time, without conflicts (MI355X, 4096 queries of 32 heads behind 4096 keys
+// in 481 us, 1071 TFLOP/s; 8192 alone in 631, 1090).  Every instruction less shows: lanes'
+// places in memory kept in registers were 6 %, a finite lowest maximum 3.  Two workgroups
+// with 64 keys a step took 743 us where three with 32 took 693.  Waves of long tiles at a
+// higher priority: no change.
 template <int DN, int TYPE>
 __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams p) {
   constexpr int kNS = DN / 32, kCT = DN / 16;
