@@ -642,6 +642,27 @@ int pace_kv_append_rope(const void* q, int64_t q_token_stride,
                         int64_t num_pages, int page_size, int32_t* err_count,
                         void* stream);
 
+/*
+ * The same into quantised pages of any size: pace_kv_append_rope, as the other
+ * calls on quantised pages, wants half a page to be a multiple of 16 bytes,
+ * which pages of few tokens and heads are not.
+ */
+int pace_kv_append_rope_packed(const void* q, int64_t q_token_stride,
+                               int64_t q_head_stride, int q_heads, void* q_out,
+                               int64_t q_out_token_stride,
+                               int64_t q_out_head_stride, const void* q_weight,
+                               const void* k, int64_t k_token_stride,
+                               int64_t k_head_stride, const void* k_weight,
+                               const void* v, int64_t v_token_stride,
+                               int64_t v_head_stride, int kv_heads,
+                               int elem_type, int head_dim, int64_t nnz,
+                               const int32_t* positions,
+                               const int64_t* slot_mapping, const float* table,
+                               int64_t table_rows, int rotary_dim,
+                               int interleaved, float eps, void* cache,
+                               int format, int64_t num_pages, int page_size,
+                               int32_t* err_count, void* stream);
+
 /* ------------------------------------------------------------------------ */
 /* Latent cache and attention                                                 */
 /* ------------------------------------------------------------------------ */

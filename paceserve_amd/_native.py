@@ -86,6 +86,10 @@ SIGNATURES = {
         c_int, [_VP, c_int64, c_int64, c_int, _VP, c_int64, c_int64, _VP, _VP, c_int64, c_int64, _VP, _VP, c_int64,
                 c_int64, c_int, c_int, c_int, c_int64, _VP, _VP, _VP, c_int64, c_int, c_int, c_float, _VP, c_int,
                 c_int64, c_int, _VP, _VP]),
+    "pace_kv_append_rope_packed": (
+        c_int, [_VP, c_int64, c_int64, c_int, _VP, c_int64, c_int64, _VP, _VP, c_int64, c_int64, _VP, _VP, c_int64,
+                c_int64, c_int, c_int, c_int, c_int64, _VP, _VP, _VP, c_int64, c_int, c_int, c_float, _VP, c_int,
+                c_int64, c_int, _VP, _VP]),
     "pace_kv_append_latent": (
         c_int, [_VP, c_int64, _VP, c_int64, _VP, c_int, c_int, c_int64, _VP, _VP, _VP, c_int64, c_int, c_float, _VP,
                 c_int64, c_int, _VP, _VP]),

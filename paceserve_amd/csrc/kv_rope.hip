@@ -263,17 +263,19 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeParams p) {
         put_vec(half + (element + eb) * 2, h < qk ? narrow<TYPE>(b) : rb);
       } else {
         // Blocks of 32 are four neighbouring lanes' runs: rotary and tail are multiples of 64.
+        // Half a page may be of any multiple of 34 or 66 bytes, so that runs lie at even bytes:
+        // packed stores, the same instructions as aligned ones.
         constexpr int kBits = mx_bits(FORMAT);
         const auto put_run = [&](const float* x, const u32x4& v, uint32_t e) {
           char* const data = half + (element + e) * kBits / 8;
           char* const scale = half + p.scale_at + (element + e) / kMxBlock;
           if (h < qk) {
             const Run<PACE_KV_FP32> r = float_run(x);
-            store_run<PACE_KV_FP32, FORMAT, false>(r, scale_byte<FORMAT>(block_amax<PACE_KV_FP32>(r)), data, scale);
+            store_run<PACE_KV_FP32, FORMAT, false, true>(r, scale_byte<FORMAT>(block_amax<PACE_KV_FP32>(r)), data, scale);
           } else {
             Run<TYPE> r;
             r.v[0] = v;
-            store_run<TYPE, FORMAT, false>(r, scale_byte<FORMAT>(block_amax<TYPE>(r)), data, scale);
+            store_run<TYPE, FORMAT, false, true>(r, scale_byte<FORMAT>(block_amax<TYPE>(r)), data, scale);
           }
         };
         put_run(a, ra, ea);
@@ -465,6 +467,57 @@ int check_dims(const char* call, int head_dim, int rotary_dim, int q_heads, int 
   return PACE_KV_OK;
 }
 
+// packed: half a page may be of any size.
+int append_rope(bool packed, const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads, void* q_out,
+                int64_t q_out_token_stride, int64_t q_out_head_stride, const void* q_weight, const void* k,
+                int64_t k_token_stride, int64_t k_head_stride, const void* k_weight, const void* v,
+                int64_t v_token_stride, int64_t v_head_stride, int kv_heads, int elem_type, int head_dim, int64_t nnz,
+                const int32_t* positions, const int64_t* slot_mapping, const float* table, int64_t table_rows,
+                int rotary_dim, int interleaved, float eps, void* cache, int format, int64_t num_pages, int page_size,
+                int32_t* err_count, void* stream) {
+  const char* const call = "append_rope";
+  PACE_KV_TRY(check_dims(call, head_dim, rotary_dim, q_heads, kv_heads));
+  PACE_KV_TRY(check_turn(call, elem_type, nnz, positions, table, table_rows, eps));
+  if (kv_heads == 0) return fail(PACE_KV_EINVAL, "%s: no KV heads", call);
+  if (format != PACE_KV_PLAIN && !is_mx_format(format)) return fail(PACE_KV_EINVAL, "%s: unknown format %d", call, format);
+  if (format != PACE_KV_PLAIN && (head_dim % 64 || rotary_dim % 64))
+    return fail(PACE_KV_EINVAL, "%s: a quantised cache takes head_dim and rotary_dim in multiples of 64", call);
+  if (num_pages < 0 || num_pages > INT32_MAX || page_size <= 0)
+    return fail(PACE_KV_EINVAL, "%s: bad number of pages or page size", call);
+  if (nnz == 0) return PACE_KV_OK;
+  if (!slot_mapping || (num_pages > 0 && !cache)) return fail(PACE_KV_EINVAL, "%s: NULL argument", call);
+  if ((reinterpret_cast<uintptr_t>(cache) & 15u) || (reinterpret_cast<uintptr_t>(slot_mapping) & 7u))
+    return fail(PACE_KV_EINVAL, "%s: the cache must be 16-byte aligned, slot_mapping 8-byte", call);
+  RopeParams p = {};
+  p.q = Rows{static_cast<const char*>(q), q_token_stride, q_head_stride, static_cast<char*>(q_out), q_out_token_stride,
+             q_out_head_stride, static_cast<const char*>(q_weight), static_cast<uint32_t>(q_heads)};
+  p.k = Rows{static_cast<const char*>(k), k_token_stride, k_head_stride, nullptr, 0, 0,
+             static_cast<const char*>(k_weight), static_cast<uint32_t>(kv_heads)};
+  p.v = Rows{static_cast<const char*>(v), v_token_stride, v_head_stride, nullptr, 0, 0, nullptr,
+             static_cast<uint32_t>(kv_heads)};
+  PACE_KV_TRY(check_rows(call, p.q, true, nnz, static_cast<uint32_t>(head_dim)));
+  PACE_KV_TRY(check_rows(call, p.k, false, nnz, static_cast<uint32_t>(head_dim)));
+  PACE_KV_TRY(check_rows(call, p.v, false, nnz, static_cast<uint32_t>(head_dim)));
+  const int64_t half = static_cast<int64_t>(page_size) * kv_heads * head_dim;
+  if (half >= int64_t(1) << 36) return fail(PACE_KV_ERANGE, "%s: pages of 2^36 elements or more", call);
+  p.half_bytes = format == PACE_KV_PLAIN ? half * 2 : mx_half_bytes(half, format);
+  if (!packed && p.half_bytes % 16)
+    return fail(PACE_KV_EINVAL, "%s: half a page must be a multiple of 16 bytes", call);
+  p.page_bytes = 2 * p.half_bytes;
+  p.scale_at = format == PACE_KV_PLAIN ? 0 : half * mx_bits(format) / 8;
+  p.positions = positions;
+  p.slots = slot_mapping;
+  p.table = table;
+  p.table_rows = table_rows;
+  p.cache = static_cast<char*>(cache);
+  p.err = err_count;
+  p.nnz = nnz;
+  p.num_slots = num_pages * page_size;
+  p.page_size = static_cast<uint32_t>(page_size);
+  p.eps = eps;
+  return launch_rope(p, elem_type, format, head_dim, rotary_dim, interleaved, static_cast<hipStream_t>(stream));
+}
+
 }  // namespace
 }  // namespace pace_kv
 
@@ -505,47 +558,26 @@ int pace_kv_append_rope(const void* q, int64_t q_token_stride, int64_t q_head_st
                         int64_t nnz, const int32_t* positions, const int64_t* slot_mapping, const float* table,
                         int64_t table_rows, int rotary_dim, int interleaved, float eps, void* cache, int format,
                         int64_t num_pages, int page_size, int32_t* err_count, void* stream) {
-  using namespace pace_kv;
-  const char* const call = "append_rope";
-  PACE_KV_TRY(check_dims(call, head_dim, rotary_dim, q_heads, kv_heads));
-  PACE_KV_TRY(check_turn(call, elem_type, nnz, positions, table, table_rows, eps));
-  if (kv_heads == 0) return fail(PACE_KV_EINVAL, "%s: no KV heads", call);
-  if (format != PACE_KV_PLAIN && !is_mx_format(format)) return fail(PACE_KV_EINVAL, "%s: unknown format %d", call, format);
-  if (format != PACE_KV_PLAIN && (head_dim % 64 || rotary_dim % 64))
-    return fail(PACE_KV_EINVAL, "%s: a quantised cache takes head_dim and rotary_dim in multiples of 64", call);
-  if (num_pages < 0 || num_pages > INT32_MAX || page_size <= 0)
-    return fail(PACE_KV_EINVAL, "%s: bad number of pages or page size", call);
-  if (nnz == 0) return PACE_KV_OK;
-  if (!slot_mapping || (num_pages > 0 && !cache)) return fail(PACE_KV_EINVAL, "%s: NULL argument", call);
-  if ((reinterpret_cast<uintptr_t>(cache) & 15u) || (reinterpret_cast<uintptr_t>(slot_mapping) & 7u))
-    return fail(PACE_KV_EINVAL, "%s: the cache must be 16-byte aligned, slot_mapping 8-byte", call);
-  RopeParams p = {};
-  p.q = Rows{static_cast<const char*>(q), q_token_stride, q_head_stride, static_cast<char*>(q_out), q_out_token_stride,
-             q_out_head_stride, static_cast<const char*>(q_weight), static_cast<uint32_t>(q_heads)};
-  p.k = Rows{static_cast<const char*>(k), k_token_stride, k_head_stride, nullptr, 0, 0,
-             static_cast<const char*>(k_weight), static_cast<uint32_t>(kv_heads)};
-  p.v = Rows{static_cast<const char*>(v), v_token_stride, v_head_stride, nullptr, 0, 0, nullptr,
-             static_cast<uint32_t>(kv_heads)};
-  PACE_KV_TRY(check_rows(call, p.q, true, nnz, static_cast<uint32_t>(head_dim)));
-  PACE_KV_TRY(check_rows(call, p.k, false, nnz, static_cast<uint32_t>(head_dim)));
-  PACE_KV_TRY(check_rows(call, p.v, false, nnz, static_cast<uint32_t>(head_dim)));
-  const int64_t half = static_cast<int64_t>(page_size) * kv_heads * head_dim;
-  if (half >= int64_t(1) << 36) return fail(PACE_KV_ERANGE, "%s: pages of 2^36 elements or more", call);
-  p.half_bytes = format == PACE_KV_PLAIN ? half * 2 : mx_half_bytes(half, format);
-  if (p.half_bytes % 16) return fail(PACE_KV_EINVAL, "%s: half a page must be a multiple of 16 bytes", call);
-  p.page_bytes = 2 * p.half_bytes;
-  p.scale_at = format == PACE_KV_PLAIN ? 0 : half * mx_bits(format) / 8;
-  p.positions = positions;
-  p.slots = slot_mapping;
-  p.table = table;
-  p.table_rows = table_rows;
-  p.cache = static_cast<char*>(cache);
-  p.err = err_count;
-  p.nnz = nnz;
-  p.num_slots = num_pages * page_size;
-  p.page_size = static_cast<uint32_t>(page_size);
-  p.eps = eps;
-  return launch_rope(p, elem_type, format, head_dim, rotary_dim, interleaved, static_cast<hipStream_t>(stream));
+  return pace_kv::append_rope(false, q, q_token_stride, q_head_stride, q_heads, q_out, q_out_token_stride,
+                              q_out_head_stride, q_weight, k, k_token_stride, k_head_stride, k_weight, v,
+                              v_token_stride, v_head_stride, kv_heads, elem_type, head_dim, nnz, positions,
+                              slot_mapping, table, table_rows, rotary_dim, interleaved, eps, cache, format, num_pages,
+                              page_size, err_count, stream);
+}
+
+int pace_kv_append_rope_packed(const void* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads, void* q_out,
+                               int64_t q_out_token_stride, int64_t q_out_head_stride, const void* q_weight,
+                               const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* k_weight,
+                               const void* v, int64_t v_token_stride, int64_t v_head_stride, int kv_heads,
+                               int elem_type, int head_dim, int64_t nnz, const int32_t* positions,
+                               const int64_t* slot_mapping, const float* table, int64_t table_rows, int rotary_dim,
+                               int interleaved, float eps, void* cache, int format, int64_t num_pages, int page_size,
+                               int32_t* err_count, void* stream) {
+  return pace_kv::append_rope(true, q, q_token_stride, q_head_stride, q_heads, q_out, q_out_token_stride,
+                              q_out_head_stride, q_weight, k, k_token_stride, k_head_stride, k_weight, v,
+                              v_token_stride, v_head_stride, kv_heads, elem_type, head_dim, nnz, positions,
+                              slot_mapping, table, table_rows, rotary_dim, interleaved, eps, cache, format, num_pages,
+                              page_size, err_count, stream);
 }
 
 int pace_kv_append_latent(const void* latent, int64_t latent_stride, const void* rope_key, int64_t rope_stride,

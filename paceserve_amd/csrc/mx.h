@@ -142,10 +142,16 @@ __device__ __forceinline__ uint32_t pair_down(uint32_t to, const Run<TYPE>& r, i
   }
 }
 
+// Where halves of pages lie at any even byte.
+typedef u32x2 packed_u32x2 __attribute__((aligned(2)));
+typedef uint32_t packed_u32 __attribute__((aligned(2)));
+
 // Stores a lane's run as elements at `data`, its place among the half page's
 // elements, and the block's scale byte at `scale` (from the block's first lane).
-template <int TYPE, int FORMAT, bool STREAM>
+// PACKED: `data` is even, and no more.
+template <int TYPE, int FORMAT, bool STREAM, bool PACKED = false>
 __device__ __forceinline__ void store_run(const Run<TYPE>& r, uint32_t byte, char* data, char* scale) {
+  static_assert(!STREAM || !PACKED);
   const float s = scale_of(byte);
   const uint32_t keep = byte == 255u ? 0u : ~0u;
   if constexpr (FORMAT == PACE_KV_MXFP8) {
@@ -154,14 +160,16 @@ __device__ __forceinline__ void store_run(const Run<TYPE>& r, uint32_t byte, cha
     q[0] = pair_down<TYPE, FORMAT, 1>(q[0], r, 1, s);
     q[1] = pair_down<TYPE, FORMAT, 0>(q[1], r, 2, s);
     q[1] = pair_down<TYPE, FORMAT, 1>(q[1], r, 3, s);
-    put<STREAM>(reinterpret_cast<u32x2*>(data), q & keep);
+    if constexpr (PACKED) *reinterpret_cast<packed_u32x2*>(data) = q & keep;
+    else put<STREAM>(reinterpret_cast<u32x2*>(data), q & keep);
   } else {
     uint32_t q = 0;
     q = pair_down<TYPE, FORMAT, 0>(q, r, 0, s);
     q = pair_down<TYPE, FORMAT, 1>(q, r, 1, s);
     q = pair_down<TYPE, FORMAT, 2>(q, r, 2, s);
     q = pair_down<TYPE, FORMAT, 3>(q, r, 3, s);
-    put<STREAM>(reinterpret_cast<uint32_t*>(data), q & keep);
+    if constexpr (PACKED) *reinterpret_cast<packed_u32*>(data) = q & keep;
+    else put<STREAM>(reinterpret_cast<uint32_t*>(data), q & keep);
   }
   if (threadIdx.x % 4 == 0) *reinterpret_cast<uint8_t*>(scale) = static_cast<uint8_t>(byte);
 }

@@ -19,6 +19,11 @@ the even one low) and then the scale bytes [page_size, H, D / 32] (e + 127);
 move, swap, the channel and KVMigrator take such pools as they are, and move
 half or a quarter of the bytes.
 
+Pages of few tokens and heads can come to halves that are no multiple of 16
+bytes (one token of one head of 128: 132 or 68).  rope.append_paged_kv_cache_rope
+writes them; the appends and conversions here and attention.paged_attention
+refuse them, and the calls that move pages those whose whole is none.
+
 Like everything in this package the calls enqueue on the current stream and
 return; tokens and pages with indices out of range are skipped and counted in
 `err`.

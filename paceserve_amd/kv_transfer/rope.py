@@ -161,8 +161,8 @@ def append_paged_kv_cache_rope(query: torch.Tensor, append_key: torch.Tensor, ap
     slot_mapping[i] = page * page_size + slot (int64, as tables.build_tables
     gives it); tokens of one call take distinct slots.  The cache is of the
     rows' type, [num_pages, 2, page_size, num_kv_heads, D], or quantised (mx;
-    D and rotary_dim then in multiples of 64): its elements are rounded once,
-    from the float32 results.
+    D and rotary_dim then in multiples of 64, pages of any size): its elements
+    are rounded once, from the float32 results.
 
     A token with slot -1 is padding: nothing of it is written.  One with another
     slot outside the cache, or a position outside the table, is counted in `err`
@@ -194,7 +194,9 @@ def append_paged_kv_cache_rope(query: torch.Tensor, append_key: torch.Tensor, ap
         out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
     else:
         _check_rows("out", out, query, query.shape[1])
-    _call(query.device, "pace_kv_append_rope", query.data_ptr(), *_strides(query), query.shape[1], out.data_ptr(),
+    # Few tokens of few heads: half a quantised page is no multiple of 16 bytes.
+    name = "pace_kv_append_rope" if fmt == _native.PLAIN or P * H * width % 16 == 0 else "pace_kv_append_rope_packed"
+    _call(query.device, name, query.data_ptr(), *_strides(query), query.shape[1], out.data_ptr(),
           *_strides(out), qw, append_key.data_ptr(), *_strides(append_key), kw, append_value.data_ptr(),
           *_strides(append_value), H, _native.ELEM_TYPES[query.dtype], D, query.shape[0], pos.data_ptr(),
           slots.data_ptr(), table.data_ptr(), rows, rotary, interleaved, eps, cache.data_ptr(), fmt, num_pages, P,

@@ -1,0 +1,122 @@
+"""norm_rotate, append_paged_kv_cache_rope and append_paged_latent_cache (HIP) at the
+ends of their ranges, against the 64-bit oracle: quantised pages of any size, rows
+whose squares leave float32's normal numbers, layouts of the outputs, and the sizes
+from which on a call takes another kernel."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx_oracle as mo
+from oracle import rope_oracle as ro
+from paceserve_amd.kv_transfer import mx, rope
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+EPS = 1e-6
+
+
+def f64(x):
+    return x.double().cpu().numpy()
+
+
+def sub_of(dtype):
+    return 2.0 ** -25 if dtype is FP16 else 0.0
+
+
+def rows(rng, shape, dtype, dev, gain=1.0):
+    return torch.from_numpy(gain * rng.standard_normal(shape) * np.exp(0.5 * rng.standard_normal(shape[-1]))).to(dtype).to(dev)
+
+
+def check_turned(got, x, weight, positions, table, interleaved=False, eps=EPS):
+    """Rows got [n, heads, D] of x at the positions."""
+    g, x, t = f64(got), f64(x), f64(table)
+    w = None if weight is None else f64(weight)
+    step, sub = torch.finfo(got.dtype).eps, sub_of(got.dtype)
+    for i, p in enumerate(positions):
+        y, size = ro.turned(x[i], w, eps, t[p], interleaved)
+        off, most = np.abs(g[i] - y), ro.bound(y, size, x.shape[-1], step, sub)
+        assert (off <= most).all(), f"token {i}: off by {np.max(off / most):.3g} of its bound"
+
+
+def scale_exponents(amax, fmt):
+    """Of blocks' largest magnitudes: the smallest exponents that bring them within the type."""
+    with np.errstate(divide="ignore"):
+        return np.clip(np.ceil(np.log2(amax / mo.TOP[fmt])), -117, 127)
+
+
+def check_quantised_keys(data, byte, x, weight, positions, table, interleaved, fmt):
+    """Element and scale bytes of keys x [n, heads, D].  The float32 result lies within the
+    bound e of y: the scale is that of a block's largest magnitude within e, and rounding
+    once adds half a step of the element, at most 2^-4 (2^-2) of the value, or half the
+    smallest step."""
+    x, t, w = f64(x), f64(table), None if weight is None else f64(weight)
+    got = mo.values(data, byte, fmt)
+    low, u = (2.0 ** -10, 2.0 ** -4) if fmt == "mxfp8" else (2.0 ** -2, 2.0 ** -2)
+    for i, p in enumerate(positions):
+        y, size = ro.turned(x[i], w, EPS, t[p], interleaved)
+        e = ro.bound(y, size, x.shape[-1], 0.0, 0.0)
+        blocks = y.shape[0], -1, mo.BLOCK
+        least, most = ((np.abs(y) + s * e).reshape(blocks).max(-1) for s in (-1, 1))
+        exponent = byte[i].astype(int) - 127
+        assert (exponent >= scale_exponents(np.maximum(least, 0), fmt)).all()
+        assert (exponent <= scale_exponents(most, fmt)).all()
+        scale = np.repeat(np.exp2(exponent.astype(np.float64)), mo.BLOCK, -1)
+        assert (np.abs(got[i] - y) <= np.maximum(u * (np.abs(y) + e), low * scale) + e).all(), f"token {i}"
+
+
+def append_and_check(gpu, n, Hq, H, D, r, P, dtype, fmt, interleaved, norm=True, tokens=None, seed=0):
+    """An append into a cache (fmt None: of the rows' type) whose other slots hold a
+    pattern; `tokens`: those looked at (all by default)."""
+    rng = np.random.default_rng(seed + n + D)
+    pages = -(-n // P) + 3
+    table = rope.rotary_table(300, r, device=gpu)
+    pos, slots = rng.integers(0, 300, n), rng.permutation(pages * P)[:n]
+    slots[rng.integers(0, n, n // 50)] = -1                            # some of them padding
+    pos_t = torch.tensor(pos, dtype=torch.int32, device=gpu)
+    slot_t = torch.tensor(slots, dtype=torch.int64, device=gpu)
+    q, k, v = rows(rng, (n, Hq + 2 * H, D), dtype, gpu).split([Hq, H, H], 1)
+    w = rows(rng, (D,), dtype, gpu) if norm else None
+    if fmt is None:
+        cache = torch.full((pages, 2, P, H, D), 5.0, dtype=dtype, device=gpu)
+    else:
+        cache = torch.full((pages, 2, P, H, mx.row_width(D, fmt)), 0x35, dtype=torch.uint8, device=gpu)
+    was, err = cache.clone(), torch.zeros(1, dtype=torch.int32, device=gpu)
+    out = torch.full_like(q, 7.0)
+    rope.append_paged_kv_cache_rope(q, k, v, pos_t, slot_t, cache, table, w, w, interleaved=interleaved, out=out, err=err)
+    torch.cuda.synchronize()
+    assert err.item() == 0
+    pad = torch.from_numpy(slots < 0).to(gpu)
+    assert (out[pad] == 7).all()
+    live = np.flatnonzero(slots >= 0)
+    page, at = torch.from_numpy(slots[live] // P).to(gpu), torch.from_numpy(slots[live] % P).to(gpu)
+    written = torch.zeros((pages, P), dtype=torch.bool, device=gpu)
+    written[page, at] = True
+    look = live if tokens is None else np.unique(np.concatenate([live[:3], live[-3:], rng.choice(live, tokens)]))
+    li = torch.from_numpy(look).to(gpu)
+    lp, la = torch.from_numpy(slots[look] // P).to(gpu), torch.from_numpy(slots[look] % P).to(gpu)
+    check_turned(out[li], q[li], w, pos[look], table, interleaved)
+    if fmt is None:
+        check_turned(cache[lp, 0, la], k[li], w, pos[look], table, interleaved)
+        assert torch.equal(cache[page, 1, at], v[torch.from_numpy(live).to(gpu)])
+        keep = ~written[:, None, :].expand(-1, 2, -1)
+        assert (cache[keep] == 5).all()
+        return
+    data, byte = mx.elements_and_scales(cache, D)
+    for new, old in zip((data, byte), mx.elements_and_scales(was, D)):
+        keep = ~written[:, None, :].expand(-1, 2, -1)
+        assert torch.equal(new[keep], old[keep])
+    codes, c = mo.quantize(f64(v[li]), fmt)                           # values as the quantising append does it
+    assert np.array_equal(data[lp, 1, la].cpu().numpy(), mo.pack(codes, fmt))
+    assert np.array_equal(byte[lp, 1, la].cpu().numpy(), c)
+    check_quantised_keys(data[lp, 0, la].cpu().numpy(), byte[lp, 0, la].cpu().numpy(), k[li], w, pos[look], table,
+                         interleaved, fmt)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("fmt", ["mxfp8", "mxfp4"])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("H,D,r,P", [(1, 64, 64, 1), (2, 64, 64, 1), (3, 64, 64, 1), (1, 128, 128, 1), (2, 128, 64, 1),
+                                     (3, 128, 128, 1), (1, 192, 64, 1), (3, 256, 256, 1), (1, 64, 64, 3), (1, 64, 64, 7)])
+def test_quantised_pages_of_any_size(gpu, H, D, r, P, dtype, fmt, interleaved):
+    """Halves of 34 and 66 bytes and their multiples, of which few are multiples of 16."""
+    append_and_check(gpu, 45, 2 * H, H, D, r, P, dtype, fmt, interleaved)
