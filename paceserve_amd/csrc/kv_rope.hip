@@ -158,6 +158,34 @@ __device__ __forceinline__ float sum_of_group(float x, uint32_t lanes) {
   return x;
 }
 
+// Sum of the squares of a lane's runs.
+template <class... R>
+__device__ __forceinline__ float squares(const R&... runs) {
+  float sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum += (... + (runs[j] * runs[j]));
+  return sum;
+}
+
+// 1 / sqrt(mean(x^2) + eps) of the rows whose runs lie with groups of `lanes` lanes.  The root's
+// instruction takes normal numbers alone, and squares of numbers below 2^-63 are none.  Where eps
+// would not hide those (below kLeastEps, which is the same for all lanes), rows whose mean square
+// does not either are scaled by 2^100 first, in place: what is returned is for the scaled runs.
+constexpr float kLeastEps = 0x1p-90f;
+
+template <class... R>
+__device__ __forceinline__ float inverse_root(uint32_t lanes, float inv_dim, float eps, R&... runs) {
+  float sum = sum_of_group(squares(runs...), lanes);
+  if (eps < kLeastEps) {
+    const float up = sum * inv_dim + eps < kLeastEps ? 0x1p100f : 1.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) (..., (runs[j] *= up));
+    sum = sum_of_group(squares(runs...), lanes);
+    eps = eps * up * up;
+  }
+  return __builtin_amdgcn_rsqf(sum * inv_dim + eps);
+}
+
 // Written through the L2 at device scope.  The asm carries the wait states that a store of
 // more than 64 bits needs before its data registers change.
 __device__ __forceinline__ void put_vec(char* to, u32x4 v) {
@@ -232,11 +260,7 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeParams p) {
       widen<TYPE>(ra, a);
       widen<TYPE>(rb, b);
       if (rows.weight != nullptr) {
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum += a[j] * a[j] + b[j] * b[j];
-        sum = sum_of_group(sum, group);
-        const float inv = __builtin_amdgcn_rsqf(sum * p.inv_dim + p.eps);
+        const float inv = inverse_root(group, p.inv_dim, p.eps, a, b);
         if (active) {
           float wa[8], wb[8];
           widen<TYPE>(*reinterpret_cast<const u32x4*>(rows.weight + ea * 2), wa);
@@ -356,12 +380,9 @@ __global__ __launch_bounds__(kThreads) void latent_rows_kernel(const LatentParam
 #pragma unroll
   for (uint32_t k = 0; k < ROWS; ++k) {
     if (p.weight != nullptr) {
-      float x[8], sum = 0.f;
+      float x[8];
       widen<TYPE>(raw[k], x);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum += x[j] * x[j];
-      sum = sum_of_group(sum, kLanes);
-      const float inv = __builtin_amdgcn_rsqf(sum * (1.f / L) + p.eps);
+      const float inv = inverse_root(kLanes, 1.f / L, p.eps, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = x[j] * inv * w[j];
       raw[k] = narrow<TYPE>(x);

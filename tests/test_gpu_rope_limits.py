@@ -8,7 +8,7 @@ import torch
 
 from oracle import mx_oracle as mo
 from oracle import rope_oracle as ro
-from paceserve_amd.kv_transfer import mx, rope
+from paceserve_amd.kv_transfer import latent, mx, rope
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -120,3 +120,35 @@ def append_and_check(gpu, n, Hq, H, D, r, P, dtype, fmt, interleaved, norm=True,
 def test_quantised_pages_of_any_size(gpu, H, D, r, P, dtype, fmt, interleaved):
     """Halves of 34 and 66 bytes and their multiples, of which few are multiples of 16."""
     append_and_check(gpu, 45, 2 * H, H, D, r, P, dtype, fmt, interleaved)
+
+
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -133, 2.0 ** -100])
+@pytest.mark.parametrize("power", [-20, -45, -62, -66, -70, -90, -126, -131])
+def test_rows_whose_squares_are_below_the_normal_numbers(gpu, power, eps):
+    """Rows of 2^power: their mean square is a subnormal number of float32 or less, and counts
+    where eps does not hide it.  Beside them rows of ordinary numbers."""
+    rng = np.random.default_rng(-power)
+    table = rope.rotary_table(8, 64, device=gpu)
+    pos = np.array([1, 2, 7])
+    at = torch.tensor(pos, dtype=torch.int32, device=gpu)
+    q, k = rows(rng, (3, 5, 128), torch.float64, gpu), rows(rng, (3, 2, 64), torch.float64, gpu)
+    q[1] *= 2.0 ** power
+    q[2, 3] *= 2.0 ** power
+    q, k = q.to(BF16), k.to(BF16)
+    w, w64 = rows(rng, (128,), BF16, gpu), rows(rng, (64,), BF16, gpu)
+    got, _ = rope.norm_rotate(q, None, at, table, w, eps=eps)
+    check_turned(got, q, w, pos, table, eps=eps)
+    # into a latent cache
+    x = rows(rng, (3, 256), torch.float64, gpu)
+    x[1:] *= 2.0 ** power
+    x = x.to(BF16)
+    cache, w = latent.empty_cache(1, 4, 256, device=gpu), rows(rng, (256,), BF16, gpu)
+    latent.append_paged_latent_cache(x, k[:, 0], at, torch.arange(3, device=gpu), cache, table, w, eps=eps)
+    y, g = f64(x), f64(cache[0, :3, :256])
+    y = y / np.sqrt((y * y).mean(-1, keepdims=True) + eps) * f64(w)
+    assert (np.abs(g - y) <= ro.bound(y, np.abs(y), 256, torch.finfo(BF16).eps, 0.0)).all()
+    # and keys on their way into pages
+    kv = torch.zeros((1, 2, 16, 2, 64), dtype=BF16, device=gpu)
+    small = (k.double() * 2.0 ** power).to(BF16)
+    rope.append_paged_kv_cache_rope(small, small, k, at, torch.arange(3, device=gpu), kv, table, None, w64, eps=eps)
+    check_turned(kv[0, 0, :3], small, w64, pos, table, eps=eps)
