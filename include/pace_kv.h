@@ -600,8 +600,9 @@ int pace_kv_build_tables(const int32_t* page_table, int64_t table_stride,
  * (a, b) = (j, j + rotary_dim / 2), or (2 j, 2 j + 1) if interleaved, become
  * (a c_j - b s_j, b c_j + a s_j), j < rotary_dim / 2.  float32, rounded once.
  * head_dim (up to 1024) and rotary_dim are multiples of 16.  Outputs may be the
- * inputs.  A token whose position is outside the table is not written, and
- * counted in err_count.
+ * inputs, each row its own; but for that they share no memory with them or with
+ * each other, and rows of one output that overlap are refused.  A token whose
+ * position is outside the table is not written, and counted in err_count.
  */
 int pace_kv_norm_rotate(const void* q, int64_t q_token_stride,
                         int64_t q_head_stride, int q_heads, void* q_out,
@@ -724,8 +725,8 @@ int pace_kv_latent_attention(const void* q, int64_t q_stride_bytes,
  * that is skipped (queries outside [0, nnz), more than max_q_len, or past the
  * row tiles of nnz rows where offsets overlap) or whose keys are cut to
  * [0, num_keys).  Token strides of keys, rotated parts and values lie in
- * [0, 2^26), and output rows do not overlap.  The keys of few rows are cut up
- * by the sizes here alone; workspace as in pace_kv_attention.
+ * [0, 2^26); output rows that overlap are refused.  The keys of few rows are cut
+ * up by the sizes here alone; workspace as in pace_kv_attention.
  */
 int pace_kv_prompt_attention_workspace(int64_t nnz, int64_t num_keys,
                                        int batch_size, int num_heads,

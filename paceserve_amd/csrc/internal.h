@@ -37,6 +37,20 @@ inline FastDiv fast_div(uint32_t divisor) {
                  log2_up > 0 ? 1u : 0u, log2_up > 0 ? log2_up - 1 : 0u};
 }
 
+// Whether rows of `bytes` at i * a + j * b, i < n, j < m, overlap: two whose indexes differ by
+// di and dj do where |di * a + dj * b| < bytes.  Signs do not matter, as dj may have either.
+inline bool rows_overlap(int64_t n, int64_t a, int64_t m, int64_t b, int64_t bytes) {
+  using wide = __int128;
+  const wide x = a < 0 ? -static_cast<wide>(a) : a, y = b < 0 ? -static_cast<wide>(b) : b;
+  if ((n > 1 && x < bytes) || (m > 1 && y < bytes)) return true;
+  if (n <= 1 || m <= 1 || (m - 1) * y + bytes <= x || (n - 1) * x + bytes <= y) return false;
+  for (wide dj = 1; dj < m && dj * y - (n - 1) * x < bytes; ++dj) {
+    const wide di = dj * y / x;
+    if ((di < n && dj * y - di * x < bytes) || (di + 1 < n && (di + 1) * x - dj * y < bytes)) return true;
+  }
+  return false;
+}
+
 #ifdef __HIP__
 __device__ __forceinline__ uint32_t over(const FastDiv& d, uint32_t n) {
   const uint32_t q = __umulhi(d.mul, n);

@@ -9,7 +9,6 @@
 // kv_len - q_len + i.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "latent.h"
 
@@ -623,8 +622,7 @@ int pace_kv_prompt_attention(const void* q, int64_t q_token_stride, int64_t q_he
        static_cast<uintptr_t>(q_token_stride | q_head_stride | k_token_stride | k_head_stride | rope_token_stride |
                               v_token_stride | v_head_stride | out_token_stride | out_head_stride)) & 15u)
     return fail(PACE_KV_EINVAL, "prompt attention: rows and strides must be multiples of 16 bytes");
-  const auto overlaps = [&](int64_t count, int64_t stride) { return count > 1 && std::abs(stride) < head_dim * 2; };
-  if (overlaps(nnz, out_token_stride) || overlaps(num_heads, out_head_stride))
+  if (rows_overlap(nnz, out_token_stride, num_heads, out_head_stride, int64_t(2) * head_dim))
     return fail(PACE_KV_EINVAL, "prompt attention: output rows overlap");
   const int64_t longest = std::max({k_token_stride, rope_token_stride, v_token_stride});
   if (longest >= int64_t(1) << 26 || std::min({k_token_stride, rope_token_stride, v_token_stride}) < 0)

@@ -16,7 +16,6 @@
 // against 32 of its rows: a lane loads them once and goes on over the token's heads.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 #include <type_traits>
 
 #include "mx.h"
@@ -433,8 +432,7 @@ int check_rows(const char* call, const Rows& r, bool writes, int64_t nnz, uint32
                    reinterpret_cast<uintptr_t>(r.weight);
   if (writes) bits |= reinterpret_cast<uintptr_t>(r.out) | static_cast<uintptr_t>(r.out_token | r.out_head);
   if (bits & 15u) return fail(PACE_KV_EINVAL, "%s: rows, weights and strides must be multiples of 16 bytes", call);
-  const auto overlaps = [&](int64_t count, int64_t stride) { return count > 1 && std::abs(stride) < int64_t(2) * head_dim; };
-  if (writes && (overlaps(nnz, r.out_token) || overlaps(r.heads, r.out_head)))
+  if (writes && rows_overlap(nnz, r.out_token, r.heads, r.out_head, int64_t(2) * head_dim))
     return fail(PACE_KV_EINVAL, "%s: output rows overlap", call);
   return PACE_KV_OK;
 }

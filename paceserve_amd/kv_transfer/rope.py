@@ -116,7 +116,7 @@ def norm_rotate(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Ten
 
     D and rotary_dim are multiples of 16; rows may be strided slices of a
     projection, each head 16-byte aligned.  out_q and out_k may be q and k
-    themselves.  A token whose position is outside the table is counted in `err`
+    themselves; otherwise they share no memory with them.  A token whose position is outside the table is counted in `err`
     and its rows are not written.  Squares are float32 sums: rows past 2^64
     normalise to zeros.  There is no backward pass."""
     _refuse_gradients("norm_rotate", q, k, q_weight, k_weight)

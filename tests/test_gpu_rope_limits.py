@@ -152,3 +152,23 @@ def test_rows_whose_squares_are_below_the_normal_numbers(gpu, power, eps):
     small = (k.double() * 2.0 ** power).to(BF16)
     rope.append_paged_kv_cache_rope(small, small, k, at, torch.arange(3, device=gpu), kv, table, None, w64, eps=eps)
     check_turned(kv[0, 0, :3], small, w64, pos, table, eps=eps)
+
+
+def test_outputs_in_any_layout_whose_rows_are_apart(gpu):
+    """Heads before tokens, rows between other rows, tokens and heads whose rows alternate."""
+    rng = np.random.default_rng(3)
+    n, H, D = 6, 4, 64
+    table = rope.rotary_table(20, 64, device=gpu)
+    pos = rng.integers(0, 20, n)
+    at = torch.tensor(pos, dtype=torch.int32, device=gpu)
+    q = rows(rng, (n, H, D), BF16, gpu)
+    want, _ = rope.norm_rotate(q, None, at, table)
+    room = torch.zeros(4096, dtype=BF16, device=gpu)
+    for strides in ((64, n * 64, 1), (512, 128, 1), (128, 1024, 1), (64 * 8, 64, 1), (64 * 5, 64 * 2, 1)):
+        room.zero_()
+        got, _ = rope.norm_rotate(q, None, at, table, out_q=room.as_strided((n, H, D), strides))
+        assert torch.equal(got, want)
+        assert (room != 0).sum() == (want != 0).sum()
+    for strides in ((64, 64, 1), (64 * 3, 64, 1), (64 * 2, 64 * 3, 1), (96, 64, 1), (64, 96, 1), (64 * 5 - 32, 64 * 2, 1)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            rope.norm_rotate(q, None, at, table, out_q=room.as_strided((n, H, D), strides))

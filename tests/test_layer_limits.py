@@ -29,3 +29,27 @@ def append_packed(q=0x1000, q_token=4096, q_head=256, heads=8, q_out=0x2000, out
 def test_packed_pages_refuse_what_others_do(args, code, msg):
     refused(append_packed(**args), args, code, msg)
     assert append_packed(nnz=0) == 0
+
+
+def turn(q_token=4096, heads=8, out_token=4096, out_head=256, k_out_token=1024, k_out_head=256, D=128, nnz=3, r=128):
+    return LIB.pace_kv_norm_rotate(0x1000, q_token, 256, heads, 0x2000, out_token, out_head, None, 0x3000, 1024, 256, 2, 0x4000,
+                                   k_out_token, k_out_head, None, 0, D, nnz, 0x100, 0x100, 9, r, 0, 1e-6, None, None)
+
+
+def prompt(o_token=16 * 256, o_head=256, heads=16, nnz=8):
+    return LIB.pace_kv_prompt_attention(0x1000, 16 * 384, 384, 0x2000, 16 * 512, 512, 0x3000, 128, 0x4000, 16 * 512, 512, 0,
+                                        heads, 128, nnz, 40, 0x100, 0x100, 2, 8, 0.1, 1, 0x5000, o_token, o_head, None, None, 0,
+                                        None, None)
+
+
+@pytest.mark.parametrize("token,head", [
+    (256, 256), (256 * 7, 256), (-256, 256), (256, -256), (512, 768), (768, 512), (256 * 8 - 16, 256), (256, 256 * 3 - 16),
+    (384, 256), (256, 384), (1 << 62, 1 << 62), (256 * 5 - 16, 512)])
+def test_rows_of_one_token_and_another_that_overlap(token, head):
+    """Each of the strides alone keeps rows of 256 bytes apart, both together do not."""
+    args = dict(token=token, head=head)
+    refused(turn(out_token=token, out_head=head, nnz=9), args, EINVAL, "overlap")
+    refused(append_packed(out_token=token, out_head=head, nnz=9), args, EINVAL, "overlap")
+    refused(prompt(o_token=token, o_head=head, nnz=9), args, EINVAL, "overlap")
+    if token == head:
+        refused(turn(k_out_token=token, k_out_head=head), args, EINVAL, "overlap")
