@@ -25,7 +25,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int64_t kMaxGroupsPerLaunch = int64_t(1) << 24;
+// Workgroups of a launch, whose threads are counted in 32 bits.
+constexpr int64_t kMostGroups = int64_t(1) << 24;
 // Rows of more bytes than this are loaded nontemporally: what a projection has just written
 // is still in the memory-side cache where it is smaller.  MI355X, 40 heads of 128: 40 MiB
 // 17.2 us plain, 18.6 so, 160 MiB 71 and 61.
@@ -446,6 +447,8 @@ int check_turn(const char* call, int elem_type, int64_t nnz, const int32_t* posi
   if (nnz > 0 && (!positions || (table_rows > 0 && !table))) return fail(PACE_KV_EINVAL, "%s: NULL argument", call);
   if (reinterpret_cast<uintptr_t>(table) & 15u)
     return fail(PACE_KV_EINVAL, "%s: the table must be 16-byte aligned", call);
+  // More than any launch takes; below, products of the number with heads and sizes fit 64 bits.
+  if (nnz > INT32_MAX) return fail(PACE_KV_ERANGE, "%s: too many tokens for one call", call);
   return PACE_KV_OK;
 }
 
@@ -466,7 +469,7 @@ int launch_rope(RopeParams& p, int elem_type, int format, int head_dim, int rota
   p.part_heads = per * turn;
   p.parts = (heads + p.part_heads - 1) / p.part_heads;
   const int64_t groups = (p.nnz * p.parts + kWaves - 1) / kWaves;
-  if (groups > kMaxGroupsPerLaunch) return fail(PACE_KV_ERANGE, "rope: too many tokens for one call");
+  if (groups >= kMostGroups) return fail(PACE_KV_ERANGE, "rope: too many tokens for one call");
   void* args[] = {&p};
   p.by_parts = fast_div(p.parts);
   p.by_page = fast_div(p.page_size);
@@ -619,7 +622,7 @@ int pace_kv_append_latent(const void* latent, int64_t latent_stride, const void*
     return fail(PACE_KV_EINVAL, "%s: rows, strides, weight and cache must be multiples of 16 bytes, slot_mapping of 8", call);
   const bool many = nnz >= kManyRows;
   const int64_t tokens = kThreads / (latent_dim / 8) * (many ? 2 : 1), groups = (nnz + tokens - 1) / tokens;
-  if (groups > kMaxGroupsPerLaunch) return fail(PACE_KV_ERANGE, "%s: too many tokens for one call", call);
+  if (groups >= kMostGroups) return fail(PACE_KV_ERANGE, "%s: too many tokens for one call", call);
   LatentParams p = {};
   p.latent = static_cast<const char*>(latent);
   p.rope_key = static_cast<const char*>(rope_key);

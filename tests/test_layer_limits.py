@@ -53,3 +53,18 @@ def test_rows_of_one_token_and_another_that_overlap(token, head):
     refused(prompt(o_token=token, o_head=head, nnz=9), args, EINVAL, "overlap")
     if token == head:
         refused(turn(k_out_token=token, k_out_head=head), args, EINVAL, "overlap")
+
+
+def append_latent(nnz, L=512):
+    return LIB.pace_kv_append_latent(0x1000, 1152, 0x2000, 1152, None, 0, L, nnz, 0x100, 0x100, 0x100, 9, 0, 1e-6, 0x5000, 4,
+                                     16, None, None)
+
+
+@pytest.mark.parametrize("nnz", [1 << 26, (1 << 26) - 3, 1 << 31, 1 << 40, (1 << 63) - 1])
+def test_launches_of_two_to_the_32_threads(nnz):
+    """Threads of a launch are counted in 32 bits: 2^24 workgroups of 256 are one too many."""
+    refused(turn(nnz=nnz), nnz, ERANGE, "too many tokens")
+    refused(append_packed(nnz=nnz), nnz, ERANGE, "too many tokens")
+    # eight rows of 512 columns a workgroup, sixteen of 256
+    for L, rows in ((512, 8), (256, 16)):
+        refused(append_latent(min(nnz * rows // 4, (1 << 63) - 1), L), nnz, ERANGE, "too many tokens")
