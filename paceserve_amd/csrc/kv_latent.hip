@@ -265,7 +265,7 @@ __global__ __launch_bounds__(kThreads, 2) void latent_kernel(const AttnParams p)
     }
   };
   // Weights of those tokens, packed by twos as they lie in s; raises the maximum where a
-  // score passes it by kSlack, for which shrink is the factor of what was summed before.
+  // score passes it, for which shrink is the factor of what was summed before.
   u32x4 pf[RW];
   float shrink[RW];
   uint32_t raised = 0;                                   // tiles whose maximum was raised
@@ -293,10 +293,10 @@ __global__ __launch_bounds__(kThreads, 2) void latent_kernel(const AttnParams p)
       top = max3_of(top, s[a][1][1], s[a][1][2]);
       top = scaled(max3_of(top, s[a][1][3], s[a][1][3]), per_score);
       shrink[a] = 1.f;
-      if (__ballot(top > m[a] + kSlack<TYPE>) != 0) {
+      if (__ballot(top > m[a]) != 0) {
         raised |= 1u << a;
         top = across_groups(top, max_of);
-        const float next = top > m[a] + kSlack<TYPE> ? top : m[a];
+        const float next = top > m[a] ? top : m[a];
         shrink[a] = exp2_of(m[a] - next);
         m[a] = next;
         l[a] *= shrink[a];

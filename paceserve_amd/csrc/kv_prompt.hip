@@ -316,9 +316,9 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
       top = max3_of(top, s[a][0][3], s[a][1][0]);
       top = max3_of(top, s[a][1][1], s[a][1][2]);
       top = scaled(max3_of(top, s[a][1][3], s[a][1][3]), per_score);
-      if (__ballot(top > m[a] + kSlack<TYPE>) != 0) {
+      if (__ballot(top > m[a]) != 0) {
         top = across_groups(top, max_of);
-        const float next = top > m[a] + kSlack<TYPE> ? top : m[a];
+        const float next = top > m[a] ? top : m[a];
         const float shrink = exp2_of(m[a] - next);
         m[a] = next;
         l[a] *= shrink;

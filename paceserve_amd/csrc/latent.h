@@ -19,20 +19,20 @@ __device__ __forceinline__ float unfused(float a, float b) {
   return a - b;
 }
 
-// Log2 of the least by which a score has to pass the running maximum before that is raised,
-// which costs a product of every sum.  (MI355X: with none, so that the maximum is exact,
-// calls of 64 rows or more and prompts take 4 to 7 % longer.)  The largest weight is then
-// rounded like the others: in bfloat16 outputs are off by 0.0019 to 0.0023 of the values,
-// where their own rounding makes 0.0017.  float16 has no room for it.
-template <int TYPE>
-constexpr float kSlack = TYPE == PACE_KV_FP16 ? 0.f : 4.f;
+// Weights are rounded to the rows' type for their product, which takes nothing wider, and sums
+// take them unrounded (attention.h).  The running maximum is exact, so that the largest weight is
+// a power of two and not rounded: outputs are off by 0.0018 to 0.0019 of the values against 64
+// bits (bfloat16, 2000 to 4096 tokens), of which their own rounding is 0.0016.  (MI355X: raising
+// it only where a score passes it by 2^4 in weight saves a product of every sum, 4 to 8 % of
+// prompts and of calls of 64 rows and more, but outputs were off by 0.0019 to 0.0021, and where
+// one token stands out by up to twice as much.)
 
 // The maximum of no scores: finite, so that differences from it are numbers.
 constexpr float kLowest = -0x1.fffffep127f;
 
 // log2 of the weight of a score that equals the maximum.  In float16 the largest weights are
 // 2^15, which leaves those down to 2^-29 of the largest their 2^-11.  bfloat16 has float32's
-// exponents: 2^-24, so that up to 2^20 values of the largest exponent have a finite sum.
+// exponents: 2^-24, so that up to 2^24 values of the largest exponent have a finite sum.
 template <int TYPE>
 constexpr float kUnit = TYPE == PACE_KV_FP16 ? 15.f : -24.f;
 
