@@ -266,10 +266,10 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
     for (int d = 0; d < kCT; ++d) acc[a][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // Scores of 32 keys from row `key` on: lane: row n of each tile, keys 16 t + 4 g + e.
+  // Scores of a buffer's keys: lane: row n of each tile, keys 16 t + 4 g + e.
   f32x4 s[kRT][2];
   const uint32_t key_at = n * kRow + (g ^ swap_of<DN>(n)) * 16, rope_at = kRopeAt + n * kRopeRow + (g ^ swap_of<kRope>(n)) * 16;
-  const auto score = [&](uint32_t from, uint32_t first) {
+  const auto score = [&](uint32_t from) {
     const uint32_t key = opaque(key_at) + from, rope = opaque(rope_at) + from;
 #pragma unroll
     for (int a = 0; a < kRT; ++a)
@@ -277,8 +277,7 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
       for (int t = 0; t < 2; ++t) s[a][t] = f32x4{0.f, 0.f, 0.f, 0.f};
     const auto read = [&](int i) {
       const int k = i / 2, t = i % 2;
-      return lds_get<u32x4>(k < kNS ? (key ^ (k * 64)) + (first + t * 16) * kRow
-                                    : (rope ^ ((k - kNS) * 64)) + (first + t * 16) * kRopeRow);
+      return lds_get<u32x4>(k < kNS ? (key ^ (k * 64)) + t * 16 * kRow : (rope ^ ((k - kNS) * 64)) + t * 16 * kRopeRow);
     };
     // Reads stay two before their products (8192 tokens of 32 heads 640 us to 631; four before,
     // registers spill).
@@ -297,7 +296,7 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
   };
   // Weights of those keys, the first of which is t0, packed by twos as they lie in s.
   u32x4 pf[kRT];
-  const auto weigh = [&](auto full, int32_t t0) {
+  const auto weigh = [&](auto full) {
     if constexpr (!decltype(full)::value) {
 #pragma unroll
       for (int a = 0; a < kRT; ++a) {
@@ -354,10 +353,10 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
   // and the same behind 16.
   const uint32_t v_row = 4 * g + n / 4;
   const uint32_t v_at = kValueAt + v_row * kRow + (n % 4 / 2 ^ swap_of<DN>(v_row)) * 16 + n % 2 * 8;
-  const auto gather = [&](uint32_t from, uint32_t first) {
+  const auto gather = [&](uint32_t from) {
     const uint32_t v = opaque(v_at) + from;
     const auto read = [&](int d) {
-      const uint32_t x = (v ^ (d * 32)) + first * kRow;
+      const uint32_t x = v ^ (d * 32);
       const u32x2 lo = lds_transposed(x), hi = lds_transposed(x + 16 * kRow);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
@@ -405,13 +404,11 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
       clean(now);
       lds_barrier();
     }
-#pragma unroll
-    for (uint32_t h = 0; h < kTile; h += 32) {
-      if constexpr (!decltype(full)::value)
-        if (t0 + static_cast<int32_t>(h) >= seen_by(wave_row0 + 16 * kRT - 1)) break;  // no row of the wave sees any
-      score(now, h);
-      weigh(full, t0 + static_cast<int32_t>(h));
-      gather(now, h);
+    // Steps of which no row of the wave sees any are passed over.
+    if (decltype(full)::value || t0 < seen_by(wave_row0 + 16 * kRT - 1)) {
+      score(now);
+      weigh(full);
+      gather(now);
     }
     const uint32_t x = now;
     now = other;
@@ -450,8 +447,8 @@ __global__ __launch_bounds__(kThreads, 3) void prompt_kernel(const PromptParams 
     if (g == 0 && p.lse != nullptr) p.lse[static_cast<int64_t>(r.q0 + row) * p.heads + head] = log_total<TYPE>(m[a], l[a]);
   }
   if (t_masked >= t_end) return;
-  // What any wave took out reaches the rows that see it.  (LDS is full: two workgroups' buffers
-  // take all of a CU's.)
+  // What any wave took out reaches the rows that see it.  The buffers, which nobody reads any
+  // more, hold who found something.
   __syncthreads();
   const bool found = __ballot(odd) != 0;
   if (lane == 0) lds_put(lds_offset(lds) + w * 4, found ? 1u : 0u);

@@ -198,7 +198,7 @@ __device__ __forceinline__ u32x4 load_vec(const char* x) {
   return STREAM ? __builtin_nontemporal_load(at) : *at;
 }
 
-// FORMAT: of the cache, or -1 without one.  STREAM: rows are loaded and stored nontemporally.
+// FORMAT: of the cache, or -1 without one.  STREAM: rows are loaded nontemporally.
 template <int TYPE, int FORMAT, bool INTERLEAVED, bool STREAM>
 __global__ __launch_bounds__(kThreads) void rope_kernel(const RopeParams p) {
   const uint32_t lane = threadIdx.x % 64;
