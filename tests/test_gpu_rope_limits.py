@@ -172,3 +172,114 @@ def test_outputs_in_any_layout_whose_rows_are_apart(gpu):
     for strides in ((64, 64, 1), (64 * 3, 64, 1), (64 * 2, 64 * 3, 1), (96, 64, 1), (64, 96, 1), (64 * 5 - 32, 64 * 2, 1)):
         with pytest.raises(RuntimeError, match="overlap"):
             rope.norm_rotate(q, None, at, table, out_q=room.as_strided((n, H, D), strides))
+
+
+def check_every_token(got, x, w, positions, table, interleaved):
+    """check_turned in torch's float64, some thousand tokens at a time; the first and the
+    last by the oracle."""
+    n, _, D = x.shape
+    ends = np.array([0, 1, n - 2, n - 1])
+    check_turned(got[ends], x[ends], w, positions[ends], table, interleaved)
+    r = table.shape[1]
+    j = torch.arange(r // 2, device=x.device)
+    a, b = (2 * j, 2 * j + 1) if interleaved else (j, j + r // 2)
+    for i in range(0, n, 4000):
+        y = x[i:i + 4000].double()
+        y = y / torch.sqrt(y.square().mean(-1, keepdim=True) + EPS) * w.double()
+        c, s = table[torch.from_numpy(positions[i:i + 4000]).to(x.device)].double()[:, None].split(r // 2, -1)
+        size, p, q = y.abs(), y[..., a], y[..., b]
+        y[..., a], y[..., b] = p * c - q * s, q * c + p * s
+        size[..., a], size[..., b] = (p * c).abs() + (q * s).abs(), (q * c).abs() + (p * s).abs()
+        e = (D / 2 + 10) * 2.0 ** -24 * size                          # as the oracle's bound
+        most = torch.finfo(x.dtype).eps / 2 * (y.abs() + e) + e + sub_of(x.dtype)
+        assert ((got[i:i + 4000].double() - y).abs() <= most).all()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("n,Hq,H,D,r", [(16400, 16, 4, 128, 128), (16385, 8, 4, 128, 64), (9001, 32, 16, 128, 128),
+                                        (2100, 40, 30, 256, 256), (20000, 1, 0, 80, 80)])
+def test_waves_of_several_turns_and_streamed_rows(gpu, n, Hq, H, D, r, dtype, interleaved):
+    """Tokens enough that a wave takes a token's heads in turns, in calls on both sides of the
+    64 MiB from which on rows are loaded nontemporally; in place too."""
+    rng = np.random.default_rng(n)
+    table = rope.rotary_table(300, r, device=gpu)
+    pos = rng.integers(0, 300, n)
+    at = torch.tensor(pos, dtype=torch.int32, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(n)
+    x = torch.randn((n, Hq + H, D), generator=g, device=gpu).to(dtype)
+    q, k = x[:, :Hq], x[:, Hq:] if H else None
+    w = rows(rng, (D,), dtype, gpu)
+    got_q, got_k = rope.norm_rotate(q, k, at, table, w, w if H else None, interleaved=interleaved)
+    check_every_token(got_q, q, w, pos, table, interleaved)
+    if H:
+        check_every_token(got_k, k, w, pos, table, interleaved)
+    rope.norm_rotate(q, k, at, table, w, w if H else None, interleaved=interleaved, out_q=q, out_k=k)
+    assert torch.equal(q, got_q) and (k is None or torch.equal(k, got_k))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("fmt", [None, "mxfp8", "mxfp4"])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("n,Hq,H,D,r,P", [(70, 8, 2, 128, 128, 16), (40, 6, 3, 192, 64, 24), (33, 4, 4, 256, 128, 1),
+                                          (16400, 8, 2, 128, 128, 16), (9001, 16, 8, 128, 64, 16)])
+def test_appends_in_both_pairings_and_many_tokens(gpu, n, Hq, H, D, r, P, dtype, fmt, interleaved):
+    append_and_check(gpu, n, Hq, H, D, r, P, dtype, fmt, interleaved, tokens=None if n < 100 else 40)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("n,L,P", [(8192, 512, 16), (8193, 512, 24), (8193, 256, 16), (8195, 256, 1), (20001, 512, 64)])
+def test_many_latent_rows(gpu, n, L, P, dtype, interleaved):
+    """From 8192 rows on a group of lanes takes two, of which the last is alone in an odd call;
+    padding and bad slots among them."""
+    rng = np.random.default_rng(n + L)
+    pages = -(-n // P) + 2
+    table = rope.rotary_table(200, 64, device=gpu)
+    pos, slots = rng.integers(0, 200, n), rng.permutation(pages * P)[:n]
+    slots[rng.integers(0, n, 300)] = -1
+    bad = rng.choice(np.flatnonzero(slots[:n - 1] >= 0), 20, replace=False)
+    slots[bad[:10]], pos[bad[10:]] = pages * P + 5, 200
+    live = slots >= 0
+    live[bad] = False
+    x, w = rows(rng, (n, L + 64), dtype, gpu), rows(rng, (L,), dtype, gpu)
+    where, at = torch.from_numpy(slots[live]).to(gpu), torch.from_numpy(np.flatnonzero(live)).to(gpu)
+    for weight in (w, None):
+        cache, err = torch.full((pages, P, L + 64), 3.0, dtype=dtype, device=gpu), torch.zeros(1, dtype=torch.int32, device=gpu)
+        latent.append_paged_latent_cache(x[:, :L], x[:, L:], torch.tensor(pos, dtype=torch.int32, device=gpu),
+                                         torch.tensor(slots, device=gpu), cache, table, weight, interleaved=interleaved,
+                                         err=err)
+        torch.cuda.synchronize()
+        assert err.item() == 20
+        flat = cache.view(-1, L + 64)
+        got = flat[where]
+        look = np.unique(np.concatenate([[0, 1, len(where) - 2, len(where) - 1], rng.integers(0, len(where), 60)]))
+        token = np.flatnonzero(live)[look]
+        check_turned(got[look][:, None, L:], x[token][:, None, L:], None, pos[token], table, interleaved)
+        if weight is None:
+            assert torch.equal(got[:, :L], x[at, :L])
+        else:
+            y, g = f64(x[at, :L]), f64(got[:, :L])
+            y = y / np.sqrt((y * y).mean(-1, keepdims=True) + EPS) * f64(w)
+            assert (np.abs(g - y) <= ro.bound(y, np.abs(y), L, torch.finfo(dtype).eps, sub_of(dtype))).all()
+        rest = torch.ones(pages * P, dtype=torch.bool, device=gpu)
+        rest[where] = False
+        assert (flat[rest] == 3).all()
+
+
+@pytest.mark.parametrize("fmt", [None, "mxfp8"])
+@pytest.mark.parametrize("n", [5, 9001])
+def test_queries_of_an_append_in_place(gpu, n, fmt):
+    rng = np.random.default_rng(n)
+    table = rope.rotary_table(50, 64, device=gpu)
+    at = torch.tensor(rng.integers(0, 50, n), dtype=torch.int32, device=gpu)
+    slots = torch.tensor(rng.permutation(n + 11)[:n], device=gpu)
+    x, w = rows(rng, (n, 14, 128), BF16, gpu), rows(rng, (128,), BF16, gpu)
+    width = 128 if fmt is None else mx.row_width(128, fmt)
+    caches = [torch.zeros((n + 11, 2, 1, 2, width), dtype=BF16 if fmt is None else torch.uint8, device=gpu) for _ in range(2)]
+    q, k, v = x.split([10, 2, 2], 1)
+    kept = x.clone()
+    want = rope.append_paged_kv_cache_rope(q, k, v, at, slots, caches[0], table, w, w)
+    got = rope.append_paged_kv_cache_rope(q, k, v, at, slots, caches[1], table, w, w, out=q)
+    assert got is q and torch.equal(q, want) and torch.equal(x[:, 10:], kept[:, 10:])
+    assert torch.equal(caches[0], caches[1])
