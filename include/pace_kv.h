@@ -569,11 +569,13 @@ int pace_kv_attention(const void* q, int64_t q_stride_bytes, int elem_type,
  *   pos = seq_lens[b] - n + j, slot = page_table[b][pos / page_size] *
  *   page_size + pos % page_size; -1 and -1 for rows of no request.
  * Lengths are cut to [0, width * page_size], page lists to num_indices
- * (kv_indptr runs on); a token before a request's first or past its pages has
- * slot -1.  err_count goes up by one for each request of which something is
- * cut, whose offsets run backwards or leave [0, nnz], or that appends more
- * tokens than it has (but for length 0 with append_indptr NULL: an unused
- * place of the batch).
+ * (kv_indptr runs on), rows to [0, nnz) (n is what is left of them); a token
+ * before a request's first or past its pages has slot -1, and so does one whose
+ * page id is below 0: a page that is not there yet, which is not counted.
+ * err_count goes up by one for each request of which something is cut, whose
+ * offsets run backwards (rows that two requests then claim hold what either
+ * says) or leave [0, nnz], or that appends more tokens than it has (but for
+ * length 0 with append_indptr NULL: an unused place of the batch).
  *
  * Stands before the producer's calls in
  * paceserve/model_executor/attention/flashinfer_attention_wrapper.py:241-255,

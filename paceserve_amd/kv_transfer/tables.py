@@ -37,12 +37,18 @@ def build_tables(page_table: torch.Tensor, seq_lens: torch.Tensor, page_size: in
     nnz is the number of token rows (batch by default; needed with
     append_indptr): rows outside every request are padding, with position and
     slot -1.  num_indices is the length of kv_indices, width * batch by default;
-    a captured step keeps it while the lengths change.  `out` takes the tables
-    of an earlier call of the same sizes to write into.
+    a captured step keeps it while the lengths change.  Attention divides its
+    work, and sizes its workspace, by that length as if the requests filled it:
+    give it what they may come to hold, not the table's room, where that is much
+    more.  `out` takes the tables of an earlier call of the same sizes to write
+    into.
 
     Sequence lengths are cut to [0, width * page_size], page lists to
     num_indices (kv_indptr runs on); a token before a request's first or past
-    its pages gets slot -1.  `err` goes up by one for each request of which
+    its pages gets slot -1.  A page id below 0 is a page that is not there yet:
+    it is listed as it is, and its tokens get slot -1, which is padding to the
+    appends; that is not counted here (attention counts the tokens on pages out
+    of range that it should read).  `err` goes up by one for each request of which
     something is cut, whose offsets run backwards or leave [0, nnz], or that
     appends more tokens than it has (without append_indptr, one of length 0 is
     an unused place of the batch: no pages, position and slot -1)."""
