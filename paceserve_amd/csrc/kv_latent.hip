@@ -55,12 +55,13 @@ __device__ __forceinline__ uint32_t swap_of_weights(uint32_t n) { return (0u - n
 // Bound by memory where a tile is 16 or 32 rows (16 heads read 1152 bytes a token for 35
 // thousand operations): the steps read 6.4 TB/s, 128 requests of up to 8192 tokens all in all
 // 4.8 in 125 us; the rest is the start, where tables, page ids and rows wait for one another,
-// and the last workgroups.  A step of 64 rows takes 4700 cycles with two workgroups a CU:
-// 2050 the scores (of them 750 to issue the next rows' loads), 600 the weights, 650 the
-// barriers, 1200 the values; matrix instructions are busy 46 % of it (256 requests of 4096
-// tokens and 128 heads in 400 us, 730 TFLOP/s).  128 rows, which would halve the reads of
-// LDS, need more registers than four waves have (they spill), or two groups of waves that
-// take turns, which wait for each other (560 us where this took 425).
+// and the last workgroups.  A step of 64 rows takes 5200 to 5500 cycles with two workgroups a
+// CU: 2100 to 2500 the scores and the issue of the next rows' loads, 700 the weights, 700 the
+// barriers, 1650 to 1800 the values and the products that follow a raised maximum; matrix
+// instructions are busy 40 % of it (256 requests of 4096 tokens and 128 heads in 405 us, 720
+// TFLOP/s).  128 rows, which would halve the reads of LDS, need more registers than four waves
+// have (they spill), or two groups of waves that take turns, which wait for each other (560 us
+// where this took 425).
 template <int L, int TYPE, int RT>
 __global__ __launch_bounds__(kThreads, 2) void latent_kernel(const AttnParams p) {
   constexpr int kW = L + kRope, kKS = L / 32, kCT = L / 64;

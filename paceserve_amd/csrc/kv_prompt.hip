@@ -149,10 +149,11 @@ __device__ __forceinline__ uint32_t swap_of(uint32_t r) {
 // other is read.  With 128 columns the buffers take 40 KiB, so that three workgroups fit a CU
 // and one's softmax may lie under another's products.
 //
-// Bound by the SIMDs' issue: of 1290 cycles that a wave's step takes of one, matrix
-// instructions are 640 and vector ones about 600, 256 of them exponentials; LDS is busy a
-// quarter of the time, without conflicts (MI355X, 4096 queries of 32 heads behind 4096 keys
-// in 481 us, 1071 TFLOP/s; 8192 alone in 631, 1090).  Every instruction less shows: lanes'
+// Bound by the SIMDs' issue: of 1390 cycles that a wave's step takes of one, matrix
+// instructions are 640 and vector ones about 720, 256 of them exponentials and some 80 the
+// products that follow a raised maximum; LDS is busy a quarter of the time, without conflicts
+// (MI355X, 4096 queries of 32 heads behind 4096 keys in 499 us, 1033 TFLOP/s; 8192 alone in
+// 628, 1095).  Every instruction less shows: lanes'
 // places in memory kept in registers were 6 %, a finite lowest maximum 3.  Two workgroups
 // with 64 keys a step took 743 us where three with 32 took 693.  Waves of long tiles at a
 // higher priority: no change.
@@ -548,10 +549,10 @@ int64_t parts_of_call(int64_t nnz, int64_t keys, int64_t batch, int64_t heads, i
 
 // LDS that a workgroup asks for beyond its own, so that two fit a CU instead of three: the
 // last turn of few workgroups a CU costs more than three at a time gain.  One, two and three
-// workgroups a CU take about 10, 13 and 18 for the same keys (MI355X, 128 columns: 600, 925
-// and 991 TFLOP/s): four a CU take 26 by twos and 28 by threes.
+// workgroups a CU take about 10, 11 and 15 for the same keys (MI355X, 8192 tokens of 32 heads
+// of 128 columns: 536, 993 and 1060 TFLOP/s): four a CU take 22 by twos and 25 by threes.
 uint32_t spare_lds(int64_t groups, int head_dim) {
-  constexpr int64_t kCus = 256, kTime[4] = {0, 10, 13, 18};
+  constexpr int64_t kCus = 256, kTime[4] = {0, 10, 11, 15};
   const int64_t each = (groups + kCus - 1) / kCus;
   const auto time_of = [&](int64_t at_once) { return each / at_once * kTime[at_once] + kTime[each % at_once]; };
   if (time_of(3) <= time_of(2)) return 0;

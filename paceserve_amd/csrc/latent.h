@@ -21,10 +21,10 @@ __device__ __forceinline__ float unfused(float a, float b) {
 
 // Weights are rounded to the rows' type for their product, which takes nothing wider, and sums
 // take them unrounded (attention.h).  The running maximum is exact, so that the largest weight is
-// a power of two and not rounded: outputs are off by 0.0018 to 0.0019 of the values against 64
-// bits (bfloat16, 2000 to 4096 tokens), of which their own rounding is 0.0016.  (MI355X: raising
+// a power of two and not rounded: outputs are off by 0.0018 to 0.0021 of the values against 64
+// bits (bfloat16, 2000 to 8192 tokens), of which their own rounding is 0.0016.  (MI355X: raising
 // it only where a score passes it by 2^4 in weight saves a product of every sum, 4 to 8 % of
-// prompts and of calls of 64 rows and more, but outputs were off by 0.0019 to 0.0021, and where
+// prompts and of calls of 64 rows and more, but outputs were off by 0.0019 to 0.0023, and where
 // one token stands out by up to twice as much.)
 
 // The maximum of no scores: finite, so that differences from it are numbers.
