@@ -205,3 +205,36 @@ def test_latent_pages_through_the_channel_and_move(gpu, P, L, dtype):
         tx.close()
         rx.close()
     assert not failed, failed
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("q_len,kv_len,heads,D", [([2049], [2049], 50, 128), ([130, 700], [600, 700], 130, 64),
+                                                  ([2300], [3000], 50, 64), ([511] * 8, [600] * 8, 26, 128)])
+def test_prompts_of_four_workgroups_a_cu(gpu, q_len, kv_len, heads, D, dtype, causal):
+    """769 to 1024 workgroups, of which two at a time run on a CU instead of three."""
+    tiles = -(-sum(q_len) // 128) + (len(q_len) - 1) // 2
+    assert 768 < tiles * heads <= 1024
+    nnz, n, scale = sum(q_len), sum(kv_len), 1 / math.sqrt(D + 64)
+    assert latent._prompt_workspace_bytes(nnz, n, len(q_len), heads, D, int(causal)) == 0
+    rng = np.random.default_rng(nnz)
+    g = torch.Generator(device=gpu).manual_seed(nnz)
+    q = (1.5 * torch.randn((nnz, heads, D + 64), generator=g, device=gpu)).to(dtype)
+    kv = torch.randn((n, heads, 2 * D), generator=g, device=gpu).to(dtype)
+    rope = torch.randn((n, 64), generator=g, device=gpu).to(dtype)
+    qo, ip = (np.concatenate([[0], np.cumsum(x)]) for x in (q_len, kv_len))
+    out, lse = latent.latent_prompt_attention(q, kv[..., :D], rope, kv[..., D:], i32(qo, gpu), i32(ip, gpu), causal=causal,
+                                              return_lse=True)
+    torch.cuda.synchronize()
+    eps, sub = torch.finfo(dtype).eps, 2.0 ** -25 if dtype is FP16 else 0.0
+    for b, (t, m) in enumerate(zip(q_len, kv_len)):
+        at = np.unique(np.concatenate([[0, t - 1], rng.integers(0, t, 6)]))
+        sees = (np.arange(m)[None, :] <= (m - t + at)[:, None]) if causal else np.ones((len(at), m), bool)
+        for h in (0, int(rng.integers(1, heads - 1)), heads - 1):
+            key = torch.cat([kv[ip[b]:ip[b + 1], h, :D], rope[ip[b]:ip[b + 1]]], 1).double().cpu().numpy()
+            value = np.concatenate([kv[ip[b]:ip[b + 1], h, D:].double().cpu().numpy(), np.zeros((m, 64))], 1)
+            o, s, mean, dots, spread = ao.attend(q[qo[b] + at, h].double().cpu().numpy()[:, None], key[:, None], value[:, None],
+                                                 scale, 0.0, sees)
+            bo, bs = ao.bounds(D + 64, eps, o, s, mean, dots, spread, 0.0, m, sub)
+            got, sums = (x[qo[b] + at, h].double().cpu().numpy() for x in (out, lse))
+            assert (np.abs(got - o[:, 0, :D]) <= bo[:, 0, :D]).all() and (np.abs(sums - s[:, 0]) <= bs[:, 0]).all()
